@@ -418,6 +418,119 @@ int umic_add_rmsnorm_gate_silu_mul_bf16(const void* x, const void* r, const void
                                         float eps, void* stream);
 
 /*
+ * One step of a paged key / value pool: block tables and slot maps from
+ * request lengths, on the device.  Request r of R holds kv_len[r] tokens in the
+ * pages table[r][0 ..] (row stride table_ld, W entries) of page_size tokens
+ * each; ring [pages] is the queue of free pages and cursor = {head, count, -, -}
+ * its state.  The request keeps its first
+ *   kept = clamp(keep[r], 0, kv_len[r])         (keep NULL: all)
+ * tokens and gets new_len[r] more (negative: none).  With
+ *   have = ceil(kv_len / page_size), need = ceil((kept + new) / page_size)
+ * pages [need, have) of its row go to the queue's tail and pages [have, need)
+ * come from the queue's head, requests in order, all pages given back before the
+ * first is taken.  Row entries from need on are left as they are.
+ * Outputs: kv_len_out[r] = kept + new; cursor_out = {head, count, tokens,
+ * status}; starts[R + 1], the sums of the new lengths; and for its new token i
+ *   slots[t] = table[r][p / page_size] * page_size + p % page_size,
+ *   positions[t] = p + delta[r]                 (delta NULL: 0)
+ * with p = kept + i, at t = starts[r] + i (row == 0) or t = r * row + i (row >
+ * 0; tokens == R * row).  Every other slots entry is -1, every other position 0.
+ * kv_len_out may be kv_len and cursor_out may be cursor.  A step that cannot be
+ * made changes nothing but cursor_out[3] (one of UMIC_PLAN_*): lengths and queue
+ * as they were, starts 0, every slot -1.  A repeated call on the same kv_len and
+ * cursor gives the same results again.  page_size: a power of two from 16 (else
+ * UMIC_ERR_UNSUPPORTED).  No counterpart in the reference, whose cache holds one
+ * batch of equal lengths (cache.py:25-160).
+ */
+#define UMIC_PLAN_OK 0
+#define UMIC_PLAN_NO_PAGES 1  /* more pages are needed than are free */
+#define UMIC_PLAN_TOO_LONG 2  /* a request outgrows its table row */
+#define UMIC_PLAN_NO_ROOM 3   /* more new tokens than tokens, or than row */
+#define UMIC_PLAN_BAD_STATE 4 /* a length or the queue's state out of range */
+int umic_page_plan(const int32_t* kv_len, const int32_t* new_len, const int32_t* keep,
+                   const int32_t* delta, int32_t* table, int32_t* ring, const int32_t* cursor,
+                   int32_t* kv_len_out, int32_t* cursor_out, int32_t* starts, int64_t* slots,
+                   int64_t* positions, int64_t R, int64_t W, int64_t table_ld, int64_t pages,
+                   int64_t page_size, int64_t tokens, int64_t row, void* stream);
+
+/*
+ * Rotary embedding of q and k from positions of several axes (time, height,
+ * width), one launch.  Pair f of a head row, elements f and f + D/2, turns by
+ *   positions[axis[f]][t] * inv_freq[f]  radians:
+ *   out[f] = x[f] cos - x[f + D/2] sin,  out[f + D/2] = x[f + D/2] cos + x[f] sin
+ * with cos and sin times scale.  turn[f] = round(2^64 inv_freq[f] / (2 pi)) mod
+ * 2^64, the frequency in 64-bit fractions of a turn per position: the angle of
+ * any int64 position is then exact to |position| 2^-65 turns.  With q_w / k_w ([D]
+ * bf16; both or neither) each head row is normalised first, x * rsqrt(mean(x^2) +
+ * eps) * w.  fp32 throughout, one rounding to bf16 (unlike UMIC_ROPE_TEXT).
+ * q: T x Hq x D, element strides (q_st, q_sh); k: T x Hk x D; positions: axes x
+ * T, strides (p_sa, p_st); axis[f] outside [0, axes) does not turn.  D % 8 == 0,
+ * D <= 512; strides and pointers multiples of 8 elements (D % 16 == 0), else of
+ * 4 (else UMIC_ERR_UNSUPPORTED).  Outputs may be the inputs.
+ * Replaces: the rotary table of HF Qwen3VLTextRotaryEmbedding followed by
+ * kernels/rope.py:86-107 (make_text_rope), and likewise :78-84 for the vision
+ * encoder's rows and columns.
+ */
+int umic_axial_rope_bf16(const void* q, const void* k, void* q_out, void* k_out,
+                         const int64_t* positions, const uint64_t* turn, const int32_t* axis,
+                         float scale, const void* q_w, const void* k_w, float eps, int64_t T,
+                         int64_t Hq, int64_t Hk, int64_t D, int64_t axes, int64_t p_sa,
+                         int64_t p_st, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+                         int64_t qo_st, int64_t qo_sh, int64_t ko_st, int64_t ko_sh,
+                         void* stream);
+
+/*
+ * umic_axial_rope_bf16 of q, with k's rotated rows and v's rows written to the
+ * slots of a paged pool: row (slot % page_size) of page (slot / page_size), strides
+ * (c_sb page, c_sh head, c_ss row), the same for both.  A slot outside [0, pages *
+ * page_size) is not written (its q row is computed).  slots must not repeat.
+ * page_size: a power of two from 16.  Replaces: the same, followed by the cache
+ * append of cache.py:50-80, for requests of different lengths.
+ */
+int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, void* q_out,
+                                void* k_pages, void* v_pages, const int64_t* positions,
+                                const uint64_t* turn, const int32_t* axis, const int64_t* slots,
+                                float scale, const void* q_w, const void* k_w, float eps,
+                                int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t axes,
+                                int64_t p_sa, int64_t p_st, int64_t q_st, int64_t q_sh,
+                                int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
+                                int64_t qo_st, int64_t qo_sh, int64_t c_sb, int64_t c_sh,
+                                int64_t c_ss, int64_t pages, int64_t page_size, void* stream);
+
+/*
+ * Attention of the last S tokens of each of B requests over its cache:
+ *   out[b,s,h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * q[b,s,h] . k_j),
+ * over the keys j < n_b of request b (causal: j <= n_b - m_b + s), fp32 softmax,
+ * one rounding to bf16.  n_b = kv_lens[b] (device; NULL: kv_len for all), the new
+ * tokens included, clamped to what the cache can hold; m_b = q_lens[b] (NULL:
+ * S): rows s >= m_b, and rows that see no key, are zero.
+ * q: B x S x Hq x D, strides (q_sb, q_ss, q_sh); out likewise (o_*).  Query head
+ * h reads key head h / (Hq / Hk).
+ * k, v: blocks of block_rows rows, strides (c_sb block, c_sh head, c_ss row).
+ * table NULL: request b is block b (blocks == B).  Else row j of request b is
+ * row j % block_rows of block table[b * table_ld + j / block_rows], table_w
+ * entries a request; block_rows a power of two from 16; an entry outside [0,
+ * blocks) is read as keys that are not there.  Rows past n_b are not used,
+ * whatever they hold.  A later new token's v that is infinite or NaN does not
+ * reach the rows that do not see it.
+ * D: 64, 128 or 256; strides multiples of 8, pointers 16-byte aligned (else
+ * UMIC_ERR_UNSUPPORTED).  workspace: umic_cache_attention_workspace_bytes, for
+ * this call alone until it has run (contents need not be kept or cleared).
+ * Results do not depend on what ran before, and repeat bit for bit.
+ * Replaces: the attention that HF Qwen3VLTextAttention calls after cache.py:50-80
+ * (InplaceLayer.update, whose single-token steps copy the whole cache for it).
+ */
+int64_t umic_cache_attention_workspace_bytes(int64_t S, int64_t Hq, int64_t Hk, int64_t D);
+int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void* out,
+                              const int32_t* table, const int32_t* kv_lens,
+                              const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
+                              int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t o_sb,
+                              int64_t o_ss, int64_t o_sh, int64_t c_sb, int64_t c_sh,
+                              int64_t c_ss, int64_t blocks, int64_t block_rows, int64_t table_ld,
+                              int64_t table_w, int64_t kv_len, int causal, float scale,
+                              void* workspace, int64_t workspace_bytes, void* stream);
+
+/*
  * Measurement helper: reads `bytes` bytes at p once (16-byte non-temporal
  * loads; p 16-byte aligned, bytes a multiple of 16, else
  * UMIC_ERR_UNSUPPORTED) and writes one xor-fold word per workgroup to

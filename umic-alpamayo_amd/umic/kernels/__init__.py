@@ -26,7 +26,8 @@ def get_kernel(pattern_name: str) -> Callable | None:
 
 
 def _register_builtin() -> None:
-    from umic.kernels import fused_ffn, layernorm, linear, rmsnorm, rope
+    from umic.kernels import (attention, axial, fused_ffn, layernorm, linear, paged, rmsnorm,
+                              rope)
 
     for name, fn in (
         ("gate_silu_mul", fused_ffn.gate_silu_mul_hip),
@@ -37,6 +38,10 @@ def _register_builtin() -> None:
         ("add_layernorm", layernorm.add_layernorm_hip),
         ("rope_text", rope.apply_rotary_text_hip),
         ("rope_vision", rope.apply_rotary_vision_hip),
+        ("rope_axial", axial.rotate),
+        ("rope_axial_append", axial.rotate_append),
+        ("plan_pages", paged.plan_pages),
+        ("cache_attention", attention.cache_attention),
     ):
         _KERNELS[name] = fn
 

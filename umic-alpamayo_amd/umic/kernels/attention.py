@@ -1,0 +1,125 @@
+"""Attention of new tokens over a key / value cache on gfx950 (libumic_hip.so):
+the decode step's single tokens, an action expert's few, a prompt's next chunk.
+
+The cache is contiguous (``umic.cache.KVArena``'s layer views) or paged
+(``paged.plan_pages``); it is read where it lies, once, by workgroups that share
+the keys of all requests evenly, and their parts are joined.  In the reference the
+cache hands such steps to the library's attention, single tokens as a copy of the
+whole prefix (src/umic/cache.py:50-80).
+
+Numerics: bf16 products in fp32, softmax in fp32, one rounding of the output.
+"""
+
+from __future__ import annotations
+
+import functools
+
+import torch
+
+from umic import _lib
+from umic.kernels._common import grad_needed, require_device
+
+HEAD_DIMS = (64, 128, 256)
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(dev: int, S: int, Hq: int, Hk: int, D: int) -> int:
+    return _lib.lib().umic_cache_attention_workspace_bytes(S, Hq, Hk, D)
+
+
+def _chunks_ok(t: torch.Tensor) -> bool:
+    """Contiguous rows of 16-byte chunks."""
+    s = t.stride()
+    return s[3] == 1 and not ((s[0] | s[1] | s[2]) & 7) and t.data_ptr() % 16 == 0
+
+
+def cache_ok(k_cache: torch.Tensor, v_cache: torch.Tensor) -> bool:
+    """Caches the kernel reads: bf16 GPU [blocks, Hk, rows, D] of one layout, D one of
+    HEAD_DIMS, 16-byte chunks."""
+    return (k_cache.is_cuda and k_cache.dtype is torch.bfloat16 and k_cache.dim() == 4
+            and v_cache.dtype is torch.bfloat16 and v_cache.get_device() == k_cache.get_device()
+            and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride()
+            and k_cache.shape[3] in HEAD_DIMS and _chunks_ok(k_cache) and _chunks_ok(v_cache))
+
+
+def _lengths(name: str, t: torch.Tensor, B: int, dev: int) -> None:
+    if (t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != B or t.get_device() != dev
+            or not t.is_contiguous()):
+        raise ValueError(f"cache_attention: {name} must be a contiguous int32 vector of {B} on "
+                         f"q's device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
+def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, kv_len, *,
+                    table: torch.Tensor | None = None, q_len: torch.Tensor | None = None,
+                    causal: bool = True, scale: float | None = None,
+                    out: torch.Tensor | None = None) -> torch.Tensor:
+    """softmax(scale q k^T) v of the last S tokens of each request over its cache.
+
+    Args:
+        q: [B, Hq, S, D], rotated queries of the new tokens.
+        k_cache, v_cache: [B, Hk, rows, D] (request b's rows in block b), or with
+            ``table`` [pages, Hk, page_size, D].  The new tokens' rows are in them.
+        kv_len: tokens of each request, the new ones included: an int for all, or int32
+            [B] on the device (clamped there to what the cache can hold).
+        table: int32 [B, W], request b's pages in order.  page_size: a power of two from 16.
+        q_len: int32 [B], new tokens of each request (None: S); rows past it are zero.
+        causal: new token s sees keys up to its own, kv_len - q_len + s; else all.
+        scale: of the scores (None: D ** -0.5).
+        out: [B, S, Hq, D] to write to.
+
+    Returns [B, S, Hq, D].  A row that sees no key is zero.
+    """
+    require_device(q, k_cache, v_cache)
+    if grad_needed(q, k_cache, v_cache):
+        raise RuntimeError("cache_attention: the kernel has no backward; call it under "
+                           "torch.no_grad()")
+    if q.dim() != 4 or not cache_ok(k_cache, v_cache):
+        raise ValueError(f"cache_attention: unsupported layout q{tuple(q.shape)} "
+                         f"cache{tuple(k_cache.shape)} (head sizes {HEAD_DIMS})")
+    B, Hq, S, D = q.shape
+    blocks, Hk, rows, Dk = k_cache.shape
+    if Dk != D or Hk == 0 or Hq % Hk:
+        raise ValueError(f"cache_attention: {Hq} heads of {D} over a cache of {Hk} of {Dk}")
+    dev = q.get_device()
+    if table is None:
+        if blocks != B:
+            raise ValueError(f"cache_attention: {B} requests over a cache of {blocks} blocks")
+        cap, ld, width = rows, 0, 0
+    else:
+        if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B
+                or table.get_device() != dev or table.stride(1) != 1):
+            raise ValueError(f"cache_attention: table must be int32 [{B}, W] with contiguous rows "
+                             f"on q's device, got {table.dtype} {tuple(table.shape)}")
+        width = table.shape[1]
+        cap, ld = width * rows, table.stride(0) if B > 1 else width
+    if isinstance(kv_len, torch.Tensor):
+        _lengths("kv_len", kv_len, B, dev)
+        lens, n = kv_len.data_ptr(), 0
+    else:
+        lens, n = None, int(kv_len)
+        if not 0 <= n <= cap:
+            raise ValueError(f"cache_attention: kv_len {n} of a cache that holds {cap}")
+    if q_len is not None:
+        _lengths("q_len", q_len, B, dev)
+    if not _chunks_ok(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if out is None:
+        out = q.new_empty(B, S, Hq, D)
+    else:
+        require_device(q, out)
+        if tuple(out.shape) != (B, S, Hq, D) or not _chunks_ok(out):
+            raise ValueError(f"cache_attention: out must be [{B}, {S}, {Hq}, {D}] of 16-byte "
+                             f"chunks, got {tuple(out.shape)}")
+    if out.numel() == 0:
+        return out
+    qs, os_, cs = q.stride(), out.stride(), k_cache.stride()
+    with _lib.device_of(q):
+        size = _workspace_bytes(dev, S, Hq, Hk, D)
+        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        _lib.call("umic_cache_attention_bf16", q.data_ptr(), k_cache.data_ptr(),
+                  v_cache.data_ptr(), out.data_ptr(), _lib.ptr(table), lens, _lib.ptr(q_len),
+                  B, S, Hq, Hk, D, qs[0], qs[2], qs[1], os_[0], os_[1], os_[2], cs[0], cs[1],
+                  cs[2], blocks, rows, ld, width, n, int(causal),
+                  float(D ** -0.5 if scale is None else scale), ws.data_ptr(), size,
+                  _lib.stream_of(q))
+    return out

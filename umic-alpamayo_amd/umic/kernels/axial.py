@@ -1,0 +1,185 @@
+"""Rotary embedding from positions of several axes (time, height and width of
+images and video) on gfx950 (libumic_hip.so), with the attention's q_norm /
+k_norm in front and the append into a paged pool behind, in one launch.
+
+The reference rotates by cos / sin tables that the model makes from the
+positions (src/umic/kernels/rope.py:62-107).  Here the positions are the input: an
+``AxisPlan`` says which axis turns which pair of a head row, and how fast.
+
+Numerics: fp32 with one rounding to bf16 (the eager text chain rounds the
+tables, both products and the sum: ``rope``).  Angles are 64-bit fractions of a
+turn, so positions of any size turn exactly.
+"""
+
+from __future__ import annotations
+
+from fractions import Fraction
+
+import torch
+
+from umic import _lib
+from umic.kernels._common import grad_needed, require_device
+
+MAX_HEAD_DIM = 512
+_PI = Fraction(314159265358979323846264338327950288419716939937510582097494, 10 ** 59)
+
+
+class AxisPlan:
+    """Which axis turns which pair of a head row, and how fast.
+
+    inv_freq: [D/2] radians per position of each pair (its fp32 values are taken
+        exactly); axis: [D/2] the axis whose positions turn it; scale: factor of
+        cos and sin (a rotary module's ``attention_scaling``).
+    """
+
+    def __init__(self, inv_freq: torch.Tensor, axis, scale: float = 1.0,
+                 device: torch.device | str | None = None) -> None:
+        device = inv_freq.device if device is None else torch.device(device)
+        freq = inv_freq.detach().double().cpu().tolist()
+        axis = torch.as_tensor(axis).detach().cpu().to(torch.int32)
+        if inv_freq.dim() != 1 or axis.shape != inv_freq.shape:
+            raise ValueError(f"AxisPlan: inv_freq {tuple(inv_freq.shape)} and axis "
+                             f"{tuple(axis.shape)} must be vectors of one length")
+        if not freq or not all(abs(f) < float("inf") for f in freq) or int(axis.min()) < 0:
+            raise ValueError("AxisPlan: frequencies must be finite and axes not negative")
+        turn = [round(Fraction(f) / (2 * _PI) * 2 ** 64) % 2 ** 64 for f in freq]
+        self.turn = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turn],
+                                 dtype=torch.int64).to(device)
+        self.axis = axis.to(device)
+        self.axes = int(axis.max()) + 1
+        self.head_dim = 2 * len(freq)
+        self.scale = float(scale)
+
+    @classmethod
+    def text(cls, head_dim: int, theta: float, sections, interleaved: bool = True,
+             scale: float = 1.0, device: torch.device | str = "cuda") -> "AxisPlan":
+        """The text trunk's plan: pair f turns at theta^(-2 f / head_dim).
+        ``sections`` are the pairs of each axis.  Interleaved (Qwen3-VL): axis a >
+        0 has pairs a, a + n, a + 2 n .. (n axes), as many as its section, and axis
+        0 the rest; else (Qwen2-VL) one axis after the other."""
+        half, n = head_dim // 2, len(sections)
+        if head_dim % 2 or sum(sections) != half:
+            raise ValueError(f"AxisPlan.text: sections {tuple(sections)} are not the {half} pairs "
+                             f"of a head of {head_dim}")
+        if interleaved:
+            axis = [0] * half
+            for a in range(1, n):
+                for f in range(a, min(half, n * sections[a]), n):
+                    axis[f] = a
+        else:
+            axis = [a for a, s in enumerate(sections) for _ in range(s)]
+        inv = 1.0 / theta ** (torch.arange(0, head_dim, 2, dtype=torch.float32) / head_dim)
+        return cls(inv, axis, scale, device)
+
+    @classmethod
+    def rotary(cls, module: torch.nn.Module) -> "AxisPlan":
+        """The plan of a transformers text rotary module: its ``inv_freq``,
+        ``mrope_section`` (interleaved) and ``attention_scaling``."""
+        inv = module.inv_freq
+        sections = list(getattr(module, "mrope_section", None) or [inv.shape[0]])
+        plan = cls.text(2 * inv.shape[0], 1e4, sections, device="cpu")
+        return cls(inv, plan.axis, getattr(module, "attention_scaling", 1.0))
+
+    @classmethod
+    def grid(cls, head_dim: int, theta: float = 1e4,
+             device: torch.device | str = "cuda") -> "AxisPlan":
+        """A vision encoder's plan: the first half of the pairs turns by rows, the
+        second by columns, both at theta^(-4 f / head_dim)."""
+        if head_dim % 4:
+            raise ValueError(f"AxisPlan.grid: a head of {head_dim} has no two halves of pairs")
+        half = head_dim // 2
+        inv = 1.0 / theta ** (torch.arange(0, half, 2, dtype=torch.float32) / half)
+        quarter = half // 2
+        return cls(torch.cat((inv, inv)), [0] * quarter + [1] * quarter, device=device)
+
+
+def _rows_ok(t: torch.Tensor) -> bool:
+    """Head rows the kernel reads: [T, H, D], contiguous rows on 8-byte chunks."""
+    return (t.stride(2) == 1 and t.stride(0) % 4 == 0 and t.stride(1) % 4 == 0
+            and t.data_ptr() % 8 == 0)
+
+
+def _check(who: str, q, k, positions, plan: AxisPlan, norm) -> None:
+    require_device(q, k, *(norm[:2] if norm is not None else ()))
+    if grad_needed(q, k, *(norm[:2] if norm is not None else ())):
+        raise RuntimeError(f"{who}: the kernel has no backward; call it under torch.no_grad()")
+    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [T, heads, D]")
+    T, _, D = q.shape
+    if D != plan.head_dim or D % 8 or D > MAX_HEAD_DIM:
+        raise ValueError(f"{who}: heads of {D} (the plan's have {plan.head_dim}; multiples of 8 "
+                         f"up to {MAX_HEAD_DIM})")
+    dev = q.get_device()
+    if (positions.dtype is not torch.int64 or positions.dim() != 2 or positions.shape[1] != T
+            or positions.shape[0] < plan.axes or positions.get_device() != dev):
+        raise ValueError(f"{who}: positions must be int64 [{plan.axes} axes, {T}] on q's device, "
+                         f"got {positions.dtype} {tuple(positions.shape)}")
+    if plan.turn.get_device() != dev:
+        raise ValueError(f"{who}: the plan is on {plan.turn.device}, q on {q.device}")
+    if norm is not None:
+        for w in norm[:2]:
+            if tuple(w.shape) != (D,) or not w.is_contiguous():
+                raise ValueError(f"{who}: norm weights must be contiguous vectors of {D}")
+
+
+def _ready(t: torch.Tensor) -> torch.Tensor:
+    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
+
+
+def _norm_args(norm):
+    return (None, None, 0.0) if norm is None else (norm[0].data_ptr(), norm[1].data_ptr(),
+                                                   float(norm[2]))
+
+
+def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: AxisPlan,
+           norm=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """q [T, Hq, D] and k [T, Hk, D] turned by positions [axes, T] (int64), as new
+    contiguous tensors.  With ``norm = (q_w, k_w, eps)`` each head row is RMS-normed
+    first."""
+    _check("rotate", q, k, positions, plan, norm)
+    q, k = _ready(q), _ready(k)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    q_out, k_out = q.new_empty(T, Hq, D), k.new_empty(T, Hk, D)
+    with _lib.device_of(q):
+        _lib.call("umic_axial_rope_bf16", q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
+                  k_out.data_ptr(), positions.data_ptr(), plan.turn.data_ptr(),
+                  plan.axis.data_ptr(), plan.scale, *_norm_args(norm), T, Hq, Hk, D,
+                  positions.shape[0], positions.stride(0), positions.stride(1), q.stride(0),
+                  q.stride(1), k.stride(0), k.stride(1), Hq * D, D, Hk * D, D, _lib.stream_of(q))
+    return q_out, k_out
+
+
+def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
+                  plan: AxisPlan, slots: torch.Tensor, k_pages: torch.Tensor,
+                  v_pages: torch.Tensor, norm=None) -> torch.Tensor:
+    """``rotate`` of q, with k's rotated rows and v's rows written to ``slots`` (int64
+    [T], distinct; one outside the pool writes nothing) of k_pages and v_pages [pages,
+    Hk, page_size, D].  Returns the rotated q."""
+    _check("rotate_append", q, k, positions, plan, norm)
+    require_device(q, v, k_pages, v_pages)
+    T, Hq, D = q.shape
+    Hk = k.shape[1]
+    if v.shape != k.shape or grad_needed(v):
+        raise ValueError(f"rotate_append: v {tuple(v.shape)} must be like k {tuple(k.shape)}, "
+                         "without a gradient")
+    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != Hk
+            or k_pages.shape[3] != D or k_pages.stride() != v_pages.stride()
+            or k_pages.stride(3) != 1):
+        raise ValueError(f"rotate_append: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} "
+                         f"must be [pages, {Hk}, page_size, {D}] of one layout")
+    if (slots.dtype is not torch.int64 or slots.dim() != 1 or slots.shape[0] != T
+            or slots.get_device() != q.get_device() or slots.stride(0) != 1 and T > 1):
+        raise ValueError(f"rotate_append: slots must be a contiguous int64 vector of {T} on q's "
+                         "device")
+    q, k, v = _ready(q), _ready(k), _ready(v)
+    q_out = q.new_empty(T, Hq, D)
+    with _lib.device_of(q):
+        _lib.call("umic_axial_rope_append_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), positions.data_ptr(),
+                  plan.turn.data_ptr(), plan.axis.data_ptr(), slots.data_ptr(), plan.scale,
+                  *_norm_args(norm), T, Hq, Hk, D, positions.shape[0], positions.stride(0),
+                  positions.stride(1), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
+                  v.stride(0), v.stride(1), Hq * D, D, *k_pages.stride()[:3], k_pages.shape[0],
+                  k_pages.shape[2], _lib.stream_of(q))
+    return q_out
