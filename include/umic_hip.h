@@ -516,10 +516,14 @@ int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, voi
  * D: 64, 128 or 256; strides multiples of 8, pointers 16-byte aligned (else
  * UMIC_ERR_UNSUPPORTED).  workspace: umic_cache_attention_workspace_bytes, for
  * this call alone until it has run (contents need not be kept or cleared).
- * Results do not depend on what ran before, and repeat bit for bit.
+ * counters: UMIC_ATTENTION_COUNTERS int32, zero before their first use and left
+ * zero by every call, for calls that do not overlap in time (those of one stream):
+ * up to 16 rows (S * Hq / Hk) are then one launch; NULL: two.  The results are the
+ * same, do not depend on what ran before, and repeat bit for bit.
  * Replaces: the attention that HF Qwen3VLTextAttention calls after cache.py:50-80
  * (InplaceLayer.update, whose single-token steps copy the whole cache for it).
  */
+#define UMIC_ATTENTION_COUNTERS 4096
 int64_t umic_cache_attention_workspace_bytes(int64_t S, int64_t Hq, int64_t Hk, int64_t D);
 int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void* out,
                               const int32_t* table, const int32_t* kv_lens,
@@ -528,7 +532,7 @@ int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void*
                               int64_t o_ss, int64_t o_sh, int64_t c_sb, int64_t c_sh,
                               int64_t c_ss, int64_t blocks, int64_t block_rows, int64_t table_ld,
                               int64_t table_w, int64_t kv_len, int causal, float scale,
-                              void* workspace, int64_t workspace_bytes, void* stream);
+                              int32_t* counters, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Measurement helper: reads `bytes` bytes at p once (16-byte non-temporal

@@ -62,15 +62,17 @@ def test_axial_refusals(lib):
 
 def test_cache_attention_refusals(lib):
     def f(B=2, S=1, Hq=8, Hk=2, D=128, q=FAKE, k=FAKE, v=FAKE, out=FAKE, table=None, lens=None,
-          st=1024, blocks=2, rows=64, ld=0, w=0, n=64, ws=FAKE, size=1 << 40):
+          st=1024, blocks=2, rows=64, ld=0, w=0, n=64, ws=FAKE, size=1 << 40,
+          scale=0.1):
         return lib.umic_cache_attention_bf16(
             q, k, v, out, table, lens, None, B, S, Hq, Hk, D, st, st, 128, st, st, 128, 16384, 8192,
-            128, blocks, rows, ld, w, n, 1, 0.1, ws, size, None)
+            128, blocks, rows, ld, w, n, 1, scale, None, ws, size, None)
 
     assert f(B=-1) == f(S=-1) == f(Hq=-1) == f(Hk=-1) == f(D=0) == f(rows=-1) == f(size=-1) == ARG
     assert f(B=0) == f(S=0) == f(Hq=0) == 0
     assert f(Hk=3) == f(Hk=0) == ARG
     assert f(q=None) == f(out=None) == f(ws=None) == f(k=None) == f(v=None) == ARG
+    assert f(scale=float("inf")) == f(scale=float("nan")) == ARG
     assert f(blocks=3) == ARG                              # contiguous: one block a request
     assert f(n=65) == f(n=-1) == ARG                       # past the cache
     assert f(table=FAKE, w=4, ld=3) == f(table=FAKE, w=-1) == ARG

@@ -13,17 +13,21 @@
 //    holds them: p never leaves its registers;
 //  * a key's row is read as the operand wants it, 16 bytes a lane; V is read
 //    along its rows too, and turned in registers (v_perm of row pairs).
-// Nothing goes through LDS until the four waves of a workgroup, which take 32
-// keys each of a tile of 128, are joined.
-//
-// The tiles of all requests, in one row, are dealt evenly over the launch's
-// workgroups, so requests of all lengths fill the chip alike.  A workgroup that
-// has a part of a request's tiles leaves (max, sum, output) in the workspace: at
-// most two such parts each, the first and the last of its tiles; a second kernel
-// joins the parts in a fixed order.
-//
 // p is split in two bf16 parts (p = hi + lo to 2^-17), each its own product: one
 // rounding to bf16 would weigh as much as the output's own.
+//
+// Up to 16 rows (single tokens) the four waves of a workgroup take 32 keys each,
+// and nothing goes through LDS until they are joined: HBM-bound.  More rows go
+// 16 or 32 to a wave, and the waves share the keys through LDS.
+//
+// The key tiles of all requests, in one row, are dealt evenly over the launch's
+// workgroups, so requests of all lengths fill the chip alike.  A workgroup that
+// has a part of a request's tiles leaves (max, sum, output) in the workspace: at
+// most two such parts each, of the first and the last of its segments.  They are
+// joined in the order of the keys: by the workgroup that finishes last, for up
+// to 16 rows and with counters to find that out, else by a second kernel.
+#include <algorithm>
+
 #include "common.hpp"
 #include "gemm_ks.hpp"  // device_cus
 
@@ -35,8 +39,7 @@ typedef float f32x4_t __attribute__((ext_vector_type(4)));
 
 constexpr int kThreads = 256;
 constexpr int kWaves = 4;
-constexpr int kStep = 32;              // keys of a wave's step
-constexpr int kTile = kStep * kWaves;  // keys of a workgroup's step
+constexpr int kStep = 32;             // keys of a wave's step
 
 struct AttnArgs {
   const uint16_t* q;
@@ -46,94 +49,164 @@ struct AttnArgs {
   const int32_t* table;   // or NULL: request b is block b
   const int32_t* kv_len;  // or NULL: len
   const int32_t* q_len;   // or NULL: S
-  float* part;            // [2 nwg][16 NT][D + 2]
-  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss, c_sb, c_sh, c_ss, table_ld;
-  int64_t cap;            // keys a request can hold
+  int32_t* counters;      // [nwg], zero between calls; NULL: a second kernel joins the parts
+  float* part;            // [2 nwg][rows of a block][D]
+  float* part_ml;         // [2 nwg][rows of a block] (max, sum)
+  int64_t q_sb, q_sh, q_ss, o_sb, o_sh, o_ss, c_sb, c_sh, table_ld;
+  int cap;                // keys a request can hold
+  int c_ss;               // below 2^24: row offsets inside a tile are 32-bit
   int B, S, Hk, G, rb;    // rb: row blocks of a (request, key head)
   int len, blocks, shift, causal, nwg;
-  float c;                // scale * log2(e)
+  uint32_t flip;          // sign bits of q (a negative scale)
+  float c;                // |scale| * log2(e)
 };
 
-__device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
-  const int n = a.kv_len ? a.kv_len[b] : a.len;
-  return n < 0 ? 0 : (int64_t)n > a.cap ? (int)a.cap : n;
+// A scalar load whatever the compiler can prove about the kernel's stores.
+__device__ __forceinline__ int scalar_i32(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
 }
 
-__device__ __forceinline__ int tiles_of(const AttnArgs& a, int b) {
-  return (keys_of(a, b) + kTile - 1) / kTile;
+__device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
+  return a.kv_len ? min(max(scalar_i32(a.kv_len + b), 0), a.cap) : a.len;
 }
 
 __device__ __forceinline__ int new_of(const AttnArgs& a, int b) {
-  const int n = a.q_len ? a.q_len[b] : a.S;
-  return n < 0 ? 0 : n > a.S ? a.S : n;
+  return a.q_len ? min(max(scalar_i32(a.q_len + b), 0), a.S) : a.S;
 }
 
-// Sum of one value per thread of the workgroup.
-__device__ __forceinline__ int block_sum(int v, int* sums) {
-#pragma unroll
-  for (int m = 1; m < kWave; m <<= 1) v += __shfl_xor(v, m, kWave);
-  __syncthreads();
-  if ((threadIdx.x & (kWave - 1)) == 0) sums[threadIdx.x / kWave] = v;
-  __syncthreads();
-  return sums[0] + sums[1] + sums[2] + sums[3];
-}
+// How a launch's key tiles are dealt.  A segment is one (request, key head, row
+// block); it counts as its tiles and LEAD more, what its start and end cost.  The
+// first `more` workgroups have each + 1 of the sum, the others each.
+template <int TILE, int LEAD, int LEAST>
+struct Deal {
+  unsigned each, more;
+  int nwg;
 
-// Tiles of the requests before b, and of all.
-__device__ __forceinline__ void tiles_before(const AttnArgs& a, int b, int* sums, int64_t& before,
-                                             int64_t& all) {
-  if (!a.kv_len) {
-    const int64_t n = tiles_of(a, 0);
-    before = n * b;
-    all = n * a.B;
-    return;
+  static __device__ __forceinline__ int tiles(int keys) { return (keys + TILE - 1) / TILE; }
+  static __device__ __forceinline__ int units(int keys) {
+    return keys > 0 ? tiles(keys) + LEAD : 0;
   }
-  int x = 0, y = 0;
-  for (int i = threadIdx.x; i < a.B; i += kThreads) {
-    const int n = tiles_of(a, i);
-    y += n;
-    if (i < b) x += n;
+  __device__ __forceinline__ Deal(unsigned all, int most) {
+    const unsigned fit = (all + LEAST - 1) / LEAST;
+    nwg = fit < (unsigned)most ? (int)fit : most;
+    each = nwg ? all / (unsigned)nwg : 0;
+    more = all - each * (unsigned)nwg;
   }
-  before = block_sum(x, sums);
-  all = block_sum(y, sums);
-}
+  __device__ __forceinline__ int begin(unsigned wg) const {
+    return (int)(wg * each + (wg < more ? wg : more));
+  }
+  __device__ __forceinline__ int holder(unsigned unit) const {
+    const unsigned wide = more * (each + 1);
+    return (int)(unit < wide ? unit / (each + 1) : more + (unit - wide) / each);
+  }
+  // the workgroups that hold a segment's first and last tile; it begins at unit `at`
+  __device__ __forceinline__ void holders(unsigned at, int tiles, int& w0, int& w1) const {
+    w0 = holder(at + LEAD);
+    w1 = holder(at + LEAD + tiles - 1);
+  }
+};
+typedef Deal<kStep * kWaves, 0, 1> FewDeal;  // single tokens: 128 keys, as they are
+typedef Deal<kStep, 4, 4> ManyDeal;
 
-// The request that holds tile t of all (t < all), and the tiles before it.
-__device__ __forceinline__ int request_at(const AttnArgs& a, int64_t t, int* sums, int* found,
-                                          int64_t& before) {
-  if (!a.kv_len) {
-    const int n = tiles_of(a, 0);
-    const int b = (int)(t / n);
-    before = (int64_t)b * n;
-    return b;
-  }
+// Units of all requests, and those before this thread's requests (a contiguous
+// share of them: [first, end)).
+struct Scan {
+  int all, before, first, end;
+};
+
+template <typename DEAL>
+__device__ __forceinline__ Scan scan_units(const AttnArgs& a, int* sums) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  int carry = 0;
-  for (int base = 0;; base += kThreads) {
-    const int i = base + (int)threadIdx.x;
-    const int n = i < a.B ? tiles_of(a, i) : 0;
-    int x = n;
+  const int share = (a.B + kThreads - 1) / kThreads;
+  Scan s;
+  s.first = min(a.B, (int)threadIdx.x * share);
+  s.end = min(a.B, s.first + share);
+  int n = 0;
+  for (int i = s.first; i < s.end; ++i) n += DEAL::units(min(max(a.kv_len[i], 0), a.cap));
+  int x = n;
 #pragma unroll
-    for (int d = 1; d < kWave; d <<= 1) {
-      const int y = __shfl_up(x, d, kWave);
-      if (lane >= d) x += y;
-    }
-    __syncthreads();
-    if (lane == kWave - 1) sums[wave] = x;
-    if (threadIdx.x == 0) found[0] = -1;
-    __syncthreads();
-    x += carry;
-    for (int w = 0; w < wave; ++w) x += sums[w];
-    if (t >= x - n && t < x) {
-      found[0] = i;
-      found[1] = x - n;
-    }
-    carry += sums[0] + sums[1] + sums[2] + sums[3];
-    __syncthreads();
-    if (found[0] >= 0 || base + kThreads >= a.B) break;
+  for (int d = 1; d < kWave; d <<= 1) {
+    const int y = __shfl_up(x, d, kWave);
+    if (lane >= d) x += y;
   }
-  before = found[1];
-  return found[0];
+  if (lane == kWave - 1) sums[wave] = x;
+  __syncthreads();
+  s.all = 0;
+  s.before = x - n;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    s.all += sums[w];
+    if (w < wave) s.before += sums[w];
+  }
+  return s;
 }
+
+// Part of a segment: its place in the launch, tiles [t0, t1).
+struct Segment {
+  int b, h, rb, len, tiles, t0, t1, fresh, at;
+};
+
+// A workgroup's walk over its segments.
+template <typename DEAL>
+struct Walk {
+  int u, u_end, b, before, per;
+
+  // false: this workgroup has none
+  __device__ __forceinline__ bool start(const AttnArgs& a, const DEAL& deal, const Scan& scan,
+                                        int even, int wg, int* found) {
+    per = a.Hk * a.rb;
+    u = deal.begin(wg);
+    u_end = deal.begin(wg + 1);
+    const int target = u / per;
+    if (a.kv_len) {
+      int x = scan.before;
+      for (int i = scan.first; i < scan.end; ++i) {
+        const int n = DEAL::units(min(max(a.kv_len[i], 0), a.cap));
+        if (target >= x && target < x + n) {
+          found[0] = i;
+          found[1] = x;
+        }
+        x += n;
+      }
+      __syncthreads();
+      b = __builtin_amdgcn_readfirstlane(found[0]);
+      before = __builtin_amdgcn_readfirstlane(found[1]);
+    } else {
+      b = target / even;
+      before = b * even;
+    }
+    return true;
+  }
+  __device__ __forceinline__ bool next(const AttnArgs& a, Segment& s) {
+    while (u < u_end) {
+      s.len = keys_of(a, b);
+      const int units = DEAL::units(s.len);
+      if (units == 0) {
+        ++b;
+        continue;
+      }
+      s.tiles = DEAL::tiles(s.len);
+      const int lead = units - s.tiles;
+      const int in = u - before * per;
+      const int pair = in / units;
+      const int p0 = in - pair * units, p1 = min(units, p0 + u_end - u);
+      s.at = before * per + pair * units;
+      s.b = b;
+      s.h = pair / a.rb;
+      s.rb = pair - s.h * a.rb;
+      s.t0 = max(0, p0 - lead);
+      s.t1 = max(0, p1 - lead);
+      s.fresh = new_of(a, b);
+      u += p1 - p0;
+      if (u - before * per >= units * per) {
+        before += units;
+        ++b;
+      }
+      if (s.t1 > s.t0) return true;
+    }
+    return false;
+  }
+};
 
 __device__ __forceinline__ bf16x8_t as_bf(const u32x4& v) { return __builtin_bit_cast(bf16x8_t, v); }
 
@@ -145,73 +218,70 @@ __device__ __forceinline__ uint32_t pair_hi(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// Rows of the output that one workgroup's (or the join's) result goes to.
-struct RowOf {
-  int s, g;
+// Where 32 keys lie: two key tiles of 16 rows (a page never ends inside one), the
+// first `n` rows of each there.
+struct Place {
+  int64_t at[2];
+  int n[2];
 };
 
-template <int D, int NT>
-__global__ __launch_bounds__(kThreads) void cache_attention_kernel(AttnArgs a) {
-  constexpr int KK = D / 32;  // 32-wide steps of a score's product
-  constexpr int DV = D / 16;  // output columns of a lane, V columns it reads
-  constexpr int VW = DV / 2;  // 32-bit words of those
-  constexpr int LDR = D + 4;  // row of the join's LDS, in floats
-  __shared__ int sums[kWaves];
-  __shared__ int found[2];
-  __shared__ float ml[kWaves][NT * 16][2];
-  __shared__ float acc_lds[kWaves][16][LDR];
-  const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const int n16 = lane & 15, g4 = lane >> 4;
-
-  const int per = a.Hk * a.rb;  // (key head, row block) pairs of a request
-  int64_t before, all;
-  tiles_before(a, 0, sums, before, all);
-  const int64_t units = all * per;
-  const int64_t wg = blockIdx.x;
-  const int64_t nwg = units < a.nwg ? units : a.nwg;  // each has a tile
-  if (wg >= nwg) return;
-  int64_t u = wg * units / nwg;
-  const int64_t u_end = (wg + 1) * units / nwg;
-  int b = request_at(a, u / per, sums, found, before);
-  b = __builtin_amdgcn_readfirstlane(b);
-
-  while (u < u_end) {
-    const int len = __builtin_amdgcn_readfirstlane(keys_of(a, b));
-    const int tiles = (len + kTile - 1) / kTile;
-    if (tiles == 0) {
-      ++b;
-      continue;
+__device__ __forceinline__ Place place_of(const AttnArgs& a, int b, int h, int len, int k0) {
+  Place p;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    int key = k0 + 16 * i;
+    p.n[i] = min(max(len - key, 0), 16);
+    if (p.n[i] == 0) key = 0;
+    int64_t block = b;
+    if (a.table) {
+      const int at = key >> a.shift;
+      const int page = scalar_i32(a.table + (int64_t)b * a.table_ld + at);
+      key -= at << a.shift;
+      const bool there = page >= 0 && page < a.blocks;  // a page outside the pool: not seen
+      block = there ? page : 0;
+      if (!there) p.n[i] = 0;
     }
-    const int64_t in = u - before * per;  // unit of this request
-    const int pair = (int)(in / tiles);
-    const int t0 = (int)(in - (int64_t)pair * tiles);
-    const int t1 = (int)(tiles - t0 < u_end - u ? tiles : t0 + (u_end - u));
-    const int h = pair / a.rb, rb = pair - h * a.rb;
-    const int fresh = __builtin_amdgcn_readfirstlane(new_of(a, b));
+    p.at[i] = block * a.c_sb + h * a.c_sh + (int64_t)key * a.c_ss;
+  }
+  return p;
+}
 
-    // this lane's rows: row r is head g of new token s
-    int lim[NT];
-    u32x4 qf[NT][KK];
+// A wave's rows r0 .. of a segment (row r is head r % G of new token r / G), NT
+// tiles of 16, a lane's being n16 of each; and what a step of 32 keys does to
+// them.
+template <int D, int NT>
+struct Rows {
+  static constexpr int KK = D / 32;  // 32-wide steps of a score's product
+  static constexpr int DV = D / 16;  // output columns of a lane, V columns it reads
+  static constexpr int VW = DV / 2;  // 32-bit words of those
+  static constexpr float kSlack = 8.0f;
+  u32x4 q[NT][KK];
+  int lim[NT];  // keys below it are seen
+  int lo, hi;   // keys below lo are seen by all rows, keys from hi on by none
+  float m[NT], l[NT];
+  f32x4_t acc[NT][DV];
+
+  __device__ __forceinline__ void load_q(const AttnArgs& a, const Segment& s, int r0, int n16,
+                                         int g4) {
     const int rows = a.S * a.G;
-    const int r0 = rb * 16 * NT;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      int r = r0 + nt * 16 + n16;
-      if (r >= rows) r = rows - 1;  // computed again, not written
-      const int s = r / a.G, g = r - s * a.G;
-      lim[nt] = a.causal ? min(len, len - fresh + s + 1) : len;
-      const uint16_t* qp = a.q + b * a.q_sb + (int64_t)(h * a.G + g) * a.q_sh + s * a.q_ss + g4 * 8;
+      const int r = min(r0 + nt * 16 + n16, rows - 1);  // past them: computed, not written
+      const int t = r / a.G, g = r - t * a.G;
+      lim[nt] = a.causal ? min(s.len, s.len - s.fresh + t + 1) : s.len;
+      const uint16_t* qp =
+          a.q + s.b * a.q_sb + (int64_t)(s.h * a.G + g) * a.q_sh + t * a.q_ss + g4 * 8;
 #pragma unroll
-      for (int kk = 0; kk < KK; ++kk) qf[nt][kk] = *reinterpret_cast<const u32x4*>(qp + kk * 32);
+      for (int kk = 0; kk < KK; ++kk)
+        q[nt][kk] = *reinterpret_cast<const u32x4*>(qp + kk * 32) ^ a.flip;
     }
-    // keys below lo are seen by all rows, keys from hi on by none
-    const int r1 = min(rows, r0 + 16 * NT) - 1;
-    const int lo = a.causal ? min(len, len - fresh + r0 / a.G + 1) : len;
-    const int hi = a.causal ? min(len, len - fresh + r1 / a.G + 1) : len;
-
-    float m[NT], l[NT];
-    f32x4_t acc[NT][DV];
+    lo = hi = s.len;
+    if (a.causal) {
+      lo = min(s.len, s.len - s.fresh + min(r0, rows - 1) / a.G + 1);
+      hi = min(s.len, s.len - s.fresh + (min(r0 + 16 * NT, rows) - 1) / a.G + 1);
+    }
+  }
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       m[nt] = -__builtin_inff();
@@ -219,304 +289,748 @@ __global__ __launch_bounds__(kThreads) void cache_attention_kernel(AttnArgs a) {
 #pragma unroll
       for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0, 0, 0, 0};
     }
-
-    for (int t = t0; t < t1; ++t) {
-      const int k0 = t * kTile + wave * kStep;
-      if (k0 >= hi) break;
-      // where the two key tiles of 16 lie: a page never ends inside one
-      const uint16_t* kb[2];
-      const uint16_t* vb[2];
-      int row0[2];
-      bool ok[2];
+  }
+  __device__ __forceinline__ void scores(const u32x4 (&kf)[2][KK], f32x4_t (&sc)[NT][2]) const {
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = k0 + 16 * i;
-        ok[i] = key < len;
-        int64_t block = b;
-        row0[i] = ok[i] ? key : 0;
-        if (a.table) {
-          const int at = row0[i] >> a.shift;
-          const int page = a.table[(int64_t)b * a.table_ld + at];
-          ok[i] = ok[i] && page >= 0 && page < a.blocks;  // a page outside the pool: not seen
-          block = ok[i] ? page : 0;
-          row0[i] -= at << a.shift;
-        }
-        const int64_t off = block * a.c_sb + h * a.c_sh;
-        kb[i] = a.k + off;
-        vb[i] = a.v + off;
-      }
-      const bool edge = k0 + kStep > lo || !ok[0] || !ok[1];
-      u32x4 kf[2][KK];
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        // rows past the length are read again from a row that is there
-        const int key = k0 + 16 * i + n16;
-        const int row = key < len && ok[i] ? row0[i] + n16 : row0[i];
-        const uint16_t* p = kb[i] + row * a.c_ss + g4 * 8;
+      for (int i = 0; i < 2; ++i) sc[nt][i] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kf[i][kk] = *reinterpret_cast<const u32x4*>(p + kk * 32);
-      }
-      uint32_t vr[8][VW];
+    for (int kk = 0; kk < KK; ++kk)
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int i = j >> 2, at = 4 * g4 + (j & 3);
-        const bool there = k0 + 16 * i + at < len && ok[i];
-        const uint32_t* p = reinterpret_cast<const uint32_t*>(
-            vb[i] + (row0[i] + (there ? at : 0)) * a.c_ss + n16 * DV);
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vr[j][w] = p[w];
-        if (edge && !there)  // 0 * inf is not 0
+        for (int nt = 0; nt < NT; ++nt)
+          sc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(kf[i][kk]), as_bf(q[nt][kk]),
+                                                               sc[nt][i], 0, 0, 0);
+  }
+  // Keys that are not there, and those a row does not see.
+  __device__ __forceinline__ void mask(f32x4_t (&sc)[NT][2], uint32_t (&vr)[8][VW], const int (&n)[2],
+                                       int k0, int g4) const {
 #pragma unroll
-          for (int w = 0; w < VW; ++w) vr[j][w] = 0;
-      }
-      f32x4_t sc[NT][2];
+    for (int j = 0; j < 8; ++j) {
+      const int at = 4 * g4 + (j & 3), key = k0 + 16 * (j >> 2) + at;
+      const bool there = at < n[j >> 2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
+        if (!there || key >= lim[nt]) sc[nt][j >> 2][j & 3] = -__builtin_inff();
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          sc[nt][i] = f32x4_t{0, 0, 0, 0};
+      for (int w = 0; w < VW; ++w) vr[j][w] = there ? vr[j][w] : 0;  // 0 * inf is not 0
+    }
+  }
+  // p of the scores, in two bf16 parts.  m follows a row's maximum only when it is
+  // passed by kSlack: p stays below 2^kSlack, and the outputs are rescaled a few
+  // times in all.
+  __device__ __forceinline__ void weights(const f32x4_t (&sc)[NT][2], float c, u32x4 (&ph)[NT],
+                                          u32x4 (&pl)[NT]) {
+    float mx[NT];
+    bool up = false;
 #pragma unroll
-          for (int kk = 0; kk < KK; ++kk)
-            sc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(kf[i][kk]), as_bf(qf[nt][kk]),
-                                                                 sc[nt][i], 0, 0, 0);
-        }
-      u32x4 ph[NT], pl[NT];
+    for (int nt = 0; nt < NT; ++nt) {
+      const f32x4_t &x = sc[nt][0], &y = sc[nt][1];
+      mx[nt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
+                     fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * c;
+      up |= mx[nt] > m[nt] + kSlack;
+    }
+    if (__any(up)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float x[8];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = sc[nt][j >> 2][j & 3] * a.c;
-          if (edge) {
-            const int key = k0 + 16 * (j >> 2) + 4 * g4 + (j & 3);
-            if (key >= lim[nt] || !ok[j >> 2]) x[j] = -__builtin_inff();
-          }
-        }
-        float mx = x[0];
-#pragma unroll
-        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, x[j]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
-        const float mn = fmaxf(m[nt], mx);
-        const float base = mn == -__builtin_inff() ? 0.0f : mn;
-        const float al = __builtin_amdgcn_exp2f(m[nt] - base);
-        m[nt] = mn;
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = __builtin_amdgcn_exp2f(x[j] - base);
-          sum += x[j];
-        }
-        l[nt] = l[nt] * al + sum;
+        mx[nt] = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, kWave));
+        mx[nt] = fmaxf(mx[nt], __shfl_xor(mx[nt], 32, kWave));
+        const float to = fmaxf(m[nt], mx[nt]);
+        const float al = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[nt] - to);
+        m[nt] = to;
+        l[nt] *= al;
 #pragma unroll
         for (int e = 0; e < DV; ++e) acc[nt][e] *= al;
-        ph[nt] = pack8(x);
-        float y[8];
-        unpack8(ph[nt], y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) y[j] = x[j] - y[j];
-        pl[nt] = pack8(y);
       }
-      // Where some rows do not see some of these keys, p = 0 has to hide a v that is
-      // not finite, and 0 * inf is not 0: such elements leave the product, and the rows
-      // that see them get theirs one by one.
-      if (edge && a.causal && hi > lo) {
-        bool wild = false;
+    }
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
+    for (int nt = 0; nt < NT; ++nt) {
+      const float base = m[nt] == -__builtin_inff() ? 0.0f : m[nt];
+      float x[8], y[8];
 #pragma unroll
-          for (int w = 0; w < VW; ++w) {
-            const uint32_t x = vr[j][w];
-            const bool l16 = (x & 0x7f80u) == 0x7f80u, h16 = (x & 0x7f800000u) == 0x7f800000u;
-            wild |= l16 | h16;
-            vr[j][w] = x & ~((l16 ? 0xffffu : 0u) | (h16 ? 0xffff0000u : 0u));
-          }
-        if (__any(wild)) {
-#pragma unroll 1
-          for (int key = 0; key < kStep; ++key) {
-            const int i = key >> 4, at = key & 15, j = i * 4 + (at & 3);
-            if (k0 + key >= len || !(i ? ok[1] : ok[0])) continue;
-            const uint16_t* vp = (i ? vb[1] : vb[0]) + ((i ? row0[1] : row0[0]) + at) * a.c_ss;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              uint32_t wh = ph[nt][0], wl = pl[nt][0];
-#pragma unroll
-              for (int y = 1; y < 4; ++y) {
-                wh = (j >> 1) == y ? ph[nt][y] : wh;
-                wl = (j >> 1) == y ? pl[nt][y] : wl;
-              }
-              float p = (j & 1) ? bf_hi(wh) + bf_hi(wl) : bf_lo(wh) + bf_lo(wl);
-              p = __shfl(p, n16 + 16 * (at >> 2), kWave);
-              if (k0 + key < lim[nt])
-#pragma unroll
-                for (int e = 0; e < DV; ++e)
-#pragma unroll
-                  for (int y = 0; y < 4; ++y) {
-                    const float x = bf2f(vp[(4 * g4 + y) * DV + e]);
-                    if (!(__builtin_fabsf(x) < __builtin_inff())) acc[nt][e][y] += p * x;
-                  }
-            }
-          }
-        }
+      for (int j = 0; j < 8; ++j) {
+        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[nt][j >> 2][j & 3], c, -base));
+        l[nt] += x[j];
       }
+      ph[nt] = pack8(x);
+      unpack8(ph[nt], y);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) y[j] = x[j] - y[j];
+      pl[nt] = pack8(y);
+    }
+  }
+  // Where some rows do not see some of the keys, p = 0 has to hide a v that is not
+  // finite, and 0 * inf is not 0: such elements leave the product, and the rows that
+  // see them get theirs one by one.
+  __device__ __forceinline__ void hide(uint32_t (&vr)[8][VW], const u32x4 (&ph)[NT],
+                                       const u32x4 (&pl)[NT], const AttnArgs& a, const Place& p,
+                                       int k0, int n16, int g4) {
+    bool wild = false;
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
 #pragma unroll
       for (int w = 0; w < VW; ++w) {
-        u32x4 v0, v1;
+        const uint32_t x = vr[j][w];
+        const bool l16 = (x & 0x7f80u) == 0x7f80u, h16 = (x & 0x7f800000u) == 0x7f800000u;
+        wild |= l16 | h16;
+        vr[j][w] = x & ~((l16 ? 0xffffu : 0u) | (h16 ? 0xffff0000u : 0u));
+      }
+    if (!__any(wild)) return;
+#pragma unroll 1
+    for (int key = 0; key < kStep; ++key) {
+      const int at = key & 15, j = (key >> 4) * 4 + (at & 3);
+      if (at >= (key < 16 ? p.n[0] : p.n[1])) continue;
+      const uint16_t* vp = a.v + (key < 16 ? p.at[0] : p.at[1]) + (int64_t)at * a.c_ss;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          v0[j] = pair_lo(vr[2 * j][w], vr[2 * j + 1][w]);
-          v1[j] = pair_hi(vr[2 * j][w], vr[2 * j + 1][w]);
-        }
+      for (int nt = 0; nt < NT; ++nt) {
+        uint32_t wh = ph[nt][0], wl = pl[nt][0];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          f32x4_t& c0 = acc[nt][2 * w];
-          f32x4_t& c1 = acc[nt][2 * w + 1];
-          c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(ph[nt]), c0, 0, 0, 0);
-          c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(ph[nt]), c1, 0, 0, 0);
-          c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(pl[nt]), c0, 0, 0, 0);
-          c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(pl[nt]), c1, 0, 0, 0);
+        for (int y = 1; y < 4; ++y) {
+          wh = (j >> 1) == y ? ph[nt][y] : wh;
+          wl = (j >> 1) == y ? pl[nt][y] : wl;
         }
+        float w = (j & 1) ? bf_hi(wh) + bf_hi(wl) : bf_lo(wh) + bf_lo(wl);
+        w = __shfl(w, n16 + 16 * (at >> 2), kWave);
+        if (k0 + key < lim[nt])
+#pragma unroll
+          for (int e = 0; e < DV; ++e)
+#pragma unroll
+            for (int y = 0; y < 4; ++y) {
+              const float x = bf2f(vp[(4 * g4 + y) * DV + e]);
+              if (!(__builtin_fabsf(x) < __builtin_inff())) acc[nt][e][y] += w * x;
+            }
       }
     }
+  }
+  __device__ __forceinline__ void product(const uint32_t (&vr)[8][VW], const u32x4 (&ph)[NT],
+                                          const u32x4 (&pl)[NT]) {
+#pragma unroll
+    for (int w = 0; w < VW; ++w) {
+      u32x4 v0, v1;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v0[j] = pair_lo(vr[2 * j][w], vr[2 * j + 1][w]);
+        v1[j] = pair_hi(vr[2 * j][w], vr[2 * j + 1][w]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        f32x4_t& c0 = acc[nt][2 * w];
+        f32x4_t& c1 = acc[nt][2 * w + 1];
+        c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(ph[nt]), c0, 0, 0, 0);
+        c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(ph[nt]), c1, 0, 0, 0);
+        c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(pl[nt]), c0, 0, 0, 0);
+        c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(pl[nt]), c1, 0, 0, 0);
+      }
+    }
+  }
+};
 
-    // join the waves
-    const bool whole = t0 == 0 && t1 == tiles;
-    const int slot = (int)wg * 2 + (t0 == 0 ? 1 : 0);
-    __syncthreads();
+// Stores and loads that other XCDs' workgroups see and are seen by: agent-scope
+// accesses, which pass the XCD's own cache by.  (With plain ones between
+// __threadfence() calls every workgroup wrote its XCD's cache back and emptied it:
+// 64 ragged requests 182 us, against 60 with a second kernel.)
+__device__ __forceinline__ void put2(float* p, float x, float y) {
+  const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool SHARED>
+__device__ __forceinline__ float get(const float* p) {
+  if constexpr (!SHARED) return *p;
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+template <bool SHARED>
+__device__ __forceinline__ void get2(const float* p, float& x, float& y) {
+  if constexpr (SHARED) {
+    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
+                                         __HIP_MEMORY_SCOPE_AGENT);
+    x = __uint_as_float((uint32_t)v), y = __uint_as_float((uint32_t)(v >> 32));
+  } else {
+    x = p[0], y = p[1];
+  }
+}
+
+__device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int b, int h, int r) {
+  const int t = r / a.G, g = r - t * a.G;
+  return a.out + b * a.o_sb + t * a.o_ss + (int64_t)(h * a.G + g) * a.o_sh;
+}
+
+// Joins one row of a segment that workgroups w0 .. w1 hold, a wave to a row: its
+// lanes hold the parts' maxima and sums, 64 parts at a time, then D / 64 columns
+// each, and a part's factor comes from the lane that holds it.  The first part is
+// its workgroup's second (its last segment), the others their first.  SHARED: they were written by this launch.
+template <int D, bool SHARED>
+__device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int rr, bool none,
+                                         uint16_t* op) {
+  constexpr int C = D / kWave;
+  constexpr int kAhead = 8;  // parts in flight (32: 25 parts 4.9 us for 5.5, but 9 parts 7.2 for 5.0)
+  const int lane = threadIdx.x & (kWave - 1);
+  const int n = w1 - w0 + 1;
+  const int64_t first = (int64_t)w0 * 2 * 16 + rr;
+  auto row_of = [&](int i) { return first + (2 * i + (i == 0)) * 16; };
+  float x[kAhead][C];
+  auto load = [&](int i0) {
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      l[nt] += __shfl_xor(l[nt], 16, kWave);
-      l[nt] += __shfl_xor(l[nt], 32, kWave);
-      if (g4 == 0) {
-        ml[wave][nt * 16 + n16][0] = m[nt];
-        ml[wave][nt * 16 + n16][1] = l[nt];
+    for (int j = 0; j < kAhead; ++j) {
+      const float* p = a.part + row_of(min(i0 + j, n - 1)) * D + lane * C;
+      if constexpr (C == 1) {
+        x[j][0] = get<SHARED>(p);
+      } else {
+#pragma unroll
+        for (int c = 0; c < C; c += 2) get2<SHARED>(p + c, x[j][c], x[j][c + 1]);
       }
     }
+  };
+  float mi = -__builtin_inff(), li = 0.0f;  // part `lane`'s
+  if (lane < n) get2<SHARED>(a.part_ml + row_of(lane) * 2, mi, li);
+  load(0);
+  float mx = mi;
+  for (int i = lane + kWave; i < n; i += kWave)
+    mx = fmaxf(mx, get<SHARED>(a.part_ml + row_of(i) * 2));
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      __syncthreads();
+  for (int k = 1; k < kWave; k <<= 1) mx = fmaxf(mx, __shfl_xor(mx, k, kWave));
+  const float base = mx == -__builtin_inff() ? 0.0f : mx;
+  float o[C] = {};
+  float sum = 0.0f;
+  for (int i0 = 0; i0 < n; i0 += kWave) {
+    if (i0) {
+      mi = -__builtin_inff(), li = 0.0f;
+      if (i0 + lane < n) get2<SHARED>(a.part_ml + row_of(i0 + lane) * 2, mi, li);
+    }
+    const float f = __builtin_amdgcn_exp2f(mi - base);
+    sum += li * f;
+#pragma unroll 1
+    for (int j0 = 0; j0 < kWave && i0 + j0 < n; j0 += kAhead) {
+      if (i0 + j0) load(i0 + j0);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) {
+        const float fj = __shfl(f, j0 + j, kWave);  // 0 past the last part
+#pragma unroll
+        for (int c = 0; c < C; ++c) o[c] += (i0 + j0 + j < n ? x[j][c] : 0.0f) * fj;
+      }
+    }
+  }
+  sum = group_sum<kWave>(sum);
+  if (sum == 0.0f) none = true;
+#pragma unroll
+  for (int c = 0; c < C; ++c) op[lane * C + c] = (uint16_t)f2bf(none ? 0.0f : o[c] / sum);
+}
+
+// Requests without a key: zeros.
+template <int D>
+__device__ __forceinline__ void zero_rows(const AttnArgs& a) {
+  const int chunks = D / 8;
+  for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+    if (keys_of(a, b)) continue;
+    const int64_t n = (int64_t)a.S * a.Hk * a.G * chunks;
+    for (int64_t i = threadIdx.x; i < n; i += kThreads) {
+      const int c = (int)(i % chunks), row = (int)(i / chunks);
+      const int t = row / (a.Hk * a.G), h = row - t * (a.Hk * a.G);
+      uint16_t* op = a.out + b * a.o_sb + t * a.o_ss + (int64_t)h * a.o_sh + c * 8;
+      *reinterpret_cast<u32x4*>(op) = u32x4{0, 0, 0, 0};
+    }
+  }
+}
+
+// This workgroup's place in the deal: they go round the eight XCDs, and those of
+// one XCD take neighbouring tiles.
+__device__ __forceinline__ int dealt_wg(int nwg) {
+  const int eighth = (nwg + 7) / 8;
+  const int wg = (blockIdx.x & 7) * eighth + blockIdx.x / 8;
+  return (int)(blockIdx.x / 8) < eighth && wg < nwg ? wg : -1;
+}
+
+// Up to 16 rows: a wave takes 32 of a tile's 128 keys.  The loads of a step are in
+// flight while the one before is computed, and the next segment's first while the
+// waves of this one are joined.
+template <int D>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(AttnArgs a) {
+  typedef Rows<D, 1> R;
+  constexpr int KK = R::KK, DV = R::DV, VW = R::VW;
+  constexpr int LDR = D + 4;  // row of the join's LDS, in floats
+  constexpr int kTile = kStep * kWaves;
+  __shared__ int sums[kWaves];
+  __shared__ int found[2];
+  __shared__ int arrived;
+  __shared__ float ml[kWaves][16][2];
+  __shared__ float acc_lds[kWaves][16][LDR];
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int n16 = lane & 15, g4 = lane >> 4;
+
+  Scan scan = {};
+  const int even = a.kv_len ? 0 : FewDeal::units(a.len);  // units of each, if all have as many
+  if (a.kv_len)
+    scan = scan_units<FewDeal>(a, sums);
+  else
+    scan.all = even * a.B;
+  const FewDeal deal((unsigned)(scan.all * a.Hk), a.nwg);
+  const int wg = dealt_wg(deal.nwg);
+  const int rows = a.S * a.G;
+  if (wg >= 0) {
+    Walk<FewDeal> walk;
+    walk.start(a, deal, scan, even, wg, found);
+    R r;
+    Segment seg, nxt;
+    Place here;
+    u32x4 kf[2][KK];
+    uint32_t vr[8][VW];
+    // rows that are not there are read again from one that is
+    auto load_k = [&](const Place& p) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint16_t* kp = a.k + p.at[i];
+        const unsigned off = __umul24(min(n16, max(p.n[i] - 1, 0)), a.c_ss) + g4 * 8;
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk)
+          kf[i][kk] = ld_stream(reinterpret_cast<const u32x4*>(kp + off + kk * 32));
+      }
+    };
+    auto load_v = [&](const Place& p) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int i = j >> 2;
+        const unsigned off =
+            __umul24(min(4 * g4 + (j & 3), max(p.n[i] - 1, 0)), a.c_ss) + n16 * DV;
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(a.v + p.at[i] + off);
+#pragma unroll
+        for (int w = 0; w < VW; ++w) vr[j][w] = vp[w];
+      }
+    };
+    auto first_of = [&](const Segment& s) {
+      return place_of(a, s.b, s.h, s.len, s.t0 * kTile + wave * kStep);
+    };
+    walk.next(a, seg);  // a dealt workgroup has one
+    here = first_of(seg);
+    load_k(here);
+    load_v(here);
+    r.load_q(a, seg, 0, n16, g4);
+    for (bool go = true; go;) {
+      go = walk.next(a, nxt);
+      const Place turn = go ? first_of(nxt) : here;
+      bool turned = false;  // the next segment's keys are on their way
+      r.clear();
+      for (int t = seg.t0; t < seg.t1; ++t) {
+        const int k0 = t * kTile + wave * kStep, k1 = k0 + kTile;
+        if (k0 >= r.hi) break;
+        const bool more = t + 1 < seg.t1 && k1 < r.hi;
+        Place next = turn;
+        if (more) next = place_of(a, seg.b, seg.h, seg.len, k1);
+        turned = !more;
+        f32x4_t sc[1][2];
+        r.scores(kf, sc);
+        if (more || go) load_k(next);  // under the softmax and the second product
+        const bool edge = k0 + kStep > r.lo || here.n[0] < 16 || here.n[1] < 16;
+        if (edge) r.mask(sc, vr, here.n, k0, g4);
+        u32x4 ph[1], pl[1];
+        r.weights(sc, a.c, ph, pl);
+        if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
+        r.product(vr, ph, pl);
+        if (more || go) load_v(next);
+        here = next;
+      }
+      if (go) {
+        if (!turned) {
+          load_k(turn);
+          load_v(turn);
+        }
+        here = turn;
+        r.load_q(a, nxt, 0, n16, g4);
+      }
+
+      // join the waves
+      const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
+      const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
+      r.l[0] += __shfl_xor(r.l[0], 16, kWave);
+      r.l[0] += __shfl_xor(r.l[0], 32, kWave);
+      if (g4 == 0) {
+        ml[wave][n16][0] = r.m[0];
+        ml[wave][n16][1] = r.l[0];
+      }
 #pragma unroll
       for (int i = 0; i < 4; ++i)
 #pragma unroll
-        for (int e = 0; e < DV; ++e) acc_lds[wave][n16][(4 * g4 + i) * DV + e] = acc[nt][e][i];
+        for (int e = 0; e < DV; ++e) acc_lds[wave][n16][(4 * g4 + i) * DV + e] = r.acc[0][e][i];
       __syncthreads();
       // thread: row tid / 16, columns DV (tid % 16) ..
       const int rr = threadIdx.x >> 4, col = (threadIdx.x & 15) * DV;
-      const int r = r0 + nt * 16 + rr;
-      if (r < rows) {
-        float mx = ml[0][nt * 16 + rr][0];
+      if (rr < rows) {
+        float mx = ml[0][rr][0];
 #pragma unroll
-        for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, ml[w][nt * 16 + rr][0]);
+        for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, ml[w][rr][0]);
         const float base = mx == -__builtin_inff() ? 0.0f : mx;
         float o[DV] = {};
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(ml[w][nt * 16 + rr][0] - base);
-          sum += ml[w][nt * 16 + rr][1] * f;
+          const float f = __builtin_amdgcn_exp2f(ml[w][rr][0] - base);
+          sum += ml[w][rr][1] * f;
 #pragma unroll
           for (int e = 0; e < DV; ++e) o[e] += acc_lds[w][rr][col + e] * f;
         }
         if (whole) {
-          const int s = r / a.G, g = r - s * a.G;
-          const float inv = s < fresh && sum != 0.0f ? 1.0f / sum : 0.0f;
-          uint16_t* op = a.out + b * a.o_sb + s * a.o_ss + (int64_t)(h * a.G + g) * a.o_sh + col;
+          const bool none = rr / a.G >= seg.fresh || sum == 0.0f;
+          const float inv = 1.0f / sum;
+          uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, seg.b, seg.h, rr) + col);
 #pragma unroll
-          for (int e = 0; e < DV; ++e) op[e] = (uint16_t)f2bf(inv == 0.0f ? 0.0f : o[e] * inv);
+          for (int w = 0; w < VW; ++w) op[w] = none ? 0 : pack2(o[2 * w] * inv, o[2 * w + 1] * inv);
         } else {
-          float* p = a.part + ((int64_t)slot * 16 * NT + nt * 16 + rr) * (D + 2);
+          const int64_t at = (int64_t)slot * 16 + rr;
 #pragma unroll
-          for (int e = 0; e < DV; ++e) p[col + e] = o[e];
-          if (col == 0) {
-            p[D] = mx;
-            p[D + 1] = sum;
+          for (int e = 0; e < DV; e += 2) put2(a.part + at * D + col + e, o[e], o[e + 1]);
+          if (col == 0) put2(a.part_ml + at * 2, mx, sum);
+        }
+      }
+      if (a.counters && !whole) {
+        int w0, w1;
+        deal.holders(seg.at, seg.tiles, w0, w1);
+        // each wave's stores have arrived before its workgroup is counted
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0)
+          arrived = __hip_atomic_fetch_add(a.counters + w0, 1, __ATOMIC_RELAXED,
+                                           __HIP_MEMORY_SCOPE_AGENT);
+        __syncthreads();
+        if (arrived == w1 - w0) {  // all other parts are there
+          if (threadIdx.x == 0) a.counters[w0] = 0;  // for the next call
+          for (int row = wave; row < rows; row += kWaves)
+            join_row<D, true>(a, w0, w1, row, row / a.G >= seg.fresh,
+                                  out_row(a, seg.b, seg.h, row));
+        }
+      }
+      __syncthreads();  // LDS is used again
+      seg = nxt;
+    }
+  }
+  if (a.counters) zero_rows<D>(a);
+}
+
+// All but LEFT of this wave's loads have landed and its LDS reads are done; then
+// the workgroup's barrier.  No memory access moves across.
+template <int LEFT>
+__device__ __forceinline__ void landed_barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_waitcnt((LEFT & 15) | (7 << 4) | ((LEFT >> 4) << 14));
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+typedef __attribute__((address_space(3))) void lds_void;
+
+// 16 bytes of each lane, from base + off (bytes), to 1 KB of LDS at `to`.  Written
+// out: before any LDS read the compiler waits for all loads into LDS that it knows
+// of, those of the steps to come included.  Its own counts of loads in flight stay
+// safe, as more are in flight than it counts; nothing is written to a register.
+__device__ __forceinline__ void load_to_lds(const void* base, int off, const u32x4* to) {
+  const uint64_t b = (uint64_t)base;
+  const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
+  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
+               "v"(off), "s"(rsrc)
+               : "memory", "m0");
+}
+
+// More rows: each wave has 16 NT of the workgroup's 64 NT, and the keys go through
+// a ring in LDS, kRing - 1 steps of 32 on their way: the loads take a few
+// thousand cycles, a step about one (one step ahead, through registers: 67 us for
+// 512 rows over 6100 keys).  A row's 16-byte chunks are permuted (chunk ^ row) so
+// that neither the reads down a column of chunks (K) nor those along rows (V)
+// meet in a bank.
+template <int D, int NT>
+__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel(AttnArgs a) {
+  typedef Rows<D, NT> R;
+  constexpr int KK = R::KK, DV = R::DV, VW = R::VW;
+  constexpr int CH = D / 8;                   // chunks of a row
+  constexpr int PER = kStep * CH / kThreads;  // chunks of K (and V) a thread moves a step
+  constexpr int kBlock = 16 * NT * kWaves;    // rows of a workgroup
+  constexpr int kRing = 4;
+  constexpr int LOADS = 2 * PER;  // of a wave, a step
+  __shared__ int sums[kWaves];
+  __shared__ int found[2];
+  __shared__ u32x4 kv[kRing][2][kStep * CH];  // [slot][K, V]
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int n16 = lane & 15, g4 = lane >> 4;
+  auto swizzle = [](int row) { return CH >= 16 ? row & 15 : (row >> 1) & 7; };
+  auto cell = [&](int row, int chunk) { return row * CH + (chunk ^ swizzle(row)); };
+
+  Scan scan = {};
+  const int even = a.kv_len ? 0 : ManyDeal::units(a.len);
+  if (a.kv_len)
+    scan = scan_units<ManyDeal>(a, sums);
+  else
+    scan.all = even * a.B;
+  const ManyDeal deal((unsigned)(scan.all * a.Hk * a.rb), a.nwg);
+  const int wg = dealt_wg(deal.nwg);
+  const int rows = a.S * a.G;
+  if (wg < 0) return;
+  Walk<ManyDeal> walk;
+  walk.start(a, deal, scan, even, wg, found);
+  R r;
+  Segment seg;
+  // A load instruction fills 64 neighbouring cells of LDS: which chunk a lane
+  // fetches follows from its cell.  Rows that are not there are another's again.
+  auto fetch = [&](int slot, const Place& p) {
+#pragma unroll
+    for (int x = 0; x < PER; ++x) {
+      const int c = x * kThreads + (int)threadIdx.x, row = c / CH;
+      const int i = __builtin_amdgcn_readfirstlane(row >> 4);
+      const int n = i ? p.n[1] : p.n[0];
+      const int64_t at = i ? p.at[1] : p.at[0];
+      const int off = (int)(__umul24(min(row & 15, max(n - 1, 0)), a.c_ss) * 2 +
+                            ((c % CH) ^ swizzle(row)) * 16);
+      const int first = x * kThreads + wave * kWave;
+      load_to_lds(a.k + at, off, &kv[slot][0][first]);
+      load_to_lds(a.v + at, off, &kv[slot][1][first]);
+    }
+  };
+  while (walk.next(a, seg)) {
+    const int r0 = seg.rb * kBlock + wave * 16 * NT;
+    // the block's last key that any row sees
+    int end = seg.len;
+    if (a.causal)
+      end = min(end, seg.len - seg.fresh + (min((seg.rb + 1) * kBlock, rows) - 1) / a.G + 1);
+    const int t1 = min(seg.t1, (max(end, 0) + kStep - 1) / kStep);
+    auto place = [&](int t) { return place_of(a, seg.b, seg.h, seg.len, min(t, t1 - 1) * kStep); };
+    Place ahead = {};
+    unsigned full = 0;  // bit t % 32: step t's pages are all there
+    auto send = [&](int t) {
+      fetch(t % kRing, ahead);
+      const unsigned bit = 1u << (t & 31);
+      full = ahead.n[0] == 16 && ahead.n[1] == 16 ? full | bit : full & ~bit;
+    };
+    landed_barrier<63>();  // the last segment's reads are done
+    if (seg.t0 < t1) {
+      for (int t = seg.t0; t < min(seg.t0 + kRing - 1, t1); ++t) {
+        ahead = place(t);
+        send(t);
+      }
+      ahead = place(seg.t0 + kRing - 1);
+    }
+    r.load_q(a, seg, r0, n16, g4);
+    r.clear();
+    for (int t = seg.t0; t < t1; ++t) {
+      const int k0 = t * kStep;
+      // this step's keys are there, those of the step before have been read
+      if (t + kRing - 2 < t1)
+        landed_barrier<(kRing - 2) * LOADS>();
+      else if (t + 1 < t1 && kRing == 4)
+        landed_barrier<LOADS>();
+      else
+        landed_barrier<0>();
+      if (t + kRing - 1 < t1) {
+        send(t + kRing - 1);
+        ahead = place(t + kRing);
+      }
+      if (k0 >= r.hi || r0 >= rows) continue;
+      const u32x4* const ks = kv[t % kRing][0];
+      const u32x4* const vs = kv[t % kRing][1];
+      u32x4 kf[2][KK];
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int kk = 0; kk < KK; ++kk) kf[i][kk] = ks[cell(16 * i + n16, kk * 4 + g4)];
+      f32x4_t sc[NT][2];
+      r.scores(kf, sc);
+      uint32_t vr[8][VW];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int row = 16 * (j >> 2) + 4 * g4 + (j & 3);
+        if constexpr (DV == 4) {
+          const uint32_t* p =
+              reinterpret_cast<const uint32_t*>(vs + cell(row, n16 >> 1)) + (n16 & 1) * 2;
+          vr[j][0] = p[0], vr[j][1] = p[1];
+        } else {
+#pragma unroll
+          for (int y = 0; y < DV / 8; ++y) {
+            const u32x4 x = vs[cell(row, n16 * (DV / 8) + y)];
+#pragma unroll
+            for (int w = 0; w < 4; ++w) vr[j][y * 4 + w] = x[w];
           }
         }
       }
+      const bool edge = k0 + kStep > r.lo || !(full >> (t & 31) & 1);
+      Place here = {};
+      if (edge) {
+        here = place(t);
+        r.mask(sc, vr, here.n, k0, g4);
+      }
+      u32x4 ph[NT], pl[NT];
+      r.weights(sc, a.c, ph, pl);
+      if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
+      r.product(vr, ph, pl);
     }
-
-    u += t1 - t0;
-    if (u - before * per >= (int64_t)tiles * per) {
-      before += tiles;
-      ++b;
+    const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
+    const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float sum = r.l[nt];
+      sum += __shfl_xor(sum, 16, kWave);
+      sum += __shfl_xor(sum, 32, kWave);
+      const int row = r0 + nt * 16 + n16;
+      if (row >= rows) continue;
+      // a lane's columns: 4 DV g4 .. + 4 DV
+      if (whole) {
+        const bool none = row / a.G >= seg.fresh || sum == 0.0f;
+        const float inv = 1.0f / sum;
+        uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, seg.b, seg.h, row) + 4 * DV * g4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int w = 0; w < VW; ++w)
+            op[i * VW + w] =
+                none ? 0 : pack2(r.acc[nt][2 * w][i] * inv, r.acc[nt][2 * w + 1][i] * inv);
+      } else {
+        // four columns of each lane side by side: the join reads them the same way
+        const int64_t tile = (int64_t)slot * (kBlock / 16) + wave * NT + nt;
+        f32x4_t* p = reinterpret_cast<f32x4_t*>(a.part) + tile * 4 * D + lane;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int e = 0; e < DV; e += 4)
+            p[(i * DV + e) / 4 * kWave] = f32x4_t{r.acc[nt][e][i], r.acc[nt][e + 1][i],
+                                                  r.acc[nt][e + 2][i], r.acc[nt][e + 3][i]};
+        if (g4 == 0) {
+          a.part_ml[(tile * 16 + n16) * 2] = r.m[nt];
+          a.part_ml[(tile * 16 + n16) * 2 + 1] = sum;
+        }
+      }
     }
   }
 }
 
-// Joins the parts of one (request, key head, row block), in the order of its
-// keys; rows without a key become zero.
-template <int D, int NT>
-__global__ __launch_bounds__(kThreads) void cache_attention_join_kernel(AttnArgs a) {
+// What a join needs to know of its (request, key head, row block).
+template <typename DEAL>
+__device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, int* sums, int* found,
+                                           int& w0, int& w1) {
+  const int per = a.Hk * a.rb;
+  const int len = keys_of(a, b), tiles = DEAL::tiles(len), units = DEAL::units(len);
+  int all = units * a.B, before = units * b;
+  if (a.kv_len) {
+    const Scan scan = scan_units<DEAL>(a, sums);
+    all = scan.all;
+    if (b >= scan.first && b < scan.end) {
+      int x = scan.before;
+      for (int i = scan.first; i < b; ++i) x += DEAL::units(min(max(a.kv_len[i], 0), a.cap));
+      *found = x;
+    }
+    __syncthreads();
+    before = *found;
+  }
+  w0 = 0, w1 = -1;
+  if (tiles == 0) return false;
+  const DEAL deal((unsigned)(all * per), a.nwg);
+  deal.holders((unsigned)(before * per + pair * units), tiles, w0, w1);
+  return true;
+}
+
+// Joins the parts that attend_few_kernel has left, and writes the zeros.
+template <int D>
+__global__ __launch_bounds__(kThreads) void join_few_kernel(AttnArgs a) {
   __shared__ int sums[kWaves];
+  __shared__ int found;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
+  int w0, w1;
+  const bool any = find_parts<FewDeal>(a, b, h, sums, &found, w0, w1);
+  const int row = blockIdx.y * kWaves + wave;
+  if (row >= a.S * a.G) return;
+  uint16_t* op = out_row(a, b, h, row);
+  if (!any)
+    for (int c = threadIdx.x & (kWave - 1); c < D; c += kWave) op[c] = 0;
+  else if (w0 != w1)
+    join_row<D, false>(a, w0, w1, row, row / a.G >= new_of(a, b), op);
+}
+
+// Joins those of attend_many_kernel: a workgroup to 4 of the DV column groups of a
+// tile of 16 rows, a lane to one row's four columns of a group, in the order in
+// which they were stored.
+template <int D, int NT>
+__global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
+  constexpr int DV = D / 16;
+  constexpr int kBlock = 16 * NT * kWaves, kTiles = kBlock / 16;
+  __shared__ int sums[kWaves];
+  __shared__ int found;
+  const int lane = threadIdx.x & (kWave - 1), n16 = lane & 15, g4 = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int per = a.Hk * a.rb;
   const int b = blockIdx.x / per, pair = blockIdx.x - b * per;
   const int h = pair / a.rb, rb = pair - h * a.rb;
-  int64_t before, all;
-  tiles_before(a, b, sums, before, all);
-  const int tiles = tiles_of(a, b);
-  const int64_t units = all * per;
-  const int64_t first = before * per + (int64_t)pair * tiles;
-  int64_t w0 = 0, w1 = -1;  // the workgroups that hold its tiles
-  if (tiles) {
-    const int64_t nwg = units < a.nwg ? units : a.nwg;
-    w0 = ((first + 1) * nwg - 1) / units;
-    w1 = ((first + tiles) * nwg - 1) / units;
-    if (w0 == w1) return;
+  int w0, w1;
+  const bool any = find_parts<ManyDeal>(a, b, pair, sums, &found, w0, w1);
+  const int group = blockIdx.z * kWaves + wave;
+  const int row = rb * kBlock + blockIdx.y * 16 + n16;
+  if ((any && w0 == w1) || group >= DV || row >= a.S * a.G) return;
+  const int n = w1 - w0 + 1;
+  const int64_t first = (int64_t)w0 * 2 * kTiles + blockIdx.y;
+  auto tile_of = [&](int i) { return first + (2 * i + (i == 0)) * kTiles; };
+  const float* ml = a.part_ml + n16 * 2;
+  const f32x4_t* part = reinterpret_cast<const f32x4_t*>(a.part) + group * kWave + lane;
+  float mx = -__builtin_inff();
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) mx = fmaxf(mx, ml[tile_of(i) * 32]);
+  const float base = mx == -__builtin_inff() ? 0.0f : mx;
+  f32x4_t o = {0, 0, 0, 0};
+  float sum = 0.0f;
+#pragma unroll 4
+  for (int i = 0; i < n; ++i) {
+    const int64_t t = tile_of(i);
+    const float f = __builtin_amdgcn_exp2f(ml[t * 32] - base);
+    sum += ml[t * 32 + 1] * f;
+    o += part[t * 4 * D] * f;
   }
-  const int fresh = new_of(a, b);
-  const int rows = min(a.S * a.G - rb * 16 * NT, 16 * NT);
-  for (int i = threadIdx.x; i < rows * D; i += kThreads) {
-    const int rr = i / D, col = i - rr * D;
-    const int r = rb * 16 * NT + rr, s = r / a.G, g = r - s * a.G;
-    float mx = -__builtin_inff();
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = w * 2 + (w == w0 ? 1 : 0);
-      mx = fmaxf(mx, a.part[(slot * 16 * NT + rr) * (D + 2) + D]);
-    }
-    const float base = mx == -__builtin_inff() ? 0.0f : mx;
-    float o = 0.0f, sum = 0.0f;
-    for (int64_t w = w0; w <= w1; ++w) {
-      const int64_t slot = w * 2 + (w == w0 ? 1 : 0);
-      const float* p = a.part + (slot * 16 * NT + rr) * (D + 2);
-      const float f = __builtin_amdgcn_exp2f(p[D] - base);
-      o += p[col] * f;
-      sum += p[D + 1] * f;
-    }
-    const bool none = s >= fresh || sum == 0.0f;
-    a.out[b * a.o_sb + s * a.o_ss + (int64_t)(h * a.G + g) * a.o_sh + col] =
-        (uint16_t)f2bf(none ? 0.0f : o / sum);
-  }
+  const bool none = sum == 0.0f || row / a.G >= new_of(a, b);
+  // group (i DV + e) / 4 of a lane's columns 4 DV g4 ..
+  uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, b, h, row) + 4 * DV * g4 + group * 4);
+  op[0] = none ? 0 : pack2(o[0] / sum, o[1] / sum);
+  op[1] = none ? 0 : pack2(o[2] / sum, o[3] / sum);
 }
 
 struct Shape {
-  int nt, rb, nwg;
+  int nt;     // 0: attend_few_kernel; else row tiles of a wave of attend_many_kernel
+  int block;  // rows of a workgroup
+  int rb;     // row blocks
+  int nwg;
 };
 
-// Row tiles of a workgroup, row blocks, workgroups.
 Shape shape_of(int64_t rows, int64_t D, int64_t cus) {
   Shape s;
-  s.nt = rows <= 16 ? 1 : rows <= 32 || D > 128 ? 2 : 4;
-  s.rb = (int)((rows + 16 * s.nt - 1) / (16 * s.nt));
-  s.nwg = (int)(cus * (s.nt == 1 ? 2 : 1));
+  s.nt = rows <= 16 ? 0 : rows <= 64 || D > 128 ? 1 : 2;
+  s.block = s.nt ? 16 * s.nt * kWaves : 16;
+  s.rb = (int)((rows + s.block - 1) / s.block);
+  s.nwg = (int)(cus * (D <= 128 ? 2 : 1));
   return s;
 }
 
+int64_t workspace_of(const Shape& s, int64_t D) {
+  return (int64_t)s.nwg * 2 * s.block * (D + 2) * 4;
+}
+
 template <int D, int NT>
-int launch(const AttnArgs& a, hipStream_t st) {
-  hipLaunchKernelGGL((cache_attention_kernel<D, NT>), dim3((unsigned)a.nwg), dim3(kThreads), 0, st,
-                     a);
-  if (int e = launch_status()) return e;
-  hipLaunchKernelGGL((cache_attention_join_kernel<D, NT>), dim3((unsigned)(a.B * a.Hk * a.rb)),
-                     dim3(kThreads), 0, st, a);
+int launch_many(const AttnArgs& a, hipStream_t st) {
+  const dim3 grid((unsigned)((a.nwg + 7) / 8 * 8)), threads(kThreads);
+  hipLaunchKernelGGL((attend_many_kernel<D, NT>), grid, threads, 0, st, a);
+  if (const int e = launch_status()) return e;
+  const int rows = a.S * a.G, block = 16 * NT * kWaves;
+  const dim3 joins((unsigned)(a.B * a.Hk * a.rb), (unsigned)((std::min(rows, block) + 15) / 16),
+                   (D / 16 + kWaves - 1) / kWaves);
+  hipLaunchKernelGGL((join_many_kernel<D, NT>), joins, threads, 0, st, a);
   return launch_status();
 }
 
 template <int D>
-int launch_nt(int nt, const AttnArgs& a, hipStream_t st) {
-  if (nt == 1) return launch<D, 1>(a, st);
+int launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
   if constexpr (D <= 128)
-    if (nt == 4) return launch<D, 4>(a, st);
-  return launch<D, 2>(a, st);
+    if (s.nt == 2) return launch_many<D, 2>(a, st);
+  if (s.nt) return launch_many<D, 1>(a, st);
+  const dim3 grid((unsigned)((a.nwg + 7) / 8 * 8)), threads(kThreads);
+  hipLaunchKernelGGL((attend_few_kernel<D>), grid, threads, 0, st, a);
+  const int e = launch_status();
+  if (e || a.counters) return e;
+  const dim3 joins((unsigned)(a.B * a.Hk), (unsigned)((a.S * a.G + kWaves - 1) / kWaves));
+  hipLaunchKernelGGL((join_few_kernel<D>), joins, threads, 0, st, a);
+  return launch_status();
 }
 
 bool head_dim_ok(int64_t D) { return D == 64 || D == 128 || D == 256; }
@@ -529,8 +1043,7 @@ extern "C" int64_t umic_cache_attention_workspace_bytes(int64_t S, int64_t Hq, i
   using namespace umic;
   if (S <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || !head_dim_ok(D) || S > (1 << 20) || Hq > (1 << 16))
     return 0;
-  const Shape s = shape_of(S * (Hq / Hk), D, device_cus());
-  return (int64_t)s.nwg * 2 * 16 * s.nt * (D + 2) * 4;
+  return workspace_of(shape_of(S * (Hq / Hk), D, device_cus()), D);
 }
 
 extern "C" int umic_cache_attention_bf16(
@@ -538,14 +1051,15 @@ extern "C" int umic_cache_attention_bf16(
     const int32_t* kv_lens, const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
     int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t o_sb, int64_t o_ss, int64_t o_sh,
     int64_t c_sb, int64_t c_sh, int64_t c_ss, int64_t blocks, int64_t block_rows, int64_t table_ld,
-    int64_t table_w, int64_t kv_len, int causal, float scale, void* workspace,
-    int64_t workspace_bytes, void* stream) {
+    int64_t table_w, int64_t kv_len, int causal, float scale, int32_t* counters,
+    void* workspace, int64_t workspace_bytes, void* stream) {
   using namespace umic;
   if (B < 0 || S < 0 || Hq < 0 || Hk < 0 || D <= 0 || blocks < 0 || block_rows < 0 ||
       workspace_bytes < 0)
     return UMIC_ERR_INVALID_ARG;
   if (B == 0 || S == 0 || Hq == 0) return UMIC_OK;
-  if (Hk == 0 || Hq % Hk) return UMIC_ERR_INVALID_ARG;
+  if (Hk == 0 || Hq % Hk || !(__builtin_fabsf(scale) < __builtin_inff()))
+    return UMIC_ERR_INVALID_ARG;
   if (!q || !out || !workspace) return UMIC_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return UMIC_ERR_UNSUPPORTED;
   int64_t cap = block_rows;
@@ -571,21 +1085,26 @@ extern "C" int umic_cache_attention_bf16(
       blocks > ((int64_t)1 << 30))
     return UMIC_ERR_UNSUPPORTED;
   const Shape s = shape_of(S * G, D, cus);
-  if (workspace_bytes < (int64_t)s.nwg * 2 * 16 * s.nt * (D + 2) * 4) return UMIC_ERR_INVALID_ARG;
-  // tiles of all requests, and joins, are counted in 32 bits
-  if (B * ((cap + kTile - 1) / kTile) > 0x7fffffff || B * Hk * s.rb > 0x7fffffff)
+  if (workspace_bytes < workspace_of(s, D)) return UMIC_ERR_INVALID_ARG;
+  if (s.nwg > UMIC_ATTENTION_COUNTERS) counters = nullptr;
+  // the tiles of all requests are counted in 32 bits, and row offsets in a tile
+  if (B * (cap / kStep + 8) > 0x7fffffff / (Hk * s.rb) || c_ss < 0 || c_ss >= (1 << 24))
     return UMIC_ERR_UNSUPPORTED;
   AttnArgs a = {};
   a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
   a.out = (uint16_t*)out, a.table = table, a.kv_len = kv_lens, a.q_len = q_lens;
+  a.counters = counters;
   a.part = (float*)workspace;
+  a.part_ml = a.part + (int64_t)s.nwg * 2 * s.block * D;
   a.q_sb = q_sb, a.q_ss = q_ss, a.q_sh = q_sh, a.o_sb = o_sb, a.o_ss = o_ss, a.o_sh = o_sh;
-  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = c_ss, a.table_ld = table_ld, a.cap = cap;
+  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = (int)c_ss, a.table_ld = table_ld, a.cap = (int)cap;
   a.B = (int)B, a.S = (int)S, a.Hk = (int)Hk, a.G = (int)G, a.rb = s.rb;
   a.len = kv_lens ? 0 : (int)kv_len, a.blocks = (int)blocks, a.shift = shift;
-  a.causal = causal != 0, a.nwg = s.nwg, a.c = scale * 1.4426950408889634f;
+  a.causal = causal != 0, a.nwg = s.nwg, a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
+  if (a.c < 0x1p-126f) a.c = 0x1p-126f;  // masked scores are -inf: times 0 they would be NaN
+  a.flip = scale < 0.0f ? 0x80008000u : 0u;
   hipStream_t st = as_stream(stream);
-  if (D == 64) return launch_nt<64>(s.nt, a, st);
-  if (D == 128) return launch_nt<128>(s.nt, a, st);
-  return launch_nt<256>(s.nt, a, st);
+  if (D == 64) return launch<64>(s, a, st);
+  if (D == 128) return launch<128>(s, a, st);
+  return launch<256>(s, a, st);
 }

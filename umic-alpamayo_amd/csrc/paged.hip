@@ -10,15 +10,20 @@
 // need) come from its head, in request order; token i lies at position p = kept
 // + i, in slot table[r][p / page] * page + p % page.
 //
-// Latency: a step of eight requests moves a few hundred bytes.  The prefix sums
-// over requests are what has to be waited for.
+// Latency: a step of eight requests moves a few hundred bytes.  One workgroup does
+// all that depends on the sums over requests, with one scan of all of them at once
+// for up to kPlanThreads requests, and the slots of up to kSlotsHere tokens; more
+// tokens' slots are a second launch's.
 #include "common.hpp"
 
 namespace umic {
 namespace {
 
+// A workgroup of 256 threads for up to as many requests, else of 1024: its barriers
+// are what a small step waits for.
+constexpr int kFewRequests = 256;
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanWaves = kPlanThreads / kWave;
+constexpr int kSlotsHere = 2048;
 
 struct PlanArgs {
   const int32_t* kv_len;
@@ -37,165 +42,211 @@ struct PlanArgs {
   int R, W, P, shift;
 };
 
+// What a step does to one request.
 struct Request {
-  int kept, have, need, fresh;
-  bool bad_state, too_long;
+  int kept, have, need, fresh, bad;  // bad: 1 its state is out of range, 2 too long
+  __device__ __forceinline__ int gives() const { return max(0, have - need); }
+  __device__ __forceinline__ int takes() const { return max(0, need - have); }
 };
 
 __device__ __forceinline__ Request request_of(const PlanArgs& a, int r) {
-  const int page = 1 << a.shift;
+  Request q = {};
+  if (r >= a.R) return q;
+  const int64_t most = (int64_t)a.W << a.shift;
   const int len = a.kv_len[r];
-  const int k = a.keep ? a.keep[r] : len;
-  Request q;
-  q.kept = max(0, min(k, len));
+  q.kept = max(0, min(a.keep ? a.keep[r] : len, len));
   q.fresh = max(0, a.fresh[r]);
   const int64_t after = (int64_t)q.kept + q.fresh;
-  q.bad_state = len < 0 || (int64_t)len > ((int64_t)a.W << a.shift);
-  q.too_long = after > ((int64_t)a.W << a.shift);
-  q.have = q.bad_state ? 0 : (int)(((int64_t)len + page - 1) >> a.shift);
-  q.need = q.too_long ? 0 : (int)((after + page - 1) >> a.shift);
+  const int64_t up = ((int64_t)1 << a.shift) - 1;
+  if (len < 0 || len > most)
+    q.bad = 1;
+  else
+    q.have = (int)((len + up) >> a.shift);
+  if (after > most)
+    q.bad |= 2;
+  else
+    q.need = (int)((after + up) >> a.shift);
   return q;
 }
 
-// Sums of one value per thread: exclusive prefix over the block, and the total.
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* sums, int64_t& total) {
+struct Sums {
+  int64_t gives, takes, fresh;
+};
+
+// Sums over the requests before this thread's, and over all; `bad` of all.
+template <int THREADS>
+__device__ __forceinline__ Sums scan(const Request& q, int64_t row, Sums& all, int& bad,
+                                     Sums (&part)[THREADS / kWave], int (&flag)[THREADS / kWave]) {
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
-  int64_t x = v;
+  Sums x = {q.gives(), q.takes(), q.fresh};
 #pragma unroll
   for (int d = 1; d < kWave; d <<= 1) {
-    const int64_t y = __shfl_up(x, d, kWave);
-    if (lane >= d) x += y;
+    const int64_t g = __shfl_up(x.gives, d, kWave), t = __shfl_up(x.takes, d, kWave),
+                  f = __shfl_up(x.fresh, d, kWave);
+    if (lane >= d) x.gives += g, x.takes += t, x.fresh += f;
   }
-  __syncthreads();  // sums may still be read from the call before
-  if (lane == kWave - 1) sums[wave] = x;
+  const int what = q.bad | (row > 0 && q.fresh > row ? 4 : 0);
+  const int any = (__any(what & 1) ? 1 : 0) | (__any(what & 2) ? 2 : 0) | (__any(what & 4) ? 4 : 0);
+  __syncthreads();  // part may still be read from the call before
+  if (lane == kWave - 1) part[wave] = x;
+  if (lane == 0) flag[wave] = any;
   __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kPlanWaves; ++w) {
-    if (w < wave) before += sums[w];
-    total += sums[w];
+  Sums before = {x.gives - q.gives(), x.takes - q.takes(), x.fresh - q.fresh};
+  all = {0, 0, 0};
+  bad = 0;
+#pragma unroll 2
+  for (int w = 0; w < THREADS / kWave; ++w) {
+    const Sums p = part[w];
+    if (w < wave) before.gives += p.gives, before.takes += p.takes, before.fresh += p.fresh;
+    all.gives += p.gives, all.takes += p.takes, all.fresh += p.fresh;
+    bad |= flag[w];
   }
-  return before + x - v;
+  return before;
 }
 
-// One workgroup: the sums over requests, the refusals, the pages that move, the
-// new lengths.  A refused step changes nothing: lengths and queue as they were,
-// no tokens, every slot -1, the reason in cursor_out[3].
-__global__ __launch_bounds__(kPlanThreads) void page_plan_kernel(PlanArgs a) {
-  __shared__ int64_t sums[kPlanWaves];
+// Token t's slot and position, from what the plan has written; starts(r): the
+// tokens of the requests before r, fresh ones; len(r): its length after the step.
+template <typename Starts, typename Len>
+__device__ __forceinline__ void map_slot(const PlanArgs& a, int64_t t, Starts starts, Len len) {
+  int r;
+  int64_t i;
+  if (a.row > 0) {
+    r = (int)(t / a.row);
+    i = t - (int64_t)r * a.row;
+  } else {
+    int lo = 0, hi = a.R;  // starts[lo] <= t < starts[hi], if there is such a request
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (starts(mid) <= t) lo = mid; else hi = mid;
+    }
+    r = lo;
+    i = t - starts(r);
+  }
+  const int64_t n = starts(r + 1) - starts(r);
+  int64_t slot = -1, position = 0;
+  if (i < n) {
+    const int64_t p = len(r) - n + i;
+    slot = ((int64_t)a.table[(int64_t)r * a.ld + (p >> a.shift)] << a.shift) +
+           (p & (((int64_t)1 << a.shift) - 1));
+    position = p + (a.delta ? a.delta[r] : 0);
+  }
+  a.slots[t] = slot;
+  a.positions[t] = position;
+}
+
+// The sums over requests, the refusals, the pages that move, the new lengths.  A
+// refused step changes nothing: lengths and queue as they were, no tokens, every
+// slot -1, the reason in cursor_out[3].
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void page_plan_kernel(PlanArgs a) {
+  __shared__ Sums part[THREADS / kWave];
+  __shared__ int flag[THREADS / kWave];
+  __shared__ int from[THREADS], at[THREADS];
+  __shared__ int starts[THREADS + 1], lens[THREADS];
   const int tid = threadIdx.x;
   const int head = a.cursor[0], free = a.cursor[1];
-  int64_t gave = 0, took = 0, fresh = 0, bad = 0, lng = 0, wide = 0;
-  for (int r = tid; r < a.R; r += kPlanThreads) {
-    const Request q = request_of(a, r);
-    gave += max(0, q.have - q.need);
-    took += max(0, q.need - q.have);
-    fresh += q.fresh;
-    bad |= q.bad_state;
-    lng |= q.too_long;
-    wide |= a.row > 0 && q.fresh > a.row;
+  const bool once = a.R <= THREADS;
+  const Request mine = request_of(a, tid);
+  Sums all;
+  int bad;
+  Sums before = scan<THREADS>(mine, a.row, all, bad, part, flag);
+  for (int base = THREADS; base < a.R; base += THREADS) {
+    Sums more;
+    int b;
+    scan<THREADS>(request_of(a, base + tid), a.row, more, b, part, flag);
+    all.gives += more.gives, all.takes += more.takes, all.fresh += more.fresh;
+    bad |= b;
   }
-  int64_t gave_all, took_all, fresh_all, flags;
-  block_scan(gave, sums, gave_all);
-  block_scan(took, sums, took_all);
-  block_scan(fresh, sums, fresh_all);
-  block_scan(bad | lng << 20 | wide << 40, sums, flags);
   int status = UMIC_PLAN_OK;
-  if ((flags & 0xfffff) || head < 0 || head >= a.P || free < 0 || free > a.P ||
-      free + gave_all > a.P)
+  if ((bad & 1) || head < 0 || head >= a.P || free < 0 || free > a.P || free + all.gives > a.P)
     status = UMIC_PLAN_BAD_STATE;
-  else if ((flags >> 20) & 0xfffff)
+  else if (bad & 2)
     status = UMIC_PLAN_TOO_LONG;
-  else if ((flags >> 40) || (a.row <= 0 && fresh_all > a.tokens))
+  else if ((bad & 4) || (a.row <= 0 && all.fresh > a.tokens))
     status = UMIC_PLAN_NO_ROOM;
-  else if (took_all > free + gave_all)
+  else if (all.takes > free + all.gives)
     status = UMIC_PLAN_NO_PAGES;
 
-  // pages given back, then pages taken: one wave to a request
+  // pages given back, then pages taken
   for (int phase = 0; phase < 2; ++phase) {
+    if (status || (phase ? all.takes : all.gives) == 0) continue;
     int64_t carry = 0;
-    for (int base = 0; base < a.R; base += kPlanThreads) {
-      __shared__ int from[kPlanThreads], count[kPlanThreads];
-      __shared__ int64_t at[kPlanThreads];
-      const int r = base + tid;
-      Request q = {};
-      if (r < a.R) q = request_of(a, r);
-      const int n = phase ? max(0, q.need - q.have) : max(0, q.have - q.need);
-      int64_t total, before = block_scan(n, sums, total);
-      from[tid] = phase ? q.have : q.need;
-      count[tid] = status ? 0 : n;
-      at[tid] = carry + before;
-      __syncthreads();
-      const int here = min(kPlanThreads, a.R - base);
-      for (int j = tid / kWave; j < here; j += kPlanWaves) {
-        int32_t* row = a.table + (int64_t)(base + j) * a.ld + from[j];
-        for (int w = tid & (kWave - 1); w < count[j]; w += kWave) {
-          const int64_t i = (int64_t)head + (phase ? 0 : free) + at[j] + w;
-          int32_t* cell = a.ring + i % a.P;
-          if (phase)
-            row[w] = *cell;
-          else
-            *cell = row[w];
-        }
+    for (int base = 0; base < a.R; base += THREADS) {
+      Request q = mine;
+      Sums b = before, more;
+      if (!once) {
+        int f;
+        q = request_of(a, base + tid);
+        b = scan<THREADS>(q, a.row, more, f, part, flag);
       }
-      carry += total;
+      // pages below P, as the step was not refused
+      from[tid] = phase ? q.have : q.need;
+      at[tid] = (int)(phase ? b.takes : b.gives);
+      __syncthreads();
+      const int here = min(THREADS, a.R - base);
+      const int total = (int)(once ? (phase ? all.takes : all.gives)
+                                   : (phase ? more.takes : more.gives));
+      for (int k = tid; k < total; k += THREADS) {
+        int j = 0;  // the last request with at <= k
+        for (int hi = here; hi - j > 1;) {
+          const int mid = (j + hi) >> 1;
+          if (at[mid] <= k) j = mid; else hi = mid;
+        }
+        int32_t* cell = a.table + (int64_t)(base + j) * a.ld + from[j] + (k - at[j]);
+        int64_t i = (int64_t)head + (phase ? 0 : free) + carry + k;  // below 3 P
+        if (i >= a.P) i -= a.P;
+        if (i >= a.P) i -= a.P;
+        if (phase)
+          *cell = a.ring[i];
+        else
+          a.ring[i] = *cell;
+      }
+      if (!once) carry += phase ? more.takes : more.gives;
       __syncthreads();
     }
   }
 
   // lengths and starts last: kv_out may be kv_len
   int64_t carry = 0;
-  for (int base = 0; base < a.R; base += kPlanThreads) {
-    const int r = base + tid;
-    Request q = {};
-    if (r < a.R) q = request_of(a, r);
-    int64_t total, before = block_scan(q.fresh, sums, total);
-    if (r < a.R) {
-      a.starts[r] = status ? 0 : (int32_t)(carry + before);
-      a.kv_out[r] = status ? a.kv_len[r] : q.kept + q.fresh;
+  for (int base = 0; base < a.R; base += THREADS) {
+    Request q = mine;
+    Sums b = before, more = {};
+    if (!once) {
+      int f;
+      q = request_of(a, base + tid);
+      b = scan<THREADS>(q, a.row, more, f, part, flag);
     }
-    carry += total;
+    const int r = base + tid;
+    if (r < a.R) {
+      const int s = status ? 0 : (int)(carry + b.fresh);
+      const int n = status ? a.kv_len[r] : q.kept + q.fresh;
+      a.starts[r] = s;
+      a.kv_out[r] = n;
+      if (once) starts[tid] = s, lens[tid] = n;
+    }
+    carry += more.fresh;
   }
   if (tid == 0) {
-    a.starts[a.R] = status ? 0 : (int32_t)fresh_all;
-    a.cursor_out[0] = status ? head : (int)((head + took_all) % a.P);
-    a.cursor_out[1] = status ? free : (int)(free + gave_all - took_all);
-    a.cursor_out[2] = status ? 0 : (int)fresh_all;
+    const int total = status ? 0 : (int)all.fresh;
+    a.starts[a.R] = total;
+    if (once) starts[a.R] = total;
+    int64_t h = status ? head : head + all.takes;
+    if (!status && h >= a.P) h -= a.P;
+    a.cursor_out[0] = (int)h;
+    a.cursor_out[1] = status ? free : (int)(free + all.gives - all.takes);
+    a.cursor_out[2] = total;
     a.cursor_out[3] = status;
   }
+  if (!once || a.tokens > kSlotsHere) return;
+  __syncthreads();
+  for (int64_t t = tid; t < a.tokens; t += THREADS)
+    map_slot(a, t, [&](int r) { return starts[r]; }, [&](int r) { return lens[r]; });
 }
 
-// A token's slot and position, from what the plan has written.
 __global__ __launch_bounds__(256) void slot_map_kernel(PlanArgs a) {
   const int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (t >= a.tokens) return;
-  int r;
-  int64_t i;
-  bool real;
-  if (a.row > 0) {
-    r = (int)(t / a.row);
-    i = t - (int64_t)r * a.row;
-    real = i < a.starts[r + 1] - a.starts[r];
-  } else {
-    int lo = 0, hi = a.R;  // starts[lo] <= t < starts[hi], if there is such a request
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (a.starts[mid] <= t) lo = mid; else hi = mid;
-    }
-    r = lo;
-    i = t - a.starts[r];
-    real = t < a.starts[a.R];
-  }
-  int64_t slot = -1, position = 0;
-  if (real) {
-    const int64_t p = a.kv_out[r] - (a.starts[r + 1] - a.starts[r]) + i;
-    slot = ((int64_t)a.table[(int64_t)r * a.ld + (p >> a.shift)] << a.shift) +
-           (p & ((1 << a.shift) - 1));
-    position = p + (a.delta ? a.delta[r] : 0);
-  }
-  a.slots[t] = slot;
-  a.positions[t] = position;
+  if (t < a.tokens)
+    map_slot(a, t, [&](int r) { return a.starts[r]; }, [&](int r) { return a.kv_out[r]; });
 }
 
 }  // namespace
@@ -224,9 +275,14 @@ extern "C" int umic_page_plan(const int32_t* kv_len, const int32_t* new_len, con
                 starts, slots, positions, table_ld, tokens, row, (int)R, (int)W, (int)pages,
                 __builtin_ctzll((unsigned long long)page_size)};
   hipStream_t st = as_stream(stream);
-  hipLaunchKernelGGL(page_plan_kernel, dim3(1), dim3(kPlanThreads), 0, st, a);
+  const bool few = R <= kFewRequests;
+  const int threads = few ? kFewRequests : kPlanThreads;
+  if (few)
+    hipLaunchKernelGGL(page_plan_kernel<kFewRequests>, dim3(1), dim3(threads), 0, st, a);
+  else
+    hipLaunchKernelGGL(page_plan_kernel<kPlanThreads>, dim3(1), dim3(threads), 0, st, a);
   if (int e = launch_status()) return e;
-  if (tokens == 0) return UMIC_OK;
+  if (tokens == 0 || (R <= threads && tokens <= kSlotsHere)) return UMIC_OK;
   hipLaunchKernelGGL(slot_map_kernel, dim3((unsigned)((tokens + 255) / 256)), dim3(256), 0, st, a);
   return launch_status();
 }

@@ -31,6 +31,7 @@ UMIC_ROPE_VISION = 1
 UMIC_ACT_NONE = 0
 UMIC_ACT_GELU = 1
 UMIC_ACT_GELU_TANH = 2
+UMIC_ATTENTION_COUNTERS = 4096  # counters of umic_cache_attention_bf16
 UMIC_STREAM_READ_GRID = 2048  # fold words umic_stream_read writes
 
 _P, _I64, _F32, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
@@ -66,7 +67,7 @@ SIGNATURES: dict[str, list] = {
     "umic_axial_rope_bf16": [_P] * 7 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 15 + [_P],
     "umic_axial_rope_append_bf16": [_P] * 10 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 20 + [_P],
     "umic_cache_attention_workspace_bytes": [_I64] * 4,
-    "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _I64, _P],
+    "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _P, _I64, _P],
     "umic_stream_read": [_P, _I64, _P, _P],
     "umic_stream_copy": [_P, _P, _I64, _P],
     "umic_version": [],

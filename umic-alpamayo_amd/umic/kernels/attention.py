@@ -20,6 +20,7 @@ from umic import _lib
 from umic.kernels._common import grad_needed, require_device
 
 HEAD_DIMS = (64, 128, 256)
+_BF16 = torch.bfloat16
 
 
 @functools.lru_cache(maxsize=1024)
@@ -27,19 +28,43 @@ def _workspace_bytes(dev: int, S: int, Hq: int, Hk: int, D: int) -> int:
     return _lib.lib().umic_cache_attention_workspace_bytes(S, Hq, Hk, D)
 
 
+# (counters, workspace) of each (device, stream): calls on one stream do not
+# overlap, and every call leaves the counters at zero.  A captured call has a
+# workspace of its own and no counters, as its graph may run beside anything.
+_SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
+
+
+def _scratch(q: torch.Tensor, dev: int, stream: int, need: int) -> tuple[int | None, torch.Tensor]:
+    if torch.cuda.is_current_stream_capturing():
+        return None, torch.empty(need, dtype=torch.uint8, device=q.device)
+    held = _SCRATCH.get((dev, stream))
+    if held is None or held[1].numel() < need:
+        counters = held[0] if held else torch.zeros(_lib.UMIC_ATTENTION_COUNTERS,
+                                                    dtype=torch.int32, device=q.device)
+        held = counters, torch.empty(need, dtype=torch.uint8, device=q.device)
+        _SCRATCH[dev, stream] = held
+    return held[0].data_ptr(), held[1]
+
+
 def _chunks_ok(t: torch.Tensor) -> bool:
     """Contiguous rows of 16-byte chunks."""
-    s = t.stride()
-    return s[3] == 1 and not ((s[0] | s[1] | s[2]) & 7) and t.data_ptr() % 16 == 0
+    a, b, c, inner = t.stride()
+    return inner == 1 and not ((a | b | c) & 7 or t.data_ptr() & 15)
 
 
 def cache_ok(k_cache: torch.Tensor, v_cache: torch.Tensor) -> bool:
     """Caches the kernel reads: bf16 GPU [blocks, Hk, rows, D] of one layout, D one of
     HEAD_DIMS, 16-byte chunks."""
-    return (k_cache.is_cuda and k_cache.dtype is torch.bfloat16 and k_cache.dim() == 4
-            and v_cache.dtype is torch.bfloat16 and v_cache.get_device() == k_cache.get_device()
-            and k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride()
-            and k_cache.shape[3] in HEAD_DIMS and _chunks_ok(k_cache) and _chunks_ok(v_cache))
+    return (k_cache.is_cuda and k_cache.dtype is _BF16 and v_cache.dtype is _BF16
+            and v_cache.get_device() == k_cache.get_device() and k_cache.dim() == 4
+            and _layout_ok(k_cache, v_cache))
+
+
+def _layout_ok(k_cache: torch.Tensor, v_cache: torch.Tensor) -> bool:
+    shape = k_cache.shape
+    return (shape == v_cache.shape and shape[3] in HEAD_DIMS
+            and k_cache.stride() == v_cache.stride() and v_cache.data_ptr() & 15 == 0
+            and _chunks_ok(k_cache))
 
 
 def _lengths(name: str, t: torch.Tensor, B: int, dev: int) -> None:
@@ -73,7 +98,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if grad_needed(q, k_cache, v_cache):
         raise RuntimeError("cache_attention: the kernel has no backward; call it under "
                            "torch.no_grad()")
-    if q.dim() != 4 or not cache_ok(k_cache, v_cache):
+    if q.dim() != 4 or k_cache.dim() != 4 or not _layout_ok(k_cache, v_cache):
         raise ValueError(f"cache_attention: unsupported layout q{tuple(q.shape)} "
                          f"cache{tuple(k_cache.shape)} (head sizes {HEAD_DIMS})")
     B, Hq, S, D = q.shape
@@ -104,22 +129,25 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if not _chunks_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = q.new_empty(B, S, Hq, D)
+        out = torch.empty((B, S, Hq, D), dtype=_BF16, device=q.device)
+        os_ = (S * Hq * D, Hq * D, D)
     else:
         require_device(q, out)
         if tuple(out.shape) != (B, S, Hq, D) or not _chunks_ok(out):
             raise ValueError(f"cache_attention: out must be [{B}, {S}, {Hq}, {D}] of 16-byte "
                              f"chunks, got {tuple(out.shape)}")
-    if out.numel() == 0:
+        os_ = out.stride()
+    if B == 0 or S == 0 or Hq == 0:
         return out
-    qs, os_, cs = q.stride(), out.stride(), k_cache.stride()
+    qs, cs = q.stride(), k_cache.stride()
     with _lib.device_of(q):
+        stream = _lib.stream_of(q)
         size = _workspace_bytes(dev, S, Hq, Hk, D)
-        ws = torch.empty(size, dtype=torch.uint8, device=q.device)
+        counters, ws = _scratch(q, dev, stream, size)
         _lib.call("umic_cache_attention_bf16", q.data_ptr(), k_cache.data_ptr(),
                   v_cache.data_ptr(), out.data_ptr(), _lib.ptr(table), lens, _lib.ptr(q_len),
                   B, S, Hq, Hk, D, qs[0], qs[2], qs[1], os_[0], os_[1], os_[2], cs[0], cs[1],
                   cs[2], blocks, rows, ld, width, n, int(causal),
-                  float(D ** -0.5 if scale is None else scale), ws.data_ptr(), size,
-                  _lib.stream_of(q))
+                  float(D ** -0.5 if scale is None else scale), counters,
+                  ws.data_ptr(), size, stream)
     return out

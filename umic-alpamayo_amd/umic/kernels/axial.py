@@ -93,42 +93,40 @@ class AxisPlan:
         return cls(torch.cat((inv, inv)), [0] * quarter + [1] * quarter, device=device)
 
 
-def _rows_ok(t: torch.Tensor) -> bool:
-    """Head rows the kernel reads: [T, H, D], contiguous rows on 8-byte chunks."""
-    return (t.stride(2) == 1 and t.stride(0) % 4 == 0 and t.stride(1) % 4 == 0
-            and t.data_ptr() % 8 == 0)
+def _ready(t: torch.Tensor) -> torch.Tensor:
+    """t, or a copy with the rows the kernel reads: [T, H, D], contiguous, in 8-byte
+    chunks."""
+    a, b, inner = t.stride()
+    if inner == 1 and not ((a | b) & 3 or t.data_ptr() & 7):
+        return t
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 def _check(who: str, q, k, positions, plan: AxisPlan, norm) -> None:
-    require_device(q, k, *(norm[:2] if norm is not None else ()))
-    if grad_needed(q, k, *(norm[:2] if norm is not None else ())):
+    if grad_needed(q, k) or norm is not None and grad_needed(norm[0], norm[1]):
         raise RuntimeError(f"{who}: the kernel has no backward; call it under torch.no_grad()")
-    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
-        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [T, heads, D]")
-    T, _, D = q.shape
-    if D != plan.head_dim or D % 8 or D > MAX_HEAD_DIM:
-        raise ValueError(f"{who}: heads of {D} (the plan's have {plan.head_dim}; multiples of 8 "
-                         f"up to {MAX_HEAD_DIM})")
-    dev = q.get_device()
+    T, D, dev = q.shape[0], plan.head_dim, q.get_device()
+    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != T or q.shape[2] != D or k.shape[2] != D:
+        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [T, heads, {D}]")
+    if D % 8 or D > MAX_HEAD_DIM:
+        raise ValueError(f"{who}: heads of {D} (multiples of 8 up to {MAX_HEAD_DIM})")
     if (positions.dtype is not torch.int64 or positions.dim() != 2 or positions.shape[1] != T
             or positions.shape[0] < plan.axes or positions.get_device() != dev):
         raise ValueError(f"{who}: positions must be int64 [{plan.axes} axes, {T}] on q's device, "
                          f"got {positions.dtype} {tuple(positions.shape)}")
     if plan.turn.get_device() != dev:
         raise ValueError(f"{who}: the plan is on {plan.turn.device}, q on {q.device}")
-    if norm is not None:
-        for w in norm[:2]:
-            if tuple(w.shape) != (D,) or not w.is_contiguous():
-                raise ValueError(f"{who}: norm weights must be contiguous vectors of {D}")
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
-    return t if _rows_ok(t) else t.clone(memory_format=torch.contiguous_format)
-
-
-def _norm_args(norm):
-    return (None, None, 0.0) if norm is None else (norm[0].data_ptr(), norm[1].data_ptr(),
-                                                   float(norm[2]))
+def _norm_args(who: str, norm, D: int):
+    """Pointers of the norm's weights and its eps."""
+    if norm is None:
+        return None, None, 0.0
+    for w in norm[:2]:
+        if w.shape != (D,) or not w.is_contiguous() or w.data_ptr() & 7:
+            raise ValueError(f"{who}: norm weights must be contiguous vectors of {D}, 8-byte "
+                             "aligned")
+    return norm[0].data_ptr(), norm[1].data_ptr(), float(norm[2])
 
 
 def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: AxisPlan,
@@ -136,17 +134,19 @@ def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: Axis
     """q [T, Hq, D] and k [T, Hk, D] turned by positions [axes, T] (int64), as new
     contiguous tensors.  With ``norm = (q_w, k_w, eps)`` each head row is RMS-normed
     first."""
+    require_device(q, k, *(norm[:2] if norm is not None else ()))
     _check("rotate", q, k, positions, plan, norm)
     q, k = _ready(q), _ready(k)
     T, Hq, D = q.shape
     Hk = k.shape[1]
-    q_out, k_out = q.new_empty(T, Hq, D), k.new_empty(T, Hk, D)
+    q_out, k_out = (torch.empty((T, h, D), dtype=torch.bfloat16, device=q.device)
+                    for h in (Hq, Hk))
     with _lib.device_of(q):
         _lib.call("umic_axial_rope_bf16", q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
                   k_out.data_ptr(), positions.data_ptr(), plan.turn.data_ptr(),
-                  plan.axis.data_ptr(), plan.scale, *_norm_args(norm), T, Hq, Hk, D,
-                  positions.shape[0], positions.stride(0), positions.stride(1), q.stride(0),
-                  q.stride(1), k.stride(0), k.stride(1), Hq * D, D, Hk * D, D, _lib.stream_of(q))
+                  plan.axis.data_ptr(), plan.scale, *_norm_args("rotate", norm, D), T, Hq, Hk, D,
+                  positions.shape[0], *positions.stride(), *q.stride()[:2], *k.stride()[:2],
+                  Hq * D, D, Hk * D, D, _lib.stream_of(q))
     return q_out, k_out
 
 
@@ -156,30 +156,29 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     """``rotate`` of q, with k's rotated rows and v's rows written to ``slots`` (int64
     [T], distinct; one outside the pool writes nothing) of k_pages and v_pages [pages,
     Hk, page_size, D].  Returns the rotated q."""
+    require_device(q, k, v, k_pages, v_pages, *(norm[:2] if norm is not None else ()))
     _check("rotate_append", q, k, positions, plan, norm)
-    require_device(q, v, k_pages, v_pages)
     T, Hq, D = q.shape
     Hk = k.shape[1]
     if v.shape != k.shape or grad_needed(v):
         raise ValueError(f"rotate_append: v {tuple(v.shape)} must be like k {tuple(k.shape)}, "
                          "without a gradient")
-    if (k_pages.dim() != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != Hk
-            or k_pages.shape[3] != D or k_pages.stride() != v_pages.stride()
-            or k_pages.stride(3) != 1):
+    shape, cst = k_pages.shape, k_pages.stride()
+    if (len(shape) != 4 or shape != v_pages.shape or shape[1] != Hk or shape[3] != D
+            or cst != v_pages.stride() or cst[3] != 1):
         raise ValueError(f"rotate_append: pages {tuple(k_pages.shape)} and {tuple(v_pages.shape)} "
                          f"must be [pages, {Hk}, page_size, {D}] of one layout")
-    if (slots.dtype is not torch.int64 or slots.dim() != 1 or slots.shape[0] != T
-            or slots.get_device() != q.get_device() or slots.stride(0) != 1 and T > 1):
+    if (slots.dtype is not torch.int64 or slots.shape != (T,)
+            or slots.get_device() != q.get_device() or not slots.is_contiguous()):
         raise ValueError(f"rotate_append: slots must be a contiguous int64 vector of {T} on q's "
                          "device")
     q, k, v = _ready(q), _ready(k), _ready(v)
-    q_out = q.new_empty(T, Hq, D)
+    q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
     with _lib.device_of(q):
         _lib.call("umic_axial_rope_append_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), positions.data_ptr(),
                   plan.turn.data_ptr(), plan.axis.data_ptr(), slots.data_ptr(), plan.scale,
-                  *_norm_args(norm), T, Hq, Hk, D, positions.shape[0], positions.stride(0),
-                  positions.stride(1), q.stride(0), q.stride(1), k.stride(0), k.stride(1),
-                  v.stride(0), v.stride(1), Hq * D, D, *k_pages.stride()[:3], k_pages.shape[0],
-                  k_pages.shape[2], _lib.stream_of(q))
+                  *_norm_args("rotate_append", norm, D), T, Hq, Hk, D, positions.shape[0], *positions.stride(),
+                  *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], Hq * D, D, *cst[:3], shape[0],
+                  shape[2], _lib.stream_of(q))
     return q_out

@@ -49,12 +49,15 @@ def page_size_ok(page_size: int) -> bool:
     return page_size >= 16 and page_size & (page_size - 1) == 0
 
 
+def _refuse(name: str, t: torch.Tensor, n: int, dtype: torch.dtype) -> None:
+    raise ValueError(f"plan_pages: {name} must be a contiguous {dtype} vector of {n} on kv_len's "
+                     f"device, got {t.dtype} {tuple(t.shape)} on {t.device}")
+
+
 def _vector(name: str, t: torch.Tensor, n: int, dtype: torch.dtype, dev: int) -> None:
-    if t.dtype is not dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"plan_pages: {name} must be a contiguous {dtype} vector of {n}, got "
-                         f"{t.dtype} {tuple(t.shape)}")
-    if t.get_device() != dev:
-        raise ValueError(f"plan_pages: {name} is on {t.device}, not on kv_len's device")
+    if (t.dtype is not dtype or t.shape != (n,) or t.get_device() != dev
+            or not t.is_contiguous()):
+        _refuse(name, t, n, dtype)
 
 
 def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
@@ -84,7 +87,8 @@ def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
     dev, R = kv_len.get_device(), kv_len.shape[0] if kv_len.dim() == 1 else -1
     _vector("kv_len", kv_len, R, _I32, dev)
     _vector("new_len", new_len, R, _I32, dev)
-    _vector("ring", ring, ring.numel(), _I32, dev)
+    pages = ring.shape[0] if ring.dim() == 1 else -1
+    _vector("ring", ring, pages, _I32, dev)
     _vector("cursor", cursor, 4, _I32, dev)
     if keep is not None:
         _vector("keep", keep, R, _I32, dev)
@@ -100,8 +104,9 @@ def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
         raise ValueError(f"plan_pages: {tokens} entries for {R} requests of {row} each")
     _lib.lib()
     if out is None:
-        out = PageStep(kv_len.new_empty(R), kv_len.new_empty(4), kv_len.new_empty(R + 1),
-                       kv_len.new_empty(tokens, dtype=_I64), kv_len.new_empty(tokens, dtype=_I64))
+        ints = torch.empty(2 * R + 5, dtype=_I32, device=kv_len.device)
+        longs = torch.empty((2, tokens), dtype=_I64, device=kv_len.device)
+        out = PageStep(*ints.split_with_sizes((R, 4, R + 1)), *longs.unbind())
     else:
         for name, n, dtype in (("kv_len", R, _I32), ("cursor", 4, _I32), ("starts", R + 1, _I32),
                                ("slots", tokens, _I64), ("positions", tokens, _I64)):
@@ -116,6 +121,6 @@ def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
                   _lib.ptr(delta), table.data_ptr(), ring.data_ptr(), cursor.data_ptr(),
                   out.kv_len.data_ptr(), out.cursor.data_ptr(), out.starts.data_ptr(),
                   out.slots.data_ptr(), out.positions.data_ptr(), R, table.shape[1],
-                  table.stride(0) if R > 1 else table.shape[1], ring.shape[0], page_size, tokens,
+                  table.stride(0) if R > 1 else table.shape[1], pages, page_size, tokens,
                   row, _lib.stream_of(kv_len))
     return out
