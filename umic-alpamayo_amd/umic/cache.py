@@ -33,7 +33,7 @@ import torch
 from transformers.cache_utils import DynamicCache, DynamicLayer
 
 from umic import _lib
-from umic.kernels import rope
+from umic.kernels import attention, rope
 
 
 class KVArena:
@@ -242,6 +242,27 @@ class InplaceLayer(DynamicLayer):
                                    norm)
         return (q_rot, *self._wrote(n))
 
+    def attend_rotary(self, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                      cos: torch.Tensor, sin: torch.Tensor, norm, scale: float):
+        """``append_rotary``, then attention of all q over all rows, read where they
+        lie: [B, S, Hq, D], or None -- nothing done -- for inputs the kernels do not
+        take."""
+        ar, i, n = self.arena, self.index, k.shape[2]
+        keys, values = ar.k(i), ar.v(i)
+        if not (self.can_append_rotary(q, k, v, cos, sin, norm)
+                and attention.cache_ok(keys, values)):
+            return None
+        if ar.replaying(n):
+            row, pos, rows = 0, ar.cursor, ar.window
+        else:
+            row, pos = ar.room(i, n), None
+            rows = row + n
+        q_rot = rope.kv_launch(q, k, v, cos, sin, keys, values, row, pos, norm)
+        if pos is None:
+            ar.fill[i] = rows
+        self._views_later(rows)
+        return attention.cache_attention(q_rot, keys, values, rows, causal=False, scale=scale)
+
     def get_seq_length(self, cache_position=None) -> int:
         return self.arena.fill[self.index]
 
@@ -357,7 +378,9 @@ class CacheStandIn:
 
     @staticmethod
     def convertible(cache) -> bool:
-        if not isinstance(cache, DynamicCache) or isinstance(cache, InplaceKVCache):
+        from umic.paged_cache import PagedKVCache
+
+        if not isinstance(cache, DynamicCache) or isinstance(cache, (InplaceKVCache, PagedKVCache)):
             return False
         layers = getattr(cache, "layers", None)
         return bool(layers) and all(getattr(lyr, "keys", None) is not None for lyr in layers)

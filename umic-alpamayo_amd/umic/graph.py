@@ -31,6 +31,7 @@ import torch
 from transformers.cache_utils import DynamicCache
 
 from umic.cache import InplaceKVCache
+from umic.paged_cache import PagedKVCache
 
 logger = logging.getLogger(__name__)
 
@@ -207,6 +208,7 @@ class DecodeGraphRunner:
         ids, pkv = kwargs.get("input_ids"), kwargs.get("past_key_values")
         return (not args and not self._off and isinstance(ids, torch.Tensor) and ids.is_cuda
                 and tuple(ids.shape) == (1, 1) and isinstance(pkv, DynamicCache)
+                and not isinstance(pkv, PagedKVCache)
                 and pkv.get_seq_length() > 0
                 and all(kwargs.get(name) is None for name in _MULTIMODAL)
                 and not torch.cuda.is_current_stream_capturing())

@@ -40,7 +40,7 @@ from torch.overrides import _get_current_function_mode_stack
 from torch.utils._device import DeviceContext
 
 from umic import _lib
-from umic.kernels import fused_ffn, layernorm, linear, rmsnorm, rope
+from umic.kernels import attention, fused_ffn, layernorm, linear, rmsnorm, rope
 from umic.kernels._common import grad_needed
 
 logger = logging.getLogger(__name__)
@@ -1050,6 +1050,54 @@ def _head_norms(module: nn.Module, q: torch.Tensor):
     return qw, kw, eps
 
 
+def _paged_attention(module: nn.Module, hidden_states: torch.Tensor, attention_mask, cache,
+                     pre_norm: nn.Module | None):
+    """The text attention over a ``PagedKVCache``: the projections, then the cache's
+    two launches, which rotate by the positions of the cache's step."""
+    if attention_mask is not None and not cache.unmasked:
+        raise ValueError("PagedKVCache: its lengths say which tokens are seen; pass no "
+                         "attention_mask (begin() takes the prompts' lengths)")
+    shape = (*hidden_states.shape[:-1], -1, module.head_dim)
+    q, k, v = (t.view(shape) for t in _qkv(module, hidden_states, pre_norm))
+    norm = _axial_norms(module, q)
+    if norm is None:
+        q, k = module.q_norm(q), module.k_norm(k)
+    out = cache.attend(module.layer_idx, q, k, v, norm, module.scaling)
+    return _linear(module.o_proj, out.reshape(*hidden_states.shape[:-1], -1)), None
+
+
+def _axial_norms(module: nn.Module, q: torch.Tensor):
+    """``(q_w, k_w, eps)`` of RMSNorms that ``axial.rotate_append`` takes, else None."""
+    qn, kn = module.q_norm, module.k_norm
+    if not all("rmsnorm" in type(n).__name__.lower() for n in (qn, kn)) or _hooked(qn, kn):
+        return None
+    qw, kw = getattr(qn, "weight", None), getattr(kn, "weight", None)
+    if _norm_eps(qn) != _norm_eps(kn) or not all(
+            isinstance(w, torch.Tensor) and w.dtype is torch.bfloat16 and w.device == q.device
+            and w.shape == q.shape[-1:] and w.is_contiguous() and w.data_ptr() % 16 == 0
+            for w in (qw, kw)):
+        return None
+    return qw, kw, _norm_eps(qn)
+
+
+# New tokens of a step that fuse_cache_attention's kernel takes: a decode step's
+# one, an action expert's 32 to 64.
+CACHE_ATTENTION_MAX_TOKENS = 128
+
+
+def _cache_attention_ok(module: nn.Module, q: torch.Tensor, attention_mask, kwargs) -> bool:
+    """True where fuse_cache_attention's kernel stands for the attention of q's tokens
+    over the in-place cache: no mask, and one token or an attention that is not causal
+    (all of the cache is seen), through SDPA, which returns no weights."""
+    tokens = q.shape[2]
+    return (getattr(module, "_umic_cache_attention", False) and attention_mask is None
+            and (tokens == 1 or tokens <= CACHE_ATTENTION_MAX_TOKENS
+                 and not (kwargs.get("is_causal") if kwargs.get("is_causal") is not None
+                          else getattr(module, "is_causal", True)))
+            and module.config._attn_implementation == "sdpa"
+            and not kwargs.get("output_attentions"))
+
+
 def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
                                      attention_mask=None, past_key_values=None, pre_norm=None,
                                      **kwargs):
@@ -1064,7 +1112,11 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
       append when the norms are not RMSNorms the kernel takes;
     * any other cache, or none: q_norm, k_norm and RoPE in one launch
       (``umic_qk_rmsnorm_rope_bf16``), then the cache's own ``update``;
-    * otherwise the module's norms, ``apply_rotary_pos_emb`` and ``update``.
+    * otherwise the module's norms, ``apply_rotary_pos_emb`` and ``update``;
+    * cache a ``PagedKVCache``: the same into its pages, by the positions of its
+      step, and the attention over them (``umic_cache_attention_bf16``);
+    * after ``fuse_cache_attention``, single tokens and unmasked steps over an
+      ``InplaceKVCache`` attend with that kernel too.
 
     pre_norm: the decoder layer's input norm, applied to hidden_states first
     (folded into the q/k/v GEMV at decode); the fused decoder-layer forward
@@ -1074,6 +1126,7 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
     forward.
     """
     from umic.cache import InplaceKVCache, InplaceLayer
+    from umic.paged_cache import PagedKVCache
 
     if self.training or grad_needed(hidden_states, self.q_proj.weight, self.k_proj.weight,
                                     self.v_proj.weight, getattr(self.q_norm, "weight", None),
@@ -1082,6 +1135,8 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
             hidden_states = pre_norm(hidden_states)
         return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
                                   past_key_values=past_key_values, **kwargs)
+    if isinstance(past_key_values, PagedKVCache):
+        return _paged_attention(self, hidden_states, attention_mask, past_key_values, pre_norm)
     layer = None
     if isinstance(past_key_values, InplaceKVCache) and self.layer_idx < len(
             past_key_values.layers):
@@ -1097,6 +1152,10 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
     norm = _head_norms(self, q)
     fused = None
     if norm is not None:
+        if layer is not None and _cache_attention_ok(self, q, attention_mask, kwargs):
+            out = layer.attend_rotary(q, k, v, cos, sin, norm, self.scaling)
+            if out is not None:
+                return _linear(self.o_proj, out.reshape(*input_shape, -1)), None
         if layer is not None:
             fused = layer.append_rotary(q, k, v, cos, sin, norm)
         elif rope.qk_norm_rope_eligible(q, k, cos, sin, norm[0], norm[1]):
@@ -1151,6 +1210,30 @@ def fuse_kv_rope(model: nn.Module, dry_run: bool = False) -> int:
     return count
 
 
+def fuse_cache_attention(model: nn.Module, dry_run: bool = False) -> int:
+    """Let single tokens, and the steps of attentions that are not causal, attend over an
+    ``InplaceKVCache`` with the library's kernel (``umic_cache_attention_bf16``), which
+    reads the cache where it lies: SDPA is handed a copy of it at every single-token step.
+    For modules that ``fuse_kv_rope`` has patched; calls with a mask, and back-ends other
+    than SDPA, stay as they are.  Not bit for bit SDPA (fp32 sums in another order).
+
+    Returns:
+        Number of attention modules matched (and marked unless dry_run).
+    """
+    if _qwen3_vl_module() is None or not _backend_ready("fuse_cache_attention"):
+        return 0
+    count = 0
+    for _, module in model.named_modules():
+        if not _is_text_attention(module) or module.head_dim not in attention.HEAD_DIMS:
+            continue
+        count += 1
+        if not dry_run:
+            module._umic_cache_attention = True
+    logger.info("fuse_cache_attention: %d attention module(s) %s", count,
+                "matched (dry run)" if dry_run else "marked")
+    return count
+
+
 def fuse_repeat_cache(repeat_module: nn.Module, extra_tokens_hint: int = 64) -> None:
     """Replace per-step KV concatenation in append-then-crop loops.
 
@@ -1187,6 +1270,7 @@ def unfuse_mlps(model: nn.Module) -> int:
     """Restore original forwards (delete every instance forward override)."""
     count = 0
     for _, module in model.named_modules():
+        module.__dict__.pop("_umic_cache_attention", None)
         if "forward" in module.__dict__:
             del module.__dict__["forward"]
             count += 1

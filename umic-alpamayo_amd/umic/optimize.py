@@ -54,6 +54,10 @@ class UmicConfig:
         adaptive_flow: accepted for compatibility; not implemented
             (reported False).
         max_new_tokens: decode-graph KV headroom (>= generate() budget).
+        cache_attention: with text_rope_fusion, single tokens and steps that
+            are not causal attend over the in-place cache with the library's
+            kernel instead of SDPA (no reference counterpart; off, as SDPA's
+            results are kept).
     With text_rope_fusion, attention calls that append to an in-place
     cache rotate q/k and write the cache in one launch.
     """
@@ -70,6 +74,7 @@ class UmicConfig:
     decode_graph: bool = True
     adaptive_flow: bool = False
     max_new_tokens: int = 96
+    cache_attention: bool = False
 
 
 def find_lm_module(model: nn.Module) -> nn.Module | None:
@@ -124,7 +129,8 @@ def _plan(integrate):
     report keys and their conditions are the reference's contract
     (src/umic/optimize.py:92-168), plus this runtime's additions:
     lm_kv_rope_fused / expert_kv_rope_fused (text RoPE fused into the
-    in-place cache append) and ve_gelu_mlp_fused.  The reference's ViT
+    in-place cache append), lm_cache_attention / expert_cache_attention and
+    ve_gelu_mlp_fused.  The reference's ViT
     patch-embed, packed-attention and bf16-residual rewrites are not part of
     this runtime, so their keys never appear.
     """
@@ -164,6 +170,10 @@ def _plan(integrate):
          count("fuse_add_rmsnorm")),
         (lambda c: c.flow_cache and c.text_rope_fusion, "expert", "expert_kv_rope_fused",
          count("fuse_kv_rope")),
+        (lambda c: c.cache_attention and c.text_rope_fusion, "lm", "lm_cache_attention",
+         count("fuse_cache_attention")),
+        (lambda c: c.cache_attention and c.flow_cache and c.text_rope_fusion, "expert",
+         "expert_cache_attention", count("fuse_cache_attention")),
         (lambda c: c.decode_graph, "vlm", "decode_graph",
          _hook(lambda m, c: fuse_decode_graph(m, max_new_tokens=c.max_new_tokens))),
         (lambda c: c.decode_cache and not c.decode_graph, "vlm", "decode_cache_hook",
