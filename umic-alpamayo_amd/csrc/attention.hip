@@ -248,12 +248,16 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, int b, int h, int l
 
 // A wave's rows r0 .. of a segment (row r is head r % G of new token r / G), NT
 // tiles of 16, a lane's being n16 of each; and what a step of 32 keys does to
-// them.
-template <int D, int NT>
+// them.  The V operand of output tile e holds for a lane one column of 8 keys, j =
+// 4 i + y being key 16 i + 4 g4 + y.  TURNED: it comes so from LDS, v[4 e ..] its
+// words, column 16 e + n16.  Else v[VW j ..] are DV columns of key j from DV n16 on,
+// turned in registers, tile e being column DV n16 + e of each lane.
+template <int D, int NT, bool TURNED>
 struct Rows {
   static constexpr int KK = D / 32;  // 32-wide steps of a score's product
   static constexpr int DV = D / 16;  // output columns of a lane, V columns it reads
   static constexpr int VW = DV / 2;  // 32-bit words of those
+  static constexpr int VR = 8 * VW;  // words of V a lane holds
   static constexpr float kSlack = 8.0f;
   u32x4 q[NT][KK];
   int lim[NT];  // keys below it are seen
@@ -304,18 +308,28 @@ struct Rows {
           sc[nt][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(kf[i][kk]), as_bf(q[nt][kk]),
                                                                sc[nt][i], 0, 0, 0);
   }
+  // Output column of acc[..][e][y].
+  static __device__ __forceinline__ int column(int e, int y, int g4) {
+    return TURNED ? 16 * e + 4 * g4 + y : (4 * g4 + y) * DV + e;
+  }
   // Keys that are not there, and those a row does not see.
-  __device__ __forceinline__ void mask(f32x4_t (&sc)[NT][2], uint32_t (&vr)[8][VW], const int (&n)[2],
+  __device__ __forceinline__ void mask(f32x4_t (&sc)[NT][2], uint32_t (&v)[VR], const int (&n)[2],
                                        int k0, int g4) const {
+    uint32_t keep[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int at = 4 * g4 + (j & 3), key = k0 + 16 * (j >> 2) + at;
       const bool there = at < n[j >> 2];
+      keep[j] = there ? 0xffffffffu : 0;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
         if (!there || key >= lim[nt]) sc[nt][j >> 2][j & 3] = -__builtin_inff();
+    }
+    // 0 * inf is not 0
 #pragma unroll
-      for (int w = 0; w < VW; ++w) vr[j][w] = there ? vr[j][w] : 0;  // 0 * inf is not 0
+    for (int x = 0; x < VR; ++x) {
+      const int j = TURNED ? (x & 3) * 2 : x / VW;
+      v[x] &= TURNED ? (keep[j] & 0xffffu) | (keep[j + 1] & 0xffff0000u) : keep[j];
     }
   }
   // p of the scores, in two bf16 parts.  m follows a row's maximum only when it is
@@ -364,19 +378,17 @@ struct Rows {
   // Where some rows do not see some of the keys, p = 0 has to hide a v that is not
   // finite, and 0 * inf is not 0: such elements leave the product, and the rows that
   // see them get theirs one by one.
-  __device__ __forceinline__ void hide(uint32_t (&vr)[8][VW], const u32x4 (&ph)[NT],
+  __device__ __forceinline__ void hide(uint32_t (&v)[VR], const u32x4 (&ph)[NT],
                                        const u32x4 (&pl)[NT], const AttnArgs& a, const Place& p,
                                        int k0, int n16, int g4) {
     bool wild = false;
 #pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t x = vr[j][w];
-        const bool l16 = (x & 0x7f80u) == 0x7f80u, h16 = (x & 0x7f800000u) == 0x7f800000u;
-        wild |= l16 | h16;
-        vr[j][w] = x & ~((l16 ? 0xffffu : 0u) | (h16 ? 0xffff0000u : 0u));
-      }
+    for (int w = 0; w < VR; ++w) {
+      const uint32_t x = v[w];
+      const bool l16 = (x & 0x7f80u) == 0x7f80u, h16 = (x & 0x7f800000u) == 0x7f800000u;
+      wild |= l16 | h16;
+      v[w] = x & ~((l16 ? 0xffffu : 0u) | (h16 ? 0xffff0000u : 0u));
+    }
     if (!__any(wild)) return;
 #pragma unroll 1
     for (int key = 0; key < kStep; ++key) {
@@ -398,31 +410,37 @@ struct Rows {
           for (int e = 0; e < DV; ++e)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
-              const float x = bf2f(vp[(4 * g4 + y) * DV + e]);
+              const float x = bf2f(vp[column(e, y, g4)]);
               if (!(__builtin_fabsf(x) < __builtin_inff())) acc[nt][e][y] += w * x;
             }
       }
     }
   }
-  __device__ __forceinline__ void product(const uint32_t (&vr)[8][VW], const u32x4 (&ph)[NT],
+  __device__ __forceinline__ void product(const uint32_t (&v)[VR], const u32x4 (&ph)[NT],
                                           const u32x4 (&pl)[NT]) {
 #pragma unroll
-    for (int w = 0; w < VW; ++w) {
+    for (int w = 0; w < VW; ++w) {  // two tiles at a time
       u32x4 v0, v1;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        v0[j] = pair_lo(vr[2 * j][w], vr[2 * j + 1][w]);
-        v1[j] = pair_hi(vr[2 * j][w], vr[2 * j + 1][w]);
+        if constexpr (TURNED) {
+          v0[j] = v[8 * w + j];
+          v1[j] = v[8 * w + 4 + j];
+        } else {
+          v0[j] = pair_lo(v[2 * j * VW + w], v[(2 * j + 1) * VW + w]);
+          v1[j] = pair_hi(v[2 * j * VW + w], v[(2 * j + 1) * VW + w]);
+        }
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        f32x4_t& c0 = acc[nt][2 * w];
-        f32x4_t& c1 = acc[nt][2 * w + 1];
-        c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(ph[nt]), c0, 0, 0, 0);
-        c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(ph[nt]), c1, 0, 0, 0);
-        c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), as_bf(pl[nt]), c0, 0, 0, 0);
-        c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), as_bf(pl[nt]), c1, 0, 0, 0);
-      }
+      for (int part = 0; part < 2; ++part)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          const bf16x8_t p = as_bf(part ? pl[nt] : ph[nt]);
+          f32x4_t& c0 = acc[nt][2 * w];
+          f32x4_t& c1 = acc[nt][2 * w + 1];
+          c0 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v0), p, c0, 0, 0, 0);
+          c1 = __builtin_amdgcn_mfma_f32_16x16x32_bf16(as_bf(v1), p, c1, 0, 0, 0);
+        }
     }
   }
 };
@@ -546,7 +564,7 @@ __device__ __forceinline__ int dealt_wg(int nwg) {
 // waves of this one are joined.
 template <int D>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(AttnArgs a) {
-  typedef Rows<D, 1> R;
+  typedef Rows<D, 1, false> R;
   constexpr int KK = R::KK, DV = R::DV, VW = R::VW;
   constexpr int LDR = D + 4;  // row of the join's LDS, in floats
   constexpr int kTile = kStep * kWaves;
@@ -575,7 +593,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
     Segment seg, nxt;
     Place here;
     u32x4 kf[2][KK];
-    uint32_t vr[8][VW];
+    uint32_t vr[R::VR];
     // rows that are not there are read again from one that is
     auto load_k = [&](const Place& p) {
 #pragma unroll
@@ -595,7 +613,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
             __umul24(min(4 * g4 + (j & 3), max(p.n[i] - 1, 0)), a.c_ss) + n16 * DV;
         const uint32_t* vp = reinterpret_cast<const uint32_t*>(a.v + p.at[i] + off);
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vr[j][w] = vp[w];
+        for (int w = 0; w < VW; ++w) vr[j * VW + w] = vp[w];
       }
     };
     auto first_of = [&](const Segment& s) {
@@ -717,6 +735,8 @@ __device__ __forceinline__ void landed_barrier() {
 }
 
 typedef __attribute__((address_space(3))) void lds_void;
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 
 // 16 bytes of each lane, from base + off (bytes), to 1 KB of LDS at `to`.  Written
 // out: before any LDS read the compiler waits for all loads into LDS that it knows
@@ -734,13 +754,13 @@ __device__ __forceinline__ void load_to_lds(const void* base, int off, const u32
 // More rows: each wave has 16 NT of the workgroup's 64 NT, and the keys go through
 // a ring in LDS, kRing - 1 steps of 32 on their way: the loads take a few
 // thousand cycles, a step about one (one step ahead, through registers: 67 us for
-// 512 rows over 6100 keys).  A row's 16-byte chunks are permuted (chunk ^ row) so
-// that neither the reads down a column of chunks (K) nor those along rows (V)
-// meet in a bank.
+// 512 rows over 6100 keys).  A row's 16-byte chunks are permuted so
+// that neither the reads of a chunk down the rows (K: ^ row) nor those of two
+// chunks of eight rows (V: ^ 2 row) meet in a bank.
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel(AttnArgs a) {
-  typedef Rows<D, NT> R;
-  constexpr int KK = R::KK, DV = R::DV, VW = R::VW;
+  typedef Rows<D, NT, true> R;
+  constexpr int KK = R::KK, DV = R::DV;
   constexpr int CH = D / 8;                   // chunks of a row
   constexpr int PER = kStep * CH / kThreads;  // chunks of K (and V) a thread moves a step
   constexpr int kBlock = 16 * NT * kWaves;    // rows of a workgroup
@@ -752,8 +772,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int n16 = lane & 15, g4 = lane >> 4;
-  auto swizzle = [](int row) { return CH >= 16 ? row & 15 : (row >> 1) & 7; };
-  auto cell = [&](int row, int chunk) { return row * CH + (chunk ^ swizzle(row)); };
+  auto k_swizzle = [](int row) { return CH >= 16 ? row & 15 : (row >> 1) & 7; };
+  auto v_swizzle = [](int row) { return CH >= 16 ? (row & 7) * 2 : ((row >> 1) & 3) * 2; };
 
   Scan scan = {};
   const int even = a.kv_len ? 0 : ManyDeal::units(a.len);
@@ -778,11 +798,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       const int i = __builtin_amdgcn_readfirstlane(row >> 4);
       const int n = i ? p.n[1] : p.n[0];
       const int64_t at = i ? p.at[1] : p.at[0];
-      const int off = (int)(__umul24(min(row & 15, max(n - 1, 0)), a.c_ss) * 2 +
-                            ((c % CH) ^ swizzle(row)) * 16);
+      const int off = (int)__umul24(min(row & 15, max(n - 1, 0)), a.c_ss) * 2;
       const int first = x * kThreads + wave * kWave;
-      load_to_lds(a.k + at, off, &kv[slot][0][first]);
-      load_to_lds(a.v + at, off, &kv[slot][1][first]);
+      load_to_lds(a.k + at, off + ((c % CH) ^ k_swizzle(row)) * 16, &kv[slot][0][first]);
+      load_to_lds(a.v + at, off + ((c % CH) ^ v_swizzle(row)) * 16, &kv[slot][1][first]);
     }
   };
   while (walk.next(a, seg)) {
@@ -819,35 +838,35 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
         landed_barrier<LOADS>();
       else
         landed_barrier<0>();
-      if (t + kRing - 1 < t1) {
-        send(t + kRing - 1);
-        ahead = place(t + kRing);
-      }
-      if (k0 >= r.hi || r0 >= rows) continue;
+      const bool idle = k0 >= r.hi || r0 >= rows;
       const u32x4* const ks = kv[t % kRing][0];
       const u32x4* const vs = kv[t % kRing][1];
       u32x4 kf[2][KK];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kf[i][kk] = ks[cell(16 * i + n16, kk * 4 + g4)];
+        for (int kk = 0; kk < KK; ++kk) kf[i][kk] = ks[(16 * i + n16) * CH + ((kk * 4 + g4) ^ k_swizzle(n16))];
+      if (t + kRing - 1 < t1) {
+        send(t + kRing - 1);
+        ahead = place(t + kRing);
+      }
+      if (idle) continue;
       f32x4_t sc[NT][2];
       r.scores(kf, sc);
-      uint32_t vr[8][VW];
+      // a read that turns 4 keys by 16 columns over 16 lanes: lane n16 gives the
+      // address of 4 columns of a key and gets one column of the 4 keys
+      uint32_t vr[R::VR];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const int row = 16 * (j >> 2) + 4 * g4 + (j & 3);
-        if constexpr (DV == 4) {
-          const uint32_t* p =
-              reinterpret_cast<const uint32_t*>(vs + cell(row, n16 >> 1)) + (n16 & 1) * 2;
-          vr[j][0] = p[0], vr[j][1] = p[1];
-        } else {
+      for (int i = 0; i < 2; ++i) {
+        const int row = 16 * i + 4 * g4 + (n16 >> 2);
 #pragma unroll
-          for (int y = 0; y < DV / 8; ++y) {
-            const u32x4 x = vs[cell(row, n16 * (DV / 8) + y)];
-#pragma unroll
-            for (int w = 0; w < 4; ++w) vr[j][y * 4 + w] = x[w];
-          }
+        for (int e = 0; e < DV; ++e) {
+          const u32x4* const c = vs + row * CH + ((2 * e + ((n16 >> 1) & 1)) ^ v_swizzle(row));
+          const uint64_t x = __builtin_bit_cast(
+              uint64_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s16x4*)(reinterpret_cast<const uint64_t*>(c) + (n16 & 1))));
+          vr[4 * e + 2 * i] = (uint32_t)x;
+          vr[4 * e + 2 * i + 1] = (uint32_t)(x >> 32);
         }
       }
       const bool edge = k0 + kStep > r.lo || !(full >> (t & 31) & 1);
@@ -870,27 +889,23 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       sum += __shfl_xor(sum, 32, kWave);
       const int row = r0 + nt * 16 + n16;
       if (row >= rows) continue;
-      // a lane's columns: 4 DV g4 .. + 4 DV
+      // a lane's columns: 16 e + 4 g4 .. + 4
       if (whole) {
         const bool none = row / a.G >= seg.fresh || sum == 0.0f;
         const float inv = 1.0f / sum;
-        uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, seg.b, seg.h, row) + 4 * DV * g4);
+        uint16_t* op = out_row(a, seg.b, seg.h, row) + 4 * g4;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int w = 0; w < VW; ++w)
-            op[i * VW + w] =
-                none ? 0 : pack2(r.acc[nt][2 * w][i] * inv, r.acc[nt][2 * w + 1][i] * inv);
+        for (int e = 0; e < DV; ++e) {
+          const f32x4_t x = r.acc[nt][e] * inv;
+          const u32x2 o = {none ? 0 : pack2(x[0], x[1]), none ? 0 : pack2(x[2], x[3])};
+          *reinterpret_cast<u32x2*>(op + 16 * e) = o;
+        }
       } else {
-        // four columns of each lane side by side: the join reads them the same way
+        // as the lanes hold them, side by side: the join reads them the same way
         const int64_t tile = (int64_t)slot * (kBlock / 16) + wave * NT + nt;
         f32x4_t* p = reinterpret_cast<f32x4_t*>(a.part) + tile * 4 * D + lane;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int e = 0; e < DV; e += 4)
-            p[(i * DV + e) / 4 * kWave] = f32x4_t{r.acc[nt][e][i], r.acc[nt][e + 1][i],
-                                                  r.acc[nt][e + 2][i], r.acc[nt][e + 3][i]};
+        for (int e = 0; e < DV; ++e) p[e * kWave] = r.acc[nt][e];
         if (g4 == 0) {
           a.part_ml[(tile * 16 + n16) * 2] = r.m[nt];
           a.part_ml[(tile * 16 + n16) * 2 + 1] = sum;
@@ -944,8 +959,7 @@ __global__ __launch_bounds__(kThreads) void join_few_kernel(AttnArgs a) {
 }
 
 // Joins those of attend_many_kernel: a workgroup to 4 of the DV column groups of a
-// tile of 16 rows, a lane to one row's four columns of a group, in the order in
-// which they were stored.
+// tile of 16 rows, a lane to four columns of one row.
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
   constexpr int DV = D / 16;
@@ -981,10 +995,8 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
     o += part[t * 4 * D] * f;
   }
   const bool none = sum == 0.0f || row / a.G >= new_of(a, b);
-  // group (i DV + e) / 4 of a lane's columns 4 DV g4 ..
-  uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, b, h, row) + 4 * DV * g4 + group * 4);
-  op[0] = none ? 0 : pack2(o[0] / sum, o[1] / sum);
-  op[1] = none ? 0 : pack2(o[2] / sum, o[3] / sum);
+  const u32x2 x = {none ? 0 : pack2(o[0] / sum, o[1] / sum), none ? 0 : pack2(o[2] / sum, o[3] / sum)};
+  *reinterpret_cast<u32x2*>(out_row(a, b, h, row) + 16 * group + 4 * g4) = x;
 }
 
 struct Shape {
