@@ -503,7 +503,8 @@ int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, voi
  * over the keys j < n_b of request b (causal: j <= n_b - m_b + s), fp32 softmax,
  * one rounding to bf16.  n_b = kv_lens[b] (device; NULL: kv_len for all), the new
  * tokens included, clamped to what the cache can hold; m_b = q_lens[b] (NULL:
- * S): rows s >= m_b, and rows that see no key, are zero.
+ * S): rows s >= m_b, and rows that see no key (or none whose score is above
+ * -infinity), are zero.
  * q: B x S x Hq x D, strides (q_sb, q_ss, q_sh); out likewise (o_*).  Query head
  * h reads key head h / (Hq / Hk).
  * k, v: blocks of block_rows rows, strides (c_sb block, c_sh head, c_ss row).

@@ -570,7 +570,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
   constexpr int kTile = kStep * kWaves;
   __shared__ int sums[kWaves];
   __shared__ int found[2];
-  __shared__ int arrived;
+  __shared__ int arrived[2];
   __shared__ float ml[kWaves][16][2];
   __shared__ float acc_lds[kWaves][16][LDR];
   const int lane = threadIdx.x & (kWave - 1);
@@ -591,6 +591,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
     walk.start(a, deal, scan, even, wg, found);
     R r;
     Segment seg, nxt;
+    Segment first = {}, last = {};  // those that other workgroups have a part of
     Place here;
     u32x4 kf[2][KK];
     uint32_t vr[R::VR];
@@ -700,25 +701,35 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
           if (col == 0) put2(a.part_ml + at * 2, mx, sum);
         }
       }
-      if (a.counters && !whole) {
-        int w0, w1;
-        deal.holders(seg.at, seg.tiles, w0, w1);
-        // each wave's stores have arrived before its workgroup is counted
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        __syncthreads();
-        if (threadIdx.x == 0)
-          arrived = __hip_atomic_fetch_add(a.counters + w0, 1, __ATOMIC_RELAXED,
-                                           __HIP_MEMORY_SCOPE_AGENT);
-        __syncthreads();
-        if (arrived == w1 - w0) {  // all other parts are there
-          if (threadIdx.x == 0) a.counters[w0] = 0;  // for the next call
-          for (int row = wave; row < rows; row += kWaves)
-            join_row<D, true>(a, w0, w1, row, row / a.G >= seg.fresh,
-                                  out_row(a, seg.b, seg.h, row));
-        }
-      }
+      if (!whole) (seg.t0 == 0 ? last : first) = seg;
       __syncthreads();  // LDS is used again
       seg = nxt;
+    }
+    if (a.counters && (first.tiles | last.tiles)) {
+      // Both parts are counted at the end: a count after each kept the workgroup
+      // waiting while none of its loads were on their way.  Every wave's stores have
+      // arrived before.
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      int w0[2] = {}, w1[2] = {};
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const Segment& p = i ? last : first;
+        if (p.tiles == 0) continue;
+        deal.holders(p.at, p.tiles, w0[i], w1[i]);
+        if (threadIdx.x == 0)
+          arrived[i] = __hip_atomic_fetch_add(a.counters + w0[i], 1, __ATOMIC_RELAXED,
+                                              __HIP_MEMORY_SCOPE_AGENT);
+      }
+      __syncthreads();
+#pragma unroll 1
+      for (int i = 0; i < 2; ++i) {
+        const Segment& p = i ? last : first;
+        if (p.tiles == 0 || arrived[i] != w1[i] - w0[i]) continue;  // other parts are missing
+        if (threadIdx.x == 0) a.counters[w0[i]] = 0;                // for the next call
+        for (int row = wave; row < rows; row += kWaves)
+          join_row<D, true>(a, w0[i], w1[i], row, row / a.G >= p.fresh, out_row(a, p.b, p.h, row));
+      }
     }
   }
   if (a.counters) zero_rows<D>(a);
@@ -742,13 +753,15 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 // out: before any LDS read the compiler waits for all loads into LDS that it knows
 // of, those of the steps to come included.  Its own counts of loads in flight stay
 // safe, as more are in flight than it counts; nothing is written to a register.
+// The wait states: of m0 (1), and of scalars that a vector instruction wrote (5),
+// which the compiler does not see to inside the block.  (With the builtin every step
+// waited for the loads of the steps to come: 512 rows over 6100 keys 100 us for 59.)
 __device__ __forceinline__ void load_to_lds(const void* base, int off, const u32x4* to) {
   const uint64_t b = (uint64_t)base;
   const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
-  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(at),
-               "v"(off), "s"(rsrc)
-               : "memory", "m0");
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(at), "v"(off), "s"(rsrc)
+               : "memory");
 }
 
 // More rows: each wave has 16 NT of the workgroup's 64 NT, and the keys go through
@@ -1093,8 +1106,8 @@ extern "C" int umic_cache_attention_bf16(
   const int64_t cus = device_cus();
   if (cus <= 0) return (int)hipErrorNoDevice;
   const int64_t G = Hq / Hk;
-  if (B > (1 << 20) || S > (1 << 20) || Hq > (1 << 16) || cap > ((int64_t)1 << 30) ||
-      blocks > ((int64_t)1 << 30))
+  if (B > (1 << 20) || S > (1 << 20) || Hq > (1 << 16) || S * Hq > 0x7fffffff ||
+      cap > ((int64_t)1 << 30) || blocks > ((int64_t)1 << 30))
     return UMIC_ERR_UNSUPPORTED;
   const Shape s = shape_of(S * G, D, cus);
   if (workspace_bytes < workspace_of(s, D)) return UMIC_ERR_INVALID_ARG;

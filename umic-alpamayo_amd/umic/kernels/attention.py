@@ -137,6 +137,8 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
             raise ValueError(f"cache_attention: out must be [{B}, {S}, {Hq}, {D}] of 16-byte "
                              f"chunks, got {tuple(out.shape)}")
         os_ = out.stride()
+        if any(st == 0 and n > 1 for st, n in zip(os_, out.shape)):
+            raise ValueError("cache_attention: out must not share rows")
     if B == 0 or S == 0 or Hq == 0:
         return out
     qs, cs = q.stride(), k_cache.stride()
