@@ -994,18 +994,34 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
   auto tile_of = [&](int i) { return first + (2 * i + (i == 0)) * kTiles; };
   const float* ml = a.part_ml + n16 * 2;
   const f32x4_t* part = reinterpret_cast<const f32x4_t*>(a.part) + group * kWave + lane;
-  float mx = -__builtin_inff();
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) mx = fmaxf(mx, ml[tile_of(i) * 32]);
-  const float base = mx == -__builtin_inff() ? 0.0f : mx;
+  // kAhead parts at a time, all their loads at once
+  constexpr int kAhead = 8;
+  float mx = -__builtin_inff(), sum = 0.0f;
   f32x4_t o = {0, 0, 0, 0};
-  float sum = 0.0f;
-#pragma unroll 4
-  for (int i = 0; i < n; ++i) {
-    const int64_t t = tile_of(i);
-    const float f = __builtin_amdgcn_exp2f(ml[t * 32] - base);
-    sum += ml[t * 32 + 1] * f;
-    o += part[t * 4 * D] * f;
+  for (int i0 = 0; i0 < n; i0 += kAhead) {
+    float m[kAhead], l[kAhead];
+    f32x4_t x[kAhead];
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) {
+      const int64_t t = tile_of(min(i0 + j, n - 1));
+      m[j] = ml[t * 32], l[j] = ml[t * 32 + 1];
+      x[j] = part[t * 4 * D];
+    }
+    float to = mx;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j) to = fmaxf(to, m[j]);
+    const float base = to == -__builtin_inff() ? 0.0f : to;
+    const float f0 = __builtin_amdgcn_exp2f(mx - base);
+    mx = to;
+    sum *= f0;
+    o *= f0;
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (i0 + j < n) {
+        const float f = __builtin_amdgcn_exp2f(m[j] - base);
+        sum += l[j] * f;
+        o += x[j] * f;
+      }
   }
   const bool none = sum == 0.0f || row / a.G >= new_of(a, b);
   const u32x2 x = {none ? 0 : pack2(o[0] / sum, o[1] / sum), none ? 0 : pack2(o[2] / sum, o[3] / sum)};
