@@ -478,11 +478,10 @@ __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int b, int h, in
 // lanes hold the parts' maxima and sums, 64 parts at a time, then D / 64 columns
 // each, and a part's factor comes from the lane that holds it.  The first part is
 // its workgroup's second (its last segment), the others their first.  SHARED: they were written by this launch.
-template <int D, bool SHARED>
-__device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int rr, bool none,
+template <int D, bool SHARED, int kAhead>
+__device__ __forceinline__ void join_parts(const AttnArgs& a, int w0, int w1, int rr, bool none,
                                          uint16_t* op) {
   constexpr int C = D / kWave;
-  constexpr int kAhead = 8;  // parts in flight (32: 25 parts 4.9 us for 5.5, but 9 parts 7.2 for 5.0)
   const int lane = threadIdx.x & (kWave - 1);
   const int n = w1 - w0 + 1;
   const int64_t first = (int64_t)w0 * 2 * 16 + rr;
@@ -533,6 +532,17 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int 
   if (sum == 0.0f) none = true;
 #pragma unroll
   for (int c = 0; c < C; ++c) op[lane * C + c] = (uint16_t)f2bf(none ? 0.0f : o[c] / sum);
+}
+
+// Parts in flight: 8, where there are more than 16 of them 32 (25 parts 4.9 us for
+// 5.5, 64 7 for 12; but 9 parts 7.2 for 5.0).
+template <int D, bool SHARED>
+__device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int rr, bool none,
+                                         uint16_t* op) {
+  if (w1 - w0 < 16)
+    join_parts<D, SHARED, 8>(a, w0, w1, rr, none, op);
+  else
+    join_parts<D, SHARED, D <= 128 ? 32 : 16>(a, w0, w1, rr, none, op);
 }
 
 // Requests without a key: zeros.
@@ -1141,7 +1151,11 @@ extern "C" int umic_cache_attention_bf16(
   a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = (int)c_ss, a.table_ld = table_ld, a.cap = (int)cap;
   a.B = (int)B, a.S = (int)S, a.Hk = (int)Hk, a.G = (int)G, a.rb = s.rb;
   a.len = kv_lens ? 0 : (int)kv_len, a.blocks = (int)blocks, a.shift = shift;
-  a.causal = causal != 0, a.nwg = s.nwg, a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
+  // Single tokens of a few segments, up to a quarter of the CUs': a workgroup to a
+  // CU.  The second hides the starts and ends of segments; with few it only doubles
+  // their parts (8 segments of 12288 keys 18 us for 25, 64 of 1024 14.5 for 15.4; 128
+  // of 300 15.2 for 13.6, 64 ragged requests 74 for 60).
+  a.causal = causal != 0, a.nwg = s.nt == 0 && B * Hk * 4 <= cus && s.nwg > cus ? (int)cus : s.nwg, a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
   if (a.c < 0x1p-126f) a.c = 0x1p-126f;  // masked scores are -inf: times 0 they would be NaN
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   hipStream_t st = as_stream(stream);
