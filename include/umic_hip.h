@@ -444,7 +444,7 @@ int umic_add_rmsnorm_gate_silu_mul_bf16(const void* x, const void* r, const void
  */
 #define UMIC_PLAN_OK 0
 #define UMIC_PLAN_NO_PAGES 1  /* more pages are needed than are free */
-#define UMIC_PLAN_TOO_LONG 2  /* a request outgrows its table row */
+#define UMIC_PLAN_TOO_LONG 2  /* a request outgrows its table row, or 2^31 - 1 tokens */
 #define UMIC_PLAN_NO_ROOM 3   /* more new tokens than tokens, or than row */
 #define UMIC_PLAN_BAD_STATE 4 /* a length or the queue's state out of range */
 int umic_page_plan(const int32_t* kv_len, const int32_t* new_len, const int32_t* keep,
@@ -515,7 +515,7 @@ int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, voi
  * whatever they hold.  A later new token's v that is infinite or NaN does not
  * reach the rows that do not see it.
  * D: 64, 128 or 256; strides multiples of 8, pointers 16-byte aligned (else
- * UMIC_ERR_UNSUPPORTED).  workspace: umic_cache_attention_workspace_bytes, for
+ * UMIC_ERR_UNSUPPORTED).  |scale| <= 2^127.  workspace: umic_cache_attention_workspace_bytes, for
  * this call alone until it has run (contents need not be kept or cleared).
  * counters: UMIC_ATTENTION_COUNTERS int32, zero before their first use and left
  * zero by every call, for calls that do not overlap in time (those of one stream):

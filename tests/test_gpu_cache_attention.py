@@ -111,6 +111,12 @@ def test_empty_cache_gives_zeros():
     assert none.numel() == 0
 
 
+def test_a_table_without_entries_is_refused():
+    q, k, v, table = make([48, 48], 1, 4, 2, 128, 16)
+    with pytest.raises(ValueError, match="table"):
+        call(q, k[:2], v[:2], [48, 48], table[:, :0])
+
+
 def test_lengths_past_the_cache_are_cut():
     q, k, v, table = make([48, 48], 1, 4, 2, 128, 16, seed=2)
     table = table[:, :3].contiguous()

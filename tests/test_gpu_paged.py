@@ -119,6 +119,17 @@ def test_refused_steps_change_nothing(why):
     check(run(*args), want)
 
 
+def test_lengths_end_at_32_bits():
+    page, most = 1 << 30, (1 << 31) - 1
+    table, ring = np.array([[2, 1, -1]], np.int32), np.array([0, -1, -1], np.int32)
+    for new, want in ((4, paged.PLAN_OK), (5, paged.TOO_LONG)):
+        got = run(np.array([most - 4], np.int32), [new], table, ring,
+                  np.array([0, 1, 0, 0], np.int32), page, 8, None, None, 0)
+        assert got[1][3] == want
+        assert got[0][0] == (most if want == paged.PLAN_OK else most - 4)
+        assert got[3][0] == ((1 << 30) + (most - 4) % page if want == paged.PLAN_OK else -1)
+
+
 def test_in_place_and_repeated():
     """kv_len and cursor as their own outputs; and a step repeated on the same lengths and queue."""
     rng = random.Random(3)

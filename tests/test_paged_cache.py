@@ -53,6 +53,9 @@ def test_what_it_refuses():
         c.update(x, x, 0)
     with pytest.raises(RuntimeError):
         c.crop(3)
+    for call in (c.reorder_cache, c.batch_select_indices, c.batch_repeat_interleave):
+        with pytest.raises(RuntimeError):
+            call(torch.tensor([1, 0]))
     with pytest.raises(ValueError, match="attention_mask"):
         integrate._paged_attention(torch.nn.Module(), x, torch.ones(2, 1), c, None)
     assert c.get_seq_length() == 0 and c.get_mask_sizes(5, 0) == (5, 0)

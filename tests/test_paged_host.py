@@ -72,7 +72,7 @@ def test_cache_attention_refusals(lib):
     assert f(B=0) == f(S=0) == f(Hq=0) == 0
     assert f(Hk=3) == f(Hk=0) == ARG
     assert f(q=None) == f(out=None) == f(ws=None) == f(k=None) == f(v=None) == ARG
-    assert f(scale=float("inf")) == f(scale=float("nan")) == ARG
+    assert f(scale=float("inf")) == f(scale=float("nan")) == f(scale=-3e38) == ARG
     assert f(blocks=3) == ARG                              # contiguous: one block a request
     assert f(n=65) == f(n=-1) == ARG                       # past the cache
     assert f(table=FAKE, w=4, ld=3) == f(table=FAKE, w=-1) == ARG

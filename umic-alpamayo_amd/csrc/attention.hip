@@ -477,10 +477,11 @@ __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int b, int h, in
 // Joins one row of a segment that workgroups w0 .. w1 hold, a wave to a row: its
 // lanes hold the parts' maxima and sums, 64 parts at a time, then D / 64 columns
 // each, and a part's factor comes from the lane that holds it.  The first part is
-// its workgroup's second (its last segment), the others their first.  SHARED: they were written by this launch.
+// its workgroup's second (its last segment), the others their first.  SHARED: they
+// were written by this launch.
 template <int D, bool SHARED, int kAhead>
 __device__ __forceinline__ void join_parts(const AttnArgs& a, int w0, int w1, int rr, bool none,
-                                         uint16_t* op) {
+                                           uint16_t* op) {
   constexpr int C = D / kWave;
   const int lane = threadIdx.x & (kWave - 1);
   const int n = w1 - w0 + 1;
@@ -534,8 +535,8 @@ __device__ __forceinline__ void join_parts(const AttnArgs& a, int w0, int w1, in
   for (int c = 0; c < C; ++c) op[lane * C + c] = (uint16_t)f2bf(none ? 0.0f : o[c] / sum);
 }
 
-// Parts in flight: 8, where there are more than 16 of them 32 (25 parts 4.9 us for
-// 5.5, 64 7 for 12; but 9 parts 7.2 for 5.0).
+// Parts in flight: 8, where there are more than 16 of them 32 (a join of 25 parts 4.9
+// us for 5.5 with 8; but one of 9 parts 7.2 for 5.0).
 template <int D, bool SHARED>
 __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int rr, bool none,
                                          uint16_t* op) {
@@ -770,7 +771,8 @@ __device__ __forceinline__ void load_to_lds(const void* base, int off, const u32
   const uint64_t b = (uint64_t)base;
   const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
   const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(at), "v"(off), "s"(rsrc)
+  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(at), "v"(off),
+               "s"(rsrc)
                : "memory");
 }
 
@@ -868,7 +870,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int kk = 0; kk < KK; ++kk) kf[i][kk] = ks[(16 * i + n16) * CH + ((kk * 4 + g4) ^ k_swizzle(n16))];
+        for (int kk = 0; kk < KK; ++kk)
+          kf[i][kk] = ks[(16 * i + n16) * CH + ((kk * 4 + g4) ^ k_swizzle(n16))];
       if (t + kRing - 1 < t1) {
         send(t + kRing - 1);
         ahead = place(t + kRing);
@@ -940,8 +943,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
 
 // What a join needs to know of its (request, key head, row block).
 template <typename DEAL>
-__device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, int* sums, int* found,
-                                           int& w0, int& w1) {
+__device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, int* sums,
+                                           int* found, int& w0, int& w1) {
   const int per = a.Hk * a.rb;
   const int len = keys_of(a, b), tiles = DEAL::tiles(len), units = DEAL::units(len);
   int all = units * a.B, before = units * b;
@@ -1034,7 +1037,8 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
       }
   }
   const bool none = sum == 0.0f || row / a.G >= new_of(a, b);
-  const u32x2 x = {none ? 0 : pack2(o[0] / sum, o[1] / sum), none ? 0 : pack2(o[2] / sum, o[3] / sum)};
+  const u32x2 x = {none ? 0 : pack2(o[0] / sum, o[1] / sum),
+                   none ? 0 : pack2(o[2] / sum, o[3] / sum)};
   *reinterpret_cast<u32x2*>(out_row(a, b, h, row) + 16 * group + 4 * g4) = x;
 }
 
@@ -1109,7 +1113,7 @@ extern "C" int umic_cache_attention_bf16(
       workspace_bytes < 0)
     return UMIC_ERR_INVALID_ARG;
   if (B == 0 || S == 0 || Hq == 0) return UMIC_OK;
-  if (Hk == 0 || Hq % Hk || !(__builtin_fabsf(scale) < __builtin_inff()))
+  if (Hk == 0 || Hq % Hk || !(__builtin_fabsf(scale) <= 0x1p127f))
     return UMIC_ERR_INVALID_ARG;
   if (!q || !out || !workspace) return UMIC_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return UMIC_ERR_UNSUPPORTED;
@@ -1155,7 +1159,9 @@ extern "C" int umic_cache_attention_bf16(
   // CU.  The second hides the starts and ends of segments; with few it only doubles
   // their parts (8 segments of 12288 keys 18 us for 25, 64 of 1024 14.5 for 15.4; 128
   // of 300 15.2 for 13.6, 64 ragged requests 74 for 60).
-  a.causal = causal != 0, a.nwg = s.nt == 0 && B * Hk * 4 <= cus && s.nwg > cus ? (int)cus : s.nwg, a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
+  a.nwg = s.nt == 0 && B * Hk * 4 <= cus ? (int)cus : s.nwg;
+  a.causal = causal != 0;
+  a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
   if (a.c < 0x1p-126f) a.c = 0x1p-126f;  // masked scores are -inf: times 0 they would be NaN
   a.flip = scale < 0.0f ? 0x80008000u : 0u;
   hipStream_t st = as_stream(stream);

@@ -52,7 +52,8 @@ struct Request {
 __device__ __forceinline__ Request request_of(const PlanArgs& a, int r) {
   Request q = {};
   if (r >= a.R) return q;
-  const int64_t most = (int64_t)a.W << a.shift;
+  const int64_t row = (int64_t)a.W << a.shift;
+  const int64_t most = row < 0x7fffffff ? row : 0x7fffffff;  // lengths are 32-bit
   const int len = a.kv_len[r];
   q.kept = max(0, min(a.keep ? a.keep[r] : len, len));
   q.fresh = max(0, a.fresh[r]);

@@ -112,9 +112,9 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         cap, ld, width = rows, 0, 0
     else:
         if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[0] != B
-                or table.get_device() != dev or table.stride(1) != 1):
-            raise ValueError(f"cache_attention: table must be int32 [{B}, W] with contiguous rows "
-                             f"on q's device, got {table.dtype} {tuple(table.shape)}")
+                or table.shape[1] == 0 or table.get_device() != dev or table.stride(1) != 1):
+            raise ValueError(f"cache_attention: table must be int32 [{B}, W > 0] with contiguous "
+                             f"rows on q's device, got {table.dtype} {tuple(table.shape)}")
         width = table.shape[1]
         cap, ld = width * rows, table.stride(0) if B > 1 else width
     if isinstance(kv_len, torch.Tensor):

@@ -149,7 +149,8 @@ class PagedKVCache(DynamicCache):
               keep: Sequence[int | None] | None = None, delta: Sequence[int] | None = None) -> None:
         """Plan the next forward: its tokens of each request (an int: as many of all),
         right-padded to the longest.  positions: [axes, requests, S] int64, else the
-        plan's own plus ``delta``."""
+        plan's own plus ``delta``.  That forward has to be run before the next step: it
+        writes the rows that the plan has counted."""
         ar = self.arena
         same = isinstance(new, int)
         new = [new] * ar.requests if same else list(new)
@@ -213,6 +214,11 @@ class PagedKVCache(DynamicCache):
 
     def crop(self, *args, **kwargs) -> None:
         raise RuntimeError("PagedKVCache: drop tokens with begin(..., keep=)")
+
+    def reorder_cache(self, *args, **kwargs) -> None:
+        raise RuntimeError("PagedKVCache: its requests stay where they are")
+
+    batch_repeat_interleave = batch_select_indices = reorder_cache
 
     def reset(self) -> None:
         """Every request empty."""
