@@ -381,15 +381,14 @@ struct Rows {
   __device__ __forceinline__ void hide(uint32_t (&v)[VR], const u32x4 (&ph)[NT],
                                        const u32x4 (&pl)[NT], const AttnArgs& a, const Place& p,
                                        int k0, int n16, int g4) {
-    bool wild = false;
+    // exponents of ones, both halves of a word at once: bits 15 and 31
+    auto wild = [](uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; };
+    uint32_t any = 0;
 #pragma unroll
-    for (int w = 0; w < VR; ++w) {
-      const uint32_t x = v[w];
-      const bool l16 = (x & 0x7f80u) == 0x7f80u, h16 = (x & 0x7f800000u) == 0x7f800000u;
-      wild |= l16 | h16;
-      v[w] = x & ~((l16 ? 0xffffu : 0u) | (h16 ? 0xffff0000u : 0u));
-    }
-    if (!__any(wild)) return;
+    for (int w = 0; w < VR; ++w) any |= wild(v[w]);
+    if (!__any(any & 0x80008000u)) return;
+#pragma unroll
+    for (int w = 0; w < VR; ++w) v[w] &= ~((wild(v[w]) >> 15 & 0x00010001u) * 0xffffu);
 #pragma unroll 1
     for (int key = 0; key < kStep; ++key) {
       const int at = key & 15, j = (key >> 4) * 4 + (at & 3);
