@@ -146,15 +146,15 @@ struct Segment {
   int b, h, rb, len, tiles, t0, t1, fresh, at;
 };
 
-// A workgroup's walk over its segments.
-template <typename DEAL>
+// A workgroup's walk over its segments.  BLOCKS: a (request, key head) can have more
+// than one row block.
+template <typename DEAL, bool BLOCKS>
 struct Walk {
   int u, u_end, b, before, per;
 
-  // false: this workgroup has none
-  __device__ __forceinline__ bool start(const AttnArgs& a, const DEAL& deal, const Scan& scan,
+  __device__ __forceinline__ void start(const AttnArgs& a, const DEAL& deal, const Scan& scan,
                                         int even, int wg, int* found) {
-    per = a.Hk * a.rb;
+    per = BLOCKS ? a.Hk * a.rb : a.Hk;
     u = deal.begin(wg);
     u_end = deal.begin(wg + 1);
     const int target = u / per;
@@ -175,7 +175,6 @@ struct Walk {
       b = target / even;
       before = b * even;
     }
-    return true;
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, Segment& s) {
     while (u < u_end) {
@@ -192,8 +191,8 @@ struct Walk {
       const int p0 = in - pair * units, p1 = min(units, p0 + u_end - u);
       s.at = before * per + pair * units;
       s.b = b;
-      s.h = pair / a.rb;
-      s.rb = pair - s.h * a.rb;
+      s.h = BLOCKS ? pair / a.rb : pair;
+      s.rb = BLOCKS ? pair - s.h * a.rb : 0;
       s.t0 = max(0, p0 - lead);
       s.t1 = max(0, p1 - lead);
       s.fresh = new_of(a, b);
@@ -207,6 +206,8 @@ struct Walk {
     return false;
   }
 };
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 __device__ __forceinline__ bf16x8_t as_bf(const u32x4& v) { return __builtin_bit_cast(bf16x8_t, v); }
 
@@ -452,97 +453,82 @@ __device__ __forceinline__ void put2(float* p, float x, float y) {
   const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 }
-template <bool SHARED>
-__device__ __forceinline__ float get(const float* p) {
-  if constexpr (!SHARED) return *p;
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-template <bool SHARED>
-__device__ __forceinline__ void get2(const float* p, float& x, float& y) {
-  if constexpr (SHARED) {
-    const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(p), __ATOMIC_RELAXED,
-                                         __HIP_MEMORY_SCOPE_AGENT);
-    x = __uint_as_float((uint32_t)v), y = __uint_as_float((uint32_t)(v >> 32));
-  } else {
-    x = p[0], y = p[1];
-  }
-}
-
 __device__ __forceinline__ uint16_t* out_row(const AttnArgs& a, int b, int h, int r) {
   const int t = r / a.G, g = r - t * a.G;
   return a.out + b * a.o_sb + t * a.o_ss + (int64_t)(h * a.G + g) * a.o_sh;
 }
 
-// Joins one row of a segment that workgroups w0 .. w1 hold, a wave to a row: its
-// lanes hold the parts' maxima and sums, 64 parts at a time, then D / 64 columns
-// each, and a part's factor comes from the lane that holds it.  The first part is
-// its workgroup's second (its last segment), the others their first.  SHARED: they
-// were written by this launch.
-template <int D, bool SHARED, int kAhead>
-__device__ __forceinline__ void join_parts(const AttnArgs& a, int w0, int w1, int rr, bool none,
-                                           uint16_t* op) {
-  constexpr int C = D / kWave;
-  const int lane = threadIdx.x & (kWave - 1);
-  const int n = w1 - w0 + 1;
-  const int64_t first = (int64_t)w0 * 2 * 16 + rr;
-  auto row_of = [&](int i) { return first + (2 * i + (i == 0)) * 16; };
-  float x[kAhead][C];
-  auto load = [&](int i0) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j) {
-      const float* p = a.part + row_of(min(i0 + j, n - 1)) * D + lane * C;
-      if constexpr (C == 1) {
-        x[j][0] = get<SHARED>(p);
-      } else {
-#pragma unroll
-        for (int c = 0; c < C; c += 2) get2<SHARED>(p + c, x[j][c], x[j][c + 1]);
-      }
-    }
-  };
-  float mi = -__builtin_inff(), li = 0.0f;  // part `lane`'s
-  if (lane < n) get2<SHARED>(a.part_ml + row_of(lane) * 2, mi, li);
-  load(0);
-  float mx = mi;
-  for (int i = lane + kWave; i < n; i += kWave)
-    mx = fmaxf(mx, get<SHARED>(a.part_ml + row_of(i) * 2));
-#pragma unroll
-  for (int k = 1; k < kWave; k <<= 1) mx = fmaxf(mx, __shfl_xor(mx, k, kWave));
-  const float base = mx == -__builtin_inff() ? 0.0f : mx;
-  float o[C] = {};
-  float sum = 0.0f;
-  for (int i0 = 0; i0 < n; i0 += kWave) {
-    if (i0) {
-      mi = -__builtin_inff(), li = 0.0f;
-      if (i0 + lane < n) get2<SHARED>(a.part_ml + row_of(i0 + lane) * 2, mi, li);
-    }
-    const float f = __builtin_amdgcn_exp2f(mi - base);
-    sum += li * f;
-#pragma unroll 1
-    for (int j0 = 0; j0 < kWave && i0 + j0 < n; j0 += kAhead) {
-      if (i0 + j0) load(i0 + j0);
-#pragma unroll
-      for (int j = 0; j < kAhead; ++j) {
-        const float fj = __shfl(f, j0 + j, kWave);  // 0 past the last part
-#pragma unroll
-        for (int c = 0; c < C; ++c) o[c] += (i0 + j0 + j < n ? x[j][c] : 0.0f) * fj;
-      }
-    }
-  }
-  sum = group_sum<kWave>(sum);
-  if (sum == 0.0f) none = true;
-#pragma unroll
-  for (int c = 0; c < C; ++c) op[lane * C + c] = (uint16_t)f2bf(none ? 0.0f : o[c] / sum);
-}
-
-// Parts in flight: 8, where there are more than 16 of them 32 (a join of 25 parts 4.9
-// us for 5.5 with 8; but one of 9 parts 7.2 for 5.0).
+// Joins one row of a segment that workgroups w0 .. w1 hold, a wave to a row.  Part i,
+// 64 of them at a time: lane i holds its maximum and sum, D / 4 lanes a fourth of its
+// columns each.  The first part is its workgroup's second (its last segment), the
+// others their first; loads past the last give zeros.  SHARED: the parts were written
+// by this launch.  (With 32 parts in flight, each by its own address, the code was
+// three times as long, and fetching it what the join waited for: a single token over
+// 3100 keys, 25 parts, 12.4 us for 10.4.)
 template <int D, bool SHARED>
 __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int rr, bool none,
                                          uint16_t* op) {
-  if (w1 - w0 < 16)
-    join_parts<D, SHARED, 8>(a, w0, w1, rr, none, op);
-  else
-    join_parts<D, SHARED, D <= 128 ? 32 : 16>(a, w0, w1, rr, none, op);
+  constexpr int kLanes = D / 4, kParts = kWave / kLanes;  // lanes of a part, parts a load
+  constexpr int kAhead = 8;
+  constexpr int kAux = SHARED ? 16 : 0;  // sc1: agent scope
+  constexpr int kRow = 16 * D * 4, kRowMl = 16 * 2 * 4;   // bytes from a slot to the next
+  const int lane = threadIdx.x & (kWave - 1);
+  const int sub = lane / kLanes, col = (lane & (kLanes - 1)) * 4;
+  const int n = w1 - w0 + 1;  // two at least
+  const int64_t first = (int64_t)w0 * 2 * 16 + rr;
+  const auto parts = __builtin_amdgcn_make_buffer_rsrc(a.part + first * D, 0, (2 * n - 1) * kRow,
+                                                       0x00020000);
+  const auto mls = __builtin_amdgcn_make_buffer_rsrc(a.part_ml + first * 2, 0,
+                                                     (2 * n - 1) * kRowMl, 0x00020000);
+  auto slot_of = [](int i) { return 2 * i + (i == 0); };
+  float mi, li;  // part `lane`'s
+  auto load_ml = [&](int i) {
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(mls, slot_of(i) * kRowMl, 0, kAux);
+    mi = i < n ? __uint_as_float(x[0]) : -__builtin_inff();
+    li = __uint_as_float(x[1]);
+  };
+  f32x4_t x[kAhead];
+  auto load = [&](int i0) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      x[j] = __builtin_bit_cast(
+          f32x4_t, __builtin_amdgcn_raw_buffer_load_b128(
+                       parts, slot_of(i0 + j * kParts + sub) * kRow + col * 4, 0, kAux));
+  };
+  load_ml(lane);
+  load(0);
+  float mx = mi;
+  for (int i0 = kWave; i0 < n; i0 += kWave) {
+    load_ml(i0 + lane);
+    mx = fmaxf(mx, mi);
+  }
+  if (n > kWave) load_ml(lane);
+#pragma unroll
+  for (int k = 1; k < kWave; k <<= 1) mx = fmaxf(mx, __shfl_xor(mx, k, kWave));
+  const float base = mx == -__builtin_inff() ? 0.0f : mx;
+  f32x4_t o = {0, 0, 0, 0};
+  float sum = 0.0f;
+#pragma unroll 1
+  for (int i0 = 0; i0 < n; i0 += kWave) {
+    if (i0) load_ml(i0 + lane);
+    const float f = __builtin_amdgcn_exp2f(mi - base);
+    sum += li * f;
+#pragma unroll 1
+    for (int j0 = 0; j0 < kWave && i0 + j0 < n; j0 += kAhead * kParts) {
+      if (i0 + j0) load(i0 + j0);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j) o += x[j] * __shfl(f, j0 + j * kParts + sub, kWave);
+    }
+  }
+#pragma unroll
+  for (int k = kLanes; k < kWave; k <<= 1)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] += __shfl_xor(o[c], k, kWave);
+  sum = group_sum<kWave>(sum);
+  if (sum == 0.0f) none = true;
+  const u32x2 out = {none ? 0 : pack2(o[0] / sum, o[1] / sum),
+                     none ? 0 : pack2(o[2] / sum, o[3] / sum)};
+  if (sub == 0) *reinterpret_cast<u32x2*>(op + col) = out;
 }
 
 // Requests without a key: zeros.
@@ -581,6 +567,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
   __shared__ int sums[kWaves];
   __shared__ int found[2];
   __shared__ int arrived[2];
+  __shared__ Segment kept[2];  // those that other workgroups have a part of: the first, the last
   __shared__ float ml[kWaves][16][2];
   __shared__ float acc_lds[kWaves][16][LDR];
   const int lane = threadIdx.x & (kWave - 1);
@@ -597,11 +584,11 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
   const int wg = dealt_wg(deal.nwg);
   const int rows = a.S * a.G;
   if (wg >= 0) {
-    Walk<FewDeal> walk;
+    Walk<FewDeal, false> walk;
     walk.start(a, deal, scan, even, wg, found);
     R r;
     Segment seg, nxt;
-    Segment first = {}, last = {};  // those that other workgroups have a part of
+    int split = 0;  // bits: which of `kept` there are
     Place here;
     u32x4 kf[2][KK];
     uint32_t vr[R::VR];
@@ -711,22 +698,24 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
           if (col == 0) put2(a.part_ml + at * 2, mx, sum);
         }
       }
-      if (!whole) (seg.t0 == 0 ? last : first) = seg;
+      if (!whole) {
+        split |= seg.t0 == 0 ? 2 : 1;
+        if (threadIdx.x == 0) kept[seg.t0 == 0 ? 1 : 0] = seg;
+      }
       __syncthreads();  // LDS is used again
       seg = nxt;
     }
-    if (a.counters && (first.tiles | last.tiles)) {
+    if (a.counters && split) {
       // Both parts are counted at the end: a count after each kept the workgroup
       // waiting while none of its loads were on their way.  Every wave's stores have
       // arrived before.
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
-      int w0[2] = {}, w1[2] = {};
+      int w0[2], w1[2];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const Segment& p = i ? last : first;
-        if (p.tiles == 0) continue;
-        deal.holders(p.at, p.tiles, w0[i], w1[i]);
+        if (!(split >> i & 1)) continue;
+        deal.holders(uniform(kept[i].at), uniform(kept[i].tiles), w0[i], w1[i]);
         if (threadIdx.x == 0)
           arrived[i] = __hip_atomic_fetch_add(a.counters + w0[i], 1, __ATOMIC_RELAXED,
                                               __HIP_MEMORY_SCOPE_AGENT);
@@ -734,11 +723,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
       __syncthreads();
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
-        const Segment& p = i ? last : first;
-        if (p.tiles == 0 || arrived[i] != w1[i] - w0[i]) continue;  // other parts are missing
-        if (threadIdx.x == 0) a.counters[w0[i]] = 0;                // for the next call
+        // others' parts are missing
+        if (!(split >> i & 1) || uniform(arrived[i]) != w1[i] - w0[i]) continue;
+        if (threadIdx.x == 0) a.counters[w0[i]] = 0;  // for the next call
+        const int b = uniform(kept[i].b), h = uniform(kept[i].h), fresh = uniform(kept[i].fresh);
         for (int row = wave; row < rows; row += kWaves)
-          join_row<D, true>(a, w0[i], w1[i], row, row / a.G >= p.fresh, out_row(a, p.b, p.h, row));
+          join_row<D, true>(a, w0[i], w1[i], row, row / a.G >= fresh, out_row(a, b, h, row));
       }
     }
   }
@@ -809,7 +799,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
   const int wg = dealt_wg(deal.nwg);
   const int rows = a.S * a.G;
   if (wg < 0) return;
-  Walk<ManyDeal> walk;
+  Walk<ManyDeal, true> walk;
   walk.start(a, deal, scan, even, wg, found);
   R r;
   Segment seg;
