@@ -61,12 +61,21 @@ struct AttnArgs {
   float c;                // |scale| * log2(e)
 };
 
+// The kernel's arguments, loaded again: held over the loops, they and what follows from
+// them do not fit the scalar registers.
+__device__ __forceinline__ AttnArgs args_again() {
+  typedef const __attribute__((address_space(4))) AttnArgs* Args;
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const AttnArgs*)p;
+}
+
 // A scalar load whatever the compiler can prove about the kernel's stores.
 __device__ __forceinline__ int scalar_i32(const int32_t* p) {
   return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
 }
 
-__device__ __forceinline__ int keys_of(const AttnArgs& a, int b) {
+__device__ __forceinline__ int len_of(const AttnArgs& a, int b) {
   return a.kv_len ? min(max(scalar_i32(a.kv_len + b), 0), a.cap) : a.len;
 }
 
@@ -178,7 +187,7 @@ struct Walk {
   }
   __device__ __forceinline__ bool next(const AttnArgs& a, Segment& s) {
     while (u < u_end) {
-      s.len = keys_of(a, b);
+      s.len = len_of(a, b);
       const int units = DEAL::units(s.len);
       if (units == 0) {
         ++b;
@@ -219,30 +228,56 @@ __device__ __forceinline__ uint32_t pair_hi(uint32_t a, uint32_t b) {
   return __builtin_amdgcn_perm(b, a, 0x07060302u);
 }
 
-// Where 32 keys lie: two key tiles of 16 rows (a page never ends inside one), the
-// first `n` rows of each there.
+// A segment's keys: row j is row j % 2^shift of block row[j >> shift], and base is
+// row 0 of block 0; row NULL: all are one block.
+struct Keys {
+  int64_t base;
+  const int32_t* row;
+  int len;
+};
+
+__device__ __forceinline__ Keys keys_of(const AttnArgs& a, const Segment& s) {
+  Keys k;
+  k.row = a.table ? a.table + s.b * a.table_ld : nullptr;
+  k.base = s.h * a.c_sh + (a.table ? 0 : s.b * a.c_sb);
+  k.len = s.len;
+  return k;
+}
+
+// The blocks of 32 keys from k0 on: of two tiles of 16 (a block never ends inside
+// one).  Asked for a step before their place is needed.
+struct Blocks {
+  int of[2];
+};
+
+__device__ __forceinline__ Blocks blocks_of(const AttnArgs& a, const Keys& s, int k0) {
+  Blocks x = {};
+  if (s.row) {
+    const int last = (s.len - 1) >> a.shift;
+    x.of[0] = scalar_i32(s.row + min(k0 >> a.shift, last));
+    x.of[1] = scalar_i32(s.row + min((k0 + 16) >> a.shift, last));
+  }
+  return x;
+}
+
+// Where the two tiles lie, the first `n` rows of each there.
 struct Place {
   int64_t at[2];
   int n[2];
 };
 
-__device__ __forceinline__ Place place_of(const AttnArgs& a, int b, int h, int len, int k0) {
+__device__ __forceinline__ Place place_of(const AttnArgs& a, const Keys& s, int k0,
+                                          const Blocks& x) {
   Place p;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
-    int key = k0 + 16 * i;
-    p.n[i] = min(max(len - key, 0), 16);
-    if (p.n[i] == 0) key = 0;
-    int64_t block = b;
-    if (a.table) {
-      const int at = key >> a.shift;
-      const int page = scalar_i32(a.table + (int64_t)b * a.table_ld + at);
-      key -= at << a.shift;
-      const bool there = page >= 0 && page < a.blocks;  // a page outside the pool: not seen
-      block = there ? page : 0;
-      if (!there) p.n[i] = 0;
-    }
-    p.at[i] = block * a.c_sb + h * a.c_sh + (int64_t)key * a.c_ss;
+    const int key = k0 + 16 * i;
+    p.n[i] = min(max(s.len - key, 0), 16);
+    // a block outside the pool: not there; rows that are not there are read elsewhere
+    const unsigned block = (unsigned)x.of[i];
+    if (block >= (unsigned)a.blocks) p.n[i] = 0;
+    p.at[i] = s.base;
+    if (p.n[i]) p.at[i] += block * a.c_sb + (int64_t)(key & ((1 << a.shift) - 1)) * a.c_ss;
   }
   return p;
 }
@@ -536,7 +571,7 @@ template <int D>
 __device__ __forceinline__ void zero_rows(const AttnArgs& a) {
   const int chunks = D / 8;
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
-    if (keys_of(a, b)) continue;
+    if (len_of(a, b)) continue;
     const int64_t n = (int64_t)a.S * a.Hk * a.G * chunks;
     for (int64_t i = threadIdx.x; i < n; i += kThreads) {
       const int c = (int)(i % chunks), row = (int)(i / chunks);
@@ -593,7 +628,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
     u32x4 kf[2][KK];
     uint32_t vr[R::VR];
     // rows that are not there are read again from one that is
-    auto load_k = [&](const Place& p) {
+    auto load_k = [&](const AttnArgs& a, const Place& p) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
         const uint16_t* kp = a.k + p.at[i];
@@ -603,7 +638,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
           kf[i][kk] = ld_stream(reinterpret_cast<const u32x4*>(kp + off + kk * 32));
       }
     };
-    auto load_v = [&](const Place& p) {
+    auto load_v = [&](const AttnArgs& a, const Place& p) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int i = j >> 2;
@@ -614,48 +649,52 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         for (int w = 0; w < VW; ++w) vr[j * VW + w] = vp[w];
       }
     };
-    auto first_of = [&](const Segment& s) {
-      return place_of(a, s.b, s.h, s.len, s.t0 * kTile + wave * kStep);
+    auto first_of = [&](const AttnArgs& a, const Segment& s) {
+      const Keys keys = keys_of(a, s);
+      const int k0 = s.t0 * kTile + wave * kStep;
+      return place_of(a, keys, k0, blocks_of(a, keys, k0));
     };
     walk.next(a, seg);  // a dealt workgroup has one
-    here = first_of(seg);
-    load_k(here);
-    load_v(here);
+    here = first_of(a, seg);
+    load_k(a, here);
+    load_v(a, here);
     r.load_q(a, seg, 0, n16, g4);
     for (bool go = true; go;) {
       go = walk.next(a, nxt);
-      const Place turn = go ? first_of(nxt) : here;
+      const Place turn = go ? first_of(a, nxt) : here;
       bool turned = false;  // the next segment's keys are on their way
+      const Keys keys = keys_of(a, seg);
       r.clear();
       for (int t = seg.t0; t < seg.t1; ++t) {
         const int k0 = t * kTile + wave * kStep, k1 = k0 + kTile;
         if (k0 >= r.hi) break;
         const bool more = t + 1 < seg.t1 && k1 < r.hi;
         Place next = turn;
-        if (more) next = place_of(a, seg.b, seg.h, seg.len, k1);
+        if (more) next = place_of(a, keys, k1, blocks_of(a, keys, k1));
         turned = !more;
         f32x4_t sc[1][2];
         r.scores(kf, sc);
-        if (more || go) load_k(next);  // under the softmax and the second product
+        if (more || go) load_k(a, next);  // under the softmax and the second product
         const bool edge = k0 + kStep > r.lo || here.n[0] < 16 || here.n[1] < 16;
         if (edge) r.mask(sc, vr, here.n, k0, g4);
         u32x4 ph[1], pl[1];
         r.weights(sc, a.c, ph, pl);
         if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
         r.product(vr, ph, pl);
-        if (more || go) load_v(next);
+        if (more || go) load_v(a, next);
         here = next;
       }
       if (go) {
         if (!turned) {
-          load_k(turn);
-          load_v(turn);
+          load_k(a, turn);
+          load_v(a, turn);
         }
         here = turn;
-        r.load_q(a, nxt, 0, n16, g4);
+        r.load_q(args_again(), nxt, 0, n16, g4);
       }
 
       // join the waves
+      const AttnArgs args = args_again();
       const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
       const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
       r.l[0] += __shfl_xor(r.l[0], 16, kWave);
@@ -686,16 +725,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
           for (int e = 0; e < DV; ++e) o[e] += acc_lds[w][rr][col + e] * f;
         }
         if (whole) {
-          const bool none = rr / a.G >= seg.fresh || sum == 0.0f;
+          const bool none = rr / args.G >= seg.fresh || sum == 0.0f;
           const float inv = 1.0f / sum;
-          uint32_t* op = reinterpret_cast<uint32_t*>(out_row(a, seg.b, seg.h, rr) + col);
+          uint32_t* op = reinterpret_cast<uint32_t*>(out_row(args, seg.b, seg.h, rr) + col);
 #pragma unroll
           for (int w = 0; w < VW; ++w) op[w] = none ? 0 : pack2(o[2 * w] * inv, o[2 * w + 1] * inv);
         } else {
           const int64_t at = (int64_t)slot * 16 + rr;
 #pragma unroll
-          for (int e = 0; e < DV; e += 2) put2(a.part + at * D + col + e, o[e], o[e + 1]);
-          if (col == 0) put2(a.part_ml + at * 2, mx, sum);
+          for (int e = 0; e < DV; e += 2) put2(args.part + at * D + col + e, o[e], o[e + 1]);
+          if (col == 0) put2(args.part_ml + at * 2, mx, sum);
         }
       }
       if (!whole) {
@@ -705,7 +744,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
       __syncthreads();  // LDS is used again
       seg = nxt;
     }
-    if (a.counters && split) {
+    const AttnArgs args = args_again();
+    if (args.counters && split) {
       // Both parts are counted at the end: a count after each kept the workgroup
       // waiting while none of its loads were on their way.  Every wave's stores have
       // arrived before.
@@ -717,18 +757,19 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         if (!(split >> i & 1)) continue;
         deal.holders(uniform(kept[i].at), uniform(kept[i].tiles), w0[i], w1[i]);
         if (threadIdx.x == 0)
-          arrived[i] = __hip_atomic_fetch_add(a.counters + w0[i], 1, __ATOMIC_RELAXED,
+          arrived[i] = __hip_atomic_fetch_add(args.counters + w0[i], 1, __ATOMIC_RELAXED,
                                               __HIP_MEMORY_SCOPE_AGENT);
       }
       __syncthreads();
 #pragma unroll 1
       for (int i = 0; i < 2; ++i) {
+        const int v0 = i ? w0[1] : w0[0], v1 = i ? w1[1] : w1[0];
         // others' parts are missing
-        if (!(split >> i & 1) || uniform(arrived[i]) != w1[i] - w0[i]) continue;
-        if (threadIdx.x == 0) a.counters[w0[i]] = 0;  // for the next call
+        if (!(split >> i & 1) || uniform(arrived[i]) != v1 - v0) continue;
+        if (threadIdx.x == 0) args.counters[v0] = 0;  // for the next call
         const int b = uniform(kept[i].b), h = uniform(kept[i].h), fresh = uniform(kept[i].fresh);
         for (int row = wave; row < rows; row += kWaves)
-          join_row<D, true>(a, w0[i], w1[i], row, row / a.G >= fresh, out_row(a, b, h, row));
+          join_row<D, true>(args, v0, v1, row, row / args.G >= fresh, out_row(args, b, h, row));
       }
     }
   }
@@ -756,12 +797,8 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 // The wait states: of m0 (1), and of scalars that a vector instruction wrote (5),
 // which the compiler does not see to inside the block.  (With the builtin every step
 // waited for the loads of the steps to come: 512 rows over 6100 keys 100 us for 59.)
-__device__ __forceinline__ void load_to_lds(const void* base, int off, const u32x4* to) {
-  const uint64_t b = (uint64_t)base;
-  const u32x4 rsrc = {(uint32_t)b, (uint32_t)(b >> 32) & 0xffffu, 0x7fffffffu, 0x00020000u};
-  const uint32_t at = __builtin_amdgcn_readfirstlane((uint32_t)(uintptr_t)(lds_void*)to);
-  asm volatile("s_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"{m0}"(at), "v"(off),
-               "s"(rsrc)
+__device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned to) {
+  asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(off), "s"(base)
                : "memory");
 }
 
@@ -805,43 +842,47 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
   Segment seg;
   // A load instruction fills 64 neighbouring cells of LDS: which chunk a lane
   // fetches follows from its cell.  Rows that are not there are another's again.
-  auto fetch = [&](int slot, const Place& p) {
+  const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(lds_void*)kv) +
+                       wave * kWave * 16;
+  auto fetch = [&](const AttnArgs& a, int slot, const Place& p) {
 #pragma unroll
     for (int x = 0; x < PER; ++x) {
       const int c = x * kThreads + (int)threadIdx.x, row = c / CH;
-      const int i = __builtin_amdgcn_readfirstlane(row >> 4);
+      const int i = (CH >= 16 ? x * (kThreads / CH) : wave * (kWave / CH)) >> 4;  // its tile
       const int n = i ? p.n[1] : p.n[0];
       const int64_t at = i ? p.at[1] : p.at[0];
-      const int off = (int)__umul24(min(row & 15, max(n - 1, 0)), a.c_ss) * 2;
-      const int first = x * kThreads + wave * kWave;
-      load_to_lds(a.k + at, off + ((c % CH) ^ k_swizzle(row)) * 16, &kv[slot][0][first]);
-      load_to_lds(a.v + at, off + ((c % CH) ^ v_swizzle(row)) * 16, &kv[slot][1][first]);
+      const unsigned off = __umul24(min(row & 15, max(n - 1, 0)), a.c_ss) * 2;
+      const unsigned to = lds + (slot * 2 * kStep * CH + x * kThreads) * 16;
+      load_to_lds(a.k + at, off + ((c % CH) ^ k_swizzle(row)) * 16, to);
+      load_to_lds(a.v + at, off + ((c % CH) ^ v_swizzle(row)) * 16, to + kStep * CH * 16);
     }
   };
-  while (walk.next(a, seg)) {
+  while (walk.next(args_again(), seg)) {
+    const AttnArgs a = args_again();
     const int r0 = seg.rb * kBlock + wave * 16 * NT;
     // the block's last key that any row sees
     int end = seg.len;
     if (a.causal)
       end = min(end, seg.len - seg.fresh + (min((seg.rb + 1) * kBlock, rows) - 1) / a.G + 1);
     const int t1 = min(seg.t1, (max(end, 0) + kStep - 1) / kStep);
-    auto place = [&](int t) { return place_of(a, seg.b, seg.h, seg.len, min(t, t1 - 1) * kStep); };
-    Place ahead = {};
+    const Keys keys = keys_of(a, seg);
+    auto blocks = [&](int t) { return blocks_of(a, keys, t * kStep); };
+    Blocks ahead[kRing];
     unsigned full = 0;  // bit t % 32: step t's pages are all there
-    auto send = [&](int t) {
-      fetch(t % kRing, ahead);
+    auto send = [&](int t, const Blocks& x) {
+      const Place p = place_of(a, keys, t * kStep, x);
+      fetch(a, t % kRing, p);
       const unsigned bit = 1u << (t & 31);
-      full = ahead.n[0] == 16 && ahead.n[1] == 16 ? full | bit : full & ~bit;
+      full = p.n[0] == 16 && p.n[1] == 16 ? full | bit : full & ~bit;
     };
     landed_barrier<63>();  // the last segment's reads are done
-    if (seg.t0 < t1) {
-      for (int t = seg.t0; t < min(seg.t0 + kRing - 1, t1); ++t) {
-        ahead = place(t);
-        send(t);
-      }
-      ahead = place(seg.t0 + kRing - 1);
-    }
-    r.load_q(a, seg, r0, n16, g4);
+#pragma unroll
+    for (int i = 0; i < kRing; ++i) ahead[i] = blocks(seg.t0 + i);
+#pragma unroll
+    for (int i = 0; i < kRing - 1; ++i)
+      if (seg.t0 + i < t1) send(seg.t0 + i, ahead[i]);
+    Blocks later = ahead[kRing - 1];
+    r.load_q(args_again(), seg, r0, n16, g4);
     r.clear();
     for (int t = seg.t0; t < t1; ++t) {
       const int k0 = t * kStep;
@@ -862,8 +903,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
         for (int kk = 0; kk < KK; ++kk)
           kf[i][kk] = ks[(16 * i + n16) * CH + ((kk * 4 + g4) ^ k_swizzle(n16))];
       if (t + kRing - 1 < t1) {
-        send(t + kRing - 1);
-        ahead = place(t + kRing);
+        send(t + kRing - 1, later);
+        later = blocks(t + kRing);
       }
       if (idle) continue;
       f32x4_t sc[NT][2];
@@ -887,7 +928,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       const bool edge = k0 + kStep > r.lo || !(full >> (t & 31) & 1);
       Place here = {};
       if (edge) {
-        here = place(t);
+        here = place_of(a, keys, k0, blocks(t));
         r.mask(sc, vr, here.n, k0, g4);
       }
       u32x4 ph[NT], pl[NT];
@@ -895,6 +936,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
       r.product(vr, ph, pl);
     }
+    const AttnArgs args = args_again();
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
 #pragma unroll
@@ -906,9 +948,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       if (row >= rows) continue;
       // a lane's columns: 16 e + 4 g4 .. + 4
       if (whole) {
-        const bool none = row / a.G >= seg.fresh || sum == 0.0f;
+        const bool none = row / args.G >= seg.fresh || sum == 0.0f;
         const float inv = 1.0f / sum;
-        uint16_t* op = out_row(a, seg.b, seg.h, row) + 4 * g4;
+        uint16_t* op = out_row(args, seg.b, seg.h, row) + 4 * g4;
 #pragma unroll
         for (int e = 0; e < DV; ++e) {
           const f32x4_t x = r.acc[nt][e] * inv;
@@ -918,12 +960,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       } else {
         // as the lanes hold them, side by side: the join reads them the same way
         const int64_t tile = (int64_t)slot * (kBlock / 16) + wave * NT + nt;
-        f32x4_t* p = reinterpret_cast<f32x4_t*>(a.part) + tile * 4 * D + lane;
+        f32x4_t* p = reinterpret_cast<f32x4_t*>(args.part) + tile * 4 * D + lane;
 #pragma unroll
         for (int e = 0; e < DV; ++e) p[e * kWave] = r.acc[nt][e];
         if (g4 == 0) {
-          a.part_ml[(tile * 16 + n16) * 2] = r.m[nt];
-          a.part_ml[(tile * 16 + n16) * 2 + 1] = sum;
+          args.part_ml[(tile * 16 + n16) * 2] = r.m[nt];
+          args.part_ml[(tile * 16 + n16) * 2 + 1] = sum;
         }
       }
     }
@@ -935,7 +977,7 @@ template <typename DEAL>
 __device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, int* sums,
                                            int* found, int& w0, int& w1) {
   const int per = a.Hk * a.rb;
-  const int len = keys_of(a, b), tiles = DEAL::tiles(len), units = DEAL::units(len);
+  const int len = len_of(a, b), tiles = DEAL::tiles(len), units = DEAL::units(len);
   int all = units * a.B, before = units * b;
   if (a.kv_len) {
     const Scan scan = scan_units<DEAL>(a, sums);
@@ -1107,7 +1149,7 @@ extern "C" int umic_cache_attention_bf16(
   if (!q || !out || !workspace) return UMIC_ERR_INVALID_ARG;
   if (!head_dim_ok(D)) return UMIC_ERR_UNSUPPORTED;
   int64_t cap = block_rows;
-  int shift = 0;
+  int shift = 30;
   if (table) {
     if (table_w < 0 || table_ld < table_w) return UMIC_ERR_INVALID_ARG;
     if (block_rows < 16 || (block_rows & (block_rows - 1))) return UMIC_ERR_UNSUPPORTED;
