@@ -56,7 +56,7 @@ struct AttnArgs {
   int cap;                // keys a request can hold
   int c_ss;               // below 2^24: row offsets inside a tile are 32-bit
   int B, S, Hk, G, rb;    // rb: row blocks of a (request, key head)
-  int len, blocks, shift, causal, nwg;
+  int len, blocks, shift, causal, nwg, some;  // nwg, some: see Deal
   uint32_t flip;          // sign bits of q (a negative scale)
   float c;                // |scale| * log2(e)
 };
@@ -95,9 +95,10 @@ struct Deal {
   static __device__ __forceinline__ int units(int keys) {
     return keys > 0 ? tiles(keys) + LEAD : 0;
   }
-  __device__ __forceinline__ Deal(unsigned all, int most) {
+  // most: that the chip holds; if that many have no work, no more than `some`
+  __device__ __forceinline__ Deal(unsigned all, int most, int some) {
     const unsigned fit = (all + LEAST - 1) / LEAST;
-    nwg = fit < (unsigned)most ? (int)fit : most;
+    nwg = fit >= (unsigned)most ? most : min((int)fit, some);
     each = nwg ? all / (unsigned)nwg : 0;
     more = all - each * (unsigned)nwg;
   }
@@ -615,7 +616,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
     scan = scan_units<FewDeal>(a, sums);
   else
     scan.all = even * a.B;
-  const FewDeal deal((unsigned)(scan.all * a.Hk), a.nwg);
+  const FewDeal deal((unsigned)(scan.all * a.Hk), a.nwg, a.some);
   const int wg = dealt_wg(deal.nwg);
   const int rows = a.S * a.G;
   if (wg >= 0) {
@@ -832,7 +833,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
     scan = scan_units<ManyDeal>(a, sums);
   else
     scan.all = even * a.B;
-  const ManyDeal deal((unsigned)(scan.all * a.Hk * a.rb), a.nwg);
+  const ManyDeal deal((unsigned)(scan.all * a.Hk * a.rb), a.nwg, a.some);
   const int wg = dealt_wg(deal.nwg);
   const int rows = a.S * a.G;
   if (wg < 0) return;
@@ -992,7 +993,7 @@ __device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, i
   }
   w0 = 0, w1 = -1;
   if (tiles == 0) return false;
-  const DEAL deal((unsigned)(all * per), a.nwg);
+  const DEAL deal((unsigned)(all * per), a.nwg, a.some);
   deal.holders((unsigned)(before * per + pair * units), tiles, w0, w1);
   return true;
 }
@@ -1191,6 +1192,9 @@ extern "C" int umic_cache_attention_bf16(
   // their parts (8 segments of 12288 keys 18 us for 25, 64 of 1024 14.5 for 15.4; 128
   // of 300 15.2 for 13.6, 64 ragged requests 74 for 60).
   a.nwg = s.nt == 0 && B * Hk * 4 <= cus ? (int)cus : s.nwg;
+  // Many rows: two workgroups to a CU or one.  Between the two some CUs have twice the
+  // others' work (128 tokens over 1024 keys: 288 workgroups 25 us, 256 of them 22).
+  a.some = s.nt && a.nwg > cus ? (int)cus : a.nwg;
   a.causal = causal != 0;
   a.c = __builtin_fabsf(scale) * 1.4426950408889634f;
   if (a.c < 0x1p-126f) a.c = 0x1p-126f;  // masked scores are -inf: times 0 they would be NaN
