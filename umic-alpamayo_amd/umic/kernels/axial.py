@@ -22,6 +22,14 @@ from umic.kernels._common import grad_needed, require_device
 
 MAX_HEAD_DIM = 512
 _PI = Fraction(314159265358979323846264338327950288419716939937510582097494, 10 ** 59)
+_UNIT = round(2 ** 191 / _PI)  # 2^64 / (2 pi) turns a radian, 128 bits behind the point
+
+
+def _turn(freq: float) -> int:
+    """round(2^64 freq / (2 pi)) modulo 2^64, as a signed number."""
+    n, d = freq.as_integer_ratio()
+    t = ((n * _UNIT // d >> 127) + 1 >> 1) & 2 ** 64 - 1
+    return t - 2 ** 64 if t >= 2 ** 63 else t
 
 
 class AxisPlan:
@@ -42,9 +50,7 @@ class AxisPlan:
                              f"{tuple(axis.shape)} must be vectors of one length")
         if not freq or not all(abs(f) < float("inf") for f in freq) or int(axis.min()) < 0:
             raise ValueError("AxisPlan: frequencies must be finite and axes not negative")
-        turn = [round(Fraction(f) / (2 * _PI) * 2 ** 64) % 2 ** 64 for f in freq]
-        self.turn = torch.tensor([t - 2 ** 64 if t >= 2 ** 63 else t for t in turn],
-                                 dtype=torch.int64).to(device)
+        self.turn = torch.tensor([_turn(f) for f in freq], dtype=torch.int64).to(device)
         self.axis = axis.to(device)
         self.axes = int(axis.max()) + 1
         self.head_dim = 2 * len(freq)
