@@ -26,6 +26,12 @@
 // most two such parts each, of the first and the last of its segments.  They are
 // joined in the order of the keys: by the workgroup that finishes last, for up
 // to 16 rows and with counters to find that out, else by a second kernel.
+//
+// Measured, 32 query heads over 8 of 128: a token of two requests of 131001 keys each
+// 171 us (6.3 TB/s), of 64 ragged requests up to 8192 keys 55 (4.6 TB/s), of one
+// request of 3100 keys 10.4: 4.5 until its first keys are there, 1.7 for them, 4 to
+// join 25 parts.  128 tokens over 65536 keys 240 us (577 TFLOP/s); four 128-token
+// chunks 47, of which the second kernel takes 13 for 41 MB of parts.
 #include <algorithm>
 
 #include "common.hpp"
@@ -116,6 +122,9 @@ struct Deal {
   }
 };
 typedef Deal<kStep * kWaves, 0, 1> FewDeal;  // single tokens: 128 keys, as they are
+// Many rows: a segment's start and end cost some four steps of 32 keys.  (LEAD, LEAST)
+// = (4, 4): 32 tokens over 256 keys 12.9 us, over 3126 18.8, four 128-token chunks 51;
+// (2, 3): 12.3, 21.4, 57; (4, 3): 12, 21, 51; (4, 8): 18.9, 20.2, 51.
 typedef Deal<kStep, 4, 4> ManyDeal;
 
 // Units of all requests, and those before this thread's requests (a contiguous
@@ -484,7 +493,7 @@ struct Rows {
 // Stores and loads that other XCDs' workgroups see and are seen by: agent-scope
 // accesses, which pass the XCD's own cache by.  (With plain ones between
 // __threadfence() calls every workgroup wrote its XCD's cache back and emptied it:
-// 64 ragged requests 182 us, against 60 with a second kernel.)
+// 64 ragged requests took three times as long as with a second kernel.)
 __device__ __forceinline__ void put2(float* p, float x, float y) {
   const uint64_t v = (uint64_t)__float_as_uint(y) << 32 | __float_as_uint(x);
   __hip_atomic_store(reinterpret_cast<uint64_t*>(p), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -797,7 +806,8 @@ typedef __attribute__((address_space(3))) s16x4_t lds_s16x4;
 // safe, as more are in flight than it counts; nothing is written to a register.
 // The wait states: of m0 (1), and of scalars that a vector instruction wrote (5),
 // which the compiler does not see to inside the block.  (With the builtin every step
-// waited for the loads of the steps to come: 512 rows over 6100 keys 100 us for 59.)
+// waited for the loads of the steps to come: four 128-token chunks took 1.7 times as
+// long.)
 __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsigned to) {
   asm volatile("s_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"{m0}"(to), "v"(off), "s"(base)
                : "memory");
@@ -805,10 +815,16 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsi
 
 // More rows: each wave has 16 NT of the workgroup's 64 NT, and the keys go through
 // a ring in LDS, kRing - 1 steps of 32 on their way: the loads take a few
-// thousand cycles, a step about one (one step ahead, through registers: 67 us for
-// 512 rows over 6100 keys).  A row's 16-byte chunks are permuted so
-// that neither the reads of a chunk down the rows (K: ^ row) nor those of two
-// chunks of eight rows (V: ^ 2 row) meet in a bank.
+// thousand cycles (with one step ahead, through registers, four 128-token chunks
+// took 12% longer).  A row's 16-byte chunks are permuted so that neither the reads
+// of a chunk down the rows (K: ^ row) nor those of two chunks of eight rows (V: ^ 2
+// row) meet in a bank.
+// What bounds it: of a step's 4000 cycles for two waves of a SIMD the matrix
+// instructions take 1540 (48 a wave, the second product twice) and the vector ones
+// 1880 (190 a wave, 16 of them exponentials), and they hardly overlap.  Matrix and
+// vector instructions in turn, priorities, the next K read early, a barrier for two
+// steps, eight waves that halve the parts: none was faster (240 us for 128 tokens
+// over 65536 keys stayed within 2%, the last cost the chunks 7 us).
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel(AttnArgs a) {
   typedef Rows<D, NT, true> R;
