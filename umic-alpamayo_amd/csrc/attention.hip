@@ -308,8 +308,14 @@ struct Rows {
   u32x4 q[NT][KK];
   int lim[NT];  // keys below it are seen
   int lo, hi;   // keys below lo are seen by all rows, keys from hi on by none
-  float m[NT], l[NT];
+  // p is exp2(c score - base), or 0 times it: nb = -base, 0 until a key is seen; what
+  // passes top is followed
+  float nb[NT], top[NT], l[NT];
   f32x4_t acc[NT][DV];
+
+  __device__ __forceinline__ float max_of(int nt) const {
+    return top[nt] == -__builtin_inff() ? top[nt] : -nb[nt];
+  }
 
   __device__ __forceinline__ void load_q(const AttnArgs& a, const Segment& s, int r0, int n16,
                                          int g4) {
@@ -334,8 +340,8 @@ struct Rows {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = -__builtin_inff();
-      l[nt] = 0.0f;
+      nb[nt] = l[nt] = 0.0f;
+      top[nt] = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0, 0, 0, 0};
     }
@@ -378,46 +384,58 @@ struct Rows {
       v[x] &= TURNED ? (keep[j] & 0xffffu) | (keep[j + 1] & 0xffff0000u) : keep[j];
     }
   }
-  // p of the scores, in two bf16 parts.  m follows a row's maximum only when it is
-  // passed by kSlack: p stays below 2^kSlack, and the outputs are rescaled a few
+  // p of the scores, in two bf16 parts.  The base follows a row's maximum only when it
+  // is passed by kSlack: p stays below 2^kSlack, and the outputs are rescaled a few
   // times in all.
   __device__ __forceinline__ void weights(const f32x4_t (&sc)[NT][2], float c, u32x4 (&ph)[NT],
                                           u32x4 (&pl)[NT]) {
-    float mx[NT];
+    float x[NT][8];
+    auto most = [&](int nt) {  // of exponents, which need no quieting of NaNs first
+      const float(&y)[8] = x[nt];
+      return fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])),
+                   fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+    };
+    auto exponents = [&](int nt) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x[nt][j] = __builtin_fmaf(sc[nt][j >> 2][j & 3], c, nb[nt]);
+    };
     bool up = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const f32x4_t &x = sc[nt][0], &y = sc[nt][1];
-      mx[nt] = fmaxf(fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])),
-                     fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3]))) * c;
-      up |= mx[nt] > m[nt] + kSlack;
+      exponents(nt);
+      up |= most(nt) > top[nt];
     }
     if (__any(up)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        mx[nt] = fmaxf(mx[nt], __shfl_xor(mx[nt], 16, kWave));
-        mx[nt] = fmaxf(mx[nt], __shfl_xor(mx[nt], 32, kWave));
-        const float to = fmaxf(m[nt], mx[nt]);
-        const float al = to == -__builtin_inff() ? 1.0f : __builtin_amdgcn_exp2f(m[nt] - to);
-        m[nt] = to;
-        l[nt] *= al;
+        const float from = max_of(nt);
+        float mx = most(nt) - nb[nt];
+        mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
+        mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
+        const float to = fmaxf(from, mx);
+        if (to > -__builtin_inff()) {
+          const float al = __builtin_amdgcn_exp2f(from - to);
+          nb[nt] = -to;
+          top[nt] = kSlack;
+          l[nt] *= al;
 #pragma unroll
-        for (int e = 0; e < DV; ++e) acc[nt][e] *= al;
+          for (int e = 0; e < DV; ++e) acc[nt][e] *= al;
+        }
+        exponents(nt);
       }
     }
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const float base = m[nt] == -__builtin_inff() ? 0.0f : m[nt];
-      float x[8], y[8];
+      float y[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        x[j] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[nt][j >> 2][j & 3], c, -base));
-        l[nt] += x[j];
+        x[nt][j] = __builtin_amdgcn_exp2f(x[nt][j]);
+        l[nt] += x[nt][j];
       }
-      ph[nt] = pack8(x);
+      ph[nt] = pack8(x[nt]);
       unpack8(ph[nt], y);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = x[j] - y[j];
+      for (int j = 0; j < 8; ++j) y[j] = x[nt][j] - y[j];
       pl[nt] = pack8(y);
     }
   }
@@ -670,10 +688,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
     load_v(a, here);
     r.load_q(a, seg, 0, n16, g4);
     for (bool go = true; go;) {
-      go = walk.next(a, nxt);
-      const Place turn = go ? first_of(a, nxt) : here;
+      go = walk.next(args_again(), nxt);
+      const Place turn = go ? first_of(args_again(), nxt) : here;
       bool turned = false;  // the next segment's keys are on their way
-      const Keys keys = keys_of(a, seg);
+      const Keys keys = keys_of(args_again(), seg);
       r.clear();
       for (int t = seg.t0; t < seg.t1; ++t) {
         const int k0 = t * kTile + wave * kStep, k1 = k0 + kTile;
@@ -710,7 +728,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
       r.l[0] += __shfl_xor(r.l[0], 16, kWave);
       r.l[0] += __shfl_xor(r.l[0], 32, kWave);
       if (g4 == 0) {
-        ml[wave][n16][0] = r.m[0];
+        ml[wave][n16][0] = r.max_of(0);
         ml[wave][n16][1] = r.l[0];
       }
 #pragma unroll
@@ -783,7 +801,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
       }
     }
   }
-  if (a.counters) zero_rows<D>(a);
+  const AttnArgs z = args_again();
+  if (z.counters) zero_rows<D>(z);
 }
 
 // All but LEFT of this wave's loads have landed and its LDS reads are done; then
@@ -981,7 +1000,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
 #pragma unroll
         for (int e = 0; e < DV; ++e) p[e * kWave] = r.acc[nt][e];
         if (g4 == 0) {
-          args.part_ml[(tile * 16 + n16) * 2] = r.m[nt];
+          args.part_ml[(tile * 16 + n16) * 2] = r.max_of(nt);
           args.part_ml[(tile * 16 + n16) * 2 + 1] = sum;
         }
       }
