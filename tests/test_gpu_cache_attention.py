@@ -94,6 +94,19 @@ def test_fewer_new_tokens_than_rows(causal):
         assert not got[b, m:].any()
 
 
+@pytest.mark.parametrize("S,Hq,Hk,D,page", [(80, 8, 2, 128, 64), (70, 14, 2, 64, 16), (40, 4, 2, 256, 128),
+                                            (257, 2, 2, 128, 0)])
+def test_several_row_blocks(S, Hq, Hk, D, page):
+    """More query rows than a workgroup has, over requests that many workgroups share."""
+    lens, fresh = [2900, S, 0, S + 31, 3 * S, 1500], [S, S, 0, S // 3, 0, 5]
+    q, k, v, table = make(lens, S, Hq, Hk, D, page, seed=S)
+    n = torch.tensor(fresh, dtype=torch.int32, device=DEV)
+    got = call(q, k, v, lens, table, q_len=n)
+    ref.check_attention(got, *ref.attention(q, k, v, lens, table, q_len=fresh))
+    got = call(q, k, v, lens, table, causal=False)
+    ref.check_attention(got, *ref.attention(q, k, v, lens, table, causal=False))
+
+
 def test_many_requests_of_all_lengths():
     rng = random.Random(4)
     lens = [rng.choice((0, 1, 130, rng.randint(0, 700))) for _ in range(610)]
@@ -236,9 +249,10 @@ def test_results_repeat_and_streams_agree():
         assert torch.equal(o, want)
 
 
-def test_two_captured_calls_share_nothing():
+@pytest.mark.parametrize("S", [2, 20])
+def test_two_captured_calls_share_nothing(S):
     lens = [[300, 41], [64, 1111]]
-    args = [make(x, 2, 8, 2, 128, 16, seed=i) for i, x in enumerate(lens)]
+    args = [make(x, S, 8, 2, 128, 16, seed=i) for i, x in enumerate(lens)]
     ns = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in lens]
     call(*args[0][:3], lens[0], args[0][3])
     torch.cuda.synchronize()
