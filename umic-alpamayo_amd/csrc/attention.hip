@@ -28,10 +28,10 @@
 // to 16 rows and with counters to find that out, else by a second kernel.
 //
 // Measured, 32 query heads over 8 of 128: a token of two requests of 131001 keys each
-// 171 us (6.3 TB/s), of 64 ragged requests up to 8192 keys 55 (4.6 TB/s), of one
-// request of 3100 keys 10.4: 4.5 until its first keys are there, 1.7 for them, 4 to
-// join 25 parts.  128 tokens over 65536 keys 240 us (577 TFLOP/s); four 128-token
-// chunks 47, of which the second kernel takes 13 for 41 MB of parts.
+// 173 us (6.2 TB/s), of 64 ragged requests up to 8192 keys 54 (4.7 TB/s), of one
+// request of 3100 keys 9.5: 4 until its first keys are there, 1.7 for them, 3 to join
+// 25 parts.  128 tokens over 65536 keys 230 us (595 TFLOP/s); four 128-token chunks
+// 46, of which the second kernel takes 13 for 41 MB of parts.
 #include <algorithm>
 
 #include "common.hpp"
@@ -845,8 +845,8 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsi
 // instructions take 1540 (48 a wave, the second product twice) and the vector ones
 // 1880 (190 a wave, 16 of them exponentials), and they hardly overlap.  Matrix and
 // vector instructions in turn, priorities, the next K read early, a barrier for two
-// steps, eight waves that halve the parts: none was faster (240 us for 128 tokens
-// over 65536 keys stayed within 2%, the last cost the chunks 7 us).
+// steps, eight waves that halve the parts: none was faster (128 tokens over 65536
+// keys stayed within 2%, the last cost the chunks 7 us).
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel(AttnArgs a) {
   typedef Rows<D, NT, true> R;
