@@ -17,16 +17,23 @@ def require_device(*tensors: torch.Tensor) -> None:
     ineligible inputs to the eager module is the injection layer's decision
     (umic.integrate), made before a wrapper is called.
     """
+    dev = tensors[0].get_device()
+    for t in tensors:
+        if t.dtype is not _BF16 or t.get_device() != dev or not t.is_cuda:
+            _refuse(tensors)
+    _lib.lib()  # raises UmicLibraryError if libumic_hip.so is unavailable
+
+
+def _refuse(tensors) -> None:
+    """Say what is wrong with one of ``require_device``'s tensors."""
     for t in tensors:
         if not t.is_cuda:
             raise ValueError(f"umic kernels run on the GPU; got a tensor on {t.device}")
         if t.dtype is not _BF16:
             raise TypeError(f"umic kernels take bfloat16 tensors; got {t.dtype}")
-    dev = tensors[0].get_device()
     for t in tensors[1:]:
-        if t.get_device() != dev:
+        if t.get_device() != tensors[0].get_device():
             raise ValueError(f"tensors on different devices: {tensors[0].device} vs {t.device}")
-    _lib.lib()  # raises UmicLibraryError if libumic_hip.so is unavailable
 
 
 def grad_needed(*tensors) -> bool:

@@ -28,6 +28,10 @@ def _workspace_bytes(dev: int, S: int, Hq: int, Hk: int, D: int) -> int:
     return _lib.lib().umic_cache_attention_workspace_bytes(S, Hq, Hk, D)
 
 
+# Asked at every call: without the public function's own look at the build.
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
+                     None) or torch.cuda.is_current_stream_capturing
+
 # (counters, workspace) of each (device, stream): calls on one stream do not
 # overlap, and every call leaves the counters at zero.  A captured call has a
 # workspace of its own and no counters, as its graph may run beside anything.
@@ -35,7 +39,7 @@ _SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
 
 
 def _scratch(q: torch.Tensor, dev: int, stream: int, need: int) -> tuple[int | None, torch.Tensor]:
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         return None, torch.empty(need, dtype=torch.uint8, device=q.device)
     held = _SCRATCH.get((dev, stream))
     if held is None or held[1].numel() < need:
@@ -98,11 +102,12 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if grad_needed(q, k_cache, v_cache):
         raise RuntimeError("cache_attention: the kernel has no backward; call it under "
                            "torch.no_grad()")
-    if q.dim() != 4 or k_cache.dim() != 4 or not _layout_ok(k_cache, v_cache):
-        raise ValueError(f"cache_attention: unsupported layout q{tuple(q.shape)} "
-                         f"cache{tuple(k_cache.shape)} (head sizes {HEAD_DIMS})")
-    B, Hq, S, D = q.shape
-    blocks, Hk, rows, Dk = k_cache.shape
+    shape, cshape = q.shape, k_cache.shape
+    if len(shape) != 4 or len(cshape) != 4 or not _layout_ok(k_cache, v_cache):
+        raise ValueError(f"cache_attention: unsupported layout q{tuple(shape)} "
+                         f"cache{tuple(cshape)} (head sizes {HEAD_DIMS})")
+    B, Hq, S, D = shape
+    blocks, Hk, rows, Dk = cshape
     if Dk != D or Hk == 0 or Hq % Hk:
         raise ValueError(f"cache_attention: {Hq} heads of {D} over a cache of {Hk} of {Dk}")
     dev = q.get_device()
@@ -129,7 +134,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     if not _chunks_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty((B, S, Hq, D), dtype=_BF16, device=q.device)
+        out = torch.empty(B, S, Hq, D, dtype=_BF16, device=q.device)
         os_ = (S * Hq * D, Hq * D, D)
     else:
         require_device(q, out)

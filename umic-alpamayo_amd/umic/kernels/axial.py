@@ -99,27 +99,31 @@ class AxisPlan:
         return cls(torch.cat((inv, inv)), [0] * quarter + [1] * quarter, device=device)
 
 
-def _ready(t: torch.Tensor) -> torch.Tensor:
+def _ready(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
     """t, or a copy with the rows the kernel reads: [T, H, D], contiguous, in 8-byte
-    chunks."""
+    chunks; and its strides."""
     a, b, inner = t.stride()
     if inner == 1 and not ((a | b) & 3 or t.data_ptr() & 7):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return t, a, b
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
 def _check(who: str, q, k, positions, plan: AxisPlan, norm) -> None:
-    if grad_needed(q, k) or norm is not None and grad_needed(norm[0], norm[1]):
+    if torch.is_grad_enabled() and (grad_needed(q, k) or norm is not None
+                                    and grad_needed(norm[0], norm[1])):
         raise RuntimeError(f"{who}: the kernel has no backward; call it under torch.no_grad()")
-    T, D, dev = q.shape[0], plan.head_dim, q.get_device()
-    if q.dim() != 3 or k.dim() != 3 or k.shape[0] != T or q.shape[2] != D or k.shape[2] != D:
-        raise ValueError(f"{who}: q {tuple(q.shape)} and k {tuple(k.shape)} must be [T, heads, {D}]")
+    qs, ks, D, dev = q.shape, k.shape, plan.head_dim, q.get_device()
+    T = qs[0] if qs else 0
+    if len(qs) != 3 or len(ks) != 3 or ks[0] != T or qs[2] != D or ks[2] != D:
+        raise ValueError(f"{who}: q {tuple(qs)} and k {tuple(ks)} must be [T, heads, {D}]")
     if D % 8 or D > MAX_HEAD_DIM:
         raise ValueError(f"{who}: heads of {D} (multiples of 8 up to {MAX_HEAD_DIM})")
-    if (positions.dtype is not torch.int64 or positions.dim() != 2 or positions.shape[1] != T
-            or positions.shape[0] < plan.axes or positions.get_device() != dev):
+    ps = positions.shape
+    if (positions.dtype is not torch.int64 or len(ps) != 2 or ps[1] != T or ps[0] < plan.axes
+            or positions.get_device() != dev):
         raise ValueError(f"{who}: positions must be int64 [{plan.axes} axes, {T}] on q's device, "
-                         f"got {positions.dtype} {tuple(positions.shape)}")
+                         f"got {positions.dtype} {tuple(ps)}")
     if plan.turn.get_device() != dev:
         raise ValueError(f"{who}: the plan is on {plan.turn.device}, q on {q.device}")
 
@@ -142,17 +146,17 @@ def rotate(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, plan: Axis
     first."""
     require_device(q, k, *(norm[:2] if norm is not None else ()))
     _check("rotate", q, k, positions, plan, norm)
-    q, k = _ready(q), _ready(k)
+    (q, q0, q1), (k, k0, k1) = _ready(q), _ready(k)
     T, Hq, D = q.shape
     Hk = k.shape[1]
-    q_out, k_out = (torch.empty((T, h, D), dtype=torch.bfloat16, device=q.device)
+    q_out, k_out = (torch.empty(T, h, D, dtype=torch.bfloat16, device=q.device)
                     for h in (Hq, Hk))
     with _lib.device_of(q):
         _lib.call("umic_axial_rope_bf16", q.data_ptr(), k.data_ptr(), q_out.data_ptr(),
                   k_out.data_ptr(), positions.data_ptr(), plan.turn.data_ptr(),
                   plan.axis.data_ptr(), plan.scale, *_norm_args("rotate", norm, D), T, Hq, Hk, D,
-                  positions.shape[0], *positions.stride(), *q.stride()[:2], *k.stride()[:2],
-                  Hq * D, D, Hk * D, D, _lib.stream_of(q))
+                  positions.shape[0], *positions.stride(), q0, q1, k0, k1, Hq * D, D, Hk * D, D,
+                  _lib.stream_of(q))
     return q_out, k_out
 
 
@@ -166,7 +170,7 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     _check("rotate_append", q, k, positions, plan, norm)
     T, Hq, D = q.shape
     Hk = k.shape[1]
-    if v.shape != k.shape or grad_needed(v):
+    if v.shape != k.shape or torch.is_grad_enabled() and grad_needed(v):
         raise ValueError(f"rotate_append: v {tuple(v.shape)} must be like k {tuple(k.shape)}, "
                          "without a gradient")
     shape, cst = k_pages.shape, k_pages.stride()
@@ -178,13 +182,13 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
             or slots.get_device() != q.get_device() or not slots.is_contiguous()):
         raise ValueError(f"rotate_append: slots must be a contiguous int64 vector of {T} on q's "
                          "device")
-    q, k, v = _ready(q), _ready(k), _ready(v)
-    q_out = torch.empty((T, Hq, D), dtype=torch.bfloat16, device=q.device)
+    (q, q0, q1), (k, k0, k1), (v, v0, v1) = _ready(q), _ready(k), _ready(v)
+    q_out = torch.empty(T, Hq, D, dtype=torch.bfloat16, device=q.device)
     with _lib.device_of(q):
         _lib.call("umic_axial_rope_append_bf16", q.data_ptr(), k.data_ptr(), v.data_ptr(),
                   q_out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), positions.data_ptr(),
                   plan.turn.data_ptr(), plan.axis.data_ptr(), slots.data_ptr(), plan.scale,
-                  *_norm_args("rotate_append", norm, D), T, Hq, Hk, D, positions.shape[0], *positions.stride(),
-                  *q.stride()[:2], *k.stride()[:2], *v.stride()[:2], Hq * D, D, *cst[:3], shape[0],
-                  shape[2], _lib.stream_of(q))
+                  *_norm_args("rotate_append", norm, D), T, Hq, Hk, D, positions.shape[0],
+                  *positions.stride(), q0, q1, k0, k1, v0, v1, Hq * D, D, cst[0], cst[1], cst[2],
+                  shape[0], shape[2], _lib.stream_of(q))
     return q_out

@@ -105,7 +105,7 @@ def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
     _lib.lib()
     if out is None:
         ints = torch.empty(2 * R + 5, dtype=_I32, device=kv_len.device)
-        longs = torch.empty((2, tokens), dtype=_I64, device=kv_len.device)
+        longs = torch.empty(2, tokens, dtype=_I64, device=kv_len.device)
         out = PageStep(*ints.split_with_sizes((R, 4, R + 1)), *longs.unbind())
     else:
         for name, n, dtype in (("kv_len", R, _I32), ("cursor", 4, _I32), ("starts", R + 1, _I32),
