@@ -843,8 +843,8 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsi
 // row) meet in a bank.
 // What bounds it: of a step's 4000 cycles for two waves of a SIMD the matrix
 // instructions take 1540 (48 a wave, the second product twice) and the vector ones
-// 1880 (190 a wave, 16 of them exponentials), and they hardly overlap.  Matrix and
-// vector instructions in turn, priorities, the next K read early, a barrier for two
+// 1880 (190 a wave, 16 of them exponentials), which run beside the former for a
+// quarter of their time.  Matrix and vector instructions in turn, priorities, the next K read early, a barrier for two
 // steps, eight waves that halve the parts: none was faster (128 tokens over 65536
 // keys stayed within 2%, the last cost the chunks 7 us).
 template <int D, int NT>
