@@ -231,7 +231,9 @@ struct Walk {
 
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
-__device__ __forceinline__ bf16x8_t as_bf(const u32x4& v) { return __builtin_bit_cast(bf16x8_t, v); }
+__device__ __forceinline__ bf16x8_t as_bf(const u32x4& v) {
+  return __builtin_bit_cast(bf16x8_t, v);
+}
 
 // The low (hi: high) halves of two words side by side.
 __device__ __forceinline__ uint32_t pair_lo(uint32_t a, uint32_t b) {
@@ -800,7 +802,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         if (threadIdx.x == 0) args.counters[v0] = 0;  // for the next call
         const int b = uniform(kept[i].b), h = uniform(kept[i].h), fresh = uniform(kept[i].fresh);
         for (int row = wave; row < rows; row += kWaves)
-          join_row<D, true>(args, v0, v1, row, quot(row, args.G) >= fresh, out_row(args, b, h, row));
+          join_row<D, true>(args, v0, v1, row, quot(row, args.G) >= fresh,
+                            out_row(args, b, h, row));
       }
     }
   }
@@ -844,9 +847,10 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsi
 // What bounds it: of a step's 4000 cycles for two waves of a SIMD the matrix
 // instructions take 1540 (48 a wave, the second product twice) and the vector ones
 // 1880 (190 a wave, 16 of them exponentials), which run beside the former for a
-// quarter of their time.  Matrix and vector instructions in turn, priorities, the next K read early, a barrier for two
-// steps, eight waves that halve the parts: none was faster (128 tokens over 65536
-// keys stayed within 2%, the last cost the chunks 7 us).
+// quarter of their time.  Matrix and vector instructions in turn, priorities, the
+// next K read early, a barrier for two steps, eight waves that halve the parts: none
+// was faster (128 tokens over 65536 keys stayed within 2%, the last cost the chunks
+// 7 us).
 template <int D, int NT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel(AttnArgs a) {
   typedef Rows<D, NT, true> R;
