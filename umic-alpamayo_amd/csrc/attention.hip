@@ -599,16 +599,16 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int 
   if (sub == 0) *reinterpret_cast<u32x2*>(op + col) = out;
 }
 
-// Requests without a key: zeros.
+// Requests without a key: zeros (of up to 16 rows a key head: their count is 32-bit).
 template <int D>
 __device__ __forceinline__ void zero_rows(const AttnArgs& a) {
-  const int chunks = D / 8;
+  constexpr int chunks = D / 8;
   for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
     if (len_of(a, b)) continue;
-    const int64_t n = (int64_t)a.S * a.Hk * a.G * chunks;
-    for (int64_t i = threadIdx.x; i < n; i += kThreads) {
-      const int c = (int)(i % chunks), row = (int)(i / chunks);
-      const int t = row / (a.Hk * a.G), h = row - t * (a.Hk * a.G);
+    const int heads = a.Hk * a.G;
+    for (int i = threadIdx.x; i < a.S * heads * chunks; i += kThreads) {
+      const int c = i & (chunks - 1), row = i / chunks;
+      const int t = quot(row, heads), h = row - t * heads;
       uint16_t* op = a.out + b * a.o_sb + t * a.o_ss + (int64_t)h * a.o_sh + c * 8;
       *reinterpret_cast<u32x4*>(op) = u32x4{0, 0, 0, 0};
     }
