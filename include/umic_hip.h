@@ -512,8 +512,11 @@ int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, voi
  * row j % block_rows of block table[b * table_ld + j / block_rows], table_w
  * entries a request; block_rows a power of two from 16; an entry outside [0,
  * blocks) is read as keys that are not there.  Rows past n_b are not used,
- * whatever they hold.  A later new token's v that is infinite or NaN does not
- * reach the rows that do not see it.
+ * whatever they hold.  A v that is infinite or NaN reaches the rows that see its
+ * key, whatever its weight (all are above 0): their column is the sum of such
+ * values; rows that do not see it (an earlier new token's) are as without it.  The
+ * sums of p v are fp32 ones, with weights up to 2^8: finite values of more than
+ * 2^119 / n_b can overflow them.
  * D: 64, 128 or 256; strides multiples of 8, pointers 16-byte aligned (else
  * UMIC_ERR_UNSUPPORTED).  |scale| <= 2^127.  workspace: umic_cache_attention_workspace_bytes, for
  * this call alone until it has run (contents need not be kept or cleared).

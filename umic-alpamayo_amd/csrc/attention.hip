@@ -297,6 +297,53 @@ __device__ __forceinline__ Place place_of(const AttnArgs& a, const Keys& s, int 
   return p;
 }
 
+__device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __builtin_inff(); }
+
+// Values that are not finite.  Every key a row sees has a weight above 0, so an
+// infinite v makes its column infinite, and two of both signs, or a NaN, make it NaN.
+// The products do not give that: the weight's low part is negative or 0, and 0 and
+// what underflows times infinity is NaN.  But whatever they give is not finite, and
+// stays so: where a row's o (of N groups of four columns, col + STEP g ..) is not, the
+// values among keys [from, to) below lim that are not finite take its place.  (Sums of
+// finite values that overflowed have none, and stay.)
+template <int N, int STEP>
+__device__ __forceinline__ void restore(f32x4_t (&o)[N], const AttnArgs& a, const Keys& s, int from,
+                                        int to, int lim, int col) {
+  float none = 0.0f;  // NaN: not all are finite
+#pragma unroll
+  for (int g = 0; g < N; ++g)
+#pragma unroll
+    for (int y = 0; y < 4; ++y) none = __builtin_fmaf(o[g][y], 0.0f, none);
+  if (!__any(none != none)) return;
+  f32x4_t sum[N] = {};
+#pragma unroll 1
+  for (int k0 = from; k0 < to; k0 += kStep) {
+    const Place p = place_of(a, s, k0, blocks_of(a, s, k0));
+#pragma unroll 1
+    for (int key = 0; key < kStep; ++key) {
+      const int at = key & 15;
+      if (at >= (key < 16 ? p.n[0] : p.n[1])) continue;
+      const uint16_t* vp = a.v + (key < 16 ? p.at[0] : p.at[1]) + (int64_t)at * a.c_ss + col;
+      u32x2 raw[N];
+#pragma unroll
+      for (int g = 0; g < N; ++g) raw[g] = *reinterpret_cast<const u32x2*>(vp + STEP * g);
+#pragma unroll
+      for (int g = 0; g < N; ++g) {
+        float x[4];
+        unpack4(raw[g], x);
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (k0 + key < lim && !finite(x[y])) sum[g][y] += x[y];
+      }
+    }
+  }
+#pragma unroll
+  for (int g = 0; g < N; ++g)
+#pragma unroll
+    for (int y = 0; y < 4; ++y)
+      if (sum[g][y] != 0.0f) o[g][y] = sum[g][y];
+}
+
 // A wave's rows r0 .. of a segment (row r is head r % G of new token r / G), NT
 // tiles of 16, a lane's being n16 of each; and what a step of 32 keys does to
 // them.  The V operand of output tile e holds for a lane one column of 8 keys, j =
@@ -446,10 +493,9 @@ struct Rows {
   }
   // Where some rows do not see some of the keys, p = 0 has to hide a v that is not
   // finite, and 0 * inf is not 0: such elements leave the product, and the rows that
-  // see them get theirs one by one.
-  __device__ __forceinline__ void hide(uint32_t (&v)[VR], const u32x4 (&ph)[NT],
-                                       const u32x4 (&pl)[NT], const AttnArgs& a, const Place& p,
-                                       int k0, int n16, int g4) {
+  // see them are marked by them, for `restore`.
+  __device__ __forceinline__ void hide(uint32_t (&v)[VR], const AttnArgs& a, const Place& p, int k0,
+                                       int g4) {
     // exponents of ones, both halves of a word at once: bits 15 and 31
     auto wild = [](uint32_t x) { return (x & 0x7f807f80u) + 0x00800080u; };
     uint32_t any = 0;
@@ -460,28 +506,19 @@ struct Rows {
     for (int w = 0; w < VR; ++w) v[w] &= ~((wild(v[w]) >> 15 & 0x00010001u) * 0xffffu);
 #pragma unroll 1
     for (int key = 0; key < kStep; ++key) {
-      const int at = key & 15, j = (key >> 4) * 4 + (at & 3);
+      const int at = key & 15;
       if (at >= (key < 16 ? p.n[0] : p.n[1])) continue;
       const uint16_t* vp = a.v + (key < 16 ? p.at[0] : p.at[1]) + (int64_t)at * a.c_ss;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        uint32_t wh = ph[nt][0], wl = pl[nt][0];
-#pragma unroll
-        for (int y = 1; y < 4; ++y) {
-          wh = (j >> 1) == y ? ph[nt][y] : wh;
-          wl = (j >> 1) == y ? pl[nt][y] : wl;
-        }
-        float w = (j & 1) ? bf_hi(wh) + bf_hi(wl) : bf_lo(wh) + bf_lo(wl);
-        w = __shfl(w, n16 + 16 * (at >> 2), kWave);
+      for (int nt = 0; nt < NT; ++nt)
         if (k0 + key < lim[nt])
 #pragma unroll
           for (int e = 0; e < DV; ++e)
 #pragma unroll
             for (int y = 0; y < 4; ++y) {
               const float x = bf2f(vp[column(e, y, g4)]);
-              if (!(__builtin_fabsf(x) < __builtin_inff())) acc[nt][e][y] += w * x;
+              if (!finite(x)) acc[nt][e][y] += x;
             }
-      }
     }
   }
   __device__ __forceinline__ void product(const uint32_t (&v)[VR], const u32x4 (&ph)[NT],
@@ -592,6 +629,23 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int 
   for (int k = kLanes; k < kWave; k <<= 1)
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[c] += __shfl_xor(o[c], k, kWave);
+  if (__any(!(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3])))) {
+    f32x4_t whole = {0, 0, 0, 0};  // of the parts that are not finite, whatever their weight
+#pragma unroll 1
+    for (int i = 0; i < n; i += kAhead * kParts) {
+      load(i);
+#pragma unroll
+      for (int j = 0; j < kAhead; ++j)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) whole[c] += finite(x[j][c]) ? 0.0f : x[j][c];
+    }
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int k = kLanes; k < kWave; k <<= 1) whole[c] += __shfl_xor(whole[c], k, kWave);
+      if (whole[c] != 0.0f) o[c] = whole[c];
+    }
+  }
   sum = group_sum<kWave>(sum);
   if (sum == 0.0f) none = true;
   const u32x2 out = {none ? 0 : pack2(o[0] / sum, o[1] / sum),
@@ -712,7 +766,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         if (edge) r.mask(sc, vr, here.n, k0, g4);
         u32x4 ph[1], pl[1];
         r.weights(sc, a.c, ph, pl);
-        if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
+        if (edge && r.hi > r.lo) r.hide(vr, a, here, k0, g4);
         r.product(vr, ph, pl);
         if (more || go) load_v(a, next);
         here = next;
@@ -748,25 +802,28 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
 #pragma unroll
         for (int w = 1; w < kWaves; ++w) mx = fmaxf(mx, ml[w][rr][0]);
         const float base = mx == -__builtin_inff() ? 0.0f : mx;
-        float o[DV] = {};
+        f32x4_t o[DV / 4] = {};
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
           const float f = __builtin_amdgcn_exp2f(ml[w][rr][0] - base);
           sum += ml[w][rr][1] * f;
 #pragma unroll
-          for (int e = 0; e < DV; ++e) o[e] += acc_lds[w][rr][col + e] * f;
+          for (int e = 0; e < DV; ++e) o[e / 4][e % 4] += acc_lds[w][rr][col + e] * f;
         }
+        const int lim = args.causal ? seg.len - seg.fresh + quot(rr, args.G) + 1 : seg.len;
+        restore<DV / 4, 4>(o, args, keys_of(args, seg), seg.t0 * kTile, seg.t1 * kTile, lim, col);
         if (whole) {
           const bool none = quot(rr, args.G) >= seg.fresh || sum == 0.0f;
           const float inv = 1.0f / sum;
           uint32_t* op = reinterpret_cast<uint32_t*>(out_row(args, seg.b, seg.h, rr) + col);
 #pragma unroll
-          for (int w = 0; w < VW; ++w) op[w] = none ? 0 : pack2(o[2 * w] * inv, o[2 * w + 1] * inv);
+          for (int w = 0; w < VW; ++w) op[w] = none ? 0 : pack2(o[w / 2][w % 2 * 2] * inv, o[w / 2][w % 2 * 2 + 1] * inv);
         } else {
           const int64_t at = (int64_t)slot * 16 + rr;
 #pragma unroll
-          for (int e = 0; e < DV; e += 2) put2(args.part + at * D + col + e, o[e], o[e + 1]);
+          for (int e = 0; e < DV; e += 2)
+            put2(args.part + at * D + col + e, o[e / 4][e % 4], o[e / 4][e % 4 + 1]);
           if (col == 0) put2(args.part_ml + at * 2, mx, sum);
         }
       }
@@ -976,12 +1033,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       }
       u32x4 ph[NT], pl[NT];
       r.weights(sc, a.c, ph, pl);
-      if (edge && r.hi > r.lo) r.hide(vr, ph, pl, a, here, k0, n16, g4);
+      if (edge && r.hi > r.lo) r.hide(vr, a, here, k0, g4);
       r.product(vr, ph, pl);
     }
     const AttnArgs args = args_again();
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+      restore<DV, 16>(r.acc[nt], args, keys_of(args, seg), seg.t0 * kStep, t1 * kStep, r.lim[nt],
+                      4 * g4);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float sum = r.l[nt];
@@ -1109,6 +1170,19 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
         sum += l[j] * f;
         o += x[j] * f;
       }
+  }
+  if (!(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3]))) {
+    f32x4_t whole = {0, 0, 0, 0};  // as in join_row
+#pragma unroll 1
+    for (int i = 0; i < n; ++i)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const float y = part[tile_of(i) * 4 * D][c];
+        whole[c] += finite(y) ? 0.0f : y;
+      }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if (whole[c] != 0.0f) o[c] = whole[c];
   }
   const bool none = sum == 0.0f || quot(row, a.G) >= new_of(a, b);
   const u32x2 x = {none ? 0 : pack2(o[0] / sum, o[1] / sum),
