@@ -114,3 +114,16 @@ def test_captured(n, S):
         g.replay()
         torch.cuda.synchronize()
         assert torch.equal(out.nan_to_num(7.0, 8.0, 9.0), eager.nan_to_num(7.0, 8.0, 9.0))
+
+
+@pytest.mark.parametrize("S,Hq,Hk,D", [(2, 32, 1, 128), (5, 32, 1, 128), (3, 16, 1, 64), (2, 48, 3, 256)])
+@pytest.mark.parametrize("bad", [INF, NAN])
+def test_hidden_where_a_wave_has_one_token(S, Hq, Hk, D, bad):
+    """Sixteen query heads and more a key head: all rows of a wave see the same keys, and not the
+    later new tokens' values."""
+    n = 150
+    q, k, v, table = make([n], S, Hq, Hk, D, 16, seed=S)
+    rows_of(v, table, n - 1)[0, 3:9] = bad
+    got = call(q, k, v, [n], table)
+    assert torch.isfinite(got[0, :S - 1]).all()
+    check(got, *expected(q, k, v, n, table))

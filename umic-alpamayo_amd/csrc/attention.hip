@@ -766,7 +766,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         if (edge) r.mask(sc, vr, here.n, k0, g4);
         u32x4 ph[1], pl[1];
         r.weights(sc, a.c, ph, pl);
-        if (edge && r.hi > r.lo) r.hide(vr, a, here, k0, g4);
+        if (edge && r.lo < seg.len) r.hide(vr, a, here, k0, g4);
         r.product(vr, ph, pl);
         if (more || go) load_v(a, next);
         here = next;
@@ -1033,7 +1033,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
       }
       u32x4 ph[NT], pl[NT];
       r.weights(sc, a.c, ph, pl);
-      if (edge && r.hi > r.lo) r.hide(vr, a, here, k0, g4);
+      if (edge && r.lo < seg.len) r.hide(vr, a, here, k0, g4);
       r.product(vr, ph, pl);
     }
     const AttnArgs args = args_again();
