@@ -360,13 +360,13 @@ struct Rows {
   u32x4 q[NT][KK];
   int lim[NT];  // keys below it are seen
   int lo, hi;   // keys below lo are seen by all rows, keys from hi on by none
-  // p is exp2(c score - base), or 0 times it: nb = -base, 0 until a key is seen; what
-  // passes top is followed
-  float nb[NT], top[NT], l[NT];
+  // p is exp2(c (score - base)); base is 0 until a key is seen, and what reaches top is
+  // followed
+  float base[NT], top[NT], l[NT];
   f32x4_t acc[NT][DV];
 
   __device__ __forceinline__ float max_of(int nt) const {
-    return top[nt] == -__builtin_inff() ? top[nt] : -nb[nt];
+    return top[nt] == -__builtin_inff() ? top[nt] : base[nt];
   }
 
   __device__ __forceinline__ void load_q(const AttnArgs& a, const Segment& s, int r0, int n16,
@@ -392,7 +392,7 @@ struct Rows {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      nb[nt] = l[nt] = 0.0f;
+      base[nt] = l[nt] = 0.0f;
       top[nt] = -__builtin_inff();
 #pragma unroll
       for (int e = 0; e < DV; ++e) acc[nt][e] = f32x4_t{0, 0, 0, 0};
@@ -438,7 +438,9 @@ struct Rows {
   }
   // p of the scores, in two bf16 parts.  The base follows a row's maximum only when it
   // is passed by kSlack: p stays below 2^kSlack, and the outputs are rescaled a few
-  // times in all.
+  // times in all.  The base is a score, not a rounded exponent: with fma(score, c, -base)
+  // a base above 2^31 leaves its own rounding as the exponent of the maximum.  (One more
+  // instruction an element, 1 to 2% of a step: 128 tokens over 65536 keys 226 us for 223.)
   __device__ __forceinline__ void weights(const f32x4_t (&sc)[NT][2], float c, u32x4 (&ph)[NT],
                                           u32x4 (&pl)[NT]) {
     float x[NT][8];
@@ -449,25 +451,27 @@ struct Rows {
     };
     auto exponents = [&](int nt) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[nt][j] = __builtin_fmaf(sc[nt][j >> 2][j & 3], c, nb[nt]);
+      for (int j = 0; j < 8; ++j) x[nt][j] = (sc[nt][j >> 2][j & 3] - base[nt]) * c;
     };
     bool up = false;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       exponents(nt);
-      up |= most(nt) > top[nt];
+      up |= most(nt) >= top[nt];  // -inf too, ahead of a base: the product with c overflows
     }
     if (__any(up)) {
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         const float from = max_of(nt);
-        float mx = most(nt) - nb[nt];
+        float mx = sc[nt][0][0];
+#pragma unroll
+        for (int j = 1; j < 8; ++j) mx = fmaxf(mx, sc[nt][j >> 2][j & 3]);
         mx = fmaxf(mx, __shfl_xor(mx, 16, kWave));
         mx = fmaxf(mx, __shfl_xor(mx, 32, kWave));
         const float to = fmaxf(from, mx);
         if (to > -__builtin_inff()) {
-          const float al = __builtin_amdgcn_exp2f(from - to);
-          nb[nt] = -to;
+          const float al = __builtin_amdgcn_exp2f((from - to) * c);
+          base[nt] = to;
           top[nt] = kSlack;
           l[nt] *= al;
 #pragma unroll
@@ -616,7 +620,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int 
 #pragma unroll 1
   for (int i0 = 0; i0 < n; i0 += kWave) {
     if (i0) load_ml(i0 + lane);
-    const float f = __builtin_amdgcn_exp2f(mi - base);
+    const float f = __builtin_amdgcn_exp2f((mi - base) * a.c);
     sum += li * f;
 #pragma unroll 1
     for (int j0 = 0; j0 < kWave && i0 + j0 < n; j0 += kAhead * kParts) {
@@ -806,7 +810,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
         float sum = 0.0f;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) {
-          const float f = __builtin_amdgcn_exp2f(ml[w][rr][0] - base);
+          const float f = __builtin_amdgcn_exp2f((ml[w][rr][0] - base) * args.c);
           sum += ml[w][rr][1] * f;
 #pragma unroll
           for (int e = 0; e < DV; ++e) o[e / 4][e % 4] += acc_lds[w][rr][col + e] * f;
@@ -1159,14 +1163,14 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
 #pragma unroll
     for (int j = 0; j < kAhead; ++j) to = fmaxf(to, m[j]);
     const float base = to == -__builtin_inff() ? 0.0f : to;
-    const float f0 = __builtin_amdgcn_exp2f(mx - base);
+    const float f0 = __builtin_amdgcn_exp2f((mx - base) * a.c);
     mx = to;
     sum *= f0;
     o *= f0;
 #pragma unroll
     for (int j = 0; j < kAhead; ++j)
       if (i0 + j < n) {
-        const float f = __builtin_amdgcn_exp2f(m[j] - base);
+        const float f = __builtin_amdgcn_exp2f((m[j] - base) * a.c);
         sum += l[j] * f;
         o += x[j] * f;
       }
