@@ -1,0 +1,28 @@
+"""Steps that a paged cache refuses, without a GPU: they change nothing."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from umic.kernels import axial
+from umic.paged_cache import PagedArena, PagedKVCache
+
+
+def cache(requests=2, pages=6, max_tokens=64):
+    ar = PagedArena(1, requests, pages, 2, 16, 64, max_tokens, device="cpu")
+    return PagedKVCache(ar, axial.AxisPlan(torch.ones(32), [0, 1, 2, 0] * 8))
+
+
+def refused(c, *args, match, error=ValueError, **kwargs):
+    with pytest.raises(error, match=match):
+        c.begin(*args, **kwargs)
+    assert c.arena.lens == [0, 0] and c.arena.free == 6 and c.step is None
+    assert c.arena.kv_len.tolist() == [0, 0] and c.arena.cursor.tolist() == [0, 6, 0, 0]
+
+
+@pytest.mark.parametrize("rows", [1, 2, 4])
+def test_positions_of_other_axes(rows):
+    """Four rows are transformers' text positions ahead of the three axes: read as the axes they
+    would turn height by time and width by height."""
+    refused(cache(), 1, positions=torch.zeros(rows, 2, 1, dtype=torch.int64), match="each axis")

@@ -155,9 +155,11 @@ class PagedKVCache(DynamicCache):
         same = isinstance(new, int)
         new = [new] * ar.requests if same else list(new)
         tokens = max(max(new), 1)
-        if positions is not None and tuple(positions.shape[1:]) != (ar.requests, tokens):
-            raise ValueError(f"PagedKVCache: positions {tuple(positions.shape)} of {ar.requests} "
-                             f"requests of {tokens} tokens")
+        want = (self.rotary.axes, ar.requests, tokens)
+        if positions is not None and tuple(positions.shape) != want:
+            raise ValueError(f"PagedKVCache: positions {tuple(positions.shape)}, not {want}: a row "
+                             "for each axis of the rotary plan (no row of text positions ahead of "
+                             "them), requests, tokens")
         self.step, fresh = ar.plan(new, keep, delta)
         self.tokens, self.unmasked = tokens, False
         self._before = [n - x for n, x in zip(ar.lens, new)]
