@@ -26,3 +26,20 @@ def test_positions_of_other_axes(rows):
     """Four rows are transformers' text positions ahead of the three axes: read as the axes they
     would turn height by time and width by height."""
     refused(cache(), 1, positions=torch.zeros(rows, 2, 1, dtype=torch.int64), match="each axis")
+
+
+@pytest.mark.parametrize("positions", [torch.zeros(3, 2, 1, dtype=torch.int32),
+                                       torch.zeros(3, 2, 1), torch.zeros(3, 2, dtype=torch.int64),
+                                       torch.zeros(3, 2, 1, dtype=torch.int64, device="meta")])
+def test_positions_of_another_kind(positions):
+    """Refused before the plan: the first layer's refusal came when rows were counted that nothing
+    had written."""
+    refused(cache(), 1, positions=positions, match="positions")
+
+
+def test_a_rotary_plan_of_another_kind():
+    ar = cache().arena
+    with pytest.raises(ValueError, match="rotary plan"):
+        PagedKVCache(ar, axial.AxisPlan(torch.ones(64), [0, 1] * 32))
+    with pytest.raises(ValueError, match="rotary plan"):
+        PagedKVCache(ar, axial.AxisPlan(torch.ones(32), [0] * 32, device="meta"))

@@ -119,10 +119,17 @@ def _refuse_mask(module, args, kwargs):
 
 class PagedKVCache(DynamicCache):
     """A ``PagedArena`` as the cache of a transformers text model whose attention
-    ``umic.integrate.fuse_kv_rope`` has patched."""
+    ``umic.integrate.fuse_kv_rope`` has patched.
+
+    rotary: the plan of the arena's head size, on its device.
+    """
 
     def __init__(self, arena: PagedArena, rotary: axial.AxisPlan) -> None:
         super().__init__()
+        dim = arena.storage.shape[-1]
+        if rotary.head_dim != dim or rotary.turn.device != arena.storage.device:
+            raise ValueError(f"PagedKVCache: a rotary plan of heads of {rotary.head_dim} on "
+                             f"{rotary.turn.device} for pages of {dim} on {arena.storage.device}")
         self.arena, self.rotary = arena, rotary
         self.step: paged.PageStep | None = None
         self.tokens = 0  # of a request, in the open step
@@ -149,8 +156,9 @@ class PagedKVCache(DynamicCache):
               keep: Sequence[int | None] | None = None, delta: Sequence[int] | None = None) -> None:
         """Plan the next forward: its tokens of each request (an int: as many of all),
         right-padded to the longest.  positions: [axes, requests, S] int64, else the
-        plan's own plus ``delta``.  That forward has to be run before the next step: it
-        writes the rows that the plan has counted."""
+        plan's own plus ``delta``.  What does not fit is refused here, and changes
+        nothing.  The forward has to be run before the next step: it writes the rows
+        that the plan has counted."""
         ar = self.arena
         same = isinstance(new, int)
         new = [new] * ar.requests if same else list(new)
@@ -160,6 +168,10 @@ class PagedKVCache(DynamicCache):
             raise ValueError(f"PagedKVCache: positions {tuple(positions.shape)}, not {want}: a row "
                              "for each axis of the rotary plan (no row of text positions ahead of "
                              "them), requests, tokens")
+        if positions is not None and (positions.dtype is not torch.int64
+                                      or positions.device != ar.storage.device):
+            raise ValueError(f"PagedKVCache: positions must be int64 on {ar.storage.device}, got "
+                             f"{positions.dtype} on {positions.device}")
         self.step, fresh = ar.plan(new, keep, delta)
         self.tokens, self.unmasked = tokens, False
         self._before = [n - x for n, x in zip(ar.lens, new)]
