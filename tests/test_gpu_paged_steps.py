@@ -1,0 +1,96 @@
+"""A paged cache whose steps were replayed from a graph, and steps that the device refuses."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+from test_gpu_paged_cache import text_model
+from umic.kernels import paged
+from umic.paged_cache import PagedArena, PagedKVCache
+
+pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore::FutureWarning"),
+              pytest.mark.filterwarnings("ignore::UserWarning")]
+DEV = "cuda"
+
+
+def arena(requests=3, pages=12):
+    return PagedArena(1, requests, pages, 2, 16, 64, 64)
+
+
+def replayed(ar, steps):
+    """Steps of one token each past ``ar.plan``, as a captured plan makes them."""
+    fresh = torch.ones(ar.requests, dtype=torch.int32, device=DEV)
+    slots, positions = torch.empty(2, ar.requests, dtype=torch.int64, device=DEV)
+    out = paged.PageStep(ar.kv_len, ar.cursor, fresh.new_empty(ar.requests + 1), slots, positions)
+    for _ in range(steps):
+        paged.plan_pages(ar.kv_len, fresh, ar.table, ar.ring, ar.cursor, 16, ar.requests, row=1,
+                         out=out)
+
+
+def test_what_is_kept_is_the_devices():
+    """None keeps all that a request holds on the device, and a number at most that."""
+    ar = arena()
+    ar.plan([20, 5, 13])
+    replayed(ar, 14)
+    assert ar.kv_len.tolist() == [34, 19, 27] and ar.lens == [20, 5, 13]
+    ar.plan([1, 1, 1], keep=[0, None, 25])
+    assert ar.kv_len.tolist() == [1, 20, 26]
+    ar.sync()
+    assert ar.lens == [1, 20, 26] and ar.free == 12 - 1 - 2 - 2 == ar.cursor.tolist()[1]
+
+
+def test_sync_says_what_was_refused():
+    ar = arena(pages=4)
+    ar.plan([20, 5, 13])
+    replayed(ar, 13)  # the third request would need a second page and a third
+    assert ar.kv_len.tolist() != ar.lens
+    with pytest.raises(RuntimeError, match="pages are missing"):
+        ar.sync()
+    assert ar.lens == ar.kv_len.tolist() and ar.free == ar.cursor.tolist()[1]
+    ar.plan([1, 0, 0], keep=[0, 0, 0])
+    ar.sync()
+    assert ar.lens == [1, 0, 0] and ar.free == 3
+
+
+def test_a_request_starts_anew_after_replays():
+    """A captured decode step's replays, then a step in which one request starts anew: the others'
+    tokens stay."""
+    m, _ = text_model()
+    g = torch.Generator().manual_seed(4)
+    prompt = torch.randint(0, 512, (3, 20), generator=g).to(DEV)
+    ids = torch.zeros(3, 1, dtype=torch.long, device=DEV)
+    caches = []
+    with torch.no_grad():
+        for _ in range(2):
+            c = PagedKVCache.for_model(m, requests=3, pages=12, max_tokens=64, page_size=16)
+            for new, tokens in (([20, 5, 13], prompt), (1, ids)):
+                c.begin(new)
+                m(input_ids=tokens, position_ids=c.position_ids, past_key_values=c)
+            caches.append(c)
+        graphed, eager = caches
+        ar = graphed.arena
+        fresh = torch.ones(3, dtype=torch.int32, device=DEV)
+        out = graphed.step = paged.PageStep(ar.kv_len, ar.cursor, *graphed.step[2:])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            paged.plan_pages(ar.kv_len, fresh, ar.table, ar.ring, ar.cursor, 16, 3, row=1, out=out)
+            graphed._positions = out.positions.expand(3, -1)
+            m(input_ids=ids, position_ids=graphed.position_ids, past_key_values=graphed)
+        for _ in range(15):
+            ids.copy_(torch.randint(0, 512, (3, 1), generator=g))
+            eager.begin(1)
+            m(input_ids=ids, position_ids=eager.position_ids, past_key_values=eager)
+            graph.replay()
+        graphed.sync()
+        assert ar.lens == eager.arena.lens == [36, 21, 29] and ar.free == eager.arena.free
+        for keep in ([0, None, None], [None, 7, None], None):
+            outs = []
+            for c in caches:
+                c.begin(1, keep=keep)
+                outs.append(m(input_ids=ids, position_ids=c.position_ids,
+                              past_key_values=c).last_hidden_state)
+            assert torch.equal(*outs)
+            assert ar.kv_len.tolist() == eager.arena.kv_len.tolist() == ar.lens
+            assert ar.cursor.tolist()[1::2] == [ar.free, 0]

@@ -22,6 +22,8 @@ from umic import _lib
 
 # status of a step (PageStep.cursor[3])
 PLAN_OK, NO_PAGES, TOO_LONG, NO_ROOM, BAD_STATE = range(5)
+REFUSALS = {NO_PAGES: "pages are missing", TOO_LONG: "a request is too long",
+            NO_ROOM: "too many new tokens", BAD_STATE: "lengths or free pages out of range"}
 
 _I32, _I64 = torch.int32, torch.int64
 

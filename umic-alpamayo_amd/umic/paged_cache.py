@@ -38,10 +38,18 @@ from transformers.cache_utils import DynamicCache
 from umic.kernels import attention, axial, paged
 
 
+_ALL = 2 ** 31 - 1  # keep: whatever is held
+
+
 class PagedArena:
     """Pages of ``layers`` layers that ``requests`` requests share.
 
     max_tokens: tokens that one request can hold.
+
+    ``lens`` and ``free`` mirror the device's lengths and free pages, and ``plan``
+    refuses by them what does not fit.  Steps that go past ``plan`` (a captured
+    ``paged.plan_pages`` on these tensors, replayed) leave them behind: ``sync`` reads
+    them again, before the next ``plan``.
     """
 
     def __init__(self, layers: int, requests: int, pages: int, heads: int, page_size: int,
@@ -97,11 +105,21 @@ class PagedArena:
         fresh = self._ints(new)
         step = paged.plan_pages(
             self.kv_len, fresh, self.table, self.ring, self.cursor, ps, n * row,
-            keep=None if keep is None else self._ints(kept),
+            keep=None if keep is None else self._ints(
+                [_ALL if k is None else max(0, min(k, _ALL)) for k in keep]),
             delta=None if delta is None else self._ints(delta), row=row)
         self.kv_len, self.cursor = step.kv_len, step.cursor
         self.lens, self.free = lens, free
         return step, fresh
+
+    def sync(self) -> None:
+        """lens and free as the device has them.  Raises where the last step was refused
+        there (it changed nothing: its tokens are not in the pages)."""
+        _, self.free, _, status = self.cursor.tolist()
+        self.lens = self.kv_len.tolist()
+        if status != paged.PLAN_OK:
+            raise RuntimeError(f"paged cache: the last step was refused "
+                               f"({paged.REFUSALS[status]})")
 
 
 def _refuse_mask(module, args, kwargs):
@@ -233,6 +251,10 @@ class PagedKVCache(DynamicCache):
         raise RuntimeError("PagedKVCache: its requests stay where they are")
 
     batch_repeat_interleave = batch_select_indices = reorder_cache
+
+    def sync(self) -> None:
+        """``PagedArena.sync``, after replays of a captured step."""
+        self.arena.sync()
 
     def reset(self) -> None:
         """Every request empty."""
