@@ -94,3 +94,31 @@ def test_a_request_starts_anew_after_replays():
             assert torch.equal(*outs)
             assert ar.kv_len.tolist() == eager.arena.kv_len.tolist() == ar.lens
             assert ar.cursor.tolist()[1::2] == [ar.free, 0]
+
+
+def test_replays_and_plans_in_turn():
+    """Steps replayed from a graph and steps planned between them: one set of lengths and pages."""
+    ar, other = arena(requests=4, pages=14), arena(requests=4, pages=14)
+    for a in (ar, other):
+        a.plan([20, 5, 13, 1])
+    fresh = torch.ones(4, dtype=torch.int32, device=DEV)
+    slots, positions = torch.empty(2, 4, dtype=torch.int64, device=DEV)
+    out = paged.PageStep(ar.kv_len, ar.cursor, fresh.new_empty(5), slots, positions)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        paged.plan_pages(ar.kv_len, fresh, ar.table, ar.ring, ar.cursor, 16, 4, row=1, out=out)
+    for keep in ([None, 0, None, None], [30, None, None, 2], [0, 0, None, None]):
+        for _ in range(9):
+            graph.replay()
+            want, _ = other.plan([1] * 4)
+            assert torch.equal(slots, want.slots) and torch.equal(positions, want.positions)
+        ar.sync()
+        new = [17, 2, 1, 0]
+        for got, want in zip(*(a.plan(new, keep)[0] for a in (ar, other))):
+            assert torch.equal(got, want)
+        for a in (ar, other):
+            assert a.kv_len.tolist() == a.lens and a.cursor.tolist()[1::2] == [a.free, 0]
+        # no page twice
+        held = [p for r, n in enumerate(ar.lens) for p in ar.table[r, :-(-n // 16)].tolist()]
+        assert len(set(held)) == len(held) == 14 - ar.free

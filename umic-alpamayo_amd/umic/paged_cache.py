@@ -49,7 +49,8 @@ class PagedArena:
     ``lens`` and ``free`` mirror the device's lengths and free pages, and ``plan``
     refuses by them what does not fit.  Steps that go past ``plan`` (a captured
     ``paged.plan_pages`` on these tensors, replayed) leave them behind: ``sync`` reads
-    them again, before the next ``plan``.
+    them again, before the next ``plan``.  The tensors stay the same ones; a step's
+    kv_len and cursor are the arena's.
     """
 
     def __init__(self, layers: int, requests: int, pages: int, heads: int, page_size: int,
@@ -103,12 +104,15 @@ class PagedArena:
             raise RuntimeError(f"paged cache overflow: {-free} pages of {ps} tokens are missing")
         row = max(max(new), 1)
         fresh = self._ints(new)
+        # lengths and queue in place: captured steps hold their addresses
+        starts = fresh.new_empty(n + 1)
+        slots, positions = fresh.new_empty(2, n * row, dtype=torch.int64)
         step = paged.plan_pages(
             self.kv_len, fresh, self.table, self.ring, self.cursor, ps, n * row,
             keep=None if keep is None else self._ints(
                 [_ALL if k is None else max(0, min(k, _ALL)) for k in keep]),
-            delta=None if delta is None else self._ints(delta), row=row)
-        self.kv_len, self.cursor = step.kv_len, step.cursor
+            delta=None if delta is None else self._ints(delta), row=row,
+            out=paged.PageStep(self.kv_len, self.cursor, starts, slots, positions))
         self.lens, self.free = lens, free
         return step, fresh
 
