@@ -122,3 +122,20 @@ def test_replays_and_plans_in_turn():
         # no page twice
         held = [p for r, n in enumerate(ar.lens) for p in ar.table[r, :-(-n // 16)].tolist()]
         assert len(set(held)) == len(held) == 14 - ar.free
+
+
+@pytest.mark.parametrize("given", [False, True])
+def test_no_requests_and_entries(given):
+    """Every entry says that there is no token, also in the caller's tensors."""
+    i32 = dict(dtype=torch.int32, device=DEV)
+    none, table = torch.empty(0, **i32), torch.empty(0, 3, **i32)
+    ring, cursor = torch.arange(4, **i32), torch.tensor([1, 3, 9, 9], **i32)
+    out = None
+    if given:
+        longs = torch.full((2, 7), 5, dtype=torch.int64, device=DEV)
+        out = paged.PageStep(none, torch.full((4,), 5, **i32), torch.full((1,), 5, **i32), *longs)
+    else:  # what torch.empty is likely to give
+        torch.full((2, 7), 5, dtype=torch.int64, device=DEV)
+    step = paged.plan_pages(none, none, table, ring, cursor, 16, 7, out=out)
+    assert step.slots.tolist() == [-1] * 7 and step.positions.tolist() == [0] * 7
+    assert step.cursor.tolist() == [1, 3, 0, 0] and step.starts.tolist() == [0]

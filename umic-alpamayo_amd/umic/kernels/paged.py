@@ -117,6 +117,8 @@ def plan_pages(kv_len: torch.Tensor, new_len: torch.Tensor, table: torch.Tensor,
         out.cursor.copy_(cursor)
         out.cursor[2:] = 0
         out.starts.zero_()
+        out.slots.fill_(-1)
+        out.positions.zero_()
         return out
     with _lib.device_of(kv_len):
         _lib.call("umic_page_plan", kv_len.data_ptr(), new_len.data_ptr(), _lib.ptr(keep),
