@@ -526,9 +526,15 @@ int umic_axial_rope_append_bf16(const void* q, const void* k, const void* v, voi
  * same, do not depend on what ran before, and repeat bit for bit.
  * Replaces: the attention that HF Qwen3VLTextAttention calls after cache.py:50-80
  * (InplaceLayer.update, whose single-token steps copy the whole cache for it).
+ * One call counts its work in 32 bits: it takes at most
+ * umic_cache_attention_max_requests requests (else UMIC_ERR_UNSUPPORTED), for caches
+ * that can hold `cap` keys a request (block_rows, or table_w * block_rows, whatever the
+ * lengths are): 2^31 / (Hk * row blocks * (cap / 32 + 8)), a row block being 128 of the
+ * S * Hq / Hk rows of a key head (64 where there are no more, or D is 256).
  */
 #define UMIC_ATTENTION_COUNTERS 4096
 int64_t umic_cache_attention_workspace_bytes(int64_t S, int64_t Hq, int64_t Hk, int64_t D);
+int64_t umic_cache_attention_max_requests(int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t cap);
 int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void* out,
                               const int32_t* table, const int32_t* kv_lens,
                               const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t Hk,

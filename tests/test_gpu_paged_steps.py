@@ -5,8 +5,11 @@ from __future__ import annotations
 import pytest
 import torch
 
+import paged_reference as ref
+from helpers import bf16_randn
+from test_gpu_cache_attention import make
 from test_gpu_paged_cache import text_model
-from umic.kernels import paged
+from umic.kernels import attention, paged
 from umic.paged_cache import PagedArena, PagedKVCache
 
 pytestmark = [pytest.mark.gpu, pytest.mark.filterwarnings("ignore::FutureWarning"),
@@ -139,3 +142,51 @@ def test_no_requests_and_entries(given):
     step = paged.plan_pages(none, none, table, ring, cursor, 16, 7, out=out)
     assert step.slots.tolist() == [-1] * 7 and step.positions.tolist() == [0] * 7
     assert step.cursor.tolist() == [1, 3, 0, 0] and step.starts.tolist() == [0]
+
+
+@pytest.mark.parametrize("S", [1, 3, 40])
+@pytest.mark.parametrize("own_out", [False, True])
+def test_more_requests_than_one_launch_takes(S, own_out):
+    """A table of 2^30 tokens a request: 63 requests a launch."""
+    B, W, page, Hq, D = 70, 1 << 14, 1 << 16, 2, 64
+    assert attention.max_requests(S, Hq, 1, D, W * page) == 63
+    g = torch.Generator().manual_seed(S)
+    k, v = (bf16_randn(3, 1, page, D, gen=g).to(DEV) for _ in range(2))
+    q = bf16_randn(B, S, Hq, D, scale=1.5, gen=g).to(DEV).transpose(1, 2)
+    table = torch.full((B, W), -1, dtype=torch.int32, device=DEV)
+    table[:, 0], table[:, 1] = torch.arange(B) % 3, torch.arange(1, B + 1) % 3
+    lens = [(b * b * 13) % 300 for b in range(B)]
+    lens[5], lens[62], lens[63], lens[69] = page + 100, 0, page + 7, 301
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    fresh = [min(S, b % (S + 1)) for b in range(B)]
+    m = torch.tensor(fresh, dtype=torch.int32, device=DEV)
+    out = torch.full((B, S, Hq, D), 7.0, dtype=torch.bfloat16, device=DEV) if own_out else None
+    got = attention.cache_attention(q, k, v, n, table=table, q_len=m, out=out)
+    assert out is None or got is out
+    ref.check_attention(got, *ref.attention(q, k, v, lens, table, q_len=fresh))
+    for b in (62, 63):
+        part = slice(b, b + 1)
+        alone = attention.cache_attention(q[part], k, v, n[part], table=table[part, :4], q_len=m[part])
+        ref.check_attention(alone, *ref.attention(q[part], k, v, lens[part], table[part],
+                                                  q_len=fresh[part]))
+    same = attention.cache_attention(q, k, v, 200, table=table, causal=False)
+    ref.check_attention(same, *ref.attention(q, k, v, [200] * B, table, causal=False))
+
+
+@pytest.mark.parametrize("page", [0, 16])
+def test_requests_of_several_launches(monkeypatch, page):
+    """Contiguous caches and tables, cut into launches of three requests."""
+    lens, S = [40, 0, 200, 33, 7, 90, 150], 5
+    q, k, v, table = make(lens, S, 8, 2, 128, page, seed=page)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    m = torch.tensor([5, 0, 3, 5, 5, 1, 2], dtype=torch.int32, device=DEV)
+    monkeypatch.setattr(attention, "max_requests", lambda *a: 3)
+    got = attention.cache_attention(q, k, v, n, table=table, q_len=m)
+    ref.check_attention(got, *ref.attention(q, k, v, lens, table, q_len=m.tolist()))
+    if not page:
+        k, v = k.nan_to_num(0.5), v.nan_to_num(0.5)
+        got = attention.cache_attention(q, k, v, 100)
+        ref.check_attention(got, *ref.attention(q, k, v, [100] * 7))
+    monkeypatch.setattr(attention, "max_requests", lambda *a: 0)
+    with pytest.raises(ValueError, match="one launch"):
+        attention.cache_attention(q, k, v, n, table=table)

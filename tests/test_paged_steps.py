@@ -5,6 +5,7 @@ from __future__ import annotations
 import pytest
 import torch
 
+from umic import _lib
 from umic.kernels import axial
 from umic.paged_cache import PagedArena, PagedKVCache
 
@@ -43,3 +44,18 @@ def test_a_rotary_plan_of_another_kind():
         PagedKVCache(ar, axial.AxisPlan(torch.ones(64), [0, 1] * 32))
     with pytest.raises(ValueError, match="rotary plan"):
         PagedKVCache(ar, axial.AxisPlan(torch.ones(32), [0] * 32, device="meta"))
+
+
+def test_steps_that_one_launch_does_not_take():
+    """The attention counts its work in 32 bits, by what a request can hold."""
+    f = _lib.lib().umic_cache_attention_max_requests
+    assert f(1, 32, 8, 128, 131072) == 0x7fffffff // 8 // 4104
+    assert f(32768, 32, 8, 128, 131072) == 63 and f(32768, 32, 8, 256, 131072) == 31
+    assert f(1, 8, 2, 64, 16) == 1 << 20
+    for args in ((0, 8, 2, 128, 64), (1, 8, 3, 128, 64), (1, 8, 2, 80, 64), (1, 8, 2, 128, -1),
+                 (1 << 21, 8, 2, 128, 64), (1, 8, 2, 128, 1 << 31), (1 << 20, 1 << 16, 8, 64, 64)):
+        assert f(*args) == 0
+    c = cache(max_tokens=1 << 24)
+    c.query_heads = 2
+    assert f(1 << 18, 2, 2, 64, 1 << 24) == 0
+    refused(c, [1 << 18, 0], match="one launch")

@@ -1242,6 +1242,13 @@ int launch(const Shape& s, const AttnArgs& a, hipStream_t st) {
 
 bool head_dim_ok(int64_t D) { return D == 64 || D == 128 || D == 256; }
 
+// Requests of up to `cap` keys that a call takes: the tiles of all are counted in 32 bits.
+int64_t max_requests(int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t cap) {
+  if (S > (1 << 20) || Hq > (1 << 16) || S * Hq > 0x7fffffff || cap > ((int64_t)1 << 30)) return 0;
+  const int64_t rb = shape_of(S * (Hq / Hk), D, 1).rb;
+  return std::min<int64_t>(0x7fffffff / (Hk * rb) / (cap / kStep + 8), 1 << 20);
+}
+
 }  // namespace
 }  // namespace umic
 
@@ -1251,6 +1258,13 @@ extern "C" int64_t umic_cache_attention_workspace_bytes(int64_t S, int64_t Hq, i
   if (S <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || !head_dim_ok(D) || S > (1 << 20) || Hq > (1 << 16))
     return 0;
   return workspace_of(shape_of(S * (Hq / Hk), D, device_cus()), D);
+}
+
+extern "C" int64_t umic_cache_attention_max_requests(int64_t S, int64_t Hq, int64_t Hk, int64_t D,
+                                                     int64_t cap) {
+  using namespace umic;
+  if (S <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || !head_dim_ok(D) || cap < 0) return 0;
+  return max_requests(S, Hq, Hk, D, cap);
 }
 
 extern "C" int umic_cache_attention_bf16(
@@ -1288,15 +1302,12 @@ extern "C" int umic_cache_attention_bf16(
   const int64_t cus = device_cus();
   if (cus <= 0) return (int)hipErrorNoDevice;
   const int64_t G = Hq / Hk;
-  if (B > (1 << 20) || S > (1 << 20) || Hq > (1 << 16) || S * Hq > 0x7fffffff ||
-      cap > ((int64_t)1 << 30) || blocks > ((int64_t)1 << 30))
+  if (B > max_requests(S, Hq, Hk, D, cap) || blocks > ((int64_t)1 << 30))
     return UMIC_ERR_UNSUPPORTED;
   const Shape s = shape_of(S * G, D, cus);
   if (workspace_bytes < workspace_of(s, D)) return UMIC_ERR_INVALID_ARG;
   if (s.nwg > UMIC_ATTENTION_COUNTERS) counters = nullptr;
-  // the tiles of all requests are counted in 32 bits, and row offsets in a tile
-  if (B * (cap / kStep + 8) > 0x7fffffff / (Hk * s.rb) || c_ss < 0 || c_ss >= (1 << 24))
-    return UMIC_ERR_UNSUPPORTED;
+  if (c_ss < 0 || c_ss >= (1 << 24)) return UMIC_ERR_UNSUPPORTED;  // row offsets in a tile
   AttnArgs a = {};
   a.q = (const uint16_t*)q, a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
   a.out = (uint16_t*)out, a.table = table, a.kv_len = kv_lens, a.q_len = q_lens;

@@ -67,6 +67,7 @@ SIGNATURES: dict[str, list] = {
     "umic_axial_rope_bf16": [_P] * 7 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 15 + [_P],
     "umic_axial_rope_append_bf16": [_P] * 10 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 20 + [_P],
     "umic_cache_attention_workspace_bytes": [_I64] * 4,
+    "umic_cache_attention_max_requests": [_I64] * 5,
     "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _P, _I64, _P],
     "umic_stream_read": [_P, _I64, _P, _P],
     "umic_stream_copy": [_P, _P, _I64, _P],
@@ -79,7 +80,8 @@ SIGNATURES: dict[str, list] = {
 RESTYPES = {"umic_version": ctypes.c_char_p, "umic_error_string": ctypes.c_char_p,
             "umic_linear_kernel": _I64, "umic_linear_workspace_bytes": _I64,
             "umic_linear_workspace_preferred": _I64,
-            "umic_cache_attention_workspace_bytes": _I64}
+            "umic_cache_attention_workspace_bytes": _I64,
+            "umic_cache_attention_max_requests": _I64}
 
 
 class UmicLibraryError(RuntimeError):

@@ -28,6 +28,12 @@ def _workspace_bytes(dev: int, S: int, Hq: int, Hk: int, D: int) -> int:
     return _lib.lib().umic_cache_attention_workspace_bytes(S, Hq, Hk, D)
 
 
+@functools.lru_cache(maxsize=1024)
+def max_requests(S: int, Hq: int, Hk: int, D: int, cap: int) -> int:
+    """Requests of S new tokens and up to cap keys that one launch takes; 0: not even one."""
+    return _lib.lib().umic_cache_attention_max_requests(S, Hq, Hk, D, cap)
+
+
 # Asked at every call: without the public function's own look at the build.
 _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
                      None) or torch.cuda.is_current_stream_capturing
@@ -145,6 +151,19 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
         if any(st == 0 and n > 1 for st, n in zip(os_, out.shape)):
             raise ValueError("cache_attention: out must not share rows")
     if B == 0 or S == 0 or Hq == 0:
+        return out
+    most = max_requests(S, Hq, Hk, D, cap)
+    if B > most:
+        if most == 0:
+            raise ValueError(f"cache_attention: {S} new tokens of {Hq} heads over up to {cap} keys "
+                             "are too many for one launch")
+        for b in range(0, B, most):  # requests stand for themselves
+            part = slice(b, b + most)
+            kv = (k_cache, v_cache) if table is not None else (k_cache[part], v_cache[part])
+            cache_attention(q[part], *kv, n if lens is None else kv_len[part],
+                            table=None if table is None else table[part],
+                            q_len=None if q_len is None else q_len[part], causal=causal,
+                            scale=scale, out=out[part])
         return out
     qs, cs = q.stride(), k_cache.stride()
     with _lib.device_of(q):

@@ -144,15 +144,18 @@ class PagedKVCache(DynamicCache):
     ``umic.integrate.fuse_kv_rope`` has patched.
 
     rotary: the plan of the arena's head size, on its device.
+    query_heads: of the model, if ``begin`` is to refuse a step that the attention does
+        not take.
     """
 
-    def __init__(self, arena: PagedArena, rotary: axial.AxisPlan) -> None:
+    def __init__(self, arena: PagedArena, rotary: axial.AxisPlan,
+                 query_heads: int | None = None) -> None:
         super().__init__()
         dim = arena.storage.shape[-1]
         if rotary.head_dim != dim or rotary.turn.device != arena.storage.device:
             raise ValueError(f"PagedKVCache: a rotary plan of heads of {rotary.head_dim} on "
                              f"{rotary.turn.device} for pages of {dim} on {arena.storage.device}")
-        self.arena, self.rotary = arena, rotary
+        self.arena, self.rotary, self.query_heads = arena, rotary, query_heads
         self.step: paged.PageStep | None = None
         self.tokens = 0  # of a request, in the open step
         self.unmasked = False  # the running forward was called without a mask
@@ -172,7 +175,8 @@ class PagedKVCache(DynamicCache):
                            max_tokens, weight.device)
         if getattr(lm, "_umic_paged_hook", None) is None:
             lm._umic_paged_hook = lm.register_forward_pre_hook(_refuse_mask, with_kwargs=True)
-        return cls(arena, axial.AxisPlan.rotary(lm.rotary_emb))
+        return cls(arena, axial.AxisPlan.rotary(lm.rotary_emb),
+                   attn.q_proj.weight.shape[0] // attn.head_dim)
 
     def begin(self, new: int | Sequence[int], positions: torch.Tensor | None = None,
               keep: Sequence[int | None] | None = None, delta: Sequence[int] | None = None) -> None:
@@ -194,6 +198,11 @@ class PagedKVCache(DynamicCache):
                                       or positions.device != ar.storage.device):
             raise ValueError(f"PagedKVCache: positions must be int64 on {ar.storage.device}, got "
                              f"{positions.dtype} on {positions.device}")
+        heads, dim = ar.storage.shape[3], ar.storage.shape[5]
+        if self.query_heads and not attention.max_requests(tokens, self.query_heads, heads, dim,
+                                                           ar.max_tokens):
+            raise ValueError(f"PagedKVCache: {tokens} new tokens of {self.query_heads} heads over up "
+                             f"to {ar.max_tokens} keys are too many for one launch")
         self.step, fresh = ar.plan(new, keep, delta)
         self.tokens, self.unmasked = tokens, False
         self._before = [n - x for n, x in zip(ar.lens, new)]
