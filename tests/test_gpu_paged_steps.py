@@ -190,3 +190,40 @@ def test_requests_of_several_launches(monkeypatch, page):
     monkeypatch.setattr(attention, "max_requests", lambda *a: 0)
     with pytest.raises(ValueError, match="one launch"):
         attention.cache_attention(q, k, v, n, table=table)
+
+
+def test_positions_of_the_forward():
+    """The forward's position ids are the step's, or refused: its attention turns by the step's."""
+    m, _ = text_model()
+    c = PagedKVCache.for_model(m, requests=2, pages=12, max_tokens=64, page_size=16)
+    g = torch.Generator().manual_seed(7)
+    ids = torch.randint(0, 512, (2, 9), generator=g).to(DEV)
+
+    def run(pos, *where):
+        c.reset()
+        c.begin([9, 4], *where)
+        return m(input_ids=ids, position_ids=pos, past_key_values=c).last_hidden_state
+
+    with torch.no_grad():
+        c.begin([9, 4])
+        own = c.position_ids.clone()
+        image = torch.randint(0, 30, (3, 2, 9), generator=g).to(DEV)
+        padded = own.clone()
+        padded[:, 1, 4:] = 17  # rows without a token
+        text = torch.cat((own[:1] + 3, own))
+        want = run(None)
+        for pos in (own, own[0], own[:1], padded, text):
+            assert torch.equal(run(pos)[0], want[0]) and torch.equal(run(pos)[1, :4], want[1, :4])
+        for pos in (image, own + 1, image[0], torch.cat((own, image))[:5], own.cpu()):
+            with pytest.raises(ValueError, match="position_ids"):
+                run(pos)
+        got = run(image, image)
+        assert not torch.equal(got[0], want[0])
+        c.reset()
+        c.begin([9, 4], image)
+        assert torch.equal(m(input_ids=ids, position_ids=c.position_ids,
+                             past_key_values=c).last_hidden_state[0], got[0])
+        with pytest.raises(ValueError, match="position_ids"):
+            run(own, image)
+        with pytest.raises(ValueError, match="position_ids"):
+            m(ids, None, own, c)

@@ -20,7 +20,8 @@ the pages in one launch and attends over them in another.
     cache.begin(1, keep=[0, None, ...])                # request 0 starts anew
 
 Positions come from the plan (the token's place in its request plus ``delta``) or
-from the caller, as [axes, requests, S] (image grids).  Numerics are ``axial``'s and
+from the caller, through ``begin``, as [axes, requests, S] (image grids); position ids
+of the forward that differ from them are refused.  Numerics are ``axial``'s and
 ``attention``'s: fp32 with one rounding, where the in-place cache repeats the eager
 chain's roundings.
 
@@ -126,13 +127,18 @@ class PagedArena:
                                f"({paged.REFUSALS[status]})")
 
 
-def _refuse_mask(module, args, kwargs):
-    """Forward pre-hook of a text model: a ``PagedKVCache`` goes without a mask.  What
-    transformers makes of none, where it cannot look at the lengths (a capture), is
-    then known to hold nothing."""
+def _refuse(module, args, kwargs):
+    """Forward pre-hook of a text model: a ``PagedKVCache`` goes without a mask, and with
+    the positions of its step.  What transformers makes of no mask, where it cannot look
+    at the lengths (a capture), is then known to hold nothing."""
     mask = kwargs.get("attention_mask", args[1] if len(args) > 1 else None)
+    positions = kwargs.get("position_ids", args[2] if len(args) > 2 else None)
     cache = kwargs.get("past_key_values", args[3] if len(args) > 3 else None)
     if isinstance(cache, PagedKVCache):
+        if positions is not None and not cache.turns_by(positions):
+            raise ValueError("PagedKVCache: position_ids are not those of its step, which its "
+                             "attention turns by: give them to begin(), and the forward "
+                             "cache.position_ids")
         if mask is not None:
             raise ValueError("PagedKVCache: its lengths say which tokens are seen; pass no "
                              "attention_mask (begin() takes the prompts' lengths)")
@@ -174,7 +180,7 @@ class PagedKVCache(DynamicCache):
         arena = PagedArena(len(lm.layers), requests, pages, heads, page_size, attn.head_dim,
                            max_tokens, weight.device)
         if getattr(lm, "_umic_paged_hook", None) is None:
-            lm._umic_paged_hook = lm.register_forward_pre_hook(_refuse_mask, with_kwargs=True)
+            lm._umic_paged_hook = lm.register_forward_pre_hook(_refuse, with_kwargs=True)
         return cls(arena, axial.AxisPlan.rotary(lm.rotary_emb),
                    attn.q_proj.weight.shape[0] // attn.head_dim)
 
@@ -216,6 +222,27 @@ class PagedKVCache(DynamicCache):
     def position_ids(self) -> torch.Tensor:
         """The open step's positions, [axes, requests, S], as the model takes them."""
         return self._positions.reshape(-1, self.arena.requests, self.tokens)
+
+    def turns_by(self, positions: torch.Tensor) -> bool:
+        """Whether a forward's position ids are the open step's for its tokens: this
+        object's own without a look at them, others by their values (a wait for the
+        device, and no for a capture).  [requests, S] count for every axis, and a row of
+        text positions ahead of the axes' does not."""
+        B, S = self.arena.requests, self.tokens
+        if self.step is None or tuple(positions.shape[-2:]) != (B, S):
+            return True  # attend() refuses the forward
+        mine = self.position_ids
+        if positions.dim() == 3 and positions.shape[0] == mine.shape[0] + 1:
+            positions = positions[1:]
+        if (positions.data_ptr() == mine.data_ptr() and positions.dtype is mine.dtype
+                and positions.shape == mine.shape and positions.stride() == mine.stride()):
+            return True
+        if (positions.device != mine.device or positions.dim() not in (2, 3)
+                or positions.dim() == 3 and positions.shape[0] not in (1, mine.shape[0])
+                or torch.cuda.is_current_stream_capturing()):
+            return False
+        there = self.step.slots.view(B, S) >= 0
+        return not bool(((positions != mine) & there).any())
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, norm,
                scale: float) -> torch.Tensor:
