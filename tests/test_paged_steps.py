@@ -2,10 +2,12 @@
 
 from __future__ import annotations
 
+import types
+
 import pytest
 import torch
 
-from umic import _lib
+from umic import _lib, integrate
 from umic.kernels import axial
 from umic.paged_cache import PagedArena, PagedKVCache
 
@@ -59,3 +61,30 @@ def test_steps_that_one_launch_does_not_take():
     c.query_heads = 2
     assert f(1 << 18, 2, 2, 64, 1 << 24) == 0
     refused(c, [1 << 18, 0], match="one launch")
+
+
+def test_modes_see_the_attention_that_the_kernel_would_replace():
+    """fuse_cache_attention leaves a call to SDPA where a function or dispatch mode watches."""
+    from torch.overrides import TorchFunctionMode
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Watch(TorchFunctionMode):
+        def __torch_function__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    class Below(TorchDispatchMode):
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            return func(*args, **(kwargs or {}))
+
+    attn = torch.nn.Module()
+    attn._umic_cache_attention = True
+    attn.config = types.SimpleNamespace(_attn_implementation="sdpa")
+    q = torch.zeros(1, 4, 1, 128, dtype=torch.bfloat16)
+    ok = integrate._cache_attention_ok
+    assert ok(attn, q, None, {})
+    with torch.device("cpu"):
+        assert ok(attn, q, None, {})
+    for mode in (Watch(), Below()):
+        with mode:
+            assert not ok(attn, q, None, {})
+    assert ok(attn, q, None, {})

@@ -1088,14 +1088,15 @@ CACHE_ATTENTION_MAX_TOKENS = 128
 def _cache_attention_ok(module: nn.Module, q: torch.Tensor, attention_mask, kwargs) -> bool:
     """True where fuse_cache_attention's kernel stands for the attention of q's tokens
     over the in-place cache: no mask, and one token or an attention that is not causal
-    (all of the cache is seen), through SDPA, which returns no weights."""
+    (all of the cache is seen), through SDPA, which returns no weights, with no mode that
+    would have seen SDPA's call."""
     tokens = q.shape[2]
     return (getattr(module, "_umic_cache_attention", False) and attention_mask is None
             and (tokens == 1 or tokens <= CACHE_ATTENTION_MAX_TOKENS
                  and not (kwargs.get("is_causal") if kwargs.get("is_causal") is not None
                           else getattr(module, "is_causal", True)))
             and module.config._attn_implementation == "sdpa"
-            and not kwargs.get("output_attentions"))
+            and not kwargs.get("output_attentions") and _plain_call(q))
 
 
 def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
