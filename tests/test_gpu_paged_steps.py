@@ -6,9 +6,9 @@ import pytest
 import torch
 
 import paged_reference as ref
-from helpers import bf16_randn
+from helpers import bf16_randn, rel_err
 from test_gpu_cache_attention import make
-from test_gpu_paged_cache import text_model
+from test_gpu_paged_cache import TOL, text_model
 from umic.kernels import attention, paged
 from umic.paged_cache import PagedArena, PagedKVCache
 
@@ -227,3 +227,28 @@ def test_positions_of_the_forward():
             run(own, image)
         with pytest.raises(ValueError, match="position_ids"):
             m(ids, None, own, c)
+
+
+@pytest.mark.parametrize("how", ["module", "call", "neither"])
+def test_attention_that_is_not_causal(how):
+    """By the module's attribute or the call's word: every new token of a request sees the others.
+    Against the unpatched module on the CPU, with a mask that shows all."""
+    m, plain = text_model()
+    c = PagedKVCache.for_model(m, requests=2, pages=8, max_tokens=64, page_size=16)
+    g = torch.Generator().manual_seed(8)
+    x = torch.randn(2, 12, 256, generator=g).to(torch.bfloat16)
+    attn = m.layers[0].self_attn
+    if how == "module":
+        attn.is_causal = False
+    lens = [12, 7]
+    with torch.no_grad():
+        c.begin(lens)
+        got = attn(x.to(DEV), (None, None), None, past_key_values=c,
+                   **({"is_causal": False} if how == "call" else {}))[0]
+        for r, n in enumerate(lens):
+            rot = plain.rotary_emb(x[r:r + 1], torch.arange(n).expand(3, 1, n))
+            mask = torch.zeros(1, 1, n, n, dtype=torch.bfloat16)
+            if how == "neither":
+                mask += torch.full((n, n), float("-inf")).triu(1).to(torch.bfloat16)
+            want = plain.layers[0].self_attn(x[r:r + 1, :n], rot, mask)[0]
+            assert rel_err(got[r, :n], want[0]) <= TOL

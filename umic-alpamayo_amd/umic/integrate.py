@@ -1050,8 +1050,15 @@ def _head_norms(module: nn.Module, q: torch.Tensor):
     return qw, kw, eps
 
 
+def _is_causal(module: nn.Module, kwargs) -> bool:
+    """Whether an attention without a mask hides later tokens: the call's word, then the
+    module's, as transformers' attention functions have it."""
+    causal = kwargs.get("is_causal")
+    return bool(getattr(module, "is_causal", True) if causal is None else causal)
+
+
 def _paged_attention(module: nn.Module, hidden_states: torch.Tensor, attention_mask, cache,
-                     pre_norm: nn.Module | None):
+                     pre_norm: nn.Module | None, causal: bool = True):
     """The text attention over a ``PagedKVCache``: the projections, then the cache's
     two launches, which rotate by the positions of the cache's step."""
     if attention_mask is not None and not cache.unmasked:
@@ -1062,7 +1069,7 @@ def _paged_attention(module: nn.Module, hidden_states: torch.Tensor, attention_m
     norm = _axial_norms(module, q)
     if norm is None:
         q, k = module.q_norm(q), module.k_norm(k)
-    out = cache.attend(module.layer_idx, q, k, v, norm, module.scaling)
+    out = cache.attend(module.layer_idx, q, k, v, norm, module.scaling, causal)
     return _linear(module.o_proj, out.reshape(*hidden_states.shape[:-1], -1)), None
 
 
@@ -1093,8 +1100,7 @@ def _cache_attention_ok(module: nn.Module, q: torch.Tensor, attention_mask, kwar
     tokens = q.shape[2]
     return (getattr(module, "_umic_cache_attention", False) and attention_mask is None
             and (tokens == 1 or tokens <= CACHE_ATTENTION_MAX_TOKENS
-                 and not (kwargs.get("is_causal") if kwargs.get("is_causal") is not None
-                          else getattr(module, "is_causal", True)))
+                 and not _is_causal(module, kwargs))
             and module.config._attn_implementation == "sdpa"
             and not kwargs.get("output_attentions") and _plain_call(q))
 
@@ -1137,7 +1143,8 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
         return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
                                   past_key_values=past_key_values, **kwargs)
     if isinstance(past_key_values, PagedKVCache):
-        return _paged_attention(self, hidden_states, attention_mask, past_key_values, pre_norm)
+        return _paged_attention(self, hidden_states, attention_mask, past_key_values, pre_norm,
+                                _is_causal(self, kwargs))
     layer = None
     if isinstance(past_key_values, InplaceKVCache) and self.layer_idx < len(
             past_key_values.layers):

@@ -245,9 +245,10 @@ class PagedKVCache(DynamicCache):
         return not bool(((positions != mine) & there).any())
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, norm,
-               scale: float) -> torch.Tensor:
+               scale: float, causal: bool = True) -> torch.Tensor:
         """Append the step's k and v [requests, S, heads, D] to a layer's pages, rotated
-        (and with ``norm = (q_w, k_w, eps)`` normed), and attend: [requests, S, Hq, D]."""
+        (and with ``norm = (q_w, k_w, eps)`` normed), and attend: [requests, S, Hq, D].
+        Not causal: a request's new tokens see each other too."""
         B, S, Hq, D = q.shape
         ar = self.arena
         if self.step is None or B != ar.requests or S != self.tokens:
@@ -259,7 +260,7 @@ class PagedKVCache(DynamicCache):
                                   values, norm)
         return attention.cache_attention(rot.view(B, S, Hq, D).transpose(1, 2), keys, values,
                                          ar.kv_len, table=ar.table, q_len=self._fresh,
-                                         scale=scale)
+                                         causal=causal, scale=scale)
 
     # -- what transformers asks of a cache -----------------------------------
 
