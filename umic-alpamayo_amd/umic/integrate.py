@@ -1133,7 +1133,6 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
     forward.
     """
     from umic.cache import InplaceKVCache, InplaceLayer
-    from umic.paged_cache import PagedKVCache
 
     if self.training or grad_needed(hidden_states, self.q_proj.weight, self.k_proj.weight,
                                     self.v_proj.weight, getattr(self.q_norm, "weight", None),
@@ -1142,15 +1141,18 @@ def _fused_kv_rope_attention_forward(self, hidden_states, position_embeddings,
             hidden_states = pre_norm(hidden_states)
         return type(self).forward(self, hidden_states, position_embeddings, attention_mask,
                                   past_key_values=past_key_values, **kwargs)
-    if isinstance(past_key_values, PagedKVCache):
-        return _paged_attention(self, hidden_states, attention_mask, past_key_values, pre_norm,
-                                _is_causal(self, kwargs))
     layer = None
-    if isinstance(past_key_values, InplaceKVCache) and self.layer_idx < len(
-            past_key_values.layers):
-        layer = past_key_values.layers[self.layer_idx]
-        if not isinstance(layer, InplaceLayer):
-            layer = None
+    if isinstance(past_key_values, InplaceKVCache):
+        if self.layer_idx < len(past_key_values.layers):
+            layer = past_key_values.layers[self.layer_idx]
+            if not isinstance(layer, InplaceLayer):
+                layer = None
+    elif past_key_values is not None:
+        from umic.paged_cache import PagedKVCache
+
+        if isinstance(past_key_values, PagedKVCache):
+            return _paged_attention(self, hidden_states, attention_mask, past_key_values, pre_norm,
+                                    _is_causal(self, kwargs))
     input_shape = hidden_states.shape[:-1]
     hidden_shape = (*input_shape, -1, self.head_dim)
     q_raw, k_raw, v = (t.view(hidden_shape) for t in _qkv(self, hidden_states, pre_norm))
