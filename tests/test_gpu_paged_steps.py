@@ -252,3 +252,25 @@ def test_attention_that_is_not_causal(how):
                 mask += torch.full((n, n), float("-inf")).triu(1).to(torch.bfloat16)
             want = plain.layers[0].self_attn(x[r:r + 1, :n], rot, mask)[0]
             assert rel_err(got[r, :n], want[0]) <= TOL
+
+
+def test_workspaces_of_many_streams():
+    """As many are held as the module says, whatever streams have called."""
+    lens = [900, 33, 0, 2500]
+    q, k, v, table = make(lens, 5, 8, 2, 128, 16, seed=5)
+    n = torch.tensor(lens, dtype=torch.int32, device=DEV)
+    want = attention.cache_attention(q, k, v, n, table=table)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(7)]
+    got = []
+    for i in range(21):
+        with torch.cuda.stream(streams[i * 3 % 7]):
+            got.append(attention.cache_attention(q, k, v, n, table=table))
+            if i % 2:  # single tokens, with counters
+                attention.cache_attention(q[:, :, :1], k, v, n, table=table)
+        assert len(attention._SCRATCH) <= attention.SCRATCH_STREAMS
+    torch.cuda.synchronize()
+    for o in got:
+        assert torch.equal(o, want)
+    for counters, _ in attention._SCRATCH.values():
+        assert not counters.any()

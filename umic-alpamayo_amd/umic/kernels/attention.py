@@ -41,6 +41,9 @@ _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing",
 # (counters, workspace) of each (device, stream): calls on one stream do not
 # overlap, and every call leaves the counters at zero.  A captured call has a
 # workspace of its own and no counters, as its graph may run beside anything.
+# The latest SCRATCH_STREAMS are held (68 MB each for more than 64 rows of 128);
+# what goes was allocated on its stream, and waits for it before it is used again.
+SCRATCH_STREAMS = 4
 _SCRATCH: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
 
 
@@ -52,6 +55,8 @@ def _scratch(q: torch.Tensor, dev: int, stream: int, need: int) -> tuple[int | N
         counters = held[0] if held else torch.zeros(_lib.UMIC_ATTENTION_COUNTERS,
                                                     dtype=torch.int32, device=q.device)
         held = counters, torch.empty(need, dtype=torch.uint8, device=q.device)
+        for key in [] if (dev, stream) in _SCRATCH else list(_SCRATCH)[:1 - SCRATCH_STREAMS]:
+            _SCRATCH.pop(key, None)
         _SCRATCH[dev, stream] = held
     return held[0].data_ptr(), held[1]
 
