@@ -127,3 +127,22 @@ def test_hidden_where_a_wave_has_one_token(S, Hq, Hk, D, bad):
     got = call(q, k, v, [n], table)
     assert torch.isfinite(got[0, :S - 1]).all()
     check(got, *expected(q, k, v, n, table))
+
+
+@pytest.mark.parametrize("S,Hq,Hk,D", [(5, 4, 4, 64), (4, 8, 2, 128), (40, 8, 2, 128), (20, 4, 2, 256)])
+def test_padded_rows_and_queries_that_are_not_finite(S, Hq, Hk, D):
+    """Rows past q_len are zero whatever their queries and the values hold; a NaN query's row is NaN
+    and the rows beside it are not."""
+    lens, fresh = [900, 2500, 70], [S - 2, 1, S]
+    q, k, v, table = make(lens, S, Hq, Hk, D, 16, seed=S)
+    m = torch.tensor(fresh, dtype=torch.int32, device=DEV)
+    want, tol = ref.attention(q, k, v, lens, table, q_len=fresh)
+    wild = q.clone()
+    wild[0, :, S - 2:], wild[1, :, 1:] = NAN, INF
+    wild[2, 1, S - 1] = NAN
+    got = call(wild, k, v, lens, table, q_len=m)
+    assert not got[0, S - 2:].any() and not got[1, 1:].any()
+    assert torch.isnan(got[2, S - 1, 1]).all()
+    got[2, S - 1, 1] = 0
+    want[2, S - 1, 1], tol[2, S - 1, 1] = 0, 1
+    ref.check_attention(got, want, tol)

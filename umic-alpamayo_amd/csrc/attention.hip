@@ -305,16 +305,17 @@ __device__ __forceinline__ bool finite(float x) { return __builtin_fabsf(x) < __
 // what underflows times infinity is NaN.  But whatever they give is not finite, and
 // stays so: where a row's o (of N groups of four columns, col + STEP g ..) is not, the
 // values among keys [from, to) below lim that are not finite take its place.  (Sums of
-// finite values that overflowed have none, and stay.)
+// finite values that overflowed have none, and stay.)  count: of rows that are written,
+// and not NaN as their weights are.
 template <int N, int STEP>
-__device__ __forceinline__ void restore(f32x4_t (&o)[N], const AttnArgs& a, const Keys& s, int from,
-                                        int to, int lim, int col) {
+__device__ __forceinline__ void restore(f32x4_t (&o)[N], bool count, const AttnArgs& a, const Keys& s,
+                                        int from, int to, int lim, int col) {
   float none = 0.0f;  // NaN: not all are finite
 #pragma unroll
   for (int g = 0; g < N; ++g)
 #pragma unroll
     for (int y = 0; y < 4; ++y) none = __builtin_fmaf(o[g][y], 0.0f, none);
-  if (!__any(none != none)) return;
+  if (!__any(count && none != none)) return;
   f32x4_t sum[N] = {};
 #pragma unroll 1
   for (int k0 = from; k0 < to; k0 += kStep) {
@@ -633,7 +634,7 @@ __device__ __forceinline__ void join_row(const AttnArgs& a, int w0, int w1, int 
   for (int k = kLanes; k < kWave; k <<= 1)
 #pragma unroll
     for (int c = 0; c < 4; ++c) o[c] += __shfl_xor(o[c], k, kWave);
-  if (__any(!(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3])))) {
+  if (__any(!none && !(finite(o[0]) && finite(o[1]) && finite(o[2]) && finite(o[3])))) {
     f32x4_t whole = {0, 0, 0, 0};  // of the parts that are not finite, whatever their weight
 #pragma unroll 1
     for (int i = 0; i < n; i += kAhead * kParts) {
@@ -815,10 +816,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
 #pragma unroll
           for (int e = 0; e < DV; ++e) o[e / 4][e % 4] += acc_lds[w][rr][col + e] * f;
         }
-        const int lim = args.causal ? seg.len - seg.fresh + quot(rr, args.G) + 1 : seg.len;
-        restore<DV / 4, 4>(o, args, keys_of(args, seg), seg.t0 * kTile, seg.t1 * kTile, lim, col);
+        const int token = quot(rr, args.G);
+        const int lim = args.causal ? seg.len - seg.fresh + token + 1 : seg.len;
+        restore<DV / 4, 4>(o, token < seg.fresh && sum == sum, args, keys_of(args, seg),
+                           seg.t0 * kTile, seg.t1 * kTile, lim, col);
         if (whole) {
-          const bool none = quot(rr, args.G) >= seg.fresh || sum == 0.0f;
+          const bool none = token >= seg.fresh || sum == 0.0f;
           const float inv = 1.0f / sum;
           uint32_t* op = reinterpret_cast<uint32_t*>(out_row(args, seg.b, seg.h, rr) + col);
 #pragma unroll
@@ -1044,19 +1047,18 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_many_kernel
     const bool whole = seg.t0 == 0 && seg.t1 == seg.tiles;
     const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-      restore<DV, 16>(r.acc[nt], args, keys_of(args, seg), seg.t0 * kStep, t1 * kStep, r.lim[nt],
-                      4 * g4);
-#pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       float sum = r.l[nt];
       sum += __shfl_xor(sum, 16, kWave);
       sum += __shfl_xor(sum, 32, kWave);
       const int row = r0 + nt * 16 + n16;
+      const bool padded = quot(row, args.G) >= seg.fresh;
+      restore<DV, 16>(r.acc[nt], !padded && sum == sum, args, keys_of(args, seg), seg.t0 * kStep,
+                      t1 * kStep, r.lim[nt], 4 * g4);
       if (row >= rows) continue;
       // a lane's columns: 16 e + 4 g4 .. + 4
       if (whole) {
-        const bool none = quot(row, args.G) >= seg.fresh || sum == 0.0f;
+        const bool none = padded || sum == 0.0f;
         const float inv = 1.0f / sum;
         uint16_t* op = out_row(args, seg.b, seg.h, row) + 4 * g4;
 #pragma unroll
