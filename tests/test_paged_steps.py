@@ -88,3 +88,16 @@ def test_modes_see_the_attention_that_the_kernel_would_replace():
         with mode:
             assert not ok(attn, q, None, {})
     assert ok(attn, q, None, {})
+
+
+@pytest.mark.parametrize("kind,ok", [("default", True), ("linear", True), ("yarn", True),
+                                     ("dynamic", False), ("longrope", False)])
+def test_rotary_modules_whose_frequencies_change(kind, ok):
+    """A plan holds the frequencies as they are; a module that changes them later has none."""
+    rot = torch.nn.Module()
+    rot.inv_freq, rot.rope_type, rot.attention_scaling = torch.ones(32), kind, 1.5
+    if ok:
+        assert axial.AxisPlan.rotary(rot).scale == 1.5
+    else:
+        with pytest.raises(ValueError, match="rope type"):
+            axial.AxisPlan.rotary(rot)

@@ -80,7 +80,11 @@ class AxisPlan:
     @classmethod
     def rotary(cls, module: torch.nn.Module) -> "AxisPlan":
         """The plan of a transformers text rotary module: its ``inv_freq``,
-        ``mrope_section`` (interleaved) and ``attention_scaling``."""
+        ``mrope_section`` (interleaved) and ``attention_scaling``.  A module that changes
+        its frequencies with the longest position it meets is refused."""
+        kind = str(getattr(module, "rope_type", "default"))
+        if "dynamic" in kind or kind == "longrope":
+            raise ValueError(f"AxisPlan.rotary: frequencies of rope type {kind!r} follow the length")
         inv = module.inv_freq
         sections = list(getattr(module, "mrope_section", None) or [inv.shape[0]])
         plan = cls.text(2 * inv.shape[0], 1e4, sections, device="cpu")
