@@ -28,10 +28,10 @@
 // to 16 rows and with counters to find that out, else by a second kernel.
 //
 // Measured, 32 query heads over 8 of 128: a token of two requests of 131001 keys each
-// 173 us (6.2 TB/s), of 64 ragged requests up to 8192 keys 54 (4.7 TB/s), of one
-// request of 3100 keys 9.5: 4 until its first keys are there, 1.7 for them, 3 to join
-// 25 parts.  128 tokens over 65536 keys 230 us (595 TFLOP/s); four 128-token chunks
-// 46, of which the second kernel takes 13 for 41 MB of parts.
+// 173 us (6.2 TB/s), of 64 ragged requests up to 8192 keys 49 (5.1 TB/s), of one
+// request of 3100 keys 9.9: 4 until its first keys are there, 1.7 for them, 3 to join
+// 25 parts.  128 tokens over 65536 keys 233 us (590 TFLOP/s); four 128-token chunks
+// 47, of which the second kernel takes 13 for 41 MB of parts.
 #include <algorithm>
 
 #include "common.hpp"
@@ -825,7 +825,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend_few_kernel(
           const float inv = 1.0f / sum;
           uint32_t* op = reinterpret_cast<uint32_t*>(out_row(args, seg.b, seg.h, rr) + col);
 #pragma unroll
-          for (int w = 0; w < VW; ++w) op[w] = none ? 0 : pack2(o[w / 2][w % 2 * 2] * inv, o[w / 2][w % 2 * 2 + 1] * inv);
+          for (int w = 0; w < VW; ++w) {
+            const f32x4_t& x = o[w / 2];
+            op[w] = none ? 0 : pack2(x[w % 2 * 2] * inv, x[w % 2 * 2 + 1] * inv);
+          }
         } else {
           const int64_t at = (int64_t)slot * 16 + rr;
 #pragma unroll
@@ -908,9 +911,9 @@ __device__ __forceinline__ void load_to_lds(const void* base, unsigned off, unsi
 // took 12% longer).  A row's 16-byte chunks are permuted so that neither the reads
 // of a chunk down the rows (K: ^ row) nor those of two chunks of eight rows (V: ^ 2
 // row) meet in a bank.
-// What bounds it: of a step's 4000 cycles for two waves of a SIMD the matrix
+// What bounds it: of a step's 3900 cycles for two waves of a SIMD the matrix
 // instructions take 1540 (48 a wave, the second product twice) and the vector ones
-// 1880 (190 a wave, 16 of them exponentials), which run beside the former for a
+// 1800 (177 a wave, 16 of them exponentials), which run beside the former for a
 // quarter of their time.  Matrix and vector instructions in turn, priorities, the
 // next K read early, a barrier for two steps, eight waves that halve the parts: none
 // was faster (128 tokens over 65536 keys stayed within 2%, the last cost the chunks

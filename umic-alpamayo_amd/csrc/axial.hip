@@ -14,7 +14,7 @@
 // workgroup takes a few tokens: its threads' first loads are on their way while
 // the tokens' D/2 sines and cosines are formed, once for all heads, in LDS.  32 + 8
 // heads of 128 into the pages: 16381 tokens 67 us, at the copy of their bytes (5.9
-// TB/s); 3100 with the norm 16.8, 12% over it; 8 tokens 4.5.
+// TB/s); 3100 with the norm 16.8, 12% over it; 8 tokens 5.2.
 #include "common.hpp"
 #include "gemm_ks.hpp"  // device_cus
 

@@ -13,7 +13,7 @@
 // Latency: a step of eight requests moves a few hundred bytes.  One workgroup does
 // all that depends on the sums over requests, with one scan of all of them at once
 // for up to kPlanThreads requests, and the slots of up to kSlotsHere tokens; more
-// tokens' slots are a second launch's.  8 requests' tokens 3.7 us, a launch being 2.3;
+// tokens' slots are a second launch's.  8 requests' tokens 3.5 us, a launch being 2.3;
 // 256 requests, half of them anew, with 34816 slots 7 and 4.
 #include "common.hpp"
 
