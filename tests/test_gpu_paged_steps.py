@@ -274,3 +274,28 @@ def test_workspaces_of_many_streams():
         assert torch.equal(o, want)
     for counters, _ in attention._SCRATCH.values():
         assert not counters.any()
+
+
+def test_positions_that_stand_for_several_requests():
+    """One row of position ids for all requests is compared with each, as are those of embeddings."""
+    m, _ = text_model()
+    c = PagedKVCache.for_model(m, requests=2, pages=12, max_tokens=64, page_size=16)
+    ids = torch.randint(0, 512, (2, 6), generator=torch.Generator().manual_seed(9)).to(DEV)
+    row = torch.arange(6, device=DEV)[None]
+    with torch.no_grad():
+        emb = m.embed_tokens(ids)
+        for pos in (row, row[None].expand(3, 1, 6), None):
+            c.reset()
+            c.begin(6)
+            got = m(inputs_embeds=emb, position_ids=pos, past_key_values=c).last_hidden_state
+        for pos in (row + 1, row[None].expand(3, 1, 6) * 2, row[:, :3], row[:, :5], row[None, None]):
+            for tokens in ({"input_ids": ids}, {"inputs_embeds": emb}):
+                with pytest.raises(ValueError, match="position_ids"):
+                    m(**tokens, position_ids=pos, past_key_values=c)
+        c.begin([1, 1], keep=[3, None])  # requests that are not alike
+        last = torch.tensor([[3]], device=DEV)
+        with pytest.raises(ValueError, match="position_ids"):
+            m(input_ids=ids[:, :1], position_ids=last, past_key_values=c)
+        c.reset()
+        c.begin(6)
+        assert torch.equal(m(input_ids=ids, past_key_values=c).last_hidden_state, got)

@@ -135,7 +135,10 @@ def _refuse(module, args, kwargs):
     positions = kwargs.get("position_ids", args[2] if len(args) > 2 else None)
     cache = kwargs.get("past_key_values", args[3] if len(args) > 3 else None)
     if isinstance(cache, PagedKVCache):
-        if positions is not None and not cache.turns_by(positions):
+        tokens = kwargs.get("input_ids", args[0] if args else None)
+        if tokens is None:
+            tokens = kwargs.get("inputs_embeds", args[4] if len(args) > 4 else None)
+        if positions is not None and cache.planned(tokens) and not cache.turns_by(positions):
             raise ValueError("PagedKVCache: position_ids are not those of its step, which its "
                              "attention turns by: give them to begin(), and the forward "
                              "cache.position_ids")
@@ -223,25 +226,28 @@ class PagedKVCache(DynamicCache):
         """The open step's positions, [axes, requests, S], as the model takes them."""
         return self._positions.reshape(-1, self.arena.requests, self.tokens)
 
+    def planned(self, tokens: torch.Tensor | None) -> bool:
+        """Whether a forward's input is the open step's by its shape ([requests, S, ..]);
+        ``attend`` refuses others."""
+        return (self.step is not None and tokens is not None
+                and tuple(tokens.shape[:2]) == (self.arena.requests, self.tokens))
+
     def turns_by(self, positions: torch.Tensor) -> bool:
         """Whether a forward's position ids are the open step's for its tokens: this
         object's own without a look at them, others by their values (a wait for the
-        device, and no for a capture).  [requests, S] count for every axis, and a row of
-        text positions ahead of the axes' does not."""
-        B, S = self.arena.requests, self.tokens
-        if self.step is None or tuple(positions.shape[-2:]) != (B, S):
-            return True  # attend() refuses the forward
+        device, and no for a capture).  Those of fewer axes or requests count for all,
+        and a row of text positions ahead of the axes' does not count."""
         mine = self.position_ids
         if positions.dim() == 3 and positions.shape[0] == mine.shape[0] + 1:
             positions = positions[1:]
         if (positions.data_ptr() == mine.data_ptr() and positions.dtype is mine.dtype
                 and positions.shape == mine.shape and positions.stride() == mine.stride()):
             return True
-        if (positions.device != mine.device or positions.dim() not in (2, 3)
-                or positions.dim() == 3 and positions.shape[0] not in (1, mine.shape[0])
+        if (positions.device != mine.device or positions.dim() > 3
+                or any(n not in (1, m) for n, m in zip(positions.shape[::-1], mine.shape[::-1]))
                 or torch.cuda.is_current_stream_capturing()):
             return False
-        there = self.step.slots.view(B, S) >= 0
+        there = self.step.slots.view(mine.shape[1:]) >= 0
         return not bool(((positions != mine) & there).any())
 
     def attend(self, layer: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, norm,
