@@ -1,0 +1,437 @@
+// A paged key / value cache in 8 bits: new tokens' rows rotated and written as codes, and
+// rows read back as bf16.
+//
+// A block is 16 consecutive rows of a page, of one key head.  With a = max |x| over the
+// values that come into it, its scale is s = 2^e, e = floor(log2 a) - 6 (int8) or - 7
+// (e4m3), and at least what it was where the block holds tokens already; its codes are
+// x / s to the nearest, ties to even.  Where the scale grows, the codes of the rows before
+// are rounded to it: it at least doubles, so that all roundings of such a row are within
+// half a step of the last scale and a half of that, and so on: one step.  The scale is
+// that of bf16 values' exponents, whole numbers throughout.
+//
+// The tokens of a block that one call brings stand within kSpan neighbours, so that a wave
+// finds by its lanes which are a block's, and which is its first: that one's workgroup
+// writes all of them.  A wave does one head of them, keys or values, at a time, as
+// `rotate` would lay their rows out over the lanes: the bits are those of `rotate`'s rows,
+// quantised.
+#include "axial.hpp"
+#include "codes.hpp"
+
+namespace umic {
+namespace {
+
+constexpr int kWaves = kThreads / kWave;
+constexpr int kSpan = 24;    // tokens that hold all of a block's
+constexpr int kChunk = 16;   // tokens of a workgroup, at most
+static_assert(kChunk + 2 * (kSpan - 1) <= kWave, "a wave sees a chunk and what may share its blocks");
+
+struct StoreArgs {
+  AxialArgs x;  // of q's rows: Hq heads, no keys; and what k's rotation needs
+  const uint16_t* k;
+  const uint16_t* v;
+  uint8_t* k8;
+  uint8_t* v8;
+  float* ks;
+  float* vs;
+  int64_t Hk, k_st, k_sh, v_st, v_sh;
+  int64_t c_sb, c_sh, c_ss, s_sb, s_sh;
+  int64_t slots_n;
+  int shift;         // of a page
+  int chunk;         // tokens of a workgroup: it does the blocks whose first is among them
+  int groups;        // of key heads, a workgroup each
+  int heads;         // of a group
+  unsigned blocks;   // workgroups that do so; those behind them rotate q
+};
+
+__device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
+  typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+  const u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b));
+  return __builtin_bit_cast(uint32_t, m);
+}
+
+template <int D, int FORMAT, bool TURN, bool NORM>
+__global__ __launch_bounds__(kThreads) void store_kernel(StoreArgs a) {
+  typedef Codes<FORMAT> C;
+  constexpr int kLanes = D / 16;            // of a row, 8 elements of each half a lane
+  constexpr int kRows = kWave / kLanes;     // rows of a pass
+  constexpr int kPasses = kBlockTokens / kRows;
+  constexpr int kOld = D / 64;              // 16-byte chunks of a block's codes a lane holds
+  extern __shared__ float cs[];             // [token of the run][pair] (cos, sin)
+  __shared__ int places[kBlockTokens];
+  if (blockIdx.x >= a.blocks) {
+    if constexpr (TURN) axial_rows<8, NORM, (D >= 128)>(a.x, blockIdx.x - a.blocks, cs);
+    return;
+  }
+  const int lane = threadIdx.x & (kWave - 1);
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+  const unsigned per = 2 * a.groups;
+  const int64_t t0 = (int64_t)(blockIdx.x / per) * a.chunk;
+  const int part = blockIdx.x % per;
+  const bool keys = part < a.groups;
+  const int h0 = (keys ? part : part - a.groups) * a.heads;
+  const int h1 = min((int)a.Hk, h0 + a.heads);
+  const uint16_t* const src = keys ? a.k : a.v;
+  const int64_t st = keys ? a.k_st : a.v_st, sh = keys ? a.k_sh : a.v_sh;
+  uint8_t* const codes = keys ? a.k8 : a.v8;
+  float* const scales = keys ? a.ks : a.vs;
+
+  // lane i: token t0 - (kSpan - 1) + i, its block and row; a slot outside the pool has none
+  const int64_t base = t0 - (kSpan - 1);
+  const int64_t tok = base + lane;
+  int64_t slot = -1;
+  if (lane < a.chunk + 2 * (kSpan - 1) && tok >= 0 && tok < a.x.T) slot = a.x.slots[tok];
+  const int block = slot >= 0 && slot < a.slots_n ? (int)(slot / kBlockTokens) : -1;
+  const int row = (int)(slot & (kBlockTokens - 1));
+
+  for (int c = 0; c < a.chunk; ++c) {
+    const int at = kSpan - 1 + c;
+    const int blk = __builtin_amdgcn_readlane(block, at);
+    const uint64_t mates = __ballot(block == blk);
+    // a block is its first token's to write
+    if (blk < 0 || mates << (64 - at) >> (64 - (kSpan - 1))) continue;
+    const uint64_t run = mates >> at << (64 - kSpan) >> (64 - kSpan) << at;
+    const int n = min(kBlockTokens, __builtin_popcountll(run));
+    // lane i: where the run's token i stands, and its row
+    const int below = __builtin_popcountll(run & (((uint64_t)1 << lane) - 1));
+    const int there = run >> lane & 1 ? below : __builtin_popcountll(run) + lane - below;
+    const int place = __builtin_amdgcn_ds_permute(there * 4, lane);
+    const int its_row = __shfl(row, place, kWave);
+    int row0 = lane < n ? its_row : kBlockTokens;  // the lowest
+#pragma unroll
+    for (int m = 1; m < kBlockTokens; m <<= 1) row0 = min(row0, __shfl_xor(row0, m, kWave));
+    row0 = __builtin_amdgcn_readfirstlane(row0);
+    const int64_t in = (int64_t)blk * kBlockTokens;
+    const int64_t page = in >> a.shift;
+    const int64_t r0 = in & (((int64_t)1 << a.shift) - 1);
+    if constexpr (TURN) {
+      __syncthreads();  // the last run's turns have been read
+      if (threadIdx.x < kBlockTokens) places[threadIdx.x] = place;
+      __syncthreads();
+      if (keys)
+        for (int i = threadIdx.x; i < n * (D / 2); i += kThreads) {
+          const int f = i % (D / 2), t = i / (D / 2);
+          const int64_t of = base + places[t];
+          const int ax = a.x.axis[f];
+          float s = 0.0f, c = 1.0f;
+          if (ax >= 0 && ax < a.x.A) {
+            const int64_t pos = a.x.positions[ax * a.x.p_sa + of * a.x.p_st];
+            const int32_t frac = (int32_t)(((uint64_t)pos * a.x.turn[f]) >> 32);
+            sincospif((float)frac * 0x1p-31f, &s, &c);
+          }
+          cs[2 * i] = c * a.x.scale;
+          cs[2 * i + 1] = s * a.x.scale;
+        }
+      __syncthreads();
+    }
+    const int c8 = (lane % kLanes) * 8;
+    for (int h = h0 + wave; h < h1; h += kWaves) {
+      uint8_t* const to = codes + page * a.c_sb + h * a.c_sh + r0 * a.c_ss;
+      float* const scale = scales + page * a.s_sb + h * a.s_sh + r0 / kBlockTokens;
+      u32x4 lo[kPasses], hi[kPasses], old[kOld];
+      int at_row[kPasses];  // -1: no token
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        const int i = p * kRows + lane / kLanes;
+        at_row[p] = __shfl(its_row, i, kWave);
+        const int64_t of = base + __shfl(place, i, kWave);
+        if (i >= n) at_row[p] = -1;
+        lo[p] = hi[p] = u32x4{0, 0, 0, 0};
+        if (i < n) {
+          const uint16_t* from = src + of * st + h * sh + c8;
+          lo[p] = ld_stream(reinterpret_cast<const u32x4*>(from));
+          hi[p] = ld_stream(reinterpret_cast<const u32x4*>(from + D / 2));
+        }
+      }
+      float was = 0.0f;
+      if (row0 > 0) {
+        was = *scale;
+#pragma unroll
+        for (int j = 0; j < kOld; ++j) {
+          const int c = j * kWave + lane, r = c / (D / 16);
+          old[j] = u32x4{0, 0, 0, 0};
+          if (r < row0) old[j] = *reinterpret_cast<const u32x4*>(to + r * a.c_ss + c % (D / 16) * 16);
+        }
+      }
+      if constexpr (TURN)
+        if (keys)
+#pragma unroll
+          for (int p = 0; p < kPasses; ++p) {
+            const int i = min(p * kRows + lane / kLanes, n - 1);
+            float x[8], y[8], ox[8], oy[8];
+            unpack8(lo[p], x);
+            unpack8(hi[p], y);
+            if constexpr (NORM) {
+              float ss = 0.0f;
+#pragma unroll
+              for (int j = 0; j < 8; ++j) ss += x[j] * x[j] + y[j] * y[j];
+#pragma unroll
+              for (int m = 1; m < kLanes; m <<= 1) ss += __shfl_xor(ss, m, kWave);
+              const float r = rsqrt_cr(ss / (float)D + a.x.eps);
+              float wx[8], wy[8];
+              unpack8(*reinterpret_cast<const u32x4*>(a.x.kw + c8), wx);
+              unpack8(*reinterpret_cast<const u32x4*>(a.x.kw + c8 + D / 2), wy);
+#pragma unroll
+              for (int j = 0; j < 8; ++j) {
+                x[j] = x[j] * r * wx[j];
+                y[j] = y[j] * r * wy[j];
+              }
+            }
+            const float* t = cs + 2 * (i * (D / 2) + c8);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+              ox[j] = x[j] * t[2 * j] - y[j] * t[2 * j + 1];
+              oy[j] = y[j] * t[2 * j] + x[j] * t[2 * j + 1];
+            }
+            const bool there = at_row[p] >= 0;
+            lo[p] = there ? pack8(ox) : u32x4{0, 0, 0, 0};
+            hi[p] = there ? pack8(oy) : u32x4{0, 0, 0, 0};
+          }
+      // the largest magnitude's exponent: that of bf16 numbers as whole ones
+      uint32_t top = 0;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          top = max_halves(top, max_halves(lo[p][w] & 0x7fff7fffu, hi[p][w] & 0x7fff7fffu));
+#pragma unroll
+      for (int m = 1; m < kWave; m <<= 1) top = max_halves(top, __shfl_xor(top, m, kWave));
+      const int most = __builtin_amdgcn_readfirstlane(max(top & 0xffffu, top >> 16));
+      const uint32_t was_bits = __builtin_amdgcn_readfirstlane(__float_as_uint(was));
+      // 255: infinite or NaN; the block then reads as NaN
+      const bool wild = (most >> 7) == 255 || (row0 > 0 && (was_bits << 1) >= 0xff000000u);
+      const int was_exp = (int)(was_bits >> 23 & 255) - 127;
+      int e = max((most >> 7) - 127 - C::kTop, kLeastExp);
+      if (row0 > 0) e = max(e, was_exp);
+      const float s = __uint_as_float((uint32_t)(e + 127) << 23);
+      const float inv = wild ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+      if (lane == 0) *scale = wild ? __builtin_nanf("") : s;
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        if (at_row[p] < 0) continue;
+        float x[8], y[8];
+        unpack8(lo[p], x);
+        unpack8(hi[p], y);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          x[j] = wild ? 0.0f : x[j] * inv;
+          y[j] = wild ? 0.0f : y[j] * inv;
+        }
+        uint8_t* r = to + at_row[p] * a.c_ss + c8;
+        *reinterpret_cast<u32x2*>(r) = u32x2{C::round4(x), C::round4(x + 4)};
+        *reinterpret_cast<u32x2*>(r + D / 2) = u32x2{C::round4(y), C::round4(y + 4)};
+      }
+      if (row0 > 0 && !wild && e > was_exp) {  // the rows before, at the new scale
+        const float ratio = was * inv;
+#pragma unroll
+        for (int j = 0; j < kOld; ++j) {
+          const int c = j * kWave + lane, r = c / (D / 16);
+          if (r >= row0) continue;
+          u32x4 w;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float x[4];
+            C::values4(old[j][i], x);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) x[k] *= ratio;
+            w[i] = C::round4(x);
+          }
+          *reinterpret_cast<u32x4*>(to + r * a.c_ss + c % (D / 16) * 16) = w;
+        }
+      }
+    }
+  }
+}
+
+struct ReadArgs {
+  const uint8_t* k8;
+  const uint8_t* v8;
+  const float* ks;
+  const float* vs;
+  uint16_t* ko;
+  uint16_t* vo;
+  const int32_t* table;
+  const int32_t* kv_len;  // or NULL: len
+  const int32_t* start;   // or NULL: 0
+  int64_t c_sb, c_sh, c_ss, s_sb, s_sh, table_ld;
+  int64_t rows, blocks;
+  int len, cap, shift, pages, Hk;
+};
+
+// A thread's 16 codes to 32 bytes; a workgroup does 16 rows' or more of one head.
+template <int D, int FORMAT>
+__global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
+  typedef Codes<FORMAT> C;
+  constexpr int kChunks = D / 16, kRows = kThreads / kChunks;
+  const int64_t tile = blockIdx.x % a.blocks;
+  const int64_t head = blockIdx.x / a.blocks;  // (k or v, request, key head)
+  const int h = (int)(head % a.Hk);
+  const int64_t rest = head / a.Hk;
+  const int b = (int)(rest >> 1);
+  const bool keys = !(rest & 1);
+  const int64_t row = tile * kRows + threadIdx.x / kChunks;
+  const int c = threadIdx.x % kChunks * 16;
+  if (row >= a.rows) return;
+  const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.cap) : a.len;
+  const int64_t at = row + (a.start ? max(a.start[b], 0) : 0);
+  u32x4 out[2] = {};
+  if (at < n) {
+    const int page = a.table[b * a.table_ld + (at >> a.shift)];
+    if ((unsigned)page < (unsigned)a.pages) {
+      const int64_t in = at & (((int64_t)1 << a.shift) - 1);
+      const u32x4 w = ld_stream(reinterpret_cast<const u32x4*>(
+          (keys ? a.k8 : a.v8) + page * a.c_sb + h * a.c_sh + in * a.c_ss + c));
+      const float s = (keys ? a.ks : a.vs)[page * a.s_sb + h * a.s_sh + in / kBlockTokens];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        float x[4];
+        C::values4(w[i], x);
+        out[i / 2][i % 2 * 2] = pack2(x[0] * s, x[1] * s);
+        out[i / 2][i % 2 * 2 + 1] = pack2(x[2] * s, x[3] * s);
+      }
+    }
+  }
+  u32x4* to = reinterpret_cast<u32x4*>(
+      (keys ? a.ko : a.vo) + (((int64_t)b * a.Hk + h) * a.rows + row) * D + c);
+  st_stream(to, out[0]);
+  st_stream(to + 1, out[1]);
+}
+
+template <int D, int FORMAT>
+int launch_store(StoreArgs& a, bool turn, hipStream_t st) {
+  unsigned grid = 0;
+  size_t lds = 0;
+  if (turn && a.x.Hq) {
+    AxialShape s;
+    if (const int e = axial_shape(a.x, s)) return e;
+    if (s.vec != 8) return UMIC_ERR_UNSUPPORTED;
+    grid = s.blocks;
+    lds = s.lds;
+  }
+  if (turn) lds = std::max(lds, (size_t)kBlockTokens * D * sizeof(float));
+  a.chunk = a.x.T <= 2048 ? 1 : kChunk;
+  a.heads = kWaves;
+  a.groups = (int)((a.Hk + a.heads - 1) / a.heads);
+  const int64_t blocks = (a.x.T + a.chunk - 1) / a.chunk * 2 * a.groups;
+  if (blocks + grid > 0x7fffffff) return UMIC_ERR_UNSUPPORTED;
+  a.blocks = (unsigned)blocks;
+  auto* kern = !turn    ? store_kernel<D, FORMAT, false, false>
+               : a.x.kw ? store_kernel<D, FORMAT, true, true>
+                        : store_kernel<D, FORMAT, true, false>;
+  hipLaunchKernelGGL(kern, dim3(a.blocks + grid), dim3(kThreads), lds, st, a);
+  return launch_status();
+}
+
+template <int D, int FORMAT>
+int launch_read(const ReadArgs& a, int64_t heads, hipStream_t st) {
+  hipLaunchKernelGGL((read_kernel<D, FORMAT>), dim3((unsigned)(a.blocks * heads)), dim3(kThreads),
+                     0, st, a);
+  return launch_status();
+}
+
+bool codes_ok(int64_t D, int64_t pages, int64_t page_size, int format) {
+  return (D == 64 || D == 128 || D == 256) && page_size >= 16 &&
+         !(page_size & (page_size - 1)) && page_size <= ((int64_t)1 << 30) &&
+         pages <= ((int64_t)1 << 30) && pages * page_size <= ((int64_t)1 << 34) &&
+         (format == UMIC_CODES_E4M3 || format == UMIC_CODES_INT8);
+}
+
+}  // namespace
+}  // namespace umic
+
+extern "C" int umic_cache8_append_bf16(
+    const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes,
+    float* k_scale, float* v_scale, const int64_t* positions, const uint64_t* turn,
+    const int32_t* axis, const int64_t* slots, float scale, const void* q_w, const void* k_w,
+    float eps, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t axes, int64_t p_sa,
+    int64_t p_st, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
+    int64_t v_sh, int64_t qo_st, int64_t qo_sh, int64_t c_sb, int64_t c_sh, int64_t c_ss,
+    int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size, int format, void* stream) {
+  using namespace umic;
+  if (T < 0 || Hq < 0 || Hk <= 0 || D <= 0 || pages < 0 || page_size <= 0)
+    return UMIC_ERR_INVALID_ARG;
+  if (T == 0) return UMIC_OK;
+  if (!k || !v || !slots) return UMIC_ERR_INVALID_ARG;
+  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return UMIC_ERR_INVALID_ARG;
+  if (turn) {
+    if (axes <= 0 || !positions || !axis || (Hq && (!q || !q_out)) || (!q_w != !k_w))
+      return UMIC_ERR_INVALID_ARG;
+  } else if (Hq || q_w || k_w) {
+    return UMIC_ERR_INVALID_ARG;
+  }
+  if (!codes_ok(D, pages, page_size, format) || Hq > (1 << 16) || Hk > (1 << 16))
+    return UMIC_ERR_UNSUPPORTED;
+  if (((q_st | q_sh | k_st | k_sh | v_st | v_sh | qo_st | qo_sh) & 7) ||
+      ((c_sb | c_sh | c_ss) & 15) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
+      !aligned16(q_out) || !aligned16(k_codes) || !aligned16(v_codes) || !aligned16(q_w) ||
+      !aligned16(k_w))
+    return UMIC_ERR_UNSUPPORTED;
+  StoreArgs a = {};
+  a.x.q = (const uint16_t*)q, a.x.qo = (uint16_t*)q_out;
+  a.x.positions = positions, a.x.turn = turn, a.x.axis = axis;
+  a.x.qw = (const uint16_t*)q_w, a.x.kw = (const uint16_t*)k_w;
+  a.x.T = T, a.x.Hq = Hq, a.x.D = D, a.x.A = axes, a.x.p_sa = p_sa, a.x.p_st = p_st;
+  a.x.q_st = q_st, a.x.q_sh = q_sh, a.x.qo_st = qo_st, a.x.qo_sh = qo_sh;
+  a.x.eps = eps, a.x.scale = scale;
+  a.x.slots = slots;
+  a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
+  a.k8 = (uint8_t*)k_codes, a.v8 = (uint8_t*)v_codes, a.ks = k_scale, a.vs = v_scale;
+  a.Hk = Hk, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = c_ss, a.s_sb = s_sb, a.s_sh = s_sh;
+  a.slots_n = pages * page_size;
+  a.shift = __builtin_ctzll((unsigned long long)page_size);
+  hipStream_t st = as_stream(stream);
+  const bool t = turn != nullptr, f = format == UMIC_CODES_INT8;
+  if (D == 64)
+    return f ? launch_store<64, UMIC_CODES_INT8>(a, t, st) : launch_store<64, UMIC_CODES_E4M3>(a, t, st);
+  if (D == 128)
+    return f ? launch_store<128, UMIC_CODES_INT8>(a, t, st)
+             : launch_store<128, UMIC_CODES_E4M3>(a, t, st);
+  return f ? launch_store<256, UMIC_CODES_INT8>(a, t, st) : launch_store<256, UMIC_CODES_E4M3>(a, t, st);
+}
+
+extern "C" int umic_cache8_read_bf16(const void* k_codes, const void* v_codes, const float* k_scale,
+                                     const float* v_scale, void* k_out, void* v_out,
+                                     const int32_t* table, const int32_t* kv_lens,
+                                     const int32_t* starts, int64_t B, int64_t Hk, int64_t rows,
+                                     int64_t D, int64_t c_sb, int64_t c_sh, int64_t c_ss,
+                                     int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size,
+                                     int64_t table_ld, int64_t table_w, int64_t kv_len, int format,
+                                     void* stream) {
+  using namespace umic;
+  if (B < 0 || Hk <= 0 || rows < 0 || D <= 0 || pages < 0 || page_size <= 0 || table_w < 0 ||
+      table_ld < table_w)
+    return UMIC_ERR_INVALID_ARG;
+  if (B == 0 || rows == 0) return UMIC_OK;
+  if (!k_out || !v_out || !table) return UMIC_ERR_INVALID_ARG;
+  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return UMIC_ERR_INVALID_ARG;
+  if (!codes_ok(D, pages, page_size, format) || table_w > ((int64_t)1 << 30) / page_size ||
+      Hk > (1 << 16) || B > (1 << 20) || rows > ((int64_t)1 << 31))
+    return UMIC_ERR_UNSUPPORTED;
+  const int64_t cap = pages ? table_w * page_size : 0;
+  if (!kv_lens && (kv_len < 0 || kv_len > cap)) return UMIC_ERR_INVALID_ARG;
+  if (((c_sb | c_sh | c_ss) & 15) || !aligned16(k_codes) || !aligned16(v_codes) ||
+      !aligned16(k_out) || !aligned16(v_out))
+    return UMIC_ERR_UNSUPPORTED;
+  ReadArgs a = {};
+  a.k8 = (const uint8_t*)k_codes, a.v8 = (const uint8_t*)v_codes, a.ks = k_scale, a.vs = v_scale;
+  a.ko = (uint16_t*)k_out, a.vo = (uint16_t*)v_out;
+  a.table = table, a.kv_len = kv_lens, a.start = starts;
+  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = c_ss, a.s_sb = s_sb, a.s_sh = s_sh;
+  a.table_ld = table_ld, a.rows = rows, a.len = (int)kv_len, a.cap = (int)cap;
+  a.shift = __builtin_ctzll((unsigned long long)page_size);
+  a.pages = (int)pages, a.Hk = (int)Hk;
+  const int64_t per = kThreads / (D / 16);
+  a.blocks = (rows + per - 1) / per;
+  const int64_t heads = 2 * B * Hk;
+  if (a.blocks > 0x7fffffff / heads) return UMIC_ERR_UNSUPPORTED;
+  hipStream_t st = as_stream(stream);
+  const bool f = format == UMIC_CODES_INT8;
+  if (D == 64)
+    return f ? launch_read<64, UMIC_CODES_INT8>(a, heads, st)
+             : launch_read<64, UMIC_CODES_E4M3>(a, heads, st);
+  if (D == 128)
+    return f ? launch_read<128, UMIC_CODES_INT8>(a, heads, st)
+             : launch_read<128, UMIC_CODES_E4M3>(a, heads, st);
+  return f ? launch_read<256, UMIC_CODES_INT8>(a, heads, st)
+           : launch_read<256, UMIC_CODES_E4M3>(a, heads, st);
+}

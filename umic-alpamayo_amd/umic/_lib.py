@@ -32,6 +32,8 @@ UMIC_ACT_NONE = 0
 UMIC_ACT_GELU = 1
 UMIC_ACT_GELU_TANH = 2
 UMIC_ATTENTION_COUNTERS = 4096  # counters of umic_cache_attention_bf16
+UMIC_CODES_E4M3 = 0  # code types of umic_cache8_*
+UMIC_CODES_INT8 = 1
 UMIC_STREAM_READ_GRID = 2048  # fold words umic_stream_read writes
 
 _P, _I64, _F32, _I = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float, ctypes.c_int
@@ -69,6 +71,9 @@ SIGNATURES: dict[str, list] = {
     "umic_cache_attention_workspace_bytes": [_I64] * 4,
     "umic_cache_attention_max_requests": [_I64] * 5,
     "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _P, _I64, _P],
+    "umic_cache8_append_bf16": [_P] * 12 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 22 + [_I, _P],
+    "umic_cache8_read_bf16": [_P] * 9 + [_I64] * 14 + [_I, _P],
+    "umic_cache8_attention_bf16": [_P] * 9 + [_I64] * 21 + [_I, _I, _F32, _P, _P, _I64, _P],
     "umic_stream_read": [_P, _I64, _P, _P],
     "umic_stream_copy": [_P, _P, _I64, _P],
     "umic_version": [],

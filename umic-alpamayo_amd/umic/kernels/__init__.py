@@ -26,8 +26,8 @@ def get_kernel(pattern_name: str) -> Callable | None:
 
 
 def _register_builtin() -> None:
-    from umic.kernels import (attention, axial, fused_ffn, layernorm, linear, paged, rmsnorm,
-                              rope)
+    from umic.kernels import (attention, axial, cache8, fused_ffn, layernorm, linear, paged,
+                              rmsnorm, rope)
 
     for name, fn in (
         ("gate_silu_mul", fused_ffn.gate_silu_mul_hip),
@@ -42,6 +42,10 @@ def _register_builtin() -> None:
         ("rope_axial_append", axial.rotate_append),
         ("plan_pages", paged.plan_pages),
         ("cache_attention", attention.cache_attention),
+        ("cache8_rotate_append", cache8.rotate_append),
+        ("cache8_append", cache8.append),
+        ("cache8_read", cache8.read),
+        ("cache8_attention", cache8.attention),
     ):
         _KERNELS[name] = fn
 

@@ -5,7 +5,8 @@ Storage.  ``PagedArena`` holds every layer's pages, ``[layers, 2, pages, kv_head
 page_size, head_dim]`` (a layer's keys and values are what the kernels of
 ``umic.kernels.axial`` and ``umic.kernels.attention`` take), and one set of block
 tables, lengths and free pages for all layers, on the device, with the lengths
-mirrored on the host.
+mirrored on the host.  With ``dtype`` int8 or float8_e4m3fn the pages hold codes of 8
+bits, and ``scales`` theirs (``umic.kernels.cache8``).
 
 A step.  ``cache.begin(new)`` plans it: the tokens each request drops and gets,
 their pages, slots and positions (``paged.plan_pages``).  The model's forward is
@@ -23,7 +24,7 @@ Positions come from the plan (the token's place in its request plus ``delta``) o
 from the caller, through ``begin``, as [axes, requests, S] (image grids); position ids
 of the forward that differ from them are refused.  Numerics are ``axial``'s and
 ``attention``'s: fp32 with one rounding, where the in-place cache repeats the eager
-chain's roundings.
+chain's roundings; and ``cache8``'s, whose rows are rounded to 8-bit codes.
 
 No counterpart in the reference, whose cache is of one batch of equal lengths
 (src/umic/cache.py:25-160).
@@ -36,7 +37,7 @@ from typing import Sequence
 import torch
 from transformers.cache_utils import DynamicCache
 
-from umic.kernels import attention, axial, paged
+from umic.kernels import attention, axial, cache8, paged
 
 
 _ALL = 2 ** 31 - 1  # keep: whatever is held
@@ -46,6 +47,7 @@ class PagedArena:
     """Pages of ``layers`` layers that ``requests`` requests share.
 
     max_tokens: tokens that one request can hold.
+    dtype: of the pages, bf16, or int8 or float8_e4m3fn codes (``cache8``).
 
     ``lens`` and ``free`` mirror the device's lengths and free pages, and ``plan``
     refuses by them what does not fit.  Steps that go past ``plan`` (a captured
@@ -55,18 +57,24 @@ class PagedArena:
     """
 
     def __init__(self, layers: int, requests: int, pages: int, heads: int, page_size: int,
-                 head_dim: int, max_tokens: int, device: torch.device | str = "cuda") -> None:
+                 head_dim: int, max_tokens: int, device: torch.device | str = "cuda",
+                 dtype: torch.dtype = torch.bfloat16) -> None:
         if min(layers, requests, pages, heads, max_tokens) <= 0:
             raise ValueError(f"PagedArena: bad geometry layers={layers} requests={requests} "
                              f"pages={pages} heads={heads} max_tokens={max_tokens}")
         if not paged.page_size_ok(page_size) or head_dim not in attention.HEAD_DIMS:
             raise ValueError(f"PagedArena: page_size {page_size} (powers of two from 16), "
                              f"head_dim {head_dim} (one of {attention.HEAD_DIMS})")
+        if dtype is not torch.bfloat16 and dtype not in cache8.DTYPES:
+            raise ValueError(f"PagedArena: pages of {dtype} (bfloat16, or one of "
+                             f"{list(cache8.DTYPES)})")
         self.page_size, self.requests, self.pages = page_size, requests, pages
         width = -(-max_tokens // page_size)
         self.max_tokens = width * page_size
-        self.storage = torch.empty(layers, 2, pages, heads, page_size, head_dim,
-                                   dtype=torch.bfloat16, device=device)
+        self.storage = torch.empty(layers, 2, pages, heads, page_size, head_dim, dtype=dtype,
+                                   device=device)
+        self.scales = None if dtype is torch.bfloat16 else torch.ones(
+            layers, 2, pages, heads, page_size // cache8.BLOCK, device=device)
         ints = dict(dtype=torch.int32, device=device)
         self.table = torch.zeros(requests, width, **ints)
         self.ring = torch.arange(pages, **ints)
@@ -80,6 +88,22 @@ class PagedArena:
 
     def v(self, layer: int) -> torch.Tensor:
         return self.storage[layer, 1]
+
+    def codes(self, layer: int) -> cache8.Pages8:
+        """A layer's pages of 8-bit codes."""
+        return cache8.Pages8(*self.storage[layer], *self.scales[layer])
+
+    def read(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
+        """A layer's keys and values as bf16, two [requests, heads, n, D]: rows of each
+        request in order, n of the longest, zero past a request's own."""
+        n = max(self.lens)
+        if self.scales is not None:
+            return cache8.read(self.codes(layer), self.table, self.kv_len, n)
+        pages = self.table[:, :-(-n // self.page_size)].clamp(0, self.pages - 1).long()
+        there = torch.arange(n, device=pages.device)[None] < self.kv_len[:, None]
+        k, v = (x[pages].transpose(1, 2).flatten(2, 3)[:, :, :n].masked_fill(
+            ~there[:, None, :, None], 0.0) for x in (self.k(layer), self.v(layer)))
+        return k, v
 
     def _ints(self, values: Sequence[int]) -> torch.Tensor:
         return torch.tensor(values, dtype=torch.int32, device=self.kv_len.device)
@@ -174,14 +198,14 @@ class PagedKVCache(DynamicCache):
 
     @classmethod
     def for_model(cls, lm: torch.nn.Module, requests: int, pages: int, max_tokens: int,
-                  page_size: int = 64) -> "PagedKVCache":
+                  page_size: int = 64, dtype: torch.dtype = torch.bfloat16) -> "PagedKVCache":
         """A cache for the text model ``lm`` (``layers`` with ``self_attn``, and
-        ``rotary_emb``)."""
+        ``rotary_emb``), of bf16 pages or of 8-bit codes (dtype int8, float8_e4m3fn)."""
         attn = lm.layers[0].self_attn
         weight = attn.k_proj.weight
         heads = weight.shape[0] // attn.head_dim
         arena = PagedArena(len(lm.layers), requests, pages, heads, page_size, attn.head_dim,
-                           max_tokens, weight.device)
+                           max_tokens, weight.device, dtype)
         if getattr(lm, "_umic_paged_hook", None) is None:
             lm._umic_paged_hook = lm.register_forward_pre_hook(_refuse, with_kwargs=True)
         return cls(arena, axial.AxisPlan.rotary(lm.rotary_emb),
@@ -260,8 +284,14 @@ class PagedKVCache(DynamicCache):
         if self.step is None or B != ar.requests or S != self.tokens:
             raise RuntimeError(f"PagedKVCache: a forward of {B} x {S} tokens; begin() planned "
                                f"{ar.requests} x {self.tokens}")
-        keys, values = ar.k(layer), ar.v(layer)
         flat = (t.reshape(B * S, -1, D) for t in (q, k, v))
+        if ar.scales is not None:
+            codes = ar.codes(layer)
+            rot = cache8.rotate_append(*flat, self._positions, self.rotary, self.step.slots, codes,
+                                       norm)
+            return cache8.attention(rot.view(B, S, Hq, D).transpose(1, 2), codes, ar.kv_len,
+                                    ar.table, q_len=self._fresh, causal=causal, scale=scale)
+        keys, values = ar.k(layer), ar.v(layer)
         rot = axial.rotate_append(*flat, self._positions, self.rotary, self.step.slots, keys,
                                   values, norm)
         return attention.cache_attention(rot.view(B, S, Hq, D).transpose(1, 2), keys, values,
