@@ -545,11 +545,26 @@ int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void*
                               int32_t* counters, void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
- * New tokens' keys and values into a paged cache of 8-bit codes.  A block is 16
- * consecutive rows of a page, of one key head; its values are code * scale, with
- * k_scale / v_scale[page * s_sb + head * s_sh + row / 16] = 2^e.  Codes: 8-bit floats
- * of 4 exponent and 3 fraction bits without infinities (UMIC_CODES_E4M3), or signed
- * integers in [-127, 127] (UMIC_CODES_INT8).
+ * A paged cache of 8-bit codes.  A block is 16 consecutive rows of a page, of one key head;
+ * its values are code * scale, scale = {k,v}_scale[page * s_sb + head * s_sh + row / 16] =
+ * 2^e.  Codes: 8-bit floats of 4 exponent and 3 fraction bits without infinities
+ * (UMIC_CODES_E4M3), or signed integers in [-127, 127] (UMIC_CODES_INT8), at page * c_sb +
+ * head * c_sh + row * c_ss of k_codes and v_codes, 16-byte aligned, strides multiples of
+ * 16.  head_dim: 64, 128 or 256; page_size: a power of two from 16; at most 2^30 pages and
+ * 2^34 rows of a head.
+ */
+#define UMIC_CODES_E4M3 0
+#define UMIC_CODES_INT8 1
+typedef struct {
+  void *k_codes, *v_codes;
+  float *k_scale, *v_scale;
+  int64_t pages, page_size, heads, head_dim;
+  int64_t c_sb, c_sh, c_ss, s_sb, s_sh;
+  int64_t format;
+} umic_cache8_t;
+
+/*
+ * New tokens' keys and values [T, heads, head_dim] into such a cache.
  * Slots do not repeat, and the tokens whose slots are of one block stand within 24
  * neighbouring tokens (tokens of other blocks, or of none, may stand between them): they
  * are written as a whole.  With a = max |x| over them for a head, and n their lowest row of
@@ -561,38 +576,29 @@ int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void*
  * count as dropped, and are left as they are.  A NaN or an infinity among the values
  * makes its block's scale NaN, until the block is begun anew (n == 0).
  * turn NULL: k's rows are written as they are (Hq 0, q_w and k_w NULL).  Else q and k are
- * turned, and normed, as by umic_axial_rope_bf16, to its bits, before k is written.
- * k, v: T x Hk x D.  Codes: strides (c_sb page, c_sh head, c_ss row), the same for both,
- * multiples of 16; the other strides multiples of 8, pointers of 16-bit and 8-bit elements
- * 16-byte aligned.  D: 64, 128 or 256; page_size: a power of two from 16.  A slot outside
- * [0, pages * page_size) is not written.
+ * turned, and normed, as by umic_axial_rope_bf16, to q_out [T, Hq, head_dim] (contiguous)
+ * and the cache, k by way of bf16.  Strides of q, k and v: multiples of 8, pointers
+ * 16-byte aligned.  A slot outside [0, pages * page_size) is not written.
  * No counterpart in the reference, whose cache holds 16-bit rows (cache.py:50-80).
  */
-#define UMIC_CODES_E4M3 0
-#define UMIC_CODES_INT8 1
-int umic_cache8_append_bf16(const void* q, const void* k, const void* v, void* q_out,
-                            void* k_codes, void* v_codes, float* k_scale, float* v_scale,
-                            const int64_t* positions, const uint64_t* turn, const int32_t* axis,
-                            const int64_t* slots, float scale, const void* q_w, const void* k_w,
-                            float eps, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t axes,
-                            int64_t p_sa, int64_t p_st, int64_t q_st, int64_t q_sh, int64_t k_st,
-                            int64_t k_sh, int64_t v_st, int64_t v_sh, int64_t qo_st,
-                            int64_t qo_sh, int64_t c_sb, int64_t c_sh, int64_t c_ss, int64_t s_sb,
-                            int64_t s_sh, int64_t pages, int64_t page_size, int format,
+int umic_cache8_append_bf16(const umic_cache8_t* cache, const void* q, const void* k,
+                            const void* v, void* q_out, const int64_t* positions,
+                            const uint64_t* turn, const int32_t* axis, const int64_t* slots,
+                            float scale, const void* q_w, const void* k_w, float eps, int64_t T,
+                            int64_t Hq, int64_t axes, int64_t p_sa, int64_t p_st, int64_t q_st,
+                            int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st, int64_t v_sh,
                             void* stream);
 
 /*
- * Rows of such a cache as bf16, exactly: k_out and v_out [B, Hk, rows, D], row i of request
- * b being its token starts[b] + i (starts NULL, or negative: 0).  Tokens from kv_lens[b]
- * (NULL: kv_len for all) on, and those of table entries outside [0, pages), are zero.
+ * Rows of such a cache as bf16, exactly: k_out and v_out [B, heads, rows, head_dim], row i
+ * of request b being its token starts[b] + i (starts NULL, or negative: 0).  Tokens from
+ * kv_lens[b] (NULL: kv_len for all) on, and those of table entries outside [0, pages), are
+ * zero.  table: as in umic_cache_attention_bf16.
  */
-int umic_cache8_read_bf16(const void* k_codes, const void* v_codes, const float* k_scale,
-                          const float* v_scale, void* k_out, void* v_out, const int32_t* table,
-                          const int32_t* kv_lens, const int32_t* starts, int64_t B, int64_t Hk,
-                          int64_t rows, int64_t D, int64_t c_sb, int64_t c_sh, int64_t c_ss,
-                          int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size,
-                          int64_t table_ld, int64_t table_w, int64_t kv_len, int format,
-                          void* stream);
+int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, void* v_out,
+                          const int32_t* table, const int32_t* kv_lens, const int32_t* starts,
+                          int64_t B, int64_t rows, int64_t table_ld, int64_t table_w,
+                          int64_t kv_len, void* stream);
 
 /*
  * umic_cache_attention_bf16 over such a cache: the same rows, lengths, workspace, counters
@@ -600,17 +606,13 @@ int umic_cache8_read_bf16(const void* k_codes, const void* v_codes, const float*
  * whose k or v scale is NaN makes the rows that see one of its keys NaN, and no other; a
  * NaN code of v (umic_cache8_append_bf16 writes none) can reach every row of its request.
  */
-int umic_cache8_attention_bf16(const void* q, const void* k_codes, const void* v_codes,
-                               const float* k_scale, const float* v_scale, void* out,
+int umic_cache8_attention_bf16(const umic_cache8_t* cache, const void* q, void* out,
                                const int32_t* table, const int32_t* kv_lens,
-                               const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t Hk,
-                               int64_t D, int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t o_sb,
-                               int64_t o_ss, int64_t o_sh, int64_t c_sb, int64_t c_sh,
-                               int64_t c_ss, int64_t s_sb, int64_t s_sh, int64_t pages,
-                               int64_t page_size, int64_t table_ld, int64_t table_w,
-                               int64_t kv_len, int format, int causal, float scale,
-                               int32_t* counters, void* workspace, int64_t workspace_bytes,
-                               void* stream);
+                               const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq,
+                               int64_t q_sb, int64_t q_ss, int64_t q_sh, int64_t o_sb,
+                               int64_t o_ss, int64_t o_sh, int64_t table_ld, int64_t table_w,
+                               int64_t kv_len, int causal, float scale, int32_t* counters,
+                               void* workspace, int64_t workspace_bytes, void* stream);
 
 /*
  * Measurement helper: reads `bytes` bytes at p once (16-byte non-temporal

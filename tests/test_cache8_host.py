@@ -2,6 +2,9 @@
 
 from __future__ import annotations
 
+import copy
+import ctypes
+
 import pytest
 import torch
 
@@ -19,62 +22,94 @@ def lib():
     return _lib.load()
 
 
+def struct(**kw):
+    """A cache's description, as (address, structure)."""
+    from umic import _lib
+
+    f = dict(k_codes=FAKE, v_codes=FAKE, k_scale=FAKE, v_scale=FAKE, pages=8, page_size=16, heads=2,
+             head_dim=64, c_sb=2048, c_sh=1024, c_ss=64, s_sb=2, s_sh=1, format=1) | kw
+    c = _lib.Cache8(**f)
+    return ctypes.addressof(c), c
+
+
+CACHE_ARG = [dict(pages=-1), dict(page_size=0), dict(heads=0), dict(head_dim=0), dict(k_codes=None),
+             dict(v_codes=None), dict(k_scale=None), dict(v_scale=None)]
+CACHE_UNS = [dict(head_dim=80), dict(head_dim=512), dict(page_size=8), dict(page_size=24),
+             dict(page_size=1 << 31), dict(pages=1 << 31), dict(pages=1 << 30, page_size=32),
+             dict(heads=1 << 17), dict(format=2), dict(format=-1), dict(c_sb=2056), dict(c_sh=1032),
+             dict(c_ss=72), dict(k_codes=FAKE + 8), dict(v_codes=FAKE + 4)]
+
+
+def test_cache_refusals(lib):
+    """Each entry point's own look at a cache."""
+    def each(**kw):
+        at, keep = struct(**kw)
+        return {lib.umic_cache8_append_bf16(at, *[FAKE] * 8, 1.0, None, None, 1e-6, 3, 4, 3, 3, 1,
+                                            *[256, 64] * 3, None),
+                lib.umic_cache8_read_bf16(at, *[FAKE] * 5, 2, 9, 4, 4, 9, None),
+                lib.umic_cache8_attention_bf16(at, *[FAKE] * 5, 2, 1, 4, *[1024] * 6, 4, 4, 9, 1, 0.1,
+                                               None, FAKE, 1 << 40, None)}
+
+    for bad in CACHE_ARG:
+        assert each(**bad) == {ARG}, bad
+    for bad in CACHE_UNS:
+        assert each(**bad) == {UNS}, bad
+
+
 def test_append_refusals(lib):
-    names = ("q", "k", "v", "qo", "kc", "vc", "ks", "vs", "pos", "turn", "axis", "slots")
+    names = ("cache", "q", "k", "v", "qo", "pos", "turn", "axis", "slots")
+    at, keep = struct()
 
-    def f(T=3, Hq=4, Hk=2, D=128, axes=3, st=1024, c=2048, pages=8, page=16, fmt=0, qw=None, kw=None, **p):
-        p = {n: FAKE for n in names} | p
-        return lib.umic_cache8_append_bf16(
-            *(p[n] for n in names), 1.0, qw, kw, 1e-6, T, Hq, Hk, D, axes, T, 1, st, 128, st, 128, st,
-            128, st, 128, 4096, c, 128, 2, 1, pages, page, fmt, None)
+    def f(T=3, Hq=4, axes=3, st=1024, qw=None, kw=None, **p):
+        p = dict.fromkeys(names, FAKE) | {"cache": at} | p
+        return lib.umic_cache8_append_bf16(*(p[n] for n in names), 1.0, qw, kw, 1e-6, T, Hq, axes, T,
+                                           1, *[st, 64] * 3, None)
 
-    none = dict.fromkeys(names)
-    assert f(T=-1) == f(Hq=-1) == f(Hk=0) == f(D=0) == f(axes=0) == f(pages=-1) == f(page=0) == ARG
-    assert f(T=0, **none) == 0
+    assert f(T=-1) == f(Hq=-1) == f(axes=0) == ARG
+    assert f(T=0, **dict.fromkeys(names[1:])) == 0
     for n in names:
         if n != "turn":
             assert f(**{n: None}) == ARG, n
     assert f(turn=None) == ARG                             # q without a rotation
     assert f(turn=None, Hq=0, kw=FAKE) == f(turn=None, Hq=0, qw=FAKE) == ARG
     assert f(qw=FAKE) == f(kw=FAKE) == ARG                 # one norm without the other
-    assert f(D=80) == f(D=512) == f(page=8) == f(page=24) == f(page=1 << 31) == UNS
-    assert f(fmt=2) == f(fmt=-1) == f(pages=1 << 31) == f(pages=1 << 30, page=32) == UNS
-    assert f(st=1020) == f(c=2056) == f(k=FAKE + 8) == f(kc=FAKE + 8) == f(qw=FAKE + 8, kw=FAKE) == UNS
-    assert f(Hk=1 << 17) == f(T=1 << 40) == UNS
+    assert f(st=1020) == f(k=FAKE + 8) == f(qo=FAKE + 2) == f(qw=FAKE + 8, kw=FAKE) == UNS
+    assert f(Hq=1 << 17) == f(T=1 << 40) == UNS
 
 
 def test_read_refusals(lib):
-    def f(B=2, Hk=2, rows=9, D=64, c=1024, pages=8, page=16, ld=4, w=4, n=9, fmt=1, lens=None,
-          p=(FAKE,) * 7):
-        return lib.umic_cache8_read_bf16(*p, lens, None, B, Hk, rows, D, 4096, c, 64, 2, 1, pages,
-                                         page, ld, w, n, fmt, None)
+    at, keep = struct()
+    none, none_keep = struct(pages=0)
+    tall, tall_keep = struct(heads=1 << 15)
 
-    assert f(B=-1) == f(Hk=0) == f(rows=-1) == f(D=0) == f(pages=-1) == f(page=0) == f(w=-1) == ARG
-    assert f(ld=3) == f(n=65) == f(n=-1) == f(pages=0) == ARG
-    assert f(B=0, p=(None,) * 7) == f(rows=0, p=(None,) * 7) == 0
-    for i in range(7):
-        assert f(p=tuple(None if j == i else FAKE for j in range(7))) == ARG, i
-    assert f(D=80) == f(page=8) == f(page=48) == f(fmt=7) == f(c=1032) == UNS
-    assert f(w=1 << 40, ld=1 << 40) == f(B=1 << 21) == f(Hk=1 << 17) == f(rows=1 << 32) == UNS
-    assert f(B=1 << 20, Hk=1 << 15) == UNS                 # more than a grid counts
-    assert f(p=(FAKE + 8,) + (FAKE,) * 6) == f(p=(FAKE,) * 4 + (FAKE + 8, FAKE, FAKE)) == UNS
+    def f(cache=at, B=2, rows=9, ld=4, w=4, n=9, lens=None, p=(FAKE,) * 3):
+        return lib.umic_cache8_read_bf16(cache, *p, lens, None, B, rows, ld, w, n, None)
+
+    assert f(B=-1) == f(rows=-1) == f(w=-1) == f(ld=3) == f(n=65) == f(n=-1) == f(none) == ARG
+    assert f(B=0, p=(None,) * 3) == f(rows=0, p=(None,) * 3) == 0
+    for i in range(3):
+        assert f(p=tuple(None if j == i else FAKE for j in range(3))) == ARG, i
+    assert f(w=1 << 40, ld=1 << 40) == f(B=1 << 21) == f(rows=1 << 32) == UNS
+    assert f(tall, B=1 << 20) == UNS                       # more than a grid counts
+    assert f(p=(FAKE + 8, FAKE, FAKE)) == f(p=(FAKE, FAKE + 8, FAKE)) == UNS
 
 
 def test_attention_refusals(lib):
-    def f(B=2, S=1, Hq=8, Hk=2, D=128, q=FAKE, k=FAKE, v=FAKE, ks=FAKE, vs=FAKE, out=FAKE, table=FAKE,
-          lens=None, st=1024, c=8192, pages=2, page=64, ld=1, w=1, n=64, fmt=0, scale=0.1, ws=FAKE,
-          size=1 << 40):
-        return lib.umic_cache8_attention_bf16(
-            q, k, v, ks, vs, out, table, lens, None, B, S, Hq, Hk, D, st, st, 128, st, st, 128, 16384, c,
-            128, 8, 4, pages, page, ld, w, n, fmt, 1, scale, None, ws, size, None)
+    at, keep = struct()
+    odd, odd_keep = struct(heads=3)
 
-    assert f(B=-1) == f(S=-1) == f(Hq=-1) == f(Hk=-1) == f(D=0) == f(page=-1) == f(size=-1) == ARG
+    def f(cache=at, B=2, S=1, Hq=8, q=FAKE, out=FAKE, table=FAKE, lens=None, st=1024, ld=4, w=4, n=64,
+          scale=0.1, ws=FAKE, size=1 << 40):
+        return lib.umic_cache8_attention_bf16(cache, q, out, table, lens, None, B, S, Hq, st, st, 64,
+                                              st, st, 64, ld, w, n, 1, scale, None, ws, size, None)
+
+    assert f(B=-1) == f(S=-1) == f(Hq=-1) == f(size=-1) == f(None) == ARG
     assert f(B=0) == f(S=0) == f(Hq=0) == 0
-    assert f(Hk=3) == f(Hk=0) == ARG
-    assert f(q=None) == f(out=None) == f(ws=None) == f(k=None) == f(v=None) == ARG
+    assert f(odd) == ARG
+    assert f(q=None) == f(out=None) == f(ws=None) == f(table=None) == ARG
     assert f(scale=float("inf")) == f(scale=float("nan")) == ARG
-    assert f(n=65) == f(n=-1) == f(ld=0) == f(w=-1) == ARG
-    assert f(D=80) == f(st=1028) == f(c=8200) == f(q=FAKE + 8) == f(k=FAKE + 8) == f(page=8) == UNS
+    assert f(n=65) == f(n=-1) == f(ld=3) == f(w=-1) == ARG
+    assert f(st=1028) == f(q=FAKE + 8) == f(ws=FAKE + 4) == f(w=1 << 40, ld=1 << 40) == UNS
 
 
 def pages8(**kw):
@@ -89,7 +124,7 @@ def test_pages():
                 dict(page_size=24), dict(page_size=8)):
         with pytest.raises(ValueError):
             pages8(**bad)
-    assert cache8._pages("x", c, -1)[0] == 1
+    assert c.layout("x", -1).struct.format == 1
     wide = torch.zeros(4, 2, 32, 72, dtype=torch.int8)
     for bad in (c._replace(v=c.v.view(torch.float8_e4m3fn)), c._replace(k=c.k[:3]),
                 c._replace(k=wide[..., :64], v=wide[..., :64]),                 # rows of 72 bytes
@@ -97,9 +132,15 @@ def test_pages():
                 c._replace(v_scale=c.v_scale.double()), c._replace(v_scale=c.v_scale[:, :1]),
                 cache8.Pages8(*(t[:, :, :24] for t in c[:2]), *c[2:])):
         with pytest.raises(ValueError):
-            cache8._pages("x", bad, -1)
+            bad.layout("x", -1)
+    held = c.layout("x", -1)
+    assert c.layout("x", -1) is held and (held.pages, held.heads, held.page_size, held.head_dim) == (4, 2, 32, 64)
+    c.k.set_(torch.zeros_like(c.k))                        # its tensors elsewhere: looked at again
+    assert c.layout("x", -1).struct.k_codes == c.k.data_ptr() != held.struct.k_codes
+    twin = copy.deepcopy(c)
+    assert type(twin) is cache8.Pages8 and twin.layout("x", -1).struct.k_codes == twin.k.data_ptr()
     with pytest.raises(ValueError, match="cache is on"):
-        cache8._pages("x", c, 0)
+        c.layout("x", 0)
 
 
 def test_wrappers_refuse_cpu_tensors():
@@ -138,7 +179,7 @@ def test_arena_of_codes():
         codes = ar.codes(1)
         assert codes.k.data_ptr() == ar.k(1).data_ptr() and codes.v.data_ptr() == ar.v(1).data_ptr()
         assert codes.v_scale.data_ptr() == ar.scales[1, 1].data_ptr()
-        assert cache8._pages("x", codes, -1)[0] == cache8.DTYPES[dtype]
+        assert codes.layout("x", -1).struct.format == cache8.DTYPES[dtype]
     assert PagedArena(1, 2, 6, 2, 32, 64, 64, device="cpu").scales is None
     with pytest.raises(ValueError, match="pages of"):
         PagedArena(1, 2, 6, 2, 32, 64, 64, device="cpu", dtype=torch.float16)

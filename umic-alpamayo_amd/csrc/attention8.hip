@@ -375,26 +375,27 @@ int launch8(const Shape& s, const Attn8Args& x, hipStream_t st) {
 }  // namespace umic
 
 extern "C" int umic_cache8_attention_bf16(
-    const void* q, const void* k_codes, const void* v_codes, const float* k_scale,
-    const float* v_scale, void* out, const int32_t* table, const int32_t* kv_lens,
-    const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t q_sb,
-    int64_t q_ss, int64_t q_sh, int64_t o_sb, int64_t o_ss, int64_t o_sh, int64_t c_sb,
-    int64_t c_sh, int64_t c_ss, int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size,
-    int64_t table_ld, int64_t table_w, int64_t kv_len, int format, int causal, float scale,
-    int32_t* counters, void* workspace, int64_t workspace_bytes, void* stream) {
+    const umic_cache8_t* cache, const void* q, void* out, const int32_t* table,
+    const int32_t* kv_lens, const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq, int64_t q_sb,
+    int64_t q_ss, int64_t q_sh, int64_t o_sb, int64_t o_ss, int64_t o_sh, int64_t table_ld,
+    int64_t table_w, int64_t kv_len, int causal, float scale, int32_t* counters, void* workspace,
+    int64_t workspace_bytes, void* stream) {
   using namespace umic;
-  const AttnCall call = {q,    k_codes, v_codes, out,   table,     kv_lens,  q_lens,  B,      S,
-                         Hq,   Hk,      D,       q_sb,  q_ss,      q_sh,     o_sb,    o_ss,   o_sh,
-                         c_sb, c_sh,    c_ss,    pages, page_size, table_ld, table_w, kv_len, causal,
-                         scale, counters, workspace, workspace_bytes};
+  int64_t cap;
+  if (const int e = check_cache8(cache, cap, table_w)) return e;
+  const umic_cache8_t& c = *cache;
+  const int64_t D = c.head_dim;
+  const AttnCall call = {q,      c.k_codes, c.v_codes, out,  table, kv_lens, q_lens, B,    S,
+                         Hq,     c.heads,   D,         q_sb, q_ss,  q_sh,    o_sb,   o_ss, o_sh,
+                         c.c_sb, c.c_sh,    c.c_ss,    c.pages, c.page_size, table_ld, table_w,
+                         kv_len, causal,    scale,     counters, workspace, workspace_bytes};
   Attn8Args x = {};
   Shape s;
+  if (!table && B > 0 && S > 0 && Hq > 0) return UMIC_ERR_INVALID_ARG;
   if (const int e = attn_args(call, 16, x.a, s)) return e == 1 ? UMIC_OK : e;
-  if (!table || (pages && (!k_scale || !v_scale))) return UMIC_ERR_INVALID_ARG;
-  if (format != UMIC_CODES_E4M3 && format != UMIC_CODES_INT8) return UMIC_ERR_UNSUPPORTED;
-  x.ks = k_scale, x.vs = v_scale, x.s_sb = s_sb, x.s_sh = s_sh;
+  x.ks = c.k_scale, x.vs = c.v_scale, x.s_sb = c.s_sb, x.s_sh = c.s_sh;
   hipStream_t st = as_stream(stream);
-  const bool f = format == UMIC_CODES_INT8;
+  const bool f = c.format == UMIC_CODES_INT8;
   if (D == 64)
     return f ? launch8<64, UMIC_CODES_INT8>(s, x, st) : launch8<64, UMIC_CODES_E4M3>(s, x, st);
   if (D == 128)

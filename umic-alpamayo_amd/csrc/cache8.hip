@@ -328,59 +328,65 @@ int launch_read(const ReadArgs& a, int64_t heads, hipStream_t st) {
   return launch_status();
 }
 
-bool codes_ok(int64_t D, int64_t pages, int64_t page_size, int format) {
-  return (D == 64 || D == 128 || D == 256) && page_size >= 16 &&
-         !(page_size & (page_size - 1)) && page_size <= ((int64_t)1 << 30) &&
-         pages <= ((int64_t)1 << 30) && pages * page_size <= ((int64_t)1 << 34) &&
-         (format == UMIC_CODES_E4M3 || format == UMIC_CODES_INT8);
+}  // namespace
+
+int check_cache8(const umic_cache8_t* c, int64_t& cap, int64_t table_w) {
+  if (!c || c->pages < 0 || c->page_size <= 0 || c->heads <= 0 || c->head_dim <= 0 || table_w < 0)
+    return UMIC_ERR_INVALID_ARG;
+  if (c->pages && (!c->k_codes || !c->v_codes || !c->k_scale || !c->v_scale))
+    return UMIC_ERR_INVALID_ARG;
+  const int64_t D = c->head_dim, ps = c->page_size;
+  if ((D != 64 && D != 128 && D != 256) || ps < 16 || (ps & (ps - 1)) || ps > ((int64_t)1 << 30) ||
+      c->pages > ((int64_t)1 << 30) || c->pages * ps > ((int64_t)1 << 34) ||
+      table_w > ((int64_t)1 << 30) / ps || c->heads > (1 << 16) ||
+      (c->format != UMIC_CODES_E4M3 && c->format != UMIC_CODES_INT8))
+    return UMIC_ERR_UNSUPPORTED;
+  if (((c->c_sb | c->c_sh | c->c_ss) & 15) || !aligned16(c->k_codes) || !aligned16(c->v_codes))
+    return UMIC_ERR_UNSUPPORTED;
+  cap = c->pages ? table_w * ps : 0;
+  return UMIC_OK;
 }
 
-}  // namespace
 }  // namespace umic
 
 extern "C" int umic_cache8_append_bf16(
-    const void* q, const void* k, const void* v, void* q_out, void* k_codes, void* v_codes,
-    float* k_scale, float* v_scale, const int64_t* positions, const uint64_t* turn,
-    const int32_t* axis, const int64_t* slots, float scale, const void* q_w, const void* k_w,
-    float eps, int64_t T, int64_t Hq, int64_t Hk, int64_t D, int64_t axes, int64_t p_sa,
-    int64_t p_st, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh, int64_t v_st,
-    int64_t v_sh, int64_t qo_st, int64_t qo_sh, int64_t c_sb, int64_t c_sh, int64_t c_ss,
-    int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size, int format, void* stream) {
+    const umic_cache8_t* cache, const void* q, const void* k, const void* v, void* q_out,
+    const int64_t* positions, const uint64_t* turn, const int32_t* axis, const int64_t* slots,
+    float scale, const void* q_w, const void* k_w, float eps, int64_t T, int64_t Hq, int64_t axes,
+    int64_t p_sa, int64_t p_st, int64_t q_st, int64_t q_sh, int64_t k_st, int64_t k_sh,
+    int64_t v_st, int64_t v_sh, void* stream) {
   using namespace umic;
-  if (T < 0 || Hq < 0 || Hk <= 0 || D <= 0 || pages < 0 || page_size <= 0)
-    return UMIC_ERR_INVALID_ARG;
+  int64_t cap;
+  if (const int e = check_cache8(cache, cap, 0)) return e;
+  if (T < 0 || Hq < 0) return UMIC_ERR_INVALID_ARG;
   if (T == 0) return UMIC_OK;
   if (!k || !v || !slots) return UMIC_ERR_INVALID_ARG;
-  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return UMIC_ERR_INVALID_ARG;
   if (turn) {
     if (axes <= 0 || !positions || !axis || (Hq && (!q || !q_out)) || (!q_w != !k_w))
       return UMIC_ERR_INVALID_ARG;
   } else if (Hq || q_w || k_w) {
     return UMIC_ERR_INVALID_ARG;
   }
-  if (!codes_ok(D, pages, page_size, format) || Hq > (1 << 16) || Hk > (1 << 16))
+  if (Hq > (1 << 16) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7) || !aligned16(q) ||
+      !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_w) || !aligned16(k_w))
     return UMIC_ERR_UNSUPPORTED;
-  if (((q_st | q_sh | k_st | k_sh | v_st | v_sh | qo_st | qo_sh) & 7) ||
-      ((c_sb | c_sh | c_ss) & 15) || !aligned16(q) || !aligned16(k) || !aligned16(v) ||
-      !aligned16(q_out) || !aligned16(k_codes) || !aligned16(v_codes) || !aligned16(q_w) ||
-      !aligned16(k_w))
-    return UMIC_ERR_UNSUPPORTED;
+  const umic_cache8_t& c = *cache;
+  const int64_t D = c.head_dim;
   StoreArgs a = {};
   a.x.q = (const uint16_t*)q, a.x.qo = (uint16_t*)q_out;
-  a.x.positions = positions, a.x.turn = turn, a.x.axis = axis;
+  a.x.positions = positions, a.x.turn = turn, a.x.axis = axis, a.x.slots = slots;
   a.x.qw = (const uint16_t*)q_w, a.x.kw = (const uint16_t*)k_w;
   a.x.T = T, a.x.Hq = Hq, a.x.D = D, a.x.A = axes, a.x.p_sa = p_sa, a.x.p_st = p_st;
-  a.x.q_st = q_st, a.x.q_sh = q_sh, a.x.qo_st = qo_st, a.x.qo_sh = qo_sh;
+  a.x.q_st = q_st, a.x.q_sh = q_sh, a.x.qo_st = Hq * D, a.x.qo_sh = D;
   a.x.eps = eps, a.x.scale = scale;
-  a.x.slots = slots;
   a.k = (const uint16_t*)k, a.v = (const uint16_t*)v;
-  a.k8 = (uint8_t*)k_codes, a.v8 = (uint8_t*)v_codes, a.ks = k_scale, a.vs = v_scale;
-  a.Hk = Hk, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
-  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = c_ss, a.s_sb = s_sb, a.s_sh = s_sh;
-  a.slots_n = pages * page_size;
-  a.shift = __builtin_ctzll((unsigned long long)page_size);
+  a.k8 = (uint8_t*)c.k_codes, a.v8 = (uint8_t*)c.v_codes, a.ks = c.k_scale, a.vs = c.v_scale;
+  a.Hk = c.heads, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  a.c_sb = c.c_sb, a.c_sh = c.c_sh, a.c_ss = c.c_ss, a.s_sb = c.s_sb, a.s_sh = c.s_sh;
+  a.slots_n = c.pages * c.page_size;
+  a.shift = __builtin_ctzll((unsigned long long)c.page_size);
   hipStream_t st = as_stream(stream);
-  const bool t = turn != nullptr, f = format == UMIC_CODES_INT8;
+  const bool t = turn != nullptr, f = c.format == UMIC_CODES_INT8;
   if (D == 64)
     return f ? launch_store<64, UMIC_CODES_INT8>(a, t, st) : launch_store<64, UMIC_CODES_E4M3>(a, t, st);
   if (D == 128)
@@ -389,43 +395,37 @@ extern "C" int umic_cache8_append_bf16(
   return f ? launch_store<256, UMIC_CODES_INT8>(a, t, st) : launch_store<256, UMIC_CODES_E4M3>(a, t, st);
 }
 
-extern "C" int umic_cache8_read_bf16(const void* k_codes, const void* v_codes, const float* k_scale,
-                                     const float* v_scale, void* k_out, void* v_out,
+extern "C" int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, void* v_out,
                                      const int32_t* table, const int32_t* kv_lens,
-                                     const int32_t* starts, int64_t B, int64_t Hk, int64_t rows,
-                                     int64_t D, int64_t c_sb, int64_t c_sh, int64_t c_ss,
-                                     int64_t s_sb, int64_t s_sh, int64_t pages, int64_t page_size,
-                                     int64_t table_ld, int64_t table_w, int64_t kv_len, int format,
+                                     const int32_t* starts, int64_t B, int64_t rows,
+                                     int64_t table_ld, int64_t table_w, int64_t kv_len,
                                      void* stream) {
   using namespace umic;
-  if (B < 0 || Hk <= 0 || rows < 0 || D <= 0 || pages < 0 || page_size <= 0 || table_w < 0 ||
-      table_ld < table_w)
-    return UMIC_ERR_INVALID_ARG;
+  int64_t cap;
+  if (const int e = check_cache8(cache, cap, table_w)) return e;
+  if (B < 0 || rows < 0 || table_ld < table_w) return UMIC_ERR_INVALID_ARG;
   if (B == 0 || rows == 0) return UMIC_OK;
   if (!k_out || !v_out || !table) return UMIC_ERR_INVALID_ARG;
-  if (pages && (!k_codes || !v_codes || !k_scale || !v_scale)) return UMIC_ERR_INVALID_ARG;
-  if (!codes_ok(D, pages, page_size, format) || table_w > ((int64_t)1 << 30) / page_size ||
-      Hk > (1 << 16) || B > (1 << 20) || rows > ((int64_t)1 << 31))
-    return UMIC_ERR_UNSUPPORTED;
-  const int64_t cap = pages ? table_w * page_size : 0;
   if (!kv_lens && (kv_len < 0 || kv_len > cap)) return UMIC_ERR_INVALID_ARG;
-  if (((c_sb | c_sh | c_ss) & 15) || !aligned16(k_codes) || !aligned16(v_codes) ||
-      !aligned16(k_out) || !aligned16(v_out))
+  if (B > (1 << 20) || rows > ((int64_t)1 << 31) || !aligned16(k_out) || !aligned16(v_out))
     return UMIC_ERR_UNSUPPORTED;
+  const umic_cache8_t& c = *cache;
+  const int64_t D = c.head_dim;
   ReadArgs a = {};
-  a.k8 = (const uint8_t*)k_codes, a.v8 = (const uint8_t*)v_codes, a.ks = k_scale, a.vs = v_scale;
+  a.k8 = (const uint8_t*)c.k_codes, a.v8 = (const uint8_t*)c.v_codes;
+  a.ks = c.k_scale, a.vs = c.v_scale;
   a.ko = (uint16_t*)k_out, a.vo = (uint16_t*)v_out;
   a.table = table, a.kv_len = kv_lens, a.start = starts;
-  a.c_sb = c_sb, a.c_sh = c_sh, a.c_ss = c_ss, a.s_sb = s_sb, a.s_sh = s_sh;
+  a.c_sb = c.c_sb, a.c_sh = c.c_sh, a.c_ss = c.c_ss, a.s_sb = c.s_sb, a.s_sh = c.s_sh;
   a.table_ld = table_ld, a.rows = rows, a.len = (int)kv_len, a.cap = (int)cap;
-  a.shift = __builtin_ctzll((unsigned long long)page_size);
-  a.pages = (int)pages, a.Hk = (int)Hk;
+  a.shift = __builtin_ctzll((unsigned long long)c.page_size);
+  a.pages = (int)c.pages, a.Hk = (int)c.heads;
   const int64_t per = kThreads / (D / 16);
   a.blocks = (rows + per - 1) / per;
-  const int64_t heads = 2 * B * Hk;
+  const int64_t heads = 2 * B * c.heads;
   if (a.blocks > 0x7fffffff / heads) return UMIC_ERR_UNSUPPORTED;
   hipStream_t st = as_stream(stream);
-  const bool f = format == UMIC_CODES_INT8;
+  const bool f = c.format == UMIC_CODES_INT8;
   if (D == 64)
     return f ? launch_read<64, UMIC_CODES_INT8>(a, heads, st)
              : launch_read<64, UMIC_CODES_E4M3>(a, heads, st);

@@ -10,6 +10,10 @@ namespace umic {
 constexpr int kBlockTokens = 16;  // that share a scale
 constexpr int kLeastExp = -100;   // of a scale
 
+// The checks of a cache that entry points share (cache8.hip); cap: keys that table_w of its
+// pages hold.
+int check_cache8(const umic_cache8_t* cache, int64_t& cap, int64_t table_w);
+
 template <int FORMAT>
 struct Codes;
 

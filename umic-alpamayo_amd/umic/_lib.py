@@ -71,14 +71,22 @@ SIGNATURES: dict[str, list] = {
     "umic_cache_attention_workspace_bytes": [_I64] * 4,
     "umic_cache_attention_max_requests": [_I64] * 5,
     "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _P, _I64, _P],
-    "umic_cache8_append_bf16": [_P] * 12 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 22 + [_I, _P],
-    "umic_cache8_read_bf16": [_P] * 9 + [_I64] * 14 + [_I, _P],
-    "umic_cache8_attention_bf16": [_P] * 9 + [_I64] * 21 + [_I, _I, _F32, _P, _P, _I64, _P],
+    "umic_cache8_append_bf16": [_P] * 9 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 11 + [_P],
+    "umic_cache8_read_bf16": [_P] * 6 + [_I64] * 5 + [_P],
+    "umic_cache8_attention_bf16": [_P] * 6 + [_I64] * 12 + [_I, _F32, _P, _P, _I64, _P],
     "umic_stream_read": [_P, _I64, _P, _P],
     "umic_stream_copy": [_P, _P, _I64, _P],
     "umic_version": [],
     "umic_error_string": [_I],
 }
+
+
+class Cache8(ctypes.Structure):
+    """umic_cache8_t: a paged cache of 8-bit codes."""
+
+    _fields_ = ([(n, _P) for n in ("k_codes", "v_codes", "k_scale", "v_scale")]
+                + [(n, _I64) for n in ("pages", "page_size", "heads", "head_dim", "c_sb", "c_sh",
+                                       "c_ss", "s_sb", "s_sh", "format")])
 
 
 # Return types other than int.

@@ -22,6 +22,7 @@ No counterpart in the reference, whose cache (src/umic/cache.py:25-160) is of 16
 
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple
 
 import torch
@@ -37,14 +38,43 @@ HEAD_DIMS = _bf16.HEAD_DIMS
 _BF16 = torch.bfloat16
 
 
-class Pages8(NamedTuple):
-    """k, v: codes [pages, Hk, page_size, D] of one type and layout, rows of 16-byte
-    chunks; k_scale, v_scale: fp32 [pages, Hk, page_size / BLOCK], powers of two."""
+class _Layout(NamedTuple):
+    """What the kernels are told of a cache, and where it was looked at."""
 
+    pointers: tuple
+    struct: _lib.Cache8
+    at: int  # the structure's address
+    pages: int
+    heads: int
+    page_size: int
+    head_dim: int
+
+
+class _Fields(NamedTuple):
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
     v_scale: torch.Tensor
+
+
+class Pages8(_Fields):
+    """k, v: codes [pages, Hk, page_size, D] of one type and layout, rows of 16-byte
+    chunks; k_scale, v_scale: fp32 [pages, Hk, page_size / BLOCK], powers of two.  Looked at
+    at its first use; one object for many calls saves looking again."""
+
+    def __reduce__(self):  # copies look for themselves
+        return type(self), tuple(self)
+
+    def layout(self, who: str, dev: int) -> _Layout:
+        """Its layout on device dev; raises where the kernels do not take it."""
+        held = self.__dict__.get("_held")
+        k, v, ks, vs = self
+        if (held is not None and held[0] == dev and held[1].pointers
+                == (k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr())):
+            return held[1]
+        got = _look(who, self, dev)
+        self._held = dev, got
+        return got
 
 
 def empty(pages: int, heads: int, page_size: int, head_dim: int,
@@ -58,12 +88,11 @@ def empty(pages: int, heads: int, page_size: int, head_dim: int,
     return Pages8(k, v, k_scale, v_scale)
 
 
-def _pages(who: str, cache: Pages8, dev: int) -> tuple:
-    """(format, shape, code strides, scale strides) of a cache on device dev."""
+def _look(who: str, cache: Pages8, dev: int) -> _Layout:
     k, v, ks, vs = cache
     shape, st, sst = k.shape, k.stride(), ks.stride()
     if (k.dtype not in DTYPES or v.dtype is not k.dtype or len(shape) != 4 or shape != v.shape
-            or shape[3] not in HEAD_DIMS or st != v.stride() or st[3] != 1
+            or shape[3] not in HEAD_DIMS or shape[1] == 0 or st != v.stride() or st[3] != 1
             or (st[0] | st[1] | st[2] | k.data_ptr() | v.data_ptr()) & 15):
         raise ValueError(f"{who}: codes k {k.dtype} {tuple(shape)} and v {v.dtype} {tuple(v.shape)} "
                          f"must be of one type ({list(DTYPES)}) and layout, [pages, heads, "
@@ -76,49 +105,32 @@ def _pages(who: str, cache: Pages8, dev: int) -> tuple:
                          f"{tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)} for pages {tuple(shape)}")
     if any(t.get_device() != dev for t in cache):
         raise ValueError(f"{who}: the cache is on {k.device}, not with the other tensors")
-    return DTYPES[k.dtype], shape, st, sst
+    pointers = tuple(t.data_ptr() for t in cache)
+    struct = _lib.Cache8(*pointers, shape[0], shape[2], shape[1], shape[3], st[0], st[1], st[2],
+                         sst[0], sst[1], DTYPES[k.dtype])
+    return _Layout(pointers, struct, ctypes.addressof(struct), shape[0], shape[1], shape[2], shape[3])
 
 
-def _chunks16(t: torch.Tensor) -> torch.Tensor:
-    """t [T, H, D], or a copy, with rows of 16-byte chunks."""
+def _chunks16(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """t [T, H, D], or a copy, with rows of 16-byte chunks; and its strides."""
     a, b, inner = t.stride()
     if inner == 1 and not ((a | b) & 7 or t.data_ptr() & 15):
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+        return t, a, b
+    t = t.clone(memory_format=torch.contiguous_format)
+    return t, t.stride(0), t.stride(1)
 
 
-def _store(who: str, q, k, v, positions, plan, slots, cache: Pages8, norm):
-    """The append of ``rotate_append`` and, q None, of ``append``."""
-    shape = k.shape
-    if len(shape) != 3 or v.shape != shape or shape[1] == 0:
-        raise ValueError(f"{who}: k {tuple(shape)} and v {tuple(v.shape)} must be [T, heads, D]")
-    T, Hk, D = shape
-    fmt, pages, cst, sst = _pages(who, cache, k.get_device())
-    if pages[1] != Hk or pages[3] != D:
-        raise ValueError(f"{who}: {Hk} heads of {D} into pages of {pages[1]} of {pages[3]}")
-    if (slots.dtype is not torch.int64 or slots.shape != (T,)
-            or slots.get_device() != k.get_device() or not slots.is_contiguous()):
-        raise ValueError(f"{who}: slots must be a contiguous int64 vector of {T} on k's device")
-    k, v = _chunks16(k), _chunks16(v)
-    if q is None:
-        out, turns, heads = None, (None, None, None, None), (None, None, 0.0)
-        Hq, axes, ps, qs, os_, scale = 0, 0, (0, 0), (0, 0), (0, 0), 1.0
-    else:
-        q, Hq = _chunks16(q), q.shape[1]
-        out = torch.empty(T, Hq, D, dtype=_BF16, device=q.device)
-        turns = (positions.data_ptr(), plan.turn.data_ptr(), plan.axis.data_ptr())
-        heads = axial._norm_args(who, norm, D)
-        if norm is not None and (norm[0].data_ptr() | norm[1].data_ptr()) & 15:
-            raise ValueError(f"{who}: norm weights must be 16-byte aligned")
-        axes, ps, qs, os_, scale = (positions.shape[0], positions.stride(), q.stride(),
-                                    (Hq * D, D), plan.scale)
-    with _lib.device_of(k):
-        _lib.call("umic_cache8_append_bf16", _lib.ptr(q), k.data_ptr(), v.data_ptr(),
-                  _lib.ptr(out), *(t.data_ptr() for t in cache), *turns[:3], slots.data_ptr(),
-                  scale, *heads, T, Hq, Hk, D, axes, ps[0], ps[1], qs[0], qs[1], k.stride(0),
-                  k.stride(1), v.stride(0), v.stride(1), *os_, cst[0], cst[1], cst[2], sst[0],
-                  sst[1], pages[0], pages[2], fmt, _lib.stream_of(k))
-    return out
+def _rows(who: str, k, v, slots, cache: Pages8) -> tuple[_Layout, tuple, tuple]:
+    """The checks and row views that both appends share."""
+    shape, dev = k.shape, k.get_device()
+    lay = cache.layout(who, dev)
+    if len(shape) != 3 or v.shape != shape or shape[1] != lay.heads or shape[2] != lay.head_dim:
+        raise ValueError(f"{who}: k {tuple(shape)} and v {tuple(v.shape)} must be [T, {lay.heads}, "
+                         f"{lay.head_dim}], as the pages")
+    if (slots.dtype is not torch.int64 or slots.shape != shape[:1] or slots.get_device() != dev
+            or not slots.is_contiguous()):
+        raise ValueError(f"{who}: slots must be a contiguous int64 vector of {shape[0]} on k's device")
+    return lay, _chunks16(k), _chunks16(v)
 
 
 def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor,
@@ -134,7 +146,20 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     if grad_needed(v):
         raise RuntimeError("cache8.rotate_append: the kernel has no backward; call it under "
                            "torch.no_grad()")
-    return _store("cache8.rotate_append", q, k, v, positions, plan, slots, cache, norm)
+    lay, (k, k0, k1), (v, v0, v1) = _rows("cache8.rotate_append", k, v, slots, cache)
+    q, q0, q1 = _chunks16(q)
+    T, Hq, D = q.shape
+    qw, kw, eps = axial._norm_args("cache8.rotate_append", norm, D)
+    if norm is not None and (qw | kw) & 15:
+        raise ValueError("cache8.rotate_append: norm weights must be 16-byte aligned")
+    out = torch.empty((T, Hq, D), dtype=_BF16, device=q.device)
+    p0, p1 = positions.stride()
+    with _lib.device_of(q):
+        _lib.call("umic_cache8_append_bf16", lay.at, q.data_ptr(), k.data_ptr(), v.data_ptr(),
+                  out.data_ptr(), positions.data_ptr(), plan.turn.data_ptr(), plan.axis.data_ptr(),
+                  slots.data_ptr(), plan.scale, qw, kw, eps, T, Hq, positions.shape[0], p0, p1, q0,
+                  q1, k0, k1, v0, v1, _lib.stream_of(q))
+    return out
 
 
 def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Pages8) -> None:
@@ -144,23 +169,29 @@ def append(k: torch.Tensor, v: torch.Tensor, slots: torch.Tensor, cache: Pages8)
     if grad_needed(k, v):
         raise RuntimeError("cache8.append: the kernel has no backward; call it under "
                            "torch.no_grad()")
-    _store("cache8.append", None, k, v, None, None, slots, cache, None)
+    lay, (k, k0, k1), (v, v0, v1) = _rows("cache8.append", k, v, slots, cache)
+    with _lib.device_of(k):
+        _lib.call("umic_cache8_append_bf16", lay.at, None, k.data_ptr(), v.data_ptr(), None, None,
+                  None, None, slots.data_ptr(), 1.0, None, None, 0.0, k.shape[0], 0, 0, 0, 0, 0, 0,
+                  k0, k1, v0, v1, _lib.stream_of(k))
 
 
 def _requests(who: str, table: torch.Tensor, kv_len, page_size: int, dev: int) -> tuple:
     """(B, table width, its row stride, lengths' pointer, length of all)."""
-    if (table.dtype is not torch.int32 or table.dim() != 2 or table.shape[1] == 0
-            or table.get_device() != dev or table.stride(1) != 1 and table.shape[1] > 1):
+    shape, st = table.shape, table.stride()
+    if (table.dtype is not torch.int32 or len(shape) != 2 or shape[1] == 0
+            or table.get_device() != dev or st[1] != 1 and shape[1] > 1):
         raise ValueError(f"{who}: table must be int32 [requests, W > 0] with contiguous rows on the "
                          f"cache's device, got {table.dtype} {tuple(table.shape)}")
-    B, width = table.shape
+    B, width = shape
+    ld = st[0] if B > 1 else width
     if isinstance(kv_len, torch.Tensor):
         _bf16._lengths("kv_len", kv_len, B, dev)
-        return B, width, table.stride(0) if B > 1 else width, kv_len.data_ptr(), 0
+        return B, width, ld, kv_len.data_ptr(), 0
     n = int(kv_len)
     if not 0 <= n <= width * page_size:
         raise ValueError(f"{who}: kv_len {n} of a table that holds {width * page_size}")
-    return B, width, table.stride(0) if B > 1 else width, None, n
+    return B, width, ld, None, n
 
 
 def read(cache: Pages8, table: torch.Tensor, kv_len, rows: int, *,
@@ -174,22 +205,21 @@ def read(cache: Pages8, table: torch.Tensor, kv_len, rows: int, *,
         rows: rows to read of each request.
         start: int32 [B], the first one (None: 0).
     """
-    dev = cache.k.get_device()
+    dev = table.get_device()
     if dev < 0:
-        raise ValueError(f"umic kernels run on the GPU; got a tensor on {cache.k.device}")
-    fmt, shape, cst, sst = _pages("cache8.read", cache, dev)
-    B, width, ld, lens, n = _requests("cache8.read", table, kv_len, shape[2], dev)
+        raise ValueError(f"umic kernels run on the GPU; got a tensor on {table.device}")
+    lay = cache.layout("cache8.read", dev)
+    B, width, ld, lens, n = _requests("cache8.read", table, kv_len, lay.page_size, dev)
     if rows < 0:
         raise ValueError(f"cache8.read: {rows} rows")
     if start is not None:
         _bf16._lengths("start", start, B, dev)
-    _lib.lib()
-    k, v = torch.empty(2, B, shape[1], rows, shape[3], dtype=_BF16, device=cache.k.device)
+    shape = (B, lay.heads, rows, lay.head_dim)
+    k = torch.empty(shape, dtype=_BF16, device=table.device)
+    v = torch.empty(shape, dtype=_BF16, device=table.device)
     with _lib.device_of(k):
-        _lib.call("umic_cache8_read_bf16", *(t.data_ptr() for t in cache), k.data_ptr(),
-                  v.data_ptr(), table.data_ptr(), lens, _lib.ptr(start), B, shape[1], rows,
-                  shape[3], cst[0], cst[1], cst[2], sst[0], sst[1], shape[0], shape[2], ld, width,
-                  n, fmt, _lib.stream_of(k))
+        _lib.call("umic_cache8_read_bf16", lay.at, k.data_ptr(), v.data_ptr(), table.data_ptr(),
+                  lens, _lib.ptr(start), B, rows, ld, width, n, _lib.stream_of(k))
     return k, v
 
 
@@ -215,13 +245,14 @@ def attention(q: torch.Tensor, cache: Pages8, kv_len, table: torch.Tensor, *,
     if grad_needed(q):
         raise RuntimeError("cache8.attention: the kernel has no backward; call it under "
                            "torch.no_grad()")
-    dev = q.get_device()
-    fmt, shape, cs, sst = _pages("cache8.attention", cache, dev)
-    pages, Hk, ps, Dk = shape
-    if q.dim() != 4 or q.shape[3] != Dk or Hk == 0 or q.shape[1] % Hk:
-        raise ValueError(f"cache8.attention: q {tuple(q.shape)} over a cache of {Hk} heads of {Dk}")
-    B, Hq, S, D = q.shape
-    rows, width, ld, lens, n = _requests("cache8.attention", table, kv_len, ps, dev)
+    dev, shape = q.get_device(), q.shape
+    lay = cache.layout("cache8.attention", dev)
+    Hk = lay.heads
+    if len(shape) != 4 or shape[3] != lay.head_dim or shape[1] % Hk:
+        raise ValueError(f"cache8.attention: q {tuple(shape)} over a cache of {Hk} heads of "
+                         f"{lay.head_dim}")
+    B, Hq, S, D = shape
+    rows, width, ld, lens, n = _requests("cache8.attention", table, kv_len, lay.page_size, dev)
     if rows != B:
         raise ValueError(f"cache8.attention: {B} requests over a table of {rows}")
     if q_len is not None:
@@ -229,7 +260,8 @@ def attention(q: torch.Tensor, cache: Pages8, kv_len, table: torch.Tensor, *,
     if not _bf16._chunks_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty(B, S, Hq, D, dtype=_BF16, device=q.device)
+        out = torch.empty((B, S, Hq, D), dtype=_BF16, device=q.device)
+        o0, o1, o2 = S * Hq * D, Hq * D, D
     else:
         require_device(q, out)
         if tuple(out.shape) != (B, S, Hq, D) or not _bf16._chunks_ok(out):
@@ -237,28 +269,27 @@ def attention(q: torch.Tensor, cache: Pages8, kv_len, table: torch.Tensor, *,
                              f"chunks, got {tuple(out.shape)}")
         if any(st == 0 and m > 1 for st, m in zip(out.stride(), out.shape)):
             raise ValueError("cache8.attention: out must not share rows")
+        o0, o1, o2, _ = out.stride()
     if B == 0 or S == 0 or Hq == 0:
         return out
-    most = _bf16.max_requests(S, Hq, Hk, D, width * ps)
+    most = _bf16.max_requests(S, Hq, Hk, D, width * lay.page_size)
     if B > most:
         if most == 0:
             raise ValueError(f"cache8.attention: {S} new tokens of {Hq} heads over up to "
-                             f"{width * ps} keys are too many for one launch")
+                             f"{width * lay.page_size} keys are too many for one launch")
         for b in range(0, B, most):  # requests stand for themselves
             part = slice(b, b + most)
             attention(q[part], cache, n if lens is None else kv_len[part], table[part],
                       q_len=None if q_len is None else q_len[part], causal=causal, scale=scale,
                       out=out[part])
         return out
-    qs, os_ = q.stride(), out.stride()
+    q0, q1, q2, _ = q.stride()
     with _lib.device_of(q):
         stream = _lib.stream_of(q)
         size = _bf16._workspace_bytes(dev, S, Hq, Hk, D)
         counters, ws = _bf16._scratch(q, dev, stream, size)
-        _lib.call("umic_cache8_attention_bf16", q.data_ptr(), *(t.data_ptr() for t in cache),
-                  out.data_ptr(), table.data_ptr(), lens, _lib.ptr(q_len), B, S, Hq, Hk, D, qs[0],
-                  qs[2], qs[1], os_[0], os_[1], os_[2], cs[0], cs[1], cs[2], sst[0], sst[1], pages,
-                  ps, ld, width, n, fmt, int(causal),
-                  float(D ** -0.5 if scale is None else scale), counters, ws.data_ptr(), size,
-                  stream)
+        _lib.call("umic_cache8_attention_bf16", lay.at, q.data_ptr(), out.data_ptr(),
+                  table.data_ptr(), lens, _lib.ptr(q_len), B, S, Hq, q0, q2, q1, o0, o1, o2, ld,
+                  width, n, int(causal), float(D ** -0.5 if scale is None else scale), counters,
+                  ws.data_ptr(), size, stream)
     return out

@@ -75,6 +75,8 @@ class PagedArena:
                                    device=device)
         self.scales = None if dtype is torch.bfloat16 else torch.ones(
             layers, 2, pages, heads, page_size // cache8.BLOCK, device=device)
+        self._codes = [] if self.scales is None else [
+            cache8.Pages8(*x, *y) for x, y in zip(self.storage, self.scales)]
         ints = dict(dtype=torch.int32, device=device)
         self.table = torch.zeros(requests, width, **ints)
         self.ring = torch.arange(pages, **ints)
@@ -91,7 +93,7 @@ class PagedArena:
 
     def codes(self, layer: int) -> cache8.Pages8:
         """A layer's pages of 8-bit codes."""
-        return cache8.Pages8(*self.storage[layer], *self.scales[layer])
+        return self._codes[layer]
 
     def read(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A layer's keys and values as bf16, two [requests, heads, n, D]: rows of each
