@@ -601,11 +601,13 @@ int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, void* v_out,
                           int64_t kv_len, void* stream);
 
 /*
- * umic_cache_attention_bf16 over such a cache: the same rows, lengths, workspace, counters
- * and limits, with a table.  The values of the codes enter the products exactly.  A block
+ * umic_cache_attention_bf16 over such a cache: the same rows, lengths, counters and limits
+ * (umic_cache_attention_max_requests), with a table; workspace_bytes from
+ * umic_cache8_attention_workspace_bytes.  The values of the codes enter the products exactly.  A block
  * whose k or v scale is NaN makes the rows that see one of its keys NaN, and no other; a
  * NaN code of v (umic_cache8_append_bf16 writes none) can reach every row of its request.
  */
+int64_t umic_cache8_attention_workspace_bytes(int64_t S, int64_t Hq, int64_t Hk, int64_t D);
 int umic_cache8_attention_bf16(const umic_cache8_t* cache, const void* q, void* out,
                                const int32_t* table, const int32_t* kv_lens,
                                const int32_t* q_lens, int64_t B, int64_t S, int64_t Hq,

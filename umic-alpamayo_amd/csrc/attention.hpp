@@ -66,7 +66,7 @@ __device__ __forceinline__ int new_of(const AttnArgs& a, int b) {
 // How a launch's key tiles are dealt.  A segment is one (request, key head, row
 // block); it counts as its tiles and LEAD more, what its start and end cost.  The
 // first `more` workgroups have each + 1 of the sum, the others each.
-template <int TILE, int LEAD, int LEAST>
+template <int TILE, int LEAD, int LEAST, int EACH = LEAST>
 struct Deal {
   unsigned each, more;
   int nwg;
@@ -75,10 +75,11 @@ struct Deal {
   static __device__ __forceinline__ int units(int keys) {
     return keys > 0 ? tiles(keys) + LEAD : 0;
   }
-  // most: that the chip holds; if that many have no work, no more than `some`
+  // most: that the chip holds; if that many have no work (LEAST units each), no more than
+  // `some`, of EACH or more
   __device__ __forceinline__ Deal(unsigned all, int most, int some) {
     const unsigned fit = (all + LEAST - 1) / LEAST;
-    nwg = fit >= (unsigned)most ? most : min((int)fit, some);
+    nwg = fit >= (unsigned)most ? most : min((int)((all + EACH - 1) / EACH), some);
     each = nwg ? all / (unsigned)nwg : 0;
     more = all - each * (unsigned)nwg;
   }
@@ -846,14 +847,14 @@ __device__ __forceinline__ bool find_parts(const AttnArgs& a, int b, int pair, i
 }
 
 // Joins the parts that attend_few_kernel has left, and writes the zeros.
-template <int D>
+template <int D, typename DEAL>
 __global__ __launch_bounds__(kThreads) void join_few_kernel(AttnArgs a) {
   __shared__ int sums[kWaves];
   __shared__ int found;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
   const int b = blockIdx.x / a.Hk, h = blockIdx.x - b * a.Hk;
   int w0, w1;
-  const bool any = find_parts<FewDeal>(a, b, h, sums, &found, w0, w1);
+  const bool any = find_parts<DEAL>(a, b, h, sums, &found, w0, w1);
   const int row = blockIdx.y * kWaves + wave;
   if (row >= a.S * a.G) return;
   uint16_t* op = out_row(a, b, h, row);
@@ -865,7 +866,7 @@ __global__ __launch_bounds__(kThreads) void join_few_kernel(AttnArgs a) {
 
 // Joins those of attend_many_kernel: a workgroup to 4 of the DV column groups of a
 // tile of 16 rows, a lane to four columns of one row.
-template <int D, int NT>
+template <int D, int NT, typename DEAL>
 __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
   constexpr int DV = D / 16;
   constexpr int kBlock = 16 * NT * kWaves, kTiles = kBlock / 16;
@@ -877,7 +878,7 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
   const int b = blockIdx.x / per, pair = blockIdx.x - b * per;
   const int h = pair / a.rb, rb = pair - h * a.rb;
   int w0, w1;
-  const bool any = find_parts<ManyDeal>(a, b, pair, sums, &found, w0, w1);
+  const bool any = find_parts<DEAL>(a, b, pair, sums, &found, w0, w1);
   const int group = blockIdx.z * kWaves + wave;
   const int row = rb * kBlock + blockIdx.y * 16 + n16;
   if ((any && w0 == w1) || group >= DV || row >= a.S * a.G) return;
@@ -934,19 +935,19 @@ __global__ __launch_bounds__(kThreads) void join_many_kernel(AttnArgs a) {
   *reinterpret_cast<u32x2*>(out_row(a, b, h, row) + 16 * group + 4 * g4) = x;
 }
 
-template <int D, int NT>
+template <int D, int NT, typename DEAL>
 int launch_join_many(const AttnArgs& a, hipStream_t st) {
   const int rows = a.S * a.G, block = 16 * NT * kWaves;
   const dim3 joins((unsigned)(a.B * a.Hk * a.rb), (unsigned)((std::min(rows, block) + 15) / 16),
                    (D / 16 + kWaves - 1) / kWaves);
-  hipLaunchKernelGGL((join_many_kernel<D, NT>), joins, dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL((join_many_kernel<D, NT, DEAL>), joins, dim3(kThreads), 0, st, a);
   return launch_status();
 }
 
-template <int D>
+template <int D, typename DEAL>
 int launch_join_few(const AttnArgs& a, hipStream_t st) {
   const dim3 joins((unsigned)(a.B * a.Hk), (unsigned)((a.S * a.G + kWaves - 1) / kWaves));
-  hipLaunchKernelGGL((join_few_kernel<D>), joins, dim3(kThreads), 0, st, a);
+  hipLaunchKernelGGL((join_few_kernel<D, DEAL>), joins, dim3(kThreads), 0, st, a);
   return launch_status();
 }
 
@@ -957,12 +958,13 @@ struct Shape {
   int nwg;
 };
 
-Shape shape_of(int64_t rows, int64_t D, int64_t cus) {
+// few: workgroups a CU holds of the kernel for up to 16 rows.
+Shape shape_of(int64_t rows, int64_t D, int64_t cus, int few) {
   Shape s;
   s.nt = rows <= 16 ? 0 : rows <= 64 || D > 128 ? 1 : 2;
   s.block = s.nt ? 16 * s.nt * kWaves : 16;
   s.rb = (int)((rows + s.block - 1) / s.block);
-  s.nwg = (int)(cus * (D <= 128 ? 2 : 1));
+  s.nwg = (int)(cus * (s.nt == 0 ? few : D <= 128 ? 2 : 1));
   return s;
 }
 
@@ -975,7 +977,7 @@ bool head_dim_ok(int64_t D) { return D == 64 || D == 128 || D == 256; }
 // Requests of up to `cap` keys that a call takes: the tiles of all are counted in 32 bits.
 int64_t max_requests(int64_t S, int64_t Hq, int64_t Hk, int64_t D, int64_t cap) {
   if (S > (1 << 20) || Hq > (1 << 16) || S * Hq > 0x7fffffff || cap > ((int64_t)1 << 30)) return 0;
-  const int64_t rb = shape_of(S * (Hq / Hk), D, 1).rb;
+  const int64_t rb = shape_of(S * (Hq / Hk), D, 1, 1).rb;
   return std::min<int64_t>(0x7fffffff / (Hk * rb) / (cap / kStep + 8), 1 << 20);
 }
 
@@ -994,8 +996,8 @@ struct AttnCall {
 };
 
 // The checks that entry points share, and the kernels' arguments.  1: nothing to do.
-// chunk: elements of 16 bytes of the cache.
-int attn_args(const AttnCall& x, int chunk, AttnArgs& a, Shape& s) {
+// chunk: elements of 16 bytes of the cache; few: as shape_of's.
+int attn_args(const AttnCall& x, int chunk, int few, AttnArgs& a, Shape& s) {
   if (x.B < 0 || x.S < 0 || x.Hq < 0 || x.Hk < 0 || x.D <= 0 || x.blocks < 0 ||
       x.block_rows < 0 || x.workspace_bytes < 0)
     return UMIC_ERR_INVALID_ARG;
@@ -1026,7 +1028,7 @@ int attn_args(const AttnCall& x, int chunk, AttnArgs& a, Shape& s) {
   const int64_t G = x.Hq / x.Hk;
   if (x.B > max_requests(x.S, x.Hq, x.Hk, x.D, cap) || x.blocks > ((int64_t)1 << 30))
     return UMIC_ERR_UNSUPPORTED;
-  s = shape_of(x.S * G, x.D, cus);
+  s = shape_of(x.S * G, x.D, cus, few);
   if (x.workspace_bytes < workspace_of(s, x.D)) return UMIC_ERR_INVALID_ARG;
   if (x.c_ss < 0 || x.c_ss >= (1 << 24)) return UMIC_ERR_UNSUPPORTED;  // row offsets in a tile
   a.q = (const uint16_t*)x.q, a.k = (const uint16_t*)x.k, a.v = (const uint16_t*)x.v;
@@ -1040,11 +1042,7 @@ int attn_args(const AttnCall& x, int chunk, AttnArgs& a, Shape& s) {
   a.cap = (int)cap;
   a.B = (int)x.B, a.S = (int)x.S, a.Hk = (int)x.Hk, a.G = (int)G, a.rb = s.rb;
   a.len = x.kv_lens ? 0 : (int)x.kv_len, a.blocks = (int)x.blocks, a.shift = shift;
-  // Single tokens of a few segments, up to a quarter of the CUs': a workgroup to a
-  // CU.  The second hides the starts and ends of segments; with few it only doubles
-  // their parts (8 segments of 12288 keys 18 us for 25, 64 of 1024 14.5 for 15.4; 128
-  // of 300 15.2 for 13.6, 64 ragged requests 74 for 60).
-  a.nwg = s.nt == 0 && x.B * x.Hk * 4 <= cus ? (int)cus : s.nwg;
+  a.nwg = s.nwg;
   // Many rows: two workgroups to a CU or one.  Between the two some CUs have twice the
   // others' work (128 tokens over 1024 keys: 288 workgroups 25 us, 256 of them 22).
   a.some = s.nt && a.nwg > cus ? (int)cus : a.nwg;
@@ -1053,6 +1051,13 @@ int attn_args(const AttnCall& x, int chunk, AttnArgs& a, Shape& s) {
   if (a.c < 0x1p-126f) a.c = 0x1p-126f;  // masked scores are -inf: times 0 they would be NaN
   a.flip = x.scale < 0.0f ? 0x80008000u : 0u;
   return UMIC_OK;
+}
+
+// Bytes of workspace that a call takes; 0: of no such call.
+int64_t workspace_bytes(int64_t S, int64_t Hq, int64_t Hk, int64_t D, int few) {
+  if (S <= 0 || Hq <= 0 || Hk <= 0 || Hq % Hk || !head_dim_ok(D) || S > (1 << 20) || Hq > (1 << 16))
+    return 0;
+  return workspace_of(shape_of(S * (Hq / Hk), D, device_cus(), few), D);
 }
 
 }  // namespace

@@ -25,36 +25,67 @@ struct Attn8Args {
   int64_t s_sb, s_sh;
 };
 
+__device__ __forceinline__ Attn8Args args8_again() {
+  typedef const __attribute__((address_space(4))) Attn8Args* Args;
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Attn8Args*)p;
+}
+
 __device__ __forceinline__ float scalar_f32(const float* p) {
   return *(const __attribute__((address_space(4))) float*)(uintptr_t)p;
 }
 
 __device__ __forceinline__ bool is_nan(float x) { return x != x; }
 
-// Two tiles of 16 keys and their scales.
-struct Place8 {
-  Place p;
-  float ks[2], vs[2];
+// A segment's codes and scales, of its key head; row j is row j % 2^shift of page
+// row[j >> shift].
+struct View {
+  const uint8_t* k;
+  const uint8_t* v;
+  const float* ks;
+  const float* vs;
+  const int32_t* row;
+  int len;
 };
 
-__device__ __forceinline__ Place8 place8_of(const Attn8Args& x, const Keys& s, int h, int k0) {
-  const Blocks blocks = blocks_of(x.a, s, k0);
-  Place8 r;
-  r.p = place_of(x.a, s, k0, blocks);
-#pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    r.ks[i] = r.vs[i] = 0.0f;
-    if (r.p.n[i]) {
-      const int in = ((k0 + 16 * i) & ((1 << x.a.shift) - 1)) / kBlockTokens;
-      const int64_t at = blocks.of[i] * x.s_sb + h * x.s_sh + in;
-      r.ks[i] = scalar_f32(x.ks + at);
-      r.vs[i] = scalar_f32(x.vs + at);
-    }
-  }
+__device__ __forceinline__ View view_of(const Attn8Args& x, const Segment& s) {
+  View w;
+  const int64_t codes = s.h * x.a.c_sh, scales = s.h * x.s_sh;
+  w.k = (const uint8_t*)x.a.k + codes;
+  w.v = (const uint8_t*)x.a.v + codes;
+  w.ks = x.ks + scales;
+  w.vs = x.vs + scales;
+  w.row = x.a.table + s.b * x.a.table_ld;
+  w.len = s.len;
+  return w;
+}
+
+// A tile of 16 keys: where it lies, the first n rows of it there, and its scales.
+struct Tile {
+  int64_t at;
+  int n;
+  float ks, vs;
+};
+
+__device__ __forceinline__ Tile tile_of(const Attn8Args& x, const View& w, int key) {
+  Tile r;
+  const int in = key & ((1 << x.a.shift) - 1);
+  const unsigned page =
+      (unsigned)scalar_i32(w.row + min(key >> x.a.shift, (w.len - 1) >> x.a.shift));
+  const bool out = page >= (unsigned)x.a.blocks;  // of the pool: not there
+  r.n = out ? 0 : min(max(w.len - key, 0), 16);
+  // rows and scales of a tile that is not there are others': nothing of it counts
+  const int64_t p = out ? 0 : page;
+  r.at = p * x.a.c_sb + (int64_t)in * x.a.c_ss;
+  const int64_t block = p * x.s_sb + in / kBlockTokens;
+  r.ks = scalar_f32(w.ks + block);
+  r.vs = scalar_f32(w.vs + block);
   return r;
 }
 
-// Rows that see a key of a tile whose values read as NaN (bit i of `wild`: tile i).
+// Rows that see a key of a tile whose values read as NaN (bit i of `wild`, of two: tile i): their
+// sum makes all of their output NaN.
 template <typename R>
 __device__ __forceinline__ void spoil(R& r, int wild, int k0) {
 #pragma unroll
@@ -62,15 +93,61 @@ __device__ __forceinline__ void spoil(R& r, int wild, int k0) {
     if (wild >> i & 1)
 #pragma unroll
       for (int nt = 0; nt < (int)(sizeof(r.lim) / sizeof(int)); ++nt)
-        if (k0 + 16 * i < r.lim[nt])
-#pragma unroll
-          for (int e = 0; e < R::DV; ++e)
-#pragma unroll
-            for (int y = 0; y < 4; ++y) r.acc[nt][e][y] = __builtin_nanf("");
+        if (k0 + 16 * i < r.lim[nt]) r.l[nt] = __builtin_nanf("");
 }
 
+// attention.hpp's Deal with the remainder spread evenly, workgroup w beginning at w all /
+// nwg: where the workgroups of a segment come out even, none has parts of two (a request
+// of 40000 keys 23.6 us for 27.7, four of 12000 22.9 for 26.6).  If the chip's workgroups
+// have less than LEAST units each, no more than `some`, of EACH or more.
+template <int TILE, int LEAD, int LEAST, int EACH>
+struct EvenDeal {
+  unsigned all, each, more;
+  int nwg;
+
+  static __device__ __forceinline__ int tiles(int keys) { return (keys + TILE - 1) / TILE; }
+  static __device__ __forceinline__ int units(int keys) {
+    return keys > 0 ? tiles(keys) + LEAD : 0;
+  }
+  __device__ __forceinline__ EvenDeal(unsigned all, int most, int some) : all(all) {
+    nwg = all / LEAST >= (unsigned)most ? most : min((int)((all + EACH - 1) / EACH), some);
+    each = nwg ? all / (unsigned)nwg : 0;
+    more = all - each * (unsigned)nwg;
+  }
+  __device__ __forceinline__ int begin(unsigned wg) const {
+    return (int)(wg * each + wg * more / (unsigned)nwg);
+  }
+  __device__ __forceinline__ int holder(unsigned unit) const {
+    // to one workgroup: there are 4096 at most, and the three roundings are of 2^-24 each
+    int w = min((int)((float)unit * ((float)nwg / (float)all)), nwg - 1);
+    if ((unsigned)begin(w) > unit) --w;
+    if ((unsigned)begin(w + 1) <= unit) ++w;
+    return w;
+  }
+  __device__ __forceinline__ void holders(unsigned at, int tiles, int& w0, int& w1) const {
+    w0 = holder(at + LEAD);
+    w1 = holder(at + LEAD + tiles - 1);
+  }
+};
+
+// Single tokens: 128 keys; a segment's start and end cost some two of them (64 ragged
+// requests 32 us; counted as nothing 39, as one or three 32 and 33).  EACH: two units, as a
+// part costs its join too (one token over 9000 keys of two heads, 16 rows each, 20 us for
+// 26; over 3100 of eight 11.9 either way; of three units 12.1).
+typedef EvenDeal<kStep * kWaves, 2, 5, 2> Few8Deal;
+
+// Workgroups of a CU.  (Three: 64 ragged requests 31 us for 32, 128 requests of 3000 keys
+// 148 for 132, two of 131001 98 for 94.  One: 57, 161, 110.)
+constexpr int few8_of(int64_t D) { return D <= 128 ? 2 : 1; }
+
+// Up to 16 rows: attention.hip's kernel, a wave to 32 of a tile's 128 keys, the loads of a
+// step in flight while the one before is computed.
+// What bounds it: HBM where the keys are many (64 requests of 8000 keys 170 us, 6.2 TB/s);
+// a request of 3100 keys 11.6 us, of which 4 pass until its first keys are there and 3 to
+// join; of a step's 350 vector instructions int8 codes take 192 (one to a number, half one
+// to pair it) and e4m3's 80.
 template <int D, int FORMAT>
-__global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_few_kernel(Attn8Args x) {
+__global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8Args x) {
   typedef Rows<D, 1, false> R;
   typedef Codes<FORMAT> C;
   constexpr int KK = R::KK, DV = R::DV;
@@ -84,64 +161,75 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_few_kernel
   const int n16 = lane & 15, g4 = lane >> 4;
 
   Scan scan = {};
-  const int even = a.kv_len ? 0 : FewDeal::units(a.len);
+  const int even = a.kv_len ? 0 : Few8Deal::units(a.len);
   if (a.kv_len)
-    scan = scan_units<FewDeal>(a, lds.sums);
+    scan = scan_units<Few8Deal>(a, lds.sums);
   else
     scan.all = even * a.B;
-  const FewDeal deal((unsigned)(scan.all * a.Hk), a.nwg, a.some);
+  const Few8Deal deal((unsigned)(scan.all * a.Hk), a.nwg, a.some);
   const int wg = dealt_wg(deal.nwg);
   if (wg >= 0) {
-    Walk<FewDeal, false> walk;
+    Walk<Few8Deal, false> walk;
     walk.start(a, deal, scan, even, wg, lds.found);
     R r;
     Segment seg, nxt;
     int split = 0;
-    Place8 here;
+    Tile here[2];
     u32x4 kc[2][KW / 4];
     uint32_t vc[8][VW];
     // a lane's 16 codes of a key at a time, those of two steps of the product
-    auto load_k = [&](const Place& p) {
+    auto load_k = [&](const uint8_t* k, const Tile (&p)[2], int c_ss) {
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const uint8_t* kp = (const uint8_t*)a.k + p.at[i];
-        const unsigned off = __umul24(min(n16, max(p.n[i] - 1, 0)), a.c_ss) + g4 * 16;
+        const uint8_t* kp = k + p[i].at;
+        const unsigned off = __umul24(min(n16, max(p[i].n - 1, 0)), c_ss) + g4 * 16;
 #pragma unroll
-        for (int w = 0; w < KW / 4; ++w)
-          kc[i][w] = ld_stream(reinterpret_cast<const u32x4*>(kp + off + w * 64));
+        for (int j = 0; j < KW / 4; ++j)
+          kc[i][j] = ld_stream(reinterpret_cast<const u32x4*>(kp + off + j * 64));
       }
     };
-    auto load_v = [&](const Place& p) {
+    auto load_v = [&](const uint8_t* v, const Tile (&p)[2], int c_ss) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int i = j >> 2;
-        const unsigned off =
-            __umul24(min(4 * g4 + (j & 3), max(p.n[i] - 1, 0)), a.c_ss) + n16 * DV;
-        const uint32_t* vp = reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + p.at[i] + off);
+        const unsigned off = __umul24(min(4 * g4 + (j & 3), max(p[i].n - 1, 0)), c_ss) + n16 * DV;
+        const uint32_t* vp = reinterpret_cast<const uint32_t*>(v + p[i].at + off);
 #pragma unroll
-        for (int w = 0; w < VW; ++w) vc[j][w] = vp[w];
+        for (int c = 0; c < VW; ++c) vc[j][c] = vp[c];
       }
     };
-    auto first_of = [&](const Segment& s) {
-      return place8_of(x, keys_of(a, s), s.h, s.t0 * kTile + wave * kStep);
+    auto tiles = [](const Attn8Args& x, const View& w, int k0, Tile (&p)[2]) {
+      p[0] = tile_of(x, w, k0);
+      p[1] = tile_of(x, w, k0 + 16);
     };
-    walk.next(a, seg);  // a dealt workgroup has one
-    here = first_of(seg);
-    load_k(here.p);
-    load_v(here.p);
-    r.template load_q<true>(a, seg, 0, n16, g4);
-    for (bool go = true; go;) {
-      go = walk.next(a, nxt);
-      const Place8 turn = go ? first_of(nxt) : here;
+    bool go = walk.next(a, seg);  // not where a segment's start is all that it was dealt
+    View view, after;
+    if (go) {
+      view = view_of(x, seg);
+      tiles(x, view, seg.t0 * kTile + wave * kStep, here);
+      load_k(view.k, here, a.c_ss);
+      load_v(view.v, here, a.c_ss);
+      r.template load_q<true>(a, seg, 0, n16, g4);
+    }
+    while (go) {
+      const Attn8Args y = args8_again();
+      go = walk.next(y.a, nxt);
+      Tile turn[2] = {here[0], here[1]};
+      after = view;
+      if (go) {
+        after = view_of(y, nxt);
+        tiles(y, after, nxt.t0 * kTile + wave * kStep, turn);
+      }
       bool turned = false;  // the next segment's keys are on their way
-      const Keys keys = keys_of(a, seg);
       r.clear();
       for (int t = seg.t0; t < seg.t1; ++t) {
         const int k0 = t * kTile + wave * kStep, k1 = k0 + kTile;
         if (k0 >= r.hi) break;
         const bool more = t + 1 < seg.t1 && k1 < r.hi;
-        Place8 next = turn;
-        if (more) next = place8_of(x, keys, seg.h, k1);
+        Tile next[2] = {turn[0], turn[1]};
+        if (more) tiles(y, view, k1, next);
+        const uint8_t* const from_k = more ? view.k : after.k;
+        const uint8_t* const from_v = more ? view.v : after.v;
         turned = !more;
         f32x4_t sc[1][2] = {};
 #pragma unroll
@@ -153,28 +241,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_few_kernel
             sc[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                 as_bf(u32x4{lo[0], lo[1], hi[0], hi[1]}), as_bf(r.q[0][kk]), sc[0][i], 0, 0, 0);
           }
-          sc[0][i] *= here.ks[i];
+          sc[0][i] *= here[i].ks;
         }
-        if (more || go) load_k(next.p);  // under the softmax and the second product
-        if (k0 + kStep > r.lo || here.p.n[0] < 16 || here.p.n[1] < 16) {
+        if (more || go) load_k(from_k, next, y.a.c_ss);  // under the softmax and the second product
+        if (k0 + kStep > r.lo || here[0].n < 16 || here[1].n < 16) {
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
             const int at = 4 * g4 + (j & 3), key = k0 + 16 * (j >> 2) + at;
-            const bool there = at < here.p.n[j >> 2];
+            const bool there = at < here[j >> 2].n;
             if (!there || key >= r.lim[0]) sc[0][j >> 2][j & 3] = -__builtin_inff();
 #pragma unroll
-            for (int w = 0; w < VW; ++w) vc[j][w] = there ? vc[j][w] : 0;
+            for (int c = 0; c < VW; ++c) vc[j][c] = there ? vc[j][c] : 0;
           }
         }
-        float vs[2] = {here.vs[0], here.vs[1]};
+        float vs[2] = {here[0].n ? here[0].vs : 0.0f, here[1].n ? here[1].vs : 0.0f};
         const int wild = (is_nan(vs[0]) ? 1 : 0) | (is_nan(vs[1]) ? 2 : 0);
-        if (wild) {
-          spoil(r, wild, k0);
-          if (wild & 1) vs[0] = 0.0f;
-          if (wild & 2) vs[1] = 0.0f;
-        }
+        if (wild & 1) vs[0] = 0.0f;
+        if (wild & 2) vs[1] = 0.0f;
         u32x4 ph[1], pl[1];
-        r.template weights<true>(sc, a.c, ph, pl, vs);
+        r.template weights<true>(sc, y.a.c, ph, pl, vs);
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t o[4][4];
@@ -188,16 +273,19 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_few_kernel
             to = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, as_bf(pl[0]), to, 0, 0, 0);
           }
         }
-        if (more || go) load_v(next.p);
-        here = next;
+        if (wild) spoil(r, wild, k0);
+        if (more || go) load_v(from_v, next, y.a.c_ss);
+        here[0] = next[0], here[1] = next[1];
       }
       if (go) {
+        const AttnArgs z = args_again();
         if (!turned) {
-          load_k(turn.p);
-          load_v(turn.p);
+          load_k(after.k, turn, z.c_ss);
+          load_v(after.v, turn, z.c_ss);
         }
-        here = turn;
-        r.template load_q<true>(a, nxt, 0, n16, g4);
+        here[0] = turn[0], here[1] = turn[1];
+        view = after;
+        r.template load_q<true>(z, nxt, 0, n16, g4);
       }
       join_waves<D, false>(args_again(), r, seg, lds, wg, split);
       seg = nxt;
@@ -208,9 +296,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_few_kernel
   if (z.counters) zero_rows<D>(z);
 }
 
-// More rows: each wave has 16 NT of the workgroup's 64 NT.  Codes are asked for two steps
-// of 32 keys ahead, in registers, and go scaled into one of two buffers of LDS while the
+// More rows: each wave has 16 NT of the workgroup's 64 NT.  Codes are asked for a step of
+// 32 keys ahead, in registers, and go scaled into one of two buffers of LDS while the
 // other is read.  Chunks of a row are permuted as attention.hip's.
+// What bounds it: attention.hip's matrix and vector instructions, and 16 (e4m3) or 80
+// (int8) vector ones of a wave's step for the codes: 128 tokens over 65536 keys 240 and 268
+// us (570 and 510 TFLOP/s; bf16 rows 233), four 128-token chunks 51 and 52 (47), of which
+// the joins take 13; 32 tokens over 3126 keys 19 (18).  (Codes asked for two steps ahead
+// took more registers than there are: 258 and 279 us.)
 template <int D, int NT, int FORMAT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kernel(Attn8Args x) {
   typedef Rows<D, NT, true> R;
@@ -222,7 +315,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
   __shared__ int sums[kWaves];
   __shared__ int found[2];
   __shared__ u32x4 kv[2][2][kStep * CH];     // [buffer][K, V]
-  __shared__ int wilds[2][2];                // [buffer][tile]: its values read as NaN
+  __shared__ int marks[2][2];  // [buffer][tile] 1: its values read as NaN, 4: not all is there
   const AttnArgs& a = x.a;
   const int lane = threadIdx.x & (kWave - 1);
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
@@ -246,60 +339,54 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
   Segment seg;
   // eight threads to a key, a wave's keys of one tile
   const int row = threadIdx.x >> 3, part = threadIdx.x & 7, tile = wave >> 1;
-  struct Raw {
-    uint32_t k[PT], v[PT];
-    float ks, vs;
-  } raw[2];
-  while (walk.next(a, seg)) {
+  uint32_t raw_k[PT], raw_v[PT];
+  float raw_ks, raw_vs;
+  bool raw_out;
+  while (walk.next(args_again(), seg)) {
+    const Attn8Args y = args8_again();
     const int r0 = seg.rb * kBlock + wave * 16 * NT;
     int end = seg.len;  // the block's last key that any row sees
-    if (a.causal)
-      end = min(end, seg.len - seg.fresh + quot(min((seg.rb + 1) * kBlock, rows) - 1, a.G) + 1);
+    if (y.a.causal)
+      end = min(end, seg.len - seg.fresh + quot(min((seg.rb + 1) * kBlock, rows) - 1, y.a.G) + 1);
     const int t1 = min(seg.t1, (max(end, 0) + kStep - 1) / kStep);
-    const Keys keys = keys_of(a, seg);
-    auto load = [&](int t, Raw& w) {
-      const Place8 p = place8_of(x, keys, seg.h, t * kStep);
-      const int n = tile ? p.p.n[1] : p.p.n[0];
-      const int64_t at = (tile ? p.p.at[1] : p.p.at[0]) +
-                         __umul24(min(row & 15, max(n - 1, 0)), a.c_ss) + part * (PT * 4);
-      w.ks = tile ? p.ks[1] : p.ks[0];
-      w.vs = tile ? p.vs[1] : p.vs[0];
-      const uint32_t* kp = reinterpret_cast<const uint32_t*>((const uint8_t*)a.k + at);
-      const uint32_t* vp = reinterpret_cast<const uint32_t*>((const uint8_t*)a.v + at);
+    const View view = view_of(y, seg);
+    auto load = [&](int t) {
+      const Tile p = tile_of(y, view, t * kStep + 16 * tile);
+      const unsigned off = __umul24(min(row & 15, max(p.n - 1, 0)), y.a.c_ss) + part * (PT * 4);
+      raw_ks = p.ks;
+      raw_vs = p.n ? p.vs : 0.0f;
+      raw_out = p.n < 16;
+      const uint32_t* kp = reinterpret_cast<const uint32_t*>(view.k + p.at + off);
+      const uint32_t* vp = reinterpret_cast<const uint32_t*>(view.v + p.at + off);
 #pragma unroll
-      for (int i = 0; i < PT; ++i) w.k[i] = kp[i], w.v[i] = vp[i];
+      for (int i = 0; i < PT; ++i) raw_k[i] = kp[i], raw_v[i] = vp[i];
     };
-    auto store = [&](int t, const Raw& w) {
+    auto store = [&](int t) {
       const int buf = t & 1;
-      const bool wild = is_nan(w.vs);
-      const float vs = wild ? 0.0f : w.vs;
+      const bool wild = is_nan(raw_vs);
+      const float vs = wild ? 0.0f : raw_vs;
 #pragma unroll
       for (int c = 0; c < PT / 2; ++c) {
         const int chunk = part * (PT / 2) + c;
-        const u32x2 k0 = C::four(w.k[2 * c], w.ks), k1 = C::four(w.k[2 * c + 1], w.ks);
-        const u32x2 v0 = C::four(w.v[2 * c], vs), v1 = C::four(w.v[2 * c + 1], vs);
+        const u32x2 k0 = C::four(raw_k[2 * c], raw_ks), k1 = C::four(raw_k[2 * c + 1], raw_ks);
+        const u32x2 v0 = C::four(raw_v[2 * c], vs), v1 = C::four(raw_v[2 * c + 1], vs);
         kv[buf][0][row * CH + (chunk ^ k_swizzle(row & 15))] = u32x4{k0[0], k0[1], k1[0], k1[1]};
         kv[buf][1][row * CH + (chunk ^ v_swizzle(row))] = u32x4{v0[0], v0[1], v1[0], v1[1]};
       }
-      if ((wave & 1) == 0 && lane == 0) wilds[buf][tile] = wild;
+      if ((wave & 1) == 0 && lane == 0) marks[buf][tile] = (wild ? 1 : 0) | (raw_out ? 4 : 0);
     };
     __syncthreads();  // the last segment's reads are done
-    if (seg.t0 < t1) load(seg.t0, raw[0]);
-    if (seg.t0 + 1 < t1) load(seg.t0 + 1, raw[1]);
-    r.load_q(a, seg, r0, n16, g4);
+    if (seg.t0 < t1) load(seg.t0);
+    r.load_q(y.a, seg, r0, n16, g4);
     r.clear();
-    if (seg.t0 < t1) {
-      store(seg.t0, raw[0]);
-      if (seg.t0 + 2 < t1) load(seg.t0 + 2, raw[0]);
-    }
-    auto step = [&](int t, Raw& next) {
+    if (seg.t0 < t1) store(seg.t0);
+    if (seg.t0 + 1 < t1) load(seg.t0 + 1);
+    for (int t = seg.t0; t < t1; ++t) {
       const int k0 = t * kStep;
       __syncthreads();  // this step's keys are there, those of the step before have been read
-      if (t + 1 < t1) {
-        store(t + 1, next);
-        if (t + 3 < t1) load(t + 3, next);
-      }
-      if (k0 >= r.hi || r0 >= rows) return;
+      if (t + 1 < t1) store(t + 1);
+      if (t + 2 < t1) load(t + 2);
+      if (k0 >= r.hi || r0 >= rows) continue;
       const u32x4* const ks = kv[t & 1][0];
       const u32x4* const vs = kv[t & 1][1];
       u32x4 kf[2][KK];
@@ -325,17 +412,16 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
           vr[4 * e + 2 * i + 1] = (uint32_t)(w >> 32);
         }
       }
-      const Place here = place_of(a, keys, k0, blocks_of(a, keys, k0));
-      if (k0 + kStep > r.lo || here.n[0] < 16 || here.n[1] < 16) r.mask(sc, vr, here.n, k0, g4);
-      const int wild = uniform(wilds[t & 1][0]) | uniform(wilds[t & 1][1]) << 1;
-      if (wild) spoil(r, wild, k0);
+      const int mark = uniform(marks[t & 1][0] | marks[t & 1][1] << 1);
+      if (k0 + kStep > r.lo || mark >> 2) {
+        const int n[2] = {tile_of(y, view, k0).n, tile_of(y, view, k0 + 16).n};
+        r.mask(sc, vr, n, k0, g4);
+      }
       u32x4 ph[NT], pl[NT];
-      r.weights(sc, a.c, ph, pl);
+      r.weights(sc, y.a.c, ph, pl);
       r.product(vr, ph, pl);
-    };
-    for (int t = seg.t0; t < t1; t += 2) {
-      step(t, raw[1]);
-      if (t + 1 < t1) step(t + 1, raw[0]);
+      // here, after the products: ahead of them their sums took other registers, and a move each
+      if (mark & 3) spoil(r, mark, k0);
     }
     const AttnArgs args = args_again();
     const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
@@ -356,7 +442,7 @@ int launch8_many(const Attn8Args& x, hipStream_t st) {
   const dim3 grid((unsigned)((x.a.nwg + 7) / 8 * 8)), threads(kThreads);
   hipLaunchKernelGGL((attend8_many_kernel<D, NT, FORMAT>), grid, threads, 0, st, x);
   if (const int e = launch_status()) return e;
-  return launch_join_many<D, NT>(x.a, st);
+  return launch_join_many<D, NT, ManyDeal>(x.a, st);
 }
 
 template <int D, int FORMAT>
@@ -368,11 +454,16 @@ int launch8(const Shape& s, const Attn8Args& x, hipStream_t st) {
   hipLaunchKernelGGL((attend8_few_kernel<D, FORMAT>), grid, threads, 0, st, x);
   const int e = launch_status();
   if (e || x.a.counters) return e;
-  return launch_join_few<D>(x.a, st);
+  return launch_join_few<D, Few8Deal>(x.a, st);
 }
 
 }  // namespace
 }  // namespace umic
+
+extern "C" int64_t umic_cache8_attention_workspace_bytes(int64_t S, int64_t Hq, int64_t Hk,
+                                                         int64_t D) {
+  return umic::workspace_bytes(S, Hq, Hk, D, umic::few8_of(D));
+}
 
 extern "C" int umic_cache8_attention_bf16(
     const umic_cache8_t* cache, const void* q, void* out, const int32_t* table,
@@ -392,7 +483,12 @@ extern "C" int umic_cache8_attention_bf16(
   Attn8Args x = {};
   Shape s;
   if (!table && B > 0 && S > 0 && Hq > 0) return UMIC_ERR_INVALID_ARG;
-  if (const int e = attn_args(call, 16, x.a, s)) return e == 1 ? UMIC_OK : e;
+  if (const int e = attn_args(call, 16, few8_of(D), x.a, s)) return e == 1 ? UMIC_OK : e;
+  // Single tokens of up to a sixteenth of the CUs' segments, and less than five units for
+  // two workgroups a CU: one, half the parts (8 segments of 12288 keys 13.1 us for 15.6, 16
+  // of 3500 21 for 28; 32 of 4000 14.0 for 13.5, 8 of 131072 60 for 53).
+  const int cus = s.nwg / few8_of(D);
+  if (s.nt == 0 && B * c.heads * 16 <= cus) x.a.some = cus;
   x.ks = c.k_scale, x.vs = c.v_scale, x.s_sb = c.s_sb, x.s_sh = c.s_sh;
   hipStream_t st = as_stream(stream);
   const bool f = c.format == UMIC_CODES_INT8;

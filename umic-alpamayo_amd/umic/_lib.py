@@ -73,6 +73,7 @@ SIGNATURES: dict[str, list] = {
     "umic_cache_attention_bf16": [_P] * 7 + [_I64] * 19 + [_I, _F32, _P, _P, _I64, _P],
     "umic_cache8_append_bf16": [_P] * 9 + [_F32] + [_P] * 2 + [_F32] + [_I64] * 11 + [_P],
     "umic_cache8_read_bf16": [_P] * 6 + [_I64] * 5 + [_P],
+    "umic_cache8_attention_workspace_bytes": [_I64] * 4,
     "umic_cache8_attention_bf16": [_P] * 6 + [_I64] * 12 + [_I, _F32, _P, _P, _I64, _P],
     "umic_stream_read": [_P, _I64, _P, _P],
     "umic_stream_copy": [_P, _P, _I64, _P],
@@ -94,7 +95,8 @@ RESTYPES = {"umic_version": ctypes.c_char_p, "umic_error_string": ctypes.c_char_
             "umic_linear_kernel": _I64, "umic_linear_workspace_bytes": _I64,
             "umic_linear_workspace_preferred": _I64,
             "umic_cache_attention_workspace_bytes": _I64,
-            "umic_cache_attention_max_requests": _I64}
+            "umic_cache_attention_max_requests": _I64,
+            "umic_cache8_attention_workspace_bytes": _I64}
 
 
 class UmicLibraryError(RuntimeError):

@@ -23,6 +23,7 @@ No counterpart in the reference, whose cache (src/umic/cache.py:25-160) is of 16
 from __future__ import annotations
 
 import ctypes
+import functools
 from typing import NamedTuple
 
 import torch
@@ -36,6 +37,11 @@ BLOCK = 16  # rows that share a scale
 DTYPES = {torch.float8_e4m3fn: _lib.UMIC_CODES_E4M3, torch.int8: _lib.UMIC_CODES_INT8}
 HEAD_DIMS = _bf16.HEAD_DIMS
 _BF16 = torch.bfloat16
+
+
+@functools.lru_cache(maxsize=1024)
+def _workspace_bytes(dev: int, S: int, Hq: int, Hk: int, D: int) -> int:
+    return _lib.lib().umic_cache8_attention_workspace_bytes(S, Hq, Hk, D)
 
 
 class _Layout(NamedTuple):
@@ -286,7 +292,7 @@ def attention(q: torch.Tensor, cache: Pages8, kv_len, table: torch.Tensor, *,
     q0, q1, q2, _ = q.stride()
     with _lib.device_of(q):
         stream = _lib.stream_of(q)
-        size = _bf16._workspace_bytes(dev, S, Hq, Hk, D)
+        size = _workspace_bytes(dev, S, Hq, Hk, D)
         counters, ws = _bf16._scratch(q, dev, stream, size)
         _lib.call("umic_cache8_attention_bf16", lay.at, q.data_ptr(), out.data_ptr(),
                   table.data_ptr(), lens, _lib.ptr(q_len), B, S, Hq, q0, q2, q1, o0, o1, o2, ld,
