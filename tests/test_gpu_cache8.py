@@ -198,21 +198,21 @@ def test_values_that_are_not_finite(kind, bad):
 @pytest.mark.parametrize("T", [1, 5, 77, 2200])
 @pytest.mark.parametrize("Hq,Hk,D", [(32, 8, 128), (14, 2, 64), (4, 3, 256)])
 @pytest.mark.parametrize("norm", [False, True])
-def test_rotate_append_is_rotate_and_append(kind, T, Hq, Hk, D, norm):
-    """To the bit, q and cache."""
+def test_rotate_append(kind, T, Hq, Hk, D, norm):
+    """q against the formula in 64 bits; the cache, to the bit, that of the same rows rotated as q
+    and appended."""
     g = torch.Generator().manual_seed(T + D)
     q, k, v = (bf16_randn(T, h, D, gen=g).to(DEV) for h in (Hq, Hk, Hk))
-    plan = axial.AxisPlan((1e4 ** (-torch.arange(D // 2) / (D // 2))).float(),
-                          torch.arange(D // 2) % 3, 1.25, DEV)
+    inv, axis = (1e4 ** (-torch.arange(D // 2) / (D // 2))).float(), torch.arange(D // 2) % 3
+    plan = axial.AxisPlan(inv, axis, 1.25, DEV)
     pos = torch.randint(-9, 40000, (3, T), generator=g).to(DEV)
-    w = tuple(bf16_randn(D, scale=0.1, shift=1.0, gen=g).to(DEV) for _ in range(2))
-    norm = (*w, 1e-5) if norm else None
-    one, two = (new_cache(kind, T // 16 + 3, Hk, 16, D) for _ in range(2))
+    qw, kw = (bf16_randn(D, scale=0.1, shift=1.0, gen=g).to(DEV) for _ in range(2))
+    one, two, spare = (new_cache(kind, T // 16 + 3, Hk, 16, D) for _ in range(3))
     slots = torch.arange(T, device=DEV) + 21
-    got = cache8.rotate_append(q, k, v, pos, plan, slots, one, norm)
-    want, turned = axial.rotate(q, k, pos, plan, norm)
+    got = cache8.rotate_append(q, k, v, pos, plan, slots, one, (qw, kw, 1e-5) if norm else None)
+    ref.check_rotated(got, *ref.rotate(q, pos, inv, axis, qw if norm else None, 1e-5, 1.25), norm)
+    turned = cache8.rotate_append(k, k, v, pos, plan, slots, spare, (kw, kw, 1e-5) if norm else None)
     cache8.append(turned, v, slots, two)
-    assert torch.equal(got, want)
     for a, b in zip(one, two):
         assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
 
@@ -560,7 +560,8 @@ def test_served_together(kind):
         q = cache8.rotate_append(q, k, v, pos, plan, t.slots, cache)
         got = cache8.attention(q.view(R, S, Hq, D).transpose(1, 2), cache, n, table,
                                q_len=torch.tensor(new, **i32))
-        turned = axial.rotate(k, k, pos, plan)[0]
+        spare = cache8.empty(R * S // 16 + 1, Hk, 16, D, ref8.TYPES[kind], DEV)
+        turned = cache8.rotate_append(k, k, v, pos, plan, torch.arange(R * S, device=DEV), spare)
         for i, x in enumerate((turned, v)):
             ref8.store(kind, model[i], model[i + 2], x.double().cpu().numpy(), t.slots.tolist())
         check_cache(cache, model)

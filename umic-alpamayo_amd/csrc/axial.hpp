@@ -42,6 +42,25 @@ struct AxialArgs {
   SmallDiv half;    // D / 2
 };
 
+// Sine and cosine of a position's angle, turn being 64-bit fractions of a turn.  FINE: of
+// its distance from the nearest quarter turn, whose rounding to fp32 is 2^-25 of at most
+// pi / 4 and not of pi.
+template <bool FINE>
+__device__ __forceinline__ void turn_of(int64_t pos, uint64_t turn, float& s, float& c) {
+  const int32_t frac = (int32_t)(((uint64_t)pos * turn) >> 32);
+  if constexpr (FINE) {
+    const int32_t quarter = (int32_t)(((uint32_t)frac + 0x20000000u) >> 30);
+    const int32_t rest = (int32_t)((uint32_t)frac - ((uint32_t)quarter << 30));
+    float x, y;
+    sincospif((float)rest * 0x1p-31f, &x, &y);
+    const float p = quarter & 1 ? y : x, q = quarter & 1 ? x : y;
+    s = quarter & 2 ? -p : p;
+    c = (quarter + 1) & 2 ? -q : q;
+  } else {
+    sincospif((float)frac * 0x1p-31f, &s, &c);
+  }
+}
+
 // VEC elements as they lie in memory
 template <int VEC>
 struct Raw;
@@ -80,8 +99,8 @@ struct Raw<4> {
 // a row.  NT: stores past the caches, where the halves of a row are whole lines
 // (16381 tokens of 32 + 8 heads of 128: 72 us for 80; rows of 80, which are not,
 // 46 for 40).
-// block: of a.tokens tokens; cs: [token][pair] (cos, sin) in LDS.
-template <int VEC, bool NORM, bool NT>
+// block: of a.tokens tokens; cs: [token][pair] (cos, sin) in LDS; FINE: turn_of's.
+template <int VEC, bool NORM, bool NT, bool FINE = false>
 __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, float* cs) {
   constexpr int kItems = kItemsOf<NORM>;
   const int half = a.half.d;
@@ -136,8 +155,7 @@ __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, f
     float s = 0.0f, c = 1.0f;
     if (ax >= 0 && ax < a.A) {  // an axis that is not there does not turn
       const int64_t pos = a.positions[ax * a.p_sa + (t0 + t) * a.p_st];
-      const int32_t frac = (int32_t)(((uint64_t)pos * a.turn[f]) >> 32);
-      sincospif((float)frac * 0x1p-31f, &s, &c);
+      turn_of<FINE>(pos, a.turn[f], s, c);
     }
     cs[2 * i] = c * a.scale;
     cs[2 * i + 1] = s * a.scale;

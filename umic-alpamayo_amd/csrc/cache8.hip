@@ -11,9 +11,11 @@
 //
 // The tokens of a block that one call brings stand within kSpan neighbours, so that a wave
 // finds by its lanes which are a block's, and which is its first: that one's workgroup
-// writes all of them.  A wave does one head of them, keys or values, at a time, as
-// `rotate` would lay their rows out over the lanes: the bits are those of `rotate`'s rows,
-// quantised.
+// writes all of them.  Behind those workgroups stand others that rotate q.
+//
+// What bounds it: at prompt sizes HBM, less what the short chains of a block (its slots,
+// rows, maximum, codes) leave idle: 16381 tokens of 32 + 8 heads of 128 70 us, 5.2 TB/s (q
+// alone 47, the codes alone 36); 3100 with the norm 19; 8 tokens 6, a chain of loads.
 #include "axial.hpp"
 #include "codes.hpp"
 
@@ -38,8 +40,7 @@ struct StoreArgs {
   int64_t slots_n;
   int shift;         // of a page
   int chunk;         // tokens of a workgroup: it does the blocks whose first is among them
-  int groups;        // of key heads, a workgroup each
-  int heads;         // of a group
+  int split;         // workgroups of a chunk, which share its blocks' heads
   unsigned blocks;   // workgroups that do so; those behind them rotate q
 };
 
@@ -49,52 +50,93 @@ __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
   return __builtin_bit_cast(uint32_t, m);
 }
 
+// A wave's task is a block's new tokens of one head, keys or values.  The sines and cosines
+// are the workgroup's, once for all heads.
 template <int D, int FORMAT, bool TURN, bool NORM>
-__global__ __launch_bounds__(kThreads) void store_kernel(StoreArgs a) {
+__global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(StoreArgs a) {
   typedef Codes<FORMAT> C;
   constexpr int kLanes = D / 16;            // of a row, 8 elements of each half a lane
   constexpr int kRows = kWave / kLanes;     // rows of a pass
   constexpr int kPasses = kBlockTokens / kRows;
   constexpr int kOld = D / 64;              // 16-byte chunks of a block's codes a lane holds
-  extern __shared__ float cs[];             // [token of the run][pair] (cos, sin)
-  __shared__ int places[kBlockTokens];
+  constexpr int kTurns = 2 * kThreads / D;  // tokens whose sines the workgroup does at a time
+  extern __shared__ float cs[];             // (cos, sin): [token][pair]
   if (blockIdx.x >= a.blocks) {
-    if constexpr (TURN) axial_rows<8, NORM, (D >= 128)>(a.x, blockIdx.x - a.blocks, cs);
+    if constexpr (TURN) axial_rows<8, NORM, (D >= 128), true>(a.x, blockIdx.x - a.blocks, cs);
     return;
   }
   const int lane = threadIdx.x & (kWave - 1);
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
-  const unsigned per = 2 * a.groups;
-  const int64_t t0 = (int64_t)(blockIdx.x / per) * a.chunk;
-  const int part = blockIdx.x % per;
-  const bool keys = part < a.groups;
-  const int h0 = (keys ? part : part - a.groups) * a.heads;
-  const int h1 = min((int)a.Hk, h0 + a.heads);
-  const uint16_t* const src = keys ? a.k : a.v;
-  const int64_t st = keys ? a.k_st : a.v_st, sh = keys ? a.k_sh : a.v_sh;
-  uint8_t* const codes = keys ? a.k8 : a.v8;
-  float* const scales = keys ? a.ks : a.vs;
+  const int waves = kWaves * a.split, parts = 2 * (int)a.Hk;
+  const int64_t t0 = (int64_t)(blockIdx.x / a.split) * a.chunk;
+  const int mine = __builtin_amdgcn_readfirstlane(blockIdx.x % a.split * kWaves + threadIdx.x / kWave);
 
   // lane i: token t0 - (kSpan - 1) + i, its block and row; a slot outside the pool has none
   const int64_t base = t0 - (kSpan - 1);
   const int64_t tok = base + lane;
   int64_t slot = -1;
   if (lane < a.chunk + 2 * (kSpan - 1) && tok >= 0 && tok < a.x.T) slot = a.x.slots[tok];
+  int axis = -1;
+  uint64_t turn = 0;
+  if constexpr (TURN) {
+    axis = a.x.axis[threadIdx.x % (D / 2)];
+    turn = a.x.turn[threadIdx.x % (D / 2)];
+  }
   const int block = slot >= 0 && slot < a.slots_n ? (int)(slot / kBlockTokens) : -1;
   const int row = (int)(slot & (kBlockTokens - 1));
+  // lane i: where the i-th of some of the lanes stands
+  auto nth = [&](uint64_t some) {
+    const int below = __builtin_popcountll(some & (((uint64_t)1 << lane) - 1));
+    const int to = some >> lane & 1 ? below : __builtin_popcountll(some) + lane - below;
+    return __builtin_amdgcn_ds_permute(to * 4, lane);
+  };
 
+  uint64_t firsts = 0, all = 0;  // of this workgroup's blocks: the first tokens, all tokens
   for (int c = 0; c < a.chunk; ++c) {
     const int at = kSpan - 1 + c;
     const int blk = __builtin_amdgcn_readlane(block, at);
     const uint64_t mates = __ballot(block == blk);
     // a block is its first token's to write
     if (blk < 0 || mates << (64 - at) >> (64 - (kSpan - 1))) continue;
-    const uint64_t run = mates >> at << (64 - kSpan) >> (64 - kSpan) << at;
+    firsts |= (uint64_t)1 << at;
+    all |= mates >> at << (64 - kSpan) >> (64 - kSpan) << at;
+  }
+  if (!firsts) return;
+  if constexpr (TURN) {
+    const int turned = nth(all), n = __builtin_popcountll(all);
+    const bool moves = axis >= 0 && axis < a.x.A;  // an axis that is not there does not turn
+    constexpr int kAhead = 4;                      // positions on their way
+    for (int i = 0; i < n; i += kAhead * kTurns) {
+      int64_t pos[kAhead];
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int t = i + u * kTurns + threadIdx.x / (D / 2);
+        const int64_t token = base + __shfl(turned, min(t, n - 1), kWave);
+        pos[u] = moves ? a.x.positions[axis * a.x.p_sa + token * a.x.p_st] : 0;
+      }
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u) {
+        const int t = i + u * kTurns + threadIdx.x / (D / 2);
+        if (i + u * kTurns >= n) break;
+        float s, c;
+        turn_of<true>(pos[u], turn, s, c);
+        if (t < n)
+          *reinterpret_cast<f32x2_t*>(cs + t * D + 2 * (threadIdx.x % (D / 2))) =
+              f32x2_t{c * a.x.scale, s * a.x.scale};
+      }
+    }
+    __syncthreads();
+  }
+
+  const int c8 = (lane % kLanes) * 8;
+  int part = mine;
+  for (; firsts; firsts &= firsts - 1, part -= parts) {
+    // the chunk's tasks, its blocks' parts in turn, are dealt over the waves
+    if (part >= parts) continue;
+    const int at = __builtin_ctzll(firsts);
+    const int blk = __builtin_amdgcn_readlane(block, at);
+    const uint64_t run = __ballot(block == blk) >> at << (64 - kSpan) >> (64 - kSpan) << at;
     const int n = min(kBlockTokens, __builtin_popcountll(run));
-    // lane i: where the run's token i stands, and its row
-    const int below = __builtin_popcountll(run & (((uint64_t)1 << lane) - 1));
-    const int there = run >> lane & 1 ? below : __builtin_popcountll(run) + lane - below;
-    const int place = __builtin_amdgcn_ds_permute(there * 4, lane);
+    const int place = nth(run);
     const int its_row = __shfl(row, place, kWave);
     int row0 = lane < n ? its_row : kBlockTokens;  // the lowest
 #pragma unroll
@@ -103,60 +145,54 @@ __global__ __launch_bounds__(kThreads) void store_kernel(StoreArgs a) {
     const int64_t in = (int64_t)blk * kBlockTokens;
     const int64_t page = in >> a.shift;
     const int64_t r0 = in & (((int64_t)1 << a.shift) - 1);
-    if constexpr (TURN) {
-      __syncthreads();  // the last run's turns have been read
-      if (threadIdx.x < kBlockTokens) places[threadIdx.x] = place;
-      __syncthreads();
-      if (keys)
-        for (int i = threadIdx.x; i < n * (D / 2); i += kThreads) {
-          const int f = i % (D / 2), t = i / (D / 2);
-          const int64_t of = base + places[t];
-          const int ax = a.x.axis[f];
-          float s = 0.0f, c = 1.0f;
-          if (ax >= 0 && ax < a.x.A) {
-            const int64_t pos = a.x.positions[ax * a.x.p_sa + of * a.x.p_st];
-            const int32_t frac = (int32_t)(((uint64_t)pos * a.x.turn[f]) >> 32);
-            sincospif((float)frac * 0x1p-31f, &s, &c);
-          }
-          cs[2 * i] = c * a.x.scale;
-          cs[2 * i + 1] = s * a.x.scale;
-        }
-      __syncthreads();
+    int at_row[kPasses];  // -1: no token
+    int of[kPasses];      // where it stands
+#pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+      const int i = p * kRows + lane / kLanes;
+      of[p] = __shfl(place, i < n ? i : 0, kWave);
+      at_row[p] = __shfl(its_row, i, kWave);
+      if (i >= n) at_row[p] = -1;
     }
-    const int c8 = (lane % kLanes) * 8;
-    for (int h = h0 + wave; h < h1; h += kWaves) {
-      uint8_t* const to = codes + page * a.c_sb + h * a.c_sh + r0 * a.c_ss;
-      float* const scale = scales + page * a.s_sb + h * a.s_sh + r0 / kBlockTokens;
-      u32x4 lo[kPasses], hi[kPasses], old[kOld];
-      int at_row[kPasses];  // -1: no token
+    u32x4 lo[kPasses], hi[kPasses];
+    auto fetch = [&](int part) {
+      const bool keys = part < a.Hk;
+      const int h = keys ? part : part - (int)a.Hk;
+      const uint16_t* const src = (keys ? a.k : a.v) + h * (keys ? a.k_sh : a.v_sh) + c8;
+      const int64_t st = keys ? a.k_st : a.v_st;
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        const int i = p * kRows + lane / kLanes;
-        at_row[p] = __shfl(its_row, i, kWave);
-        const int64_t of = base + __shfl(place, i, kWave);
-        if (i >= n) at_row[p] = -1;
         lo[p] = hi[p] = u32x4{0, 0, 0, 0};
-        if (i < n) {
-          const uint16_t* from = src + of * st + h * sh + c8;
-          lo[p] = ld_stream(reinterpret_cast<const u32x4*>(from));
-          hi[p] = ld_stream(reinterpret_cast<const u32x4*>(from + D / 2));
+        if (at_row[p] >= 0) {
+          const uint16_t* x = src + (base + of[p]) * st;
+          lo[p] = ld_stream(reinterpret_cast<const u32x4*>(x));
+          hi[p] = ld_stream(reinterpret_cast<const u32x4*>(x + D / 2));
         }
       }
+    };
+    fetch(part);
+#pragma unroll 1
+    for (; part < parts; part += waves) {
+      const bool keys = part < a.Hk;
+      const int h = keys ? part : part - (int)a.Hk;
+      uint8_t* const to = (keys ? a.k8 : a.v8) + page * a.c_sb + h * a.c_sh + r0 * a.c_ss;
+      float* const scale = (keys ? a.ks : a.vs) + page * a.s_sb + h * a.s_sh + r0 / kBlockTokens;
+      u32x4 old[kOld];
       float was = 0.0f;
       if (row0 > 0) {
         was = *scale;
 #pragma unroll
         for (int j = 0; j < kOld; ++j) {
-          const int c = j * kWave + lane, r = c / (D / 16);
+          const int i = j * kWave + lane, r = i / (D / 16);
           old[j] = u32x4{0, 0, 0, 0};
-          if (r < row0) old[j] = *reinterpret_cast<const u32x4*>(to + r * a.c_ss + c % (D / 16) * 16);
+          if (r < row0) old[j] = *reinterpret_cast<const u32x4*>(to + r * a.c_ss + i % (D / 16) * 16);
         }
       }
       if constexpr (TURN)
         if (keys)
 #pragma unroll
           for (int p = 0; p < kPasses; ++p) {
-            const int i = min(p * kRows + lane / kLanes, n - 1);
+            if (p * kRows >= n) break;
             float x[8], y[8], ox[8], oy[8];
             unpack8(lo[p], x);
             unpack8(hi[p], y);
@@ -176,15 +212,16 @@ __global__ __launch_bounds__(kThreads) void store_kernel(StoreArgs a) {
                 y[j] = y[j] * r * wy[j];
               }
             }
-            const float* t = cs + 2 * (i * (D / 2) + c8);
+            const int its = __builtin_popcountll(all & (((uint64_t)1 << of[p]) - 1));
+            const float* t = cs + its * D + 2 * c8;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
               ox[j] = x[j] * t[2 * j] - y[j] * t[2 * j + 1];
               oy[j] = y[j] * t[2 * j] + x[j] * t[2 * j + 1];
             }
-            const bool there = at_row[p] >= 0;
-            lo[p] = there ? pack8(ox) : u32x4{0, 0, 0, 0};
-            hi[p] = there ? pack8(oy) : u32x4{0, 0, 0, 0};
+            const bool is = at_row[p] >= 0;
+            lo[p] = is ? pack8(ox) : u32x4{0, 0, 0, 0};
+            hi[p] = is ? pack8(oy) : u32x4{0, 0, 0, 0};
           }
       // the largest magnitude's exponent: that of bf16 numbers as whole ones
       uint32_t top = 0;
@@ -203,39 +240,43 @@ __global__ __launch_bounds__(kThreads) void store_kernel(StoreArgs a) {
       int e = max((most >> 7) - 127 - C::kTop, kLeastExp);
       if (row0 > 0) e = max(e, was_exp);
       const float s = __uint_as_float((uint32_t)(e + 127) << 23);
-      const float inv = wild ? 0.0f : __uint_as_float((uint32_t)(127 - e) << 23);
+      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
       if (lane == 0) *scale = wild ? __builtin_nanf("") : s;
+      uint32_t w[kPasses][4];
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        if (at_row[p] < 0) continue;
         float x[8], y[8];
         unpack8(lo[p], x);
         unpack8(hi[p], y);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          x[j] = wild ? 0.0f : x[j] * inv;
-          y[j] = wild ? 0.0f : y[j] * inv;
-        }
+        for (int j = 0; j < 8; ++j) x[j] *= inv, y[j] *= inv;
+        w[p][0] = C::round4(x), w[p][1] = C::round4(x + 4);
+        w[p][2] = C::round4(y), w[p][3] = C::round4(y + 4);
+      }
+      if (part + waves < parts) fetch(part + waves);
+#pragma unroll
+      for (int p = 0; p < kPasses; ++p) {
+        if (at_row[p] < 0) continue;
         uint8_t* r = to + at_row[p] * a.c_ss + c8;
-        *reinterpret_cast<u32x2*>(r) = u32x2{C::round4(x), C::round4(x + 4)};
-        *reinterpret_cast<u32x2*>(r + D / 2) = u32x2{C::round4(y), C::round4(y + 4)};
+        *reinterpret_cast<u32x2*>(r) = wild ? u32x2{0, 0} : u32x2{w[p][0], w[p][1]};
+        *reinterpret_cast<u32x2*>(r + D / 2) = wild ? u32x2{0, 0} : u32x2{w[p][2], w[p][3]};
       }
       if (row0 > 0 && !wild && e > was_exp) {  // the rows before, at the new scale
         const float ratio = was * inv;
 #pragma unroll
         for (int j = 0; j < kOld; ++j) {
-          const int c = j * kWave + lane, r = c / (D / 16);
+          const int i = j * kWave + lane, r = i / (D / 16);
           if (r >= row0) continue;
-          u32x4 w;
+          u32x4 o;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
+          for (int q = 0; q < 4; ++q) {
             float x[4];
-            C::values4(old[j][i], x);
+            C::values4(old[j][q], x);
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k] *= ratio;
-            w[i] = C::round4(x);
+            for (int y = 0; y < 4; ++y) x[y] *= ratio;
+            o[q] = C::round4(x);
           }
-          *reinterpret_cast<u32x4*>(to + r * a.c_ss + c % (D / 16) * 16) = w;
+          *reinterpret_cast<u32x4*>(to + r * a.c_ss + i % (D / 16) * 16) = o;
         }
       }
     }
@@ -307,11 +348,20 @@ int launch_store(StoreArgs& a, bool turn, hipStream_t st) {
     grid = s.blocks;
     lds = s.lds;
   }
-  if (turn) lds = std::max(lds, (size_t)kBlockTokens * D * sizeof(float));
-  a.chunk = a.x.T <= 2048 ? 1 : kChunk;
-  a.heads = kWaves;
-  a.groups = (int)((a.Hk + a.heads - 1) / a.heads);
-  const int64_t blocks = (a.x.T + a.chunk - 1) / a.chunk * 2 * a.groups;
+  const int64_t cus = device_cus();
+  if (cus <= 0) return (int)hipErrorNoDevice;
+  // Two chunks to a CU's workgroup in four, up to kChunk tokens each; then a workgroup for
+  // each four tasks of a block while there are not two to a CU.  (Chunks of a token up to
+  // 2048 of them: 42 us for 16.5, most workgroups having no block's first token; four times
+  // the chunks 20.9.  Four workgroups to a CU: 3100 tokens 23.7 us for 19.0, and one 19.4,
+  // where 4096 tokens of 64 requests take 39 for 29.)
+  a.chunk = (int)std::min<int64_t>((2 * a.x.T + cus - 1) / cus, kChunk);
+  const int64_t chunks = (a.x.T + a.chunk - 1) / a.chunk;
+  a.split = (int)std::max<int64_t>(
+      1, std::min<int64_t>((2 * a.Hk + kWaves - 1) / kWaves, 2 * cus / chunks));
+  if (turn)
+    lds = std::max(lds, (size_t)std::min(a.chunk + kSpan - 1, a.chunk * kSpan) * D * sizeof(float));
+  const int64_t blocks = chunks * a.split;
   if (blocks + grid > 0x7fffffff) return UMIC_ERR_UNSUPPORTED;
   a.blocks = (unsigned)blocks;
   auto* kern = !turn    ? store_kernel<D, FORMAT, false, false>
