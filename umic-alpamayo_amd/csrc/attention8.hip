@@ -12,6 +12,8 @@
 //
 // A block whose scale is NaN reads as NaN: a row that sees one of its keys is NaN, others
 // are as without it.
+#include <type_traits>
+
 #include "attention.hpp"
 #include "codes.hpp"
 
@@ -298,12 +300,13 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
 
 // More rows: each wave has 16 NT of the workgroup's 64 NT.  Codes are asked for a step of
 // 32 keys ahead, in registers, and go scaled into one of two buffers of LDS while the
-// other is read.  Chunks of a row are permuted as attention.hip's.
+// other is read.  Two steps are written out, so that the buffers' addresses are known (128
+// tokens over 65536 keys 216 us for 246).  Chunks of a row are permuted as attention.hip's.
 // What bounds it: attention.hip's matrix and vector instructions, and 16 (e4m3) or 80
-// (int8) vector ones of a wave's step for the codes: 128 tokens over 65536 keys 240 and 268
-// us (570 and 510 TFLOP/s; bf16 rows 233), four 128-token chunks 51 and 52 (47), of which
-// the joins take 13; 32 tokens over 3126 keys 19 (18).  (Codes asked for two steps ahead
-// took more registers than there are: 258 and 279 us.)
+// (int8) vector ones of a wave's step for the codes: 128 tokens over 65536 keys 216 and 235
+// us (640 and 580 TFLOP/s; bf16 rows 233), four 128-token chunks 47 and 48 (47), of which
+// the joins take 13; 32 tokens over 3126 keys 18 (18).  (Codes asked for two steps ahead:
+// the same, and 6% slower through LDS.)
 template <int D, int NT, int FORMAT>
 __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kernel(Attn8Args x) {
   typedef Rows<D, NT, true> R;
@@ -361,8 +364,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
 #pragma unroll
       for (int i = 0; i < PT; ++i) raw_k[i] = kp[i], raw_v[i] = vp[i];
     };
-    auto store = [&](int t) {
-      const int buf = t & 1;
+    auto store = [&](auto buffer) {
+      constexpr int buf = buffer;
       const bool wild = is_nan(raw_vs);
       const float vs = wild ? 0.0f : raw_vs;
 #pragma unroll
@@ -379,16 +382,19 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
     if (seg.t0 < t1) load(seg.t0);
     r.load_q(y.a, seg, r0, n16, g4);
     r.clear();
-    if (seg.t0 < t1) store(seg.t0);
+    const std::integral_constant<int, 0> first;
+    const std::integral_constant<int, 1> second;
+    if (seg.t0 < t1) store(first);
     if (seg.t0 + 1 < t1) load(seg.t0 + 1);
-    for (int t = seg.t0; t < t1; ++t) {
+    auto step = [&](int t, auto buffer, auto other) {
+      constexpr int buf = buffer;
       const int k0 = t * kStep;
       __syncthreads();  // this step's keys are there, those of the step before have been read
-      if (t + 1 < t1) store(t + 1);
+      if (t + 1 < t1) store(other);
       if (t + 2 < t1) load(t + 2);
-      if (k0 >= r.hi || r0 >= rows) continue;
-      const u32x4* const ks = kv[t & 1][0];
-      const u32x4* const vs = kv[t & 1][1];
+      if (k0 >= r.hi || r0 >= rows) return;
+      const u32x4* const ks = kv[buf][0];
+      const u32x4* const vs = kv[buf][1];
       u32x4 kf[2][KK];
 #pragma unroll
       for (int i = 0; i < 2; ++i)
@@ -412,7 +418,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
           vr[4 * e + 2 * i + 1] = (uint32_t)(w >> 32);
         }
       }
-      const int mark = uniform(marks[t & 1][0] | marks[t & 1][1] << 1);
+      const int mark = uniform(marks[buf][0] | marks[buf][1] << 1);
       if (k0 + kStep > r.lo || mark >> 2) {
         const int n[2] = {tile_of(y, view, k0).n, tile_of(y, view, k0 + 16).n};
         r.mask(sc, vr, n, k0, g4);
@@ -422,6 +428,10 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
       r.product(vr, ph, pl);
       // here, after the products: ahead of them their sums took other registers, and a move each
       if (mark & 3) spoil(r, mark, k0);
+    };
+    for (int t = seg.t0; t < t1; t += 2) {
+      step(t, first, second);
+      if (t + 1 < t1) step(t + 1, second, first);
     }
     const AttnArgs args = args_again();
     const int slot = wg * 2 + (seg.t0 == 0 ? 1 : 0);
