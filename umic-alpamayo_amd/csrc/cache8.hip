@@ -298,43 +298,64 @@ struct ReadArgs {
   int len, cap, shift, pages, Hk;
 };
 
-// A thread's 16 codes to 32 bytes; a workgroup does 16 rows' or more of one head.
-template <int D, int FORMAT>
+// A scalar load whatever the compiler can prove about the kernel's stores.
+__device__ __forceinline__ int scalar_i32(const int32_t* p) {
+  return *(const __attribute__((address_space(4))) int32_t*)(uintptr_t)p;
+}
+
+// A thread's 8 codes at a time to 16 bytes, in ITEMS rows whose loads are on their way
+// together.  HBM-bound: 4 x 30011 rows of 8 heads of 128 119.9 us, 6.2 TB/s (one row a
+// thread 156, four 127, 16 codes to two stores 129); of padded rows, mostly zeros, 166 MB
+// in 31 us (one 33, four 34).
+template <int D, int FORMAT, int ITEMS>
 __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
   typedef Codes<FORMAT> C;
-  constexpr int kChunks = D / 16, kRows = kThreads / kChunks;
-  const int64_t tile = blockIdx.x % a.blocks;
-  const int64_t head = blockIdx.x / a.blocks;  // (k or v, request, key head)
-  const int h = (int)(head % a.Hk);
-  const int64_t rest = head / a.Hk;
+  constexpr int kChunks = D / 8, kRows = kThreads / kChunks;
+  const int64_t head = blockIdx.x / (unsigned)a.blocks;  // (request, k or v, key head)
+  const unsigned block = blockIdx.x % (unsigned)a.blocks;
+  const int h = (int)((unsigned)head % (unsigned)a.Hk);
+  const unsigned rest = (unsigned)head / (unsigned)a.Hk;
   const int b = (int)(rest >> 1);
   const bool keys = !(rest & 1);
-  const int64_t row = tile * kRows + threadIdx.x / kChunks;
-  const int c = threadIdx.x % kChunks * 16;
-  if (row >= a.rows) return;
-  const int n = a.kv_len ? min(max(a.kv_len[b], 0), a.cap) : a.len;
-  const int64_t at = row + (a.start ? max(a.start[b], 0) : 0);
-  u32x4 out[2] = {};
-  if (at < n) {
-    const int page = a.table[b * a.table_ld + (at >> a.shift)];
-    if ((unsigned)page < (unsigned)a.pages) {
-      const int64_t in = at & (((int64_t)1 << a.shift) - 1);
-      const u32x4 w = ld_stream(reinterpret_cast<const u32x4*>(
-          (keys ? a.k8 : a.v8) + page * a.c_sb + h * a.c_sh + in * a.c_ss + c));
-      const float s = (keys ? a.ks : a.vs)[page * a.s_sb + h * a.s_sh + in / kBlockTokens];
+  const int c = threadIdx.x % kChunks * 8;
+  const int64_t row0 = (int64_t)block * (ITEMS * kRows) + threadIdx.x / kChunks;
+  const int n = a.kv_len ? min(max(scalar_i32(a.kv_len + b), 0), a.cap) : a.len;
+  const int64_t at0 = row0 + (a.start ? max(scalar_i32(a.start + b), 0) : 0);
+  const uint8_t* const codes = (keys ? a.k8 : a.v8) + h * a.c_sh + c;
+  const float* const scales = (keys ? a.ks : a.vs) + h * a.s_sh;
+  const int32_t* const table = a.table + b * a.table_ld;
+  int page[ITEMS];
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float x[4];
-        C::values4(w[i], x);
-        out[i / 2][i % 2 * 2] = pack2(x[0] * s, x[1] * s);
-        out[i / 2][i % 2 * 2 + 1] = pack2(x[2] * s, x[3] * s);
-      }
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t at = at0 + i * kRows;
+    page[i] = at < n ? table[at >> a.shift] : -1;
+  }
+  u32x2 w[ITEMS];
+  float s[ITEMS];
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    const int64_t in = (at0 + i * kRows) & (((int64_t)1 << a.shift) - 1);
+    w[i] = u32x2{0, 0};
+    s[i] = 0.0f;
+    if ((unsigned)page[i] < (unsigned)a.pages) {  // others are not there
+      w[i] = __builtin_nontemporal_load(
+          reinterpret_cast<const u32x2*>(codes + page[i] * a.c_sb + in * a.c_ss));
+      s[i] = scales[page[i] * a.s_sb + in / kBlockTokens];
     }
   }
-  u32x4* to = reinterpret_cast<u32x4*>(
-      (keys ? a.ko : a.vo) + (((int64_t)b * a.Hk + h) * a.rows + row) * D + c);
-  st_stream(to, out[0]);
-  st_stream(to + 1, out[1]);
+  uint16_t* const to =
+      (keys ? a.ko : a.vo) + (((int64_t)b * a.Hk + h) * a.rows + row0) * D + c;
+#pragma unroll
+  for (int i = 0; i < ITEMS; ++i) {
+    if (row0 + i * kRows >= a.rows) break;
+    float x[4], y[4];
+    C::values4(w[i][0], x);
+    C::values4(w[i][1], y);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] *= s[i], y[j] *= s[i];
+    st_stream(reinterpret_cast<u32x4*>(to + (int64_t)i * kRows * D),
+              u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])});
+  }
 }
 
 template <int D, int FORMAT>
@@ -372,9 +393,17 @@ int launch_store(StoreArgs& a, bool turn, hipStream_t st) {
 }
 
 template <int D, int FORMAT>
-int launch_read(const ReadArgs& a, int64_t heads, hipStream_t st) {
-  hipLaunchKernelGGL((read_kernel<D, FORMAT>), dim3((unsigned)(a.blocks * heads)), dim3(kThreads),
-                     0, st, a);
+int launch_read(ReadArgs& a, int64_t heads, hipStream_t st) {
+  constexpr int kItems = 2, kRows = kThreads / (D / 8);
+  const int64_t cus = device_cus();
+  if (cus <= 0) return (int)hipErrorNoDevice;
+  // Two rows a thread where that leaves eight workgroups to a CU; fewer would not fill it.
+  const bool many = (a.rows + kItems * kRows - 1) / (kItems * kRows) * heads >= 8 * cus;
+  const int64_t per = kRows * (many ? kItems : 1);
+  a.blocks = (a.rows + per - 1) / per;
+  if (a.blocks > 0x7fffffff / heads) return UMIC_ERR_UNSUPPORTED;
+  auto* kern = many ? read_kernel<D, FORMAT, kItems> : read_kernel<D, FORMAT, 1>;
+  hipLaunchKernelGGL(kern, dim3((unsigned)(a.blocks * heads)), dim3(kThreads), 0, st, a);
   return launch_status();
 }
 
@@ -457,7 +486,7 @@ extern "C" int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, vo
   if (B == 0 || rows == 0) return UMIC_OK;
   if (!k_out || !v_out || !table) return UMIC_ERR_INVALID_ARG;
   if (!kv_lens && (kv_len < 0 || kv_len > cap)) return UMIC_ERR_INVALID_ARG;
-  if (B > (1 << 20) || rows > ((int64_t)1 << 31) || !aligned16(k_out) || !aligned16(v_out))
+  if (B > (1 << 20) || 2 * B * cache->heads > 0x7fffffff || rows > ((int64_t)1 << 31) || !aligned16(k_out) || !aligned16(v_out))
     return UMIC_ERR_UNSUPPORTED;
   const umic_cache8_t& c = *cache;
   const int64_t D = c.head_dim;
@@ -470,10 +499,7 @@ extern "C" int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, vo
   a.table_ld = table_ld, a.rows = rows, a.len = (int)kv_len, a.cap = (int)cap;
   a.shift = __builtin_ctzll((unsigned long long)c.page_size);
   a.pages = (int)c.pages, a.Hk = (int)c.heads;
-  const int64_t per = kThreads / (D / 16);
-  a.blocks = (rows + per - 1) / per;
   const int64_t heads = 2 * B * c.heads;
-  if (a.blocks > 0x7fffffff / heads) return UMIC_ERR_UNSUPPORTED;
   hipStream_t st = as_stream(stream);
   const bool f = c.format == UMIC_CODES_INT8;
   if (D == 64)
