@@ -686,13 +686,13 @@ __device__ __forceinline__ void zero_rows(const AttnArgs& a) {
 
 // What attend_few's waves share of a workgroup's LDS.
 template <int D>
-struct FewShared {
+struct alignas(16) FewShared {
+  float acc[kWaves][16][D + 4];  // first: read and written 16 bytes at a time
+  float ml[kWaves][16][2];
   int sums[kWaves];
   int found[2];
   int arrived[2];
   Segment kept[2];  // those that other workgroups have a part of: the first, the last
-  float ml[kWaves][16][2];
-  float acc[kWaves][16][D + 4];
 };
 
 // Joins the waves of a workgroup that has done a segment's tiles: rows of the output, or a
