@@ -99,7 +99,16 @@ struct Raw<4> {
 // a row.  NT: stores past the caches, where the halves of a row are whole lines
 // (16381 tokens of 32 + 8 heads of 128: 72 us for 80; rows of 80, which are not,
 // 46 for 40).
-// block: of a.tokens tokens; cs: [token][pair] (cos, sin) in LDS; FINE: turn_of's.
+// Where the (cos, sin) of a token's pair lies among its D floats, if lanes of 8 pairs each
+// are to read theirs 16 bytes at a time side by side: [two pairs of a lane][lane].  (Pair by
+// pair, 64 bytes a lane, the reads met in their banks: 16381 tokens of 32 + 8 heads with
+// 8-bit rows 70 us for 68.)
+__device__ __forceinline__ int turn_at(int pair, int lanes) {
+  return ((pair >> 1 & 3) * lanes + (pair >> 3)) * 4 + (pair & 1) * 2;
+}
+
+// block: of a.tokens tokens; cs: [token][pair] (cos, sin) in LDS.  FINE: turn_of's, and
+// turn_at's order (VEC 8).
 template <int VEC, bool NORM, bool NT, bool FINE = false>
 __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, float* cs) {
   constexpr int kItems = kItemsOf<NORM>;
@@ -140,7 +149,7 @@ __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, f
             dst[u] = out + page * a.ko_sb + hk * a.ko_sh + r * a.ko_st + d;
         }
       }
-      at[u] = t * half + d;
+      at[u] = FINE ? t * 2 * half + (d >> 1) : t * half + d;
       lo[u].load(src + d);
       hi[u].load(src + half + d);
     }
@@ -157,8 +166,9 @@ __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, f
       const int64_t pos = a.positions[ax * a.p_sa + (t0 + t) * a.p_st];
       turn_of<FINE>(pos, a.turn[f], s, c);
     }
-    cs[2 * i] = c * a.scale;
-    cs[2 * i + 1] = s * a.scale;
+    const int to = FINE ? t * 2 * half + turn_at(f, half >> 3) : 2 * i;
+    cs[to] = c * a.scale;
+    cs[to + 1] = s * a.scale;
   }
   __syncthreads();
   for (int base = 0; base < items; base += kItems * kThreads) {
@@ -202,7 +212,8 @@ __device__ __forceinline__ void axial_rows(const AxialArgs& a, unsigned block, f
       }
 #pragma unroll
       for (int j = 0; j < VEC; ++j) {
-        const float co = cs[2 * (t + j)], si = cs[2 * (t + j) + 1];
+        const int from = FINE ? t + (j >> 1) * (half >> 1) + (j & 1) * 2 : 2 * (t + j);
+        const float co = cs[from], si = cs[from + 1];
         ox[j] = x[j] * co - y[j] * si;
         oy[j] = y[j] * co + x[j] * si;
       }

@@ -13,9 +13,9 @@
 // finds by its lanes which are a block's, and which is its first: that one's workgroup
 // writes all of them.  Behind those workgroups stand others that rotate q.
 //
-// What bounds it: at prompt sizes HBM, less what the short chains of a block (its slots,
-// rows, maximum, codes) leave idle: 16381 tokens of 32 + 8 heads of 128 70 us, 5.2 TB/s (q
-// alone 47, the codes alone 36); 3100 with the norm 19; 8 tokens 6, a chain of loads.
+// What bounds it: HBM at prompt sizes, 16381 tokens of 32 + 8 heads of 128 63 us, 5.8 TB/s
+// (a large copy 6.1); 3100 with the norm 18.8, of which 12 are their bytes', the rest the
+// chain of a block (its slots, rows, maximum, codes); 8 tokens 6, that chain alone.
 #include "axial.hpp"
 #include "codes.hpp"
 
@@ -120,7 +120,7 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
         float s, c;
         turn_of<true>(pos[u], turn, s, c);
         if (t < n)
-          *reinterpret_cast<f32x2_t*>(cs + t * D + 2 * (threadIdx.x % (D / 2))) =
+          *reinterpret_cast<f32x2_t*>(cs + t * D + turn_at(threadIdx.x % (D / 2), kLanes)) =
               f32x2_t{c * a.x.scale, s * a.x.scale};
       }
     }
@@ -213,11 +213,12 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
               }
             }
             const int its = __builtin_popcountll(all & (((uint64_t)1 << of[p]) - 1));
-            const float* t = cs + its * D + 2 * c8;
+            const float* t = cs + its * D + c8 / 2;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-              ox[j] = x[j] * t[2 * j] - y[j] * t[2 * j + 1];
-              oy[j] = y[j] * t[2 * j] + x[j] * t[2 * j + 1];
+              const float* cosine = t + (j >> 1) * (4 * kLanes) + (j & 1) * 2;
+              ox[j] = x[j] * cosine[0] - y[j] * cosine[1];
+              oy[j] = y[j] * cosine[0] + x[j] * cosine[1];
             }
             const bool is = at_row[p] >= 0;
             lo[p] = is ? pack8(ox) : u32x4{0, 0, 0, 0};
