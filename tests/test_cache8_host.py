@@ -141,6 +141,8 @@ def test_pages():
     assert type(twin) is cache8.Pages8 and twin.layout("x", -1).struct.k_codes == twin.k.data_ptr()
     with pytest.raises(ValueError, match="cache is on"):
         c.layout("x", 0)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        c._replace(k_scale=c.k_scale.clone().requires_grad_()).layout("x", -1)
 
 
 def test_wrappers_refuse_cpu_tensors():

@@ -66,7 +66,9 @@ class _Fields(NamedTuple):
 class Pages8(_Fields):
     """k, v: codes [pages, Hk, page_size, D] of one type and layout, rows of 16-byte
     chunks; k_scale, v_scale: fp32 [pages, Hk, page_size / BLOCK], powers of two.  Looked at
-    at its first use; one object for many calls saves looking again."""
+    at its first use, and again where its tensors have moved: one object for many calls saves
+    looking.  Their shapes and strides are not changed in place (``transpose_``,
+    ``resize_``)."""
 
     def __reduce__(self):  # copies look for themselves
         return type(self), tuple(self)
@@ -111,6 +113,8 @@ def _look(who: str, cache: Pages8, dev: int) -> _Layout:
                          f"{tuple(ks.shape)} and {vs.dtype} {tuple(vs.shape)} for pages {tuple(shape)}")
     if any(t.get_device() != dev for t in cache):
         raise ValueError(f"{who}: the cache is on {k.device}, not with the other tensors")
+    if any(t.requires_grad for t in cache):
+        raise RuntimeError(f"{who}: the cache has no gradient; its tensors must not require one")
     pointers = tuple(t.data_ptr() for t in cache)
     struct = _lib.Cache8(*pointers, shape[0], shape[2], shape[1], shape[3], st[0], st[1], st[2],
                          sst[0], sst[1], DTYPES[k.dtype])

@@ -97,7 +97,8 @@ class PagedArena:
 
     def read(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
         """A layer's keys and values as bf16, two [requests, heads, n, D]: rows of each
-        request in order, n of the longest, zero past a request's own."""
+        request in order, n of the longest, zero past a request's own.  (After steps that
+        ``lens`` does not follow: ``sync`` first.)"""
         n = max(self.lens)
         if self.scales is not None:
             return cache8.read(self.codes(layer), self.table, self.kv_len, n)
