@@ -162,7 +162,7 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
     qw, kw, eps = axial._norm_args("cache8.rotate_append", norm, D)
     if norm is not None and (qw | kw) & 15:
         raise ValueError("cache8.rotate_append: norm weights must be 16-byte aligned")
-    out = torch.empty((T, Hq, D), dtype=_BF16, device=q.device)
+    out = q.new_empty((T, Hq, D))
     p0, p1 = positions.stride()
     with _lib.device_of(q):
         _lib.call("umic_cache8_append_bf16", lay.at, q.data_ptr(), k.data_ptr(), v.data_ptr(),
@@ -225,8 +225,8 @@ def read(cache: Pages8, table: torch.Tensor, kv_len, rows: int, *,
     if start is not None:
         _bf16._lengths("start", start, B, dev)
     shape = (B, lay.heads, rows, lay.head_dim)
-    k = torch.empty(shape, dtype=_BF16, device=table.device)
-    v = torch.empty(shape, dtype=_BF16, device=table.device)
+    k = table.new_empty(shape, dtype=_BF16)
+    v = torch.empty_like(k)
     with _lib.device_of(k):
         _lib.call("umic_cache8_read_bf16", lay.at, k.data_ptr(), v.data_ptr(), table.data_ptr(),
                   lens, _lib.ptr(start), B, rows, ld, width, n, _lib.stream_of(k))
@@ -270,7 +270,7 @@ def attention(q: torch.Tensor, cache: Pages8, kv_len, table: torch.Tensor, *,
     if not _bf16._chunks_ok(q):
         q = q.clone(memory_format=torch.contiguous_format)
     if out is None:
-        out = torch.empty((B, S, Hq, D), dtype=_BF16, device=q.device)
+        out = q.new_empty((B, S, Hq, D))
         o0, o1, o2 = S * Hq * D, Hq * D, D
     else:
         require_device(q, out)
