@@ -565,10 +565,9 @@ typedef struct {
 
 /*
  * New tokens' keys and values [T, heads, head_dim] into such a cache.
- * Slots do not repeat, and the tokens whose slots are of one block stand within 24
- * neighbouring tokens (tokens of other blocks, or of none, may stand between them): they
- * are written as a whole.  With a = max |x| over them for a head, and n their lowest row of
- * the block, the scale is that of
+ * Slots do not repeat; the tokens whose slots are of one block, wherever they stand among
+ * the T (2^31 - 1 at most), are written as a whole.  With a = max |x| over them for a head,
+ * and n their lowest row of the block, the scale is that of
  *   e = max(floor(log2 a) - 7 (E4M3) or 6 (INT8), -100), and where n > 0 at least what
  *   the block's was;
  * a code is x * 2^-e rounded to the nearest, ties to even (INT8: 127.5 to 127).  Where a

@@ -9,12 +9,16 @@
 // half a step of the last scale and a half of that, and so on: one step.  The scale is
 // that of bf16 values' exponents, whole numbers throughout.
 //
-// The tokens of a block that one call brings stand within kSpan neighbours, so that a wave
-// finds by its lanes which are a block's, and which is its first: that one's workgroup
-// writes all of them.  Behind those workgroups stand others that rotate q.
+// A block is its first token's workgroup's to write, with all tokens that the call brings to
+// it.  A wave finds them by its lanes where they stand within kSpan neighbours, and 16 there
+// are all.  Of a block with fewer the workgroup looks through all slots of the call, 8 bytes
+// a token, while positions and sines are on their way: tokens before the first one make it
+// another's, and with others behind it the block is done by itself, after the rest.  (Prompts
+// of one request have two such blocks; 4096 tokens of 64 requests 28.8 us, 28.0 without the
+// look, 64 single tokens 6.5 and 6.1.)  Behind those workgroups stand others that rotate q.
 //
-// What bounds it: HBM at prompt sizes, 16381 tokens of 32 + 8 heads of 128 63 us, 5.8 TB/s
-// (a large copy 6.1); 3100 with the norm 18.8, of which 12 are their bytes', the rest the
+// What bounds it: HBM at prompt sizes, 16381 tokens of 32 + 8 heads of 128 62 us, 5.9 TB/s
+// (a large copy 6.1); 3100 with the norm 19.3, of which 12 are their bytes', the rest the
 // chain of a block (its slots, rows, maximum, codes); 8 tokens 6, that chain alone.
 #include "axial.hpp"
 #include "codes.hpp"
@@ -23,9 +27,10 @@ namespace umic {
 namespace {
 
 constexpr int kWaves = kThreads / kWave;
-constexpr int kSpan = 24;    // tokens that hold all of a block's
+constexpr int kSpan = 24;    // tokens among which a wave finds a block's by its lanes
 constexpr int kChunk = 16;   // tokens of a workgroup, at most
-static_assert(kChunk + 2 * (kSpan - 1) <= kWave, "a wave sees a chunk and what may share its blocks");
+static_assert(kChunk + 2 * (kSpan - 1) <= kWave, "a wave sees a chunk and its neighbours");
+constexpr int kEarlier = 1 << 16;  // counts a block's tokens before the first one near
 
 struct StoreArgs {
   AxialArgs x;  // of q's rows: Hq heads, no keys; and what k's rotation needs
@@ -44,10 +49,34 @@ struct StoreArgs {
   unsigned blocks;   // workgroups that do so; those behind them rotate q
 };
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// x of another lane; all lanes are there.
+__device__ __forceinline__ int of_lane(int x, int lane) { return __builtin_amdgcn_ds_bpermute(lane * 4, x); }
+
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
   const u16x2 m = __builtin_elementwise_max(__builtin_bit_cast(u16x2, a), __builtin_bit_cast(u16x2, b));
   return __builtin_bit_cast(uint32_t, m);
+}
+
+// f over 16 neighbouring lanes, by moves of the vector unit: with shuffles, whose lane numbers
+// take a register each, the blocks done one by one did not fit.
+template <typename F>
+__device__ __forceinline__ int over16(int x, F f) {
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false));   // quad_perm [1,0,3,2]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false));   // quad_perm [2,3,0,1]
+  x = f(x, __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false));  // row_half_mirror
+  return f(x, __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false));  // row_mirror
+}
+
+// The kernel's arguments, loaded again: what the rare paths need of them is not held over the
+// others.
+__device__ __forceinline__ StoreArgs store_args_again() {
+  typedef const __attribute__((address_space(4))) StoreArgs* Args;
+  Args p = (Args)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const StoreArgs*)p;
 }
 
 // A wave's task is a block's new tokens of one head, keys or values.  The sines and cosines
@@ -61,6 +90,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
   constexpr int kOld = D / 64;              // 16-byte chunks of a block's codes a lane holds
   constexpr int kTurns = 2 * kThreads / D;  // tokens whose sines the workgroup does at a time
   extern __shared__ float cs[];             // (cos, sin): [token][pair]
+  __shared__ int far_n[kChunk];             // tokens of a block that are not near its first one
+  __shared__ int far[kChunk][kBlockTokens];
+  __shared__ int found[kWaves];             // a wave has seen such tokens
   if (blockIdx.x >= a.blocks) {
     if constexpr (TURN) axial_rows<8, NORM, (D >= 128), true>(a.x, blockIdx.x - a.blocks, cs);
     return;
@@ -72,212 +104,321 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
 
   // lane i: token t0 - (kSpan - 1) + i, its block and row; a slot outside the pool has none
   const int64_t base = t0 - (kSpan - 1);
-  const int64_t tok = base + lane;
-  int64_t slot = -1;
-  if (lane < a.chunk + 2 * (kSpan - 1) && tok >= 0 && tok < a.x.T) slot = a.x.slots[tok];
+  auto slot_of = [&](const StoreArgs& a, int lane) {
+    const int64_t tok = base + lane;
+    const bool in = lane < a.chunk + 2 * (kSpan - 1) && tok >= 0 && tok < a.x.T;
+    return in ? a.x.slots[tok] : -1;
+  };
+  const int64_t slot = slot_of(a, lane);
+  // The look through all slots: few are asked for here, beside the lanes' own.  (After them
+  // 64 single tokens took 7.2 us.)
+  const bool wide = a.x.T > kSpan;  // no two tokens of fewer are further apart
+  constexpr int kSlots = 8;         // a thread's at a time
+  int64_t slots[kSlots];
+  auto load_slots = [&](const StoreArgs& a, int64_t t) {
+#pragma unroll
+    for (int u = 0; u < kSlots; ++u, t += kThreads) slots[u] = t < a.x.T ? a.x.slots[t] : -1;
+  };
+  const bool few = a.x.T <= kSlots * kThreads;
+  if (wide && few) load_slots(a, threadIdx.x);
   int axis = -1;
   uint64_t turn = 0;
   if constexpr (TURN) {
     axis = a.x.axis[threadIdx.x % (D / 2)];
     turn = a.x.turn[threadIdx.x % (D / 2)];
   }
-  const int block = slot >= 0 && slot < a.slots_n ? (int)(slot / kBlockTokens) : -1;
-  const int row = (int)(slot & (kBlockTokens - 1));
+  auto block_of = [](const StoreArgs& a, int64_t slot) {
+    return slot >= 0 && slot < a.slots_n ? (int)(slot / kBlockTokens) : -1;
+  };
+  int block = block_of(a, slot), row = (int)(slot & (kBlockTokens - 1)), where = lane;
   // lane i: where the i-th of some of the lanes stands
   auto nth = [&](uint64_t some) {
-    const int below = __builtin_popcountll(some & (((uint64_t)1 << lane) - 1));
+    const int below =
+        __builtin_amdgcn_mbcnt_hi((uint32_t)(some >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some, 0));
     const int to = some >> lane & 1 ? below : __builtin_popcountll(some) + lane - below;
     return __builtin_amdgcn_ds_permute(to * 4, lane);
   };
+  // the tokens of lane at's block that stand near it
+  auto near_of = [&](int at) {
+    const int blk = __builtin_amdgcn_readlane(block, at);
+    return __ballot(block == blk) >> at << (64 - kSpan) >> (64 - kSpan) << at;
+  };
 
-  uint64_t firsts = 0, all = 0;  // of this workgroup's blocks: the first tokens, all tokens
+  // Of the chunk's tokens: those that are their block's first, and those of them whose block
+  // can have more than the ones near; and all tokens near a first.
+  uint32_t now = 0, open = 0;
+  uint64_t all = 0;
+  bool more = false;  // some has
   for (int c = 0; c < a.chunk; ++c) {
     const int at = kSpan - 1 + c;
     const int blk = __builtin_amdgcn_readlane(block, at);
     const uint64_t mates = __ballot(block == blk);
     // a block is its first token's to write
-    if (blk < 0 || mates << (64 - at) >> (64 - (kSpan - 1))) continue;
-    firsts |= (uint64_t)1 << at;
-    all |= mates >> at << (64 - kSpan) >> (64 - kSpan) << at;
+    if (blk < 0 || mates << (64 - at)) continue;
+    const uint64_t run = near_of(at);
+    now |= 1u << c;
+    all |= run;
+    if (__builtin_popcountll(run) < kBlockTokens) open |= 1u << c;
+    if (mates != run) more = true;
   }
-  if (!firsts) return;
-  if constexpr (TURN) {
-    const int turned = nth(all), n = __builtin_popcountll(all);
-    const bool moves = axis >= 0 && axis < a.x.A;  // an axis that is not there does not turn
-    constexpr int kAhead = 4;                      // positions on their way
-    for (int i = 0; i < n; i += kAhead * kTurns) {
-      int64_t pos[kAhead];
+  if (!now) return;
+  if (!wide) open = 0;
+  if (open) {
+    for (int64_t i = 0; i < a.x.T; i += kSlots * kThreads) {
+      if (!few) load_slots(a, i + threadIdx.x);
+      int blk[kSlots];
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int t = i + u * kTurns + threadIdx.x / (D / 2);
-        const int64_t token = base + __shfl(turned, min(t, n - 1), kWave);
-        pos[u] = moves ? a.x.positions[axis * a.x.p_sa + token * a.x.p_st] : 0;
+      for (int u = 0; u < kSlots; ++u) {  // the neighbours have been looked at
+        const uint64_t off = i + u * kThreads + threadIdx.x - base;
+        blk[u] = off < (uint64_t)(a.chunk + 2 * (kSpan - 1)) ? -1 : block_of(a, slots[u]);
       }
+#pragma unroll 1
+      for (uint32_t m = open; m; m &= m - 1) {
+        const int its = __builtin_amdgcn_readlane(block, kSpan - 1 + __builtin_ctz(m));
 #pragma unroll
-      for (int u = 0; u < kAhead; ++u) {
-        const int t = i + u * kTurns + threadIdx.x / (D / 2);
-        if (i + u * kTurns >= n) break;
-        float s, c;
-        turn_of<true>(pos[u], turn, s, c);
-        if (t < n)
-          *reinterpret_cast<f32x2_t*>(cs + t * D + turn_at(threadIdx.x % (D / 2), kLanes)) =
-              f32x2_t{c * a.x.scale, s * a.x.scale};
+        for (int u = 0; u < kSlots; ++u) more |= blk[u] == its;
+      }
+    }
+    const bool any = __any(more);
+    if (lane == 0) found[threadIdx.x / kWave] = any;
+  }
+  uint32_t apart = 0;  // firsts whose blocks have tokens that are not near them
+  // Tokens that are not near their block's first one: the block is another workgroup's, or apart.
+  auto gather = [&] {
+    const StoreArgs z = store_args_again();
+    if (threadIdx.x < kChunk) far_n[threadIdx.x] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int64_t i = 0; i < z.x.T; i += kSlots * kThreads) {
+      load_slots(z, i + threadIdx.x);
+#pragma unroll 1
+      for (uint32_t m = open; m; m &= m - 1) {
+        const int c = __builtin_ctz(m), its = __builtin_amdgcn_readlane(block, kSpan - 1 + c);
+#pragma unroll
+        for (int u = 0; u < kSlots; ++u) {
+          const int64_t t = i + u * kThreads + threadIdx.x, off = t - base - (kSpan - 1 + c);
+          if (block_of(z, slots[u]) != its || (off >= 0 && off < kSpan)) continue;
+          const int n = atomicAdd(&far_n[c], off < 0 ? kEarlier : 1) & (kEarlier - 1);
+          if (off > 0 && n < kBlockTokens) far[c][n] = (int)(t - base);
+        }
       }
     }
     __syncthreads();
-  }
-
-  const int c8 = (lane % kLanes) * 8;
-  int part = mine;
-  for (; firsts; firsts &= firsts - 1, part -= parts) {
-    // the chunk's tasks, its blocks' parts in turn, are dealt over the waves
-    if (part >= parts) continue;
-    const int at = __builtin_ctzll(firsts);
-    const int blk = __builtin_amdgcn_readlane(block, at);
-    const uint64_t run = __ballot(block == blk) >> at << (64 - kSpan) >> (64 - kSpan) << at;
-    const int n = min(kBlockTokens, __builtin_popcountll(run));
-    const int place = nth(run);
-    const int its_row = __shfl(row, place, kWave);
-    int row0 = lane < n ? its_row : kBlockTokens;  // the lowest
-#pragma unroll
-    for (int m = 1; m < kBlockTokens; m <<= 1) row0 = min(row0, __shfl_xor(row0, m, kWave));
-    row0 = __builtin_amdgcn_readfirstlane(row0);
-    const int64_t in = (int64_t)blk * kBlockTokens;
-    const int64_t page = in >> a.shift;
-    const int64_t r0 = in & (((int64_t)1 << a.shift) - 1);
-    int at_row[kPasses];  // -1: no token
-    int of[kPasses];      // where it stands
-#pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-      const int i = p * kRows + lane / kLanes;
-      of[p] = __shfl(place, i < n ? i : 0, kWave);
-      at_row[p] = __shfl(its_row, i, kWave);
-      if (i >= n) at_row[p] = -1;
+    for (uint32_t m = open; m; m &= m - 1) {
+      const int n = uniform(far_n[__builtin_ctz(m)]);
+      if (!n) continue;
+      now &= ~(m & -m);
+      if (n < kEarlier) apart |= m & -m;
     }
-    u32x4 lo[kPasses], hi[kPasses];
-    auto fetch = [&](int part) {
-      const bool keys = part < a.Hk;
-      const int h = keys ? part : part - (int)a.Hk;
-      const uint16_t* const src = (keys ? a.k : a.v) + h * (keys ? a.k_sh : a.v_sh) + c8;
-      const int64_t st = keys ? a.k_st : a.v_st;
+  };
+  const int c8 = (lane % kLanes) * 8;
+  // the blocks whose tokens are near, then the others one by one
+  for (bool first = true;; first = false) {
+    if (__builtin_expect(!now, 0)) {
+      if (!apart) break;
+      const StoreArgs z = store_args_again();
+      const int c = __builtin_ctz(apart), at = kSpan - 1 + c;
+      now = apart & -apart;
+      apart &= apart - 1;
+      // lanes at .. get the block's tokens
+      int again = lane;
+      asm volatile("" : "+v"(again));  // what follows from it is not held over the tasks
+      block = block_of(z, slot_of(z, again));
+      const uint64_t run = near_of(at);
+      const int near = __builtin_popcountll(run);
+      const int n = min(kBlockTokens, near + uniform(far_n[c]));
+      const int i = lane - at;
+      where = of_lane(nth(run), i & (kWave - 1));
+      if (i >= near && i < n) where = far[c][i - near];
+      block = -1;
+      if (i >= 0 && i < n) {
+        const int64_t slot = z.x.slots[base + where];
+        block = block_of(z, slot);
+        row = (int)(slot & (kBlockTokens - 1));
+      }
+      all = __ballot(block >= 0);
+      if (TURN) __syncthreads();  // the sines have been read
+    }
+    if constexpr (TURN) {
+      const int turned = of_lane(where, nth(all)), count = __builtin_popcountll(all);
+      const bool moves = axis >= 0 && axis < a.x.A;  // an axis that is not there does not turn
+      constexpr int kAhead = 4;                      // positions on their way
+      int thread = threadIdx.x;
+      asm volatile("" : "+v"(thread));  // as above
+      for (int i = 0; i < count; i += kAhead * kTurns) {
+        int64_t pos[kAhead];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int t = i + u * kTurns + thread / (D / 2);
+          const int64_t token = base + of_lane(turned, min(t, count - 1));
+          pos[u] = moves ? a.x.positions[axis * a.x.p_sa + token * a.x.p_st] : 0;
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+          const int t = i + u * kTurns + thread / (D / 2);
+          if (i + u * kTurns >= count) break;
+          float s, c;
+          turn_of<true>(pos[u], turn, s, c);
+          if (t < count)
+            *reinterpret_cast<f32x2_t*>(cs + t * D + turn_at(thread % (D / 2), kLanes)) =
+                f32x2_t{c * a.x.scale, s * a.x.scale};
+        }
+      }
+    }
+    if (TURN || (first && open)) __syncthreads();
+    if (first && open && __builtin_expect(uniform(found[0] | found[1] | found[2] | found[3]), 0))
+      gather();
+
+    int part = mine;
+    for (; now; now &= now - 1, part -= parts) {
+      // the chunk's tasks, its blocks' parts in turn, are dealt over the waves
+      if (part >= parts) continue;
+      const int at = kSpan - 1 + __builtin_ctz(now);
+      const int blk = __builtin_amdgcn_readlane(block, at);
+      const uint64_t run = near_of(at);
+      const int n = min(kBlockTokens, __builtin_popcountll(run));
+      const int place = nth(run);
+      const int its_row = of_lane(row, place), its_where = of_lane(where, place);
+      const int its_turn = __builtin_popcountll(all & (((uint64_t)1 << place) - 1));
+      int row0 = lane < n ? its_row : kBlockTokens;  // the lowest
+      row0 = uniform(over16(row0, [](int x, int y) { return min(x, y); }));
+      const int64_t first = (int64_t)blk * kBlockTokens;
+      const int64_t page = first >> a.shift;
+      const int64_t r0 = first & (((int64_t)1 << a.shift) - 1);
+      int at_row[kPasses];  // its row, and times 16 where its sines are; negative: no token
+      int of[kPasses];      // where it stands
 #pragma unroll
       for (int p = 0; p < kPasses; ++p) {
-        lo[p] = hi[p] = u32x4{0, 0, 0, 0};
-        if (at_row[p] >= 0) {
-          const uint16_t* x = src + (base + of[p]) * st;
-          lo[p] = ld_stream(reinterpret_cast<const u32x4*>(x));
-          hi[p] = ld_stream(reinterpret_cast<const u32x4*>(x + D / 2));
-        }
+        const int i = lane / kLanes + p * kRows;
+        of[p] = of_lane(its_where, i);
+        at_row[p] = of_lane(its_turn * kBlockTokens + its_row, i);
+        if (i >= n) at_row[p] = (int)0x80000000;
       }
-    };
-    fetch(part);
+      u32x4 lo[kPasses], hi[kPasses];
+      auto fetch = [&](int part) {
+        const bool keys = part < a.Hk;
+        const int h = keys ? part : part - (int)a.Hk;
+        const uint16_t* const src = (keys ? a.k : a.v) + h * (keys ? a.k_sh : a.v_sh) + c8;
+        const int64_t st = keys ? a.k_st : a.v_st;
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          lo[p] = hi[p] = u32x4{0, 0, 0, 0};
+          if (at_row[p] >= 0) {
+            const uint16_t* x = src + (base + of[p]) * st;
+            lo[p] = ld_stream(reinterpret_cast<const u32x4*>(x));
+            hi[p] = ld_stream(reinterpret_cast<const u32x4*>(x + D / 2));
+          }
+        }
+      };
+      fetch(part);
 #pragma unroll 1
-    for (; part < parts; part += waves) {
-      const bool keys = part < a.Hk;
-      const int h = keys ? part : part - (int)a.Hk;
-      uint8_t* const to = (keys ? a.k8 : a.v8) + page * a.c_sb + h * a.c_sh + r0 * a.c_ss;
-      float* const scale = (keys ? a.ks : a.vs) + page * a.s_sb + h * a.s_sh + r0 / kBlockTokens;
-      u32x4 old[kOld];
-      float was = 0.0f;
-      if (row0 > 0) {
-        was = *scale;
+      for (; part < parts; part += waves) {
+        const bool keys = part < a.Hk;
+        const int h = keys ? part : part - (int)a.Hk;
+        const StoreArgs y = store_args_again();
+        uint8_t* const to = (keys ? y.k8 : y.v8) + page * y.c_sb + h * y.c_sh + r0 * y.c_ss;
+        float* const scale = (keys ? y.ks : y.vs) + page * y.s_sb + h * y.s_sh + r0 / kBlockTokens;
+        u32x4 old[kOld];
+        float was = 0.0f;
+        if (row0 > 0) {
+          was = *scale;
 #pragma unroll
-        for (int j = 0; j < kOld; ++j) {
-          const int i = j * kWave + lane, r = i / (D / 16);
-          old[j] = u32x4{0, 0, 0, 0};
-          if (r < row0) old[j] = *reinterpret_cast<const u32x4*>(to + r * a.c_ss + i % (D / 16) * 16);
+          for (int j = 0; j < kOld; ++j) {
+            const int i = j * kWave + lane, r = i / (D / 16);
+            old[j] = u32x4{0, 0, 0, 0};
+            if (r < row0) old[j] = *reinterpret_cast<const u32x4*>(to + r * y.c_ss + i % (D / 16) * 16);
+          }
         }
-      }
-      if constexpr (TURN)
-        if (keys)
+        if constexpr (TURN)
+          if (keys)
 #pragma unroll
-          for (int p = 0; p < kPasses; ++p) {
-            if (p * kRows >= n) break;
-            float x[8], y[8], ox[8], oy[8];
-            unpack8(lo[p], x);
-            unpack8(hi[p], y);
-            if constexpr (NORM) {
-              float ss = 0.0f;
+            for (int p = 0; p < kPasses; ++p) {
+              if (p * kRows >= n) break;
+              float x[8], y[8], ox[8], oy[8];
+              unpack8(lo[p], x);
+              unpack8(hi[p], y);
+              if constexpr (NORM) {
+                float ss = 0.0f;
 #pragma unroll
-              for (int j = 0; j < 8; ++j) ss += x[j] * x[j] + y[j] * y[j];
+                for (int j = 0; j < 8; ++j) ss += x[j] * x[j] + y[j] * y[j];
+                const float r = rsqrt_cr(group_sum<kLanes>(ss) / (float)D + a.x.eps);
+                auto by = [&](float (&z)[8], const uint16_t* w) {
+                  float f[8];
+                  unpack8(*reinterpret_cast<const u32x4*>(w), f);
 #pragma unroll
-              for (int m = 1; m < kLanes; m <<= 1) ss += __shfl_xor(ss, m, kWave);
-              const float r = rsqrt_cr(ss / (float)D + a.x.eps);
-              float wx[8], wy[8];
-              unpack8(*reinterpret_cast<const u32x4*>(a.x.kw + c8), wx);
-              unpack8(*reinterpret_cast<const u32x4*>(a.x.kw + c8 + D / 2), wy);
+                  for (int j = 0; j < 8; ++j) z[j] = z[j] * r * f[j];
+                };
+                by(x, a.x.kw + c8);
+                __builtin_amdgcn_sched_barrier(0);  // both halves' weights at once do not fit
+                by(y, a.x.kw + c8 + D / 2);
+              }
+              const float* t = cs + (at_row[p] & 0xffff) / kBlockTokens * D + c8 / 2;
 #pragma unroll
               for (int j = 0; j < 8; ++j) {
-                x[j] = x[j] * r * wx[j];
-                y[j] = y[j] * r * wy[j];
+                const float* cosine = t + (j >> 1) * (4 * kLanes) + (j & 1) * 2;
+                ox[j] = x[j] * cosine[0] - y[j] * cosine[1];
+                oy[j] = y[j] * cosine[0] + x[j] * cosine[1];
               }
+              const bool is = at_row[p] >= 0;
+              lo[p] = is ? pack8(ox) : u32x4{0, 0, 0, 0};
+              hi[p] = is ? pack8(oy) : u32x4{0, 0, 0, 0};
             }
-            const int its = __builtin_popcountll(all & (((uint64_t)1 << of[p]) - 1));
-            const float* t = cs + its * D + c8 / 2;
+        // the largest magnitude's exponent: that of bf16 numbers as whole ones
+        uint32_t top = 0;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-              const float* cosine = t + (j >> 1) * (4 * kLanes) + (j & 1) * 2;
-              ox[j] = x[j] * cosine[0] - y[j] * cosine[1];
-              oy[j] = y[j] * cosine[0] + x[j] * cosine[1];
+        for (int p = 0; p < kPasses; ++p)
+#pragma unroll
+          for (int w = 0; w < 4; ++w)
+            top = max_halves(top, max_halves(lo[p][w] & 0x7fff7fffu, hi[p][w] & 0x7fff7fffu));
+        top = over16((int)top, [](int x, int y) { return (int)max_halves(x, y); });
+        const int one = (int)max(top & 0xffffu, top >> 16);
+        const int most = max(max(__builtin_amdgcn_readlane(one, 0), __builtin_amdgcn_readlane(one, 16)),
+                             max(__builtin_amdgcn_readlane(one, 32), __builtin_amdgcn_readlane(one, 48)));
+        const uint32_t was_bits = __builtin_amdgcn_readfirstlane(__float_as_uint(was));
+        // 255: infinite or NaN; the block then reads as NaN
+        const bool wild = (most >> 7) == 255 || (row0 > 0 && (was_bits << 1) >= 0xff000000u);
+        const int was_exp = (int)(was_bits >> 23 & 255) - 127;
+        int e = max((most >> 7) - 127 - C::kTop, kLeastExp);
+        if (row0 > 0) e = max(e, was_exp);
+        const float s = __uint_as_float((uint32_t)(e + 127) << 23);
+        const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+        if (lane == 0) *scale = wild ? __builtin_nanf("") : s;
+        uint32_t w[kPasses][4];
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          float x[8], y[8];
+          unpack8(lo[p], x);
+          unpack8(hi[p], y);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) x[j] *= inv, y[j] *= inv;
+          w[p][0] = C::round4(x), w[p][1] = C::round4(x + 4);
+          w[p][2] = C::round4(y), w[p][3] = C::round4(y + 4);
+        }
+        if (part + waves < parts) fetch(part + waves);
+#pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+          if (at_row[p] < 0) continue;
+          uint8_t* r = to + (at_row[p] & (kBlockTokens - 1)) * y.c_ss + c8;
+          *reinterpret_cast<u32x2*>(r) = wild ? u32x2{0, 0} : u32x2{w[p][0], w[p][1]};
+          *reinterpret_cast<u32x2*>(r + D / 2) = wild ? u32x2{0, 0} : u32x2{w[p][2], w[p][3]};
+        }
+        if (row0 > 0 && !wild && e > was_exp) {  // the rows before, at the new scale
+          const float ratio = was * inv;
+#pragma unroll
+          for (int j = 0; j < kOld; ++j) {
+            const int i = j * kWave + lane, r = i / (D / 16);
+            if (r >= row0) continue;
+            u32x4 o;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+              float x[4];
+              C::values4(old[j][q], x);
+#pragma unroll
+              for (int y = 0; y < 4; ++y) x[y] *= ratio;
+              o[q] = C::round4(x);
             }
-            const bool is = at_row[p] >= 0;
-            lo[p] = is ? pack8(ox) : u32x4{0, 0, 0, 0};
-            hi[p] = is ? pack8(oy) : u32x4{0, 0, 0, 0};
+            *reinterpret_cast<u32x4*>(to + r * y.c_ss + i % (D / 16) * 16) = o;
           }
-      // the largest magnitude's exponent: that of bf16 numbers as whole ones
-      uint32_t top = 0;
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p)
-#pragma unroll
-        for (int w = 0; w < 4; ++w)
-          top = max_halves(top, max_halves(lo[p][w] & 0x7fff7fffu, hi[p][w] & 0x7fff7fffu));
-#pragma unroll
-      for (int m = 1; m < kWave; m <<= 1) top = max_halves(top, __shfl_xor(top, m, kWave));
-      const int most = __builtin_amdgcn_readfirstlane(max(top & 0xffffu, top >> 16));
-      const uint32_t was_bits = __builtin_amdgcn_readfirstlane(__float_as_uint(was));
-      // 255: infinite or NaN; the block then reads as NaN
-      const bool wild = (most >> 7) == 255 || (row0 > 0 && (was_bits << 1) >= 0xff000000u);
-      const int was_exp = (int)(was_bits >> 23 & 255) - 127;
-      int e = max((most >> 7) - 127 - C::kTop, kLeastExp);
-      if (row0 > 0) e = max(e, was_exp);
-      const float s = __uint_as_float((uint32_t)(e + 127) << 23);
-      const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-      if (lane == 0) *scale = wild ? __builtin_nanf("") : s;
-      uint32_t w[kPasses][4];
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        float x[8], y[8];
-        unpack8(lo[p], x);
-        unpack8(hi[p], y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[j] *= inv, y[j] *= inv;
-        w[p][0] = C::round4(x), w[p][1] = C::round4(x + 4);
-        w[p][2] = C::round4(y), w[p][3] = C::round4(y + 4);
-      }
-      if (part + waves < parts) fetch(part + waves);
-#pragma unroll
-      for (int p = 0; p < kPasses; ++p) {
-        if (at_row[p] < 0) continue;
-        uint8_t* r = to + at_row[p] * a.c_ss + c8;
-        *reinterpret_cast<u32x2*>(r) = wild ? u32x2{0, 0} : u32x2{w[p][0], w[p][1]};
-        *reinterpret_cast<u32x2*>(r + D / 2) = wild ? u32x2{0, 0} : u32x2{w[p][2], w[p][3]};
-      }
-      if (row0 > 0 && !wild && e > was_exp) {  // the rows before, at the new scale
-        const float ratio = was * inv;
-#pragma unroll
-        for (int j = 0; j < kOld; ++j) {
-          const int i = j * kWave + lane, r = i / (D / 16);
-          if (r >= row0) continue;
-          u32x4 o;
-#pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            float x[4];
-            C::values4(old[j][q], x);
-#pragma unroll
-            for (int y = 0; y < 4; ++y) x[y] *= ratio;
-            o[q] = C::round4(x);
-          }
-          *reinterpret_cast<u32x4*>(to + r * a.c_ss + i % (D / 16) * 16) = o;
         }
       }
     }
@@ -447,7 +588,7 @@ extern "C" int umic_cache8_append_bf16(
   } else if (Hq || q_w || k_w) {
     return UMIC_ERR_INVALID_ARG;
   }
-  if (Hq > (1 << 16) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7) || !aligned16(q) ||
+  if (T > 0x7fffffff || Hq > (1 << 16) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7) || !aligned16(q) ||
       !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_w) || !aligned16(k_w))
     return UMIC_ERR_UNSUPPORTED;
   const umic_cache8_t& c = *cache;

@@ -147,9 +147,9 @@ def rotate_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: 
                   plan: axial.AxisPlan, slots: torch.Tensor, cache: Pages8,
                   norm=None) -> torch.Tensor:
     """``axial.rotate`` of q and k (norm: ``(q_w, k_w, eps)``), k's rotated rows and v's
-    rows written as codes to ``slots`` (int64 [T], distinct; one outside the pool writes
-    nothing).  The tokens of one block (slots that differ below BLOCK only) stand within 24
-    neighbouring tokens, as ``paged.plan_pages`` has them next to each other.  Returns the
+    rows written as codes to ``slots`` (int64 [T], distinct, in any order; one outside the
+    pool writes nothing).  Quickest where a block's tokens (slots that differ below BLOCK
+    only) stand within 24 neighbouring ones, as ``paged.plan_pages`` has them.  Returns the
     rotated q."""
     require_device(q, k, v, *(norm[:2] if norm is not None else ()))
     axial._check("cache8.rotate_append", q, k, positions, plan, norm)
