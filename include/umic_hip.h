@@ -565,6 +565,7 @@ typedef struct {
 
 /*
  * New tokens' keys and values [T, heads, head_dim] into such a cache.
+ * No two rows or scales of the cache share memory, k's and v's neither.
  * Slots do not repeat; the tokens whose slots are of one block, wherever they stand among
  * the T (2^31 - 1 at most), are written as a whole.  With a = max |x| over them for a head,
  * and n their lowest row of the block, the scale is that of

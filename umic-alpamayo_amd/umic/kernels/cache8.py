@@ -54,6 +54,7 @@ class _Layout(NamedTuple):
     heads: int
     page_size: int
     head_dim: int
+    apart: bool  # no two rows or scales share memory
 
 
 class _Fields(NamedTuple):
@@ -68,7 +69,8 @@ class Pages8(_Fields):
     chunks; k_scale, v_scale: fp32 [pages, Hk, page_size / BLOCK], powers of two.  Looked at
     at its first use, and again where its tensors have moved: one object for many calls saves
     looking.  Their shapes and strides are not changed in place (``transpose_``,
-    ``resize_``)."""
+    ``resize_``), nor are they made to require a gradient.  Rows or scales that share memory
+    (``expand``) can be read, not written."""
 
     def __reduce__(self):  # copies look for themselves
         return type(self), tuple(self)
@@ -96,6 +98,26 @@ def empty(pages: int, heads: int, page_size: int, head_dim: int,
     return Pages8(k, v, k_scale, v_scale)
 
 
+def _apart(shape, strides, width: int, between: int) -> bool:
+    """Whether blocks of ``width`` bytes, at these strides in bytes, lie each for itself (the
+    strides nest), and those of a second tensor of the layout ``between`` bytes on between
+    them."""
+    dims, span = [], width
+    for st, n in sorted((st, n) for st, n in zip(strides, shape) if n > 1):
+        if st < span:
+            return False
+        dims.append((st, n))
+        span += st * (n - 1)
+
+    def meet(gap: int, inner: int) -> bool:
+        if inner == 0:
+            return abs(gap) < width
+        st, n = dims[inner - 1]
+        return any(abs(m) < n and meet(gap - m * st, inner - 1) for m in (gap // st, gap // st + 1))
+
+    return 0 in shape or not meet(between, len(dims))
+
+
 def _look(who: str, cache: Pages8, dev: int) -> _Layout:
     k, v, ks, vs = cache
     shape, st, sst = k.shape, k.stride(), ks.stride()
@@ -118,7 +140,9 @@ def _look(who: str, cache: Pages8, dev: int) -> _Layout:
     pointers = tuple(t.data_ptr() for t in cache)
     struct = _lib.Cache8(*pointers, shape[0], shape[2], shape[1], shape[3], st[0], st[1], st[2],
                          sst[0], sst[1], DTYPES[k.dtype])
-    return _Layout(pointers, struct, ctypes.addressof(struct), shape[0], shape[1], shape[2], shape[3])
+    apart = (_apart(shape[:3], st[:3], shape[3], pointers[1] - pointers[0])
+             and _apart(ks.shape, [4 * n for n in sst], 4, pointers[3] - pointers[2]))
+    return _Layout(pointers, struct, ctypes.addressof(struct), *shape, apart)
 
 
 def _chunks16(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
@@ -137,6 +161,8 @@ def _rows(who: str, k, v, slots, cache: Pages8) -> tuple[_Layout, tuple, tuple]:
     if len(shape) != 3 or v.shape != shape or shape[1] != lay.heads or shape[2] != lay.head_dim:
         raise ValueError(f"{who}: k {tuple(shape)} and v {tuple(v.shape)} must be [T, {lay.heads}, "
                          f"{lay.head_dim}], as the pages")
+    if not lay.apart:
+        raise ValueError(f"{who}: rows or scales of the cache share memory")
     if (slots.dtype is not torch.int64 or slots.shape != shape[:1] or slots.get_device() != dev
             or not slots.is_contiguous()):
         raise ValueError(f"{who}: slots must be a contiguous int64 vector of {shape[0]} on k's device")
