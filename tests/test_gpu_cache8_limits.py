@@ -6,8 +6,10 @@ from __future__ import annotations
 import pytest
 import torch
 
+import cache8_reference as ref8
+import paged_reference as ref
 from helpers import bf16_randn
-from test_gpu_cache8 import DEV, call, filled, queries
+from test_gpu_cache8 import DEV, KINDS, call, filled, new_cache, queries
 from umic.kernels import axial, cache8
 
 pytestmark = pytest.mark.gpu
@@ -33,3 +35,55 @@ def test_rows_that_share_memory_are_read_not_written():
             cache8.rotate_append(x, x, x, at[None], plan, at, bad)
         for t, was in zip(cache, before):
             assert torch.equal(t.view(torch.uint8), was.view(torch.uint8))
+
+
+# --- the largest values, and queries past what fp32 holds of their products with codes ---------
+
+MOST = float(torch.finfo(torch.bfloat16).max)
+
+
+def values_of(cache):
+    """(k, v) [pages, Hk, page, D] that the codes stand for: none past bf16's largest number."""
+    kc, vc, ks, vs = ref8.numbers(cache)
+    return tuple(torch.tensor(ref8.values(c, s)).clamp(-MOST, MOST) for c, s in ((kc, ks), (vc, vs)))
+
+
+def cache_of(kind, k, v, page=16):
+    """A request [n, Hk, D] in pages of its own, and its table."""
+    n, Hk, D = k.shape
+    pages = -(-n // page)
+    cache = new_cache(kind, pages, Hk, page, D)
+    cache8.append(k.to(DEV), v.to(DEV), torch.arange(n, device=DEV), cache)
+    return cache, torch.arange(pages, dtype=torch.int32, device=DEV)[None]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D,S,Hq", [(64, 1, 4), (128, 1, 8), (256, 1, 2), (128, 20, 4)])
+@pytest.mark.parametrize("n", [5, 200, 3000])
+def test_large_queries_of_small_keys(kind, D, S, Hq, n):
+    """q of 2^122 over keys of 2^-93: scores of ordinary size, but not q times a code."""
+    g = torch.Generator().manual_seed(D + n)
+    k, v = (bf16_randn(n, 2, D, gen=g) for _ in range(2))
+    cache, table = cache_of(kind, (k.float() * 2.0 ** -93).to(torch.bfloat16), v)
+    q = (bf16_randn(1, S, Hq, D, gen=g).float() * 2.0 ** 122).to(torch.bfloat16).to(DEV).transpose(1, 2)
+    scale = 2.0 ** -29 * D ** -0.5
+    got = call(q, cache, [n], table, scale=scale)
+    ref.check_attention(got, *ref.attention(q, *values_of(cache), [n], table.cpu(), scale=scale))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_weights_above_one_of_large_values(kind, D):
+    """Keys 128 to 159 weigh 2^7 of what came before them, with a value of 2^127 among them: the
+    other columns are as they are."""
+    g = torch.Generator().manual_seed(D)
+    k = torch.zeros(160, 1, D, dtype=torch.bfloat16)
+    k[128:, 0, 0] = 5.1875
+    v = bf16_randn(160, 1, D, gen=g)
+    v[130, 0, 0] = 1.5 * 2.0 ** 127
+    cache, table = cache_of(kind, k, v)
+    q = torch.zeros(1, 2, 1, D, dtype=torch.bfloat16, device=DEV)
+    q[..., 0] = 1.0
+    got = call(q, cache, [160], table, scale=1.0)
+    want, tol = ref.attention(q, *values_of(cache), [160], table.cpu(), scale=1.0)
+    ref.check_attention(got[..., 1:], want[..., 1:], tol[..., 1:])

@@ -7,8 +7,10 @@
 // 16 is a block, so that its scales are a wave's scalars.
 //
 // Up to 16 rows: codes go from memory to registers; the scores of a tile are scaled by
-// its key scale, its weights by its value scale.  More rows: codes are turned into scaled
-// bf16 numbers once for the workgroup, on their way into LDS.
+// its key scale, its weights by its value scale.  Where a scale or an element of q is 2^97
+// or more, that can pass what fp32 holds: such a part of a segment is done again, from
+// scaled codes.  More rows: codes are turned into scaled bf16 numbers once for the
+// workgroup, on their way into LDS.
 //
 // A block whose scale is NaN reads as NaN: a row that sees one of its keys is NaN, others
 // are as without it.
@@ -97,6 +99,12 @@ __device__ __forceinline__ void spoil(R& r, int wild, int k0) {
       for (int nt = 0; nt < (int)(sizeof(r.lim) / sizeof(int)); ++nt)
         if (k0 + 16 * i < r.lim[nt]) r.l[nt] = __builtin_nanf("");
 }
+
+// The larger one's bits: numbers above 0, and NaN above all.
+__device__ __forceinline__ int top_of(float a, float b) {
+  return max((int)__float_as_uint(a), (int)__float_as_uint(b));
+}
+__device__ __forceinline__ int top_of(const Tile& p) { return top_of(p.ks, p.vs); }
 
 // attention.hpp's Deal with the remainder spread evenly, workgroup w beginning at w all /
 // nwg: where the workgroups of a segment come out even, none has parts of two (a request
@@ -200,9 +208,63 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         for (int c = 0; c < VW; ++c) vc[j][c] = vp[c];
       }
     };
+    // Keys that are not there, and those that a row does not see.
+    auto mask = [&](f32x4_t (&sc)[1][2], const Tile (&p)[2], int k0) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const int at = 4 * g4 + (j & 3), key = k0 + 16 * (j >> 2) + at;
+        const bool there = at < p[j >> 2].n;
+        if (!there || key >= r.lim[0]) sc[0][j >> 2][j & 3] = -__builtin_inff();
+#pragma unroll
+        for (int c = 0; c < VW; ++c) vc[j][c] = there ? vc[j][c] : 0;
+      }
+    };
     auto tiles = [](const Attn8Args& x, const View& w, int k0, Tile (&p)[2]) {
       p[0] = tile_of(x, w, k0);
       p[1] = tile_of(x, w, k0 + 16);
+    };
+    // A segment's tiles of this wave from scaled codes, one step at a time.
+    auto again = [&](const Segment& s, const View& w) {
+      const Attn8Args y = args8_again();
+      r.clear();
+#pragma unroll 1
+      for (int t = s.t0; t < s.t1; ++t) {
+        const int k0 = t * kTile + wave * kStep;
+        Tile p[2];
+        tiles(y, w, k0, p);
+        load_k(w.k, p, y.a.c_ss);
+        load_v(w.v, p, y.a.c_ss);
+        f32x4_t sc[1][2] = {};
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int kk = 0; kk < KK; ++kk) {
+            const u32x2 lo = C::four(kc[i][kk / 2][kk % 2 * 2], p[i].ks);
+            const u32x2 hi = C::four(kc[i][kk / 2][kk % 2 * 2 + 1], p[i].ks);
+            sc[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                as_bf(u32x4{lo[0], lo[1], hi[0], hi[1]}), as_bf(r.q[0][kk]), sc[0][i], 0, 0, 0);
+          }
+        mask(sc, p, k0);
+        u32x4 ph[1], pl[1];
+        r.weights(sc, y.a.c, ph, pl);
+        float vs[2];
+        int wild = 0;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          vs[i] = p[i].n ? p[i].vs : 0.0f;
+          if (is_nan(vs[i])) wild |= 1 << i, vs[i] = 0.0f;
+        }
+        uint32_t v[R::VR];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int c = 0; c < VW; ++c) {
+            const u32x2 x = C::four(vc[j][c], vs[j >> 2]);
+            v[R::VW * j + 2 * c] = x[0], v[R::VW * j + 2 * c + 1] = x[1];
+          }
+        r.product(v, ph, pl);
+        if (wild) spoil(r, wild, k0);
+      }
     };
     bool go = walk.next(a, seg);  // not where a segment's start is all that it was dealt
     View view, after;
@@ -223,6 +285,7 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         tiles(y, after, nxt.t0 * kTile + wave * kStep, turn);
       }
       bool turned = false;  // the next segment's keys are on their way
+      int top = 0;          // bits of the largest scale
       r.clear();
       for (int t = seg.t0; t < seg.t1; ++t) {
         const int k0 = t * kTile + wave * kStep, k1 = k0 + kTile;
@@ -247,19 +310,13 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         }
         if (more || go) load_k(from_k, next, y.a.c_ss);  // under the softmax and the second product
         if (k0 + kStep > r.lo || here[0].n < 16 || here[1].n < 16) {
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int at = 4 * g4 + (j & 3), key = k0 + 16 * (j >> 2) + at;
-            const bool there = at < here[j >> 2].n;
-            if (!there || key >= r.lim[0]) sc[0][j >> 2][j & 3] = -__builtin_inff();
-#pragma unroll
-            for (int c = 0; c < VW; ++c) vc[j][c] = there ? vc[j][c] : 0;
-          }
+          mask(sc, here, k0);
         }
         float vs[2] = {here[0].n ? here[0].vs : 0.0f, here[1].n ? here[1].vs : 0.0f};
         const int wild = (is_nan(vs[0]) ? 1 : 0) | (is_nan(vs[1]) ? 2 : 0);
         if (wild & 1) vs[0] = 0.0f;
         if (wild & 2) vs[1] = 0.0f;
+        top = max(top, max(top_of(here[0]), top_of(here[1])));
         u32x4 ph[1], pl[1];
         r.template weights<true>(sc, y.a.c, ph, pl, vs);
 #pragma unroll
@@ -278,6 +335,15 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         if (wild) spoil(r, wild, k0);
         if (more || go) load_v(from_v, next, y.a.c_ss);
         here[0] = next[0], here[1] = next[1];
+      }
+      // q is looked at here: ahead of the loop its wait changed those inside (a token over
+      // 131001 keys 97 us for 93)
+      uint32_t any = 0;
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) any |= wide_q(r.q[0][kk]);
+      if (__builtin_expect(top >= kWideBits || __any(any != 0), 0)) {
+        turned = false;
+        again(seg, view);
       }
       if (go) {
         const AttnArgs z = args_again();

@@ -17,6 +17,19 @@ int check_cache8(const umic_cache8_t* cache, int64_t& cap, int64_t table_w);
 template <int FORMAT>
 struct Codes;
 
+// 2^97.  From it on a scale, times a weight of the softmax, can pass what fp32 holds, and so
+// can products of codes with elements of q (wide_q).
+constexpr int kWideBits = (127 + 97) << 23;
+
+// Whether one of these bf16 numbers is 2^97 or more, infinite or NaN: the exponents' upper
+// three bits, both halves of a word at once.
+__device__ __forceinline__ uint32_t wide_q(u32x4 v) {
+  uint32_t any = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) any |= (v[i] & 0x70007000u) + 0x10001000u;
+  return any & 0x80008000u;
+}
+
 // Scales are such that a block's largest magnitude is 2^7 to 2^8 codes, below e4m3's
 // largest, 448: its bits, but for the three of a code's fraction, are the exponent's.
 template <>
