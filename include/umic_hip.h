@@ -547,7 +547,8 @@ int umic_cache_attention_bf16(const void* q, const void* k, const void* v, void*
 /*
  * A paged cache of 8-bit codes.  A block is 16 consecutive rows of a page, of one key head;
  * its values are code * scale, scale = {k,v}_scale[page * s_sb + head * s_sh + row / 16] =
- * 2^e.  Codes: 8-bit floats of 4 exponent and 3 fraction bits without infinities
+ * 2^e; where that passes the largest bf16 number (E4M3 codes from 256 on of 2^120), that
+ * one.  Codes: 8-bit floats of 4 exponent and 3 fraction bits without infinities
  * (UMIC_CODES_E4M3), or signed integers in [-127, 127] (UMIC_CODES_INT8), at page * c_sb +
  * head * c_sh + row * c_ss of k_codes and v_codes, 16-byte aligned, strides multiples of
  * 16.  head_dim: 64, 128 or 256; page_size: a power of two from 16; at most 2^30 pages and

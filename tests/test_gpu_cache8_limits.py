@@ -58,6 +58,49 @@ def cache_of(kind, k, v, page=16):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_the_largest_values_are_finite(kind, D):
+    """Numbers that round up to a code past bf16's range are read, and attended to, as the largest."""
+    steps = torch.tensor([1.0, 0.99609375, 0.9765625, 0.97265625, 0.5, 0.25])  # of the largest: 255 to 248, 247 ..
+    row = torch.cat((steps, -steps, torch.zeros(D - 12))) * MOST
+    x = torch.stack((row, row.flip(0), torch.full((D,), MOST)))[:, None].to(torch.bfloat16)  # [3, 1, D]
+    x = torch.cat([x[i:i + 1] for i in range(3) for _ in range(16)])  # a block of each
+    cache, table = cache_of(kind, x, x)
+    k, _ = values_of(cache)
+    got = cache8.read(cache, table, 48, 48)
+    for y in got:
+        assert torch.equal(y[0, 0].double().cpu(), k.flatten(0, 2))
+        assert y.isfinite().all()
+        err = (y[0, 0].double().cpu() - x[:, 0].double()).abs()
+        assert (err <= (2.0 ** -4 * x[:, 0].double().abs() if kind == "e4m3" else 2.0 ** 120)).all()
+    for S in (1, 20):  # one key: its own value
+        out = call(queries(1, S, 2, D, S) * 0, cache, [1], table)
+        assert torch.equal(out[0, -1, 0], got[1][0, 0, 0]) and not out[0, :-1].any()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("D,S", [(64, 1), (128, 1), (256, 1), (128, 3), (64, 20), (128, 40), (256, 9)])
+def test_large_values_that_rows_do_not_see(kind, D, S):
+    """The largest values behind a row leave it as it is; keys of that size that q is 0 for count as
+    any other."""
+    g = torch.Generator().manual_seed(D + S)
+    n, Hk = 150, 2
+    k, v = (bf16_randn(n, Hk, D, gen=g) for _ in range(2))
+    v[n - 1, 0, ::3] = MOST
+    v[n - 1, 1, 1::3] = -MOST
+    k[77:79, :, 5] = MOST
+    cache, table = cache_of(kind, k, v)
+    q = queries(1, S, 4, D, S)
+    q[..., 5] = 0
+    got = call(q, cache, [n], table)
+    want, tol = ref.attention(q, *values_of(cache), [n], table.cpu())
+    others = torch.arange(D) % 3 == 2
+    for rows in ((got[:, :-1], want[:, :-1], tol[:, :-1]),
+                 (got[:, -1:][..., others], want[:, -1:][..., others], tol[:, -1:][..., others])):
+        ref.check_attention(*rows)
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D,S,Hq", [(64, 1, 4), (128, 1, 8), (256, 1, 2), (128, 20, 4)])
 @pytest.mark.parametrize("n", [5, 200, 3000])
 def test_large_queries_of_small_keys(kind, D, S, Hq, n):

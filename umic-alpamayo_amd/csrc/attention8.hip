@@ -100,6 +100,13 @@ __device__ __forceinline__ void spoil(R& r, int wild, int k0) {
         if (k0 + 16 * i < r.lim[nt]) r.l[nt] = __builtin_nanf("");
 }
 
+// Four codes as scaled bf16 numbers, infinite ones as the largest.
+template <typename C>
+__device__ __forceinline__ u32x2 scaled4(uint32_t w, float scale) {
+  const u32x2 v = C::four(w, scale);
+  return C::kPasses ? at_most(v) : v;
+}
+
 // The larger one's bits: numbers above 0, and NaN above all.
 __device__ __forceinline__ int top_of(float a, float b) {
   return max((int)__float_as_uint(a), (int)__float_as_uint(b));
@@ -239,8 +246,8 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         for (int i = 0; i < 2; ++i)
 #pragma unroll
           for (int kk = 0; kk < KK; ++kk) {
-            const u32x2 lo = C::four(kc[i][kk / 2][kk % 2 * 2], p[i].ks);
-            const u32x2 hi = C::four(kc[i][kk / 2][kk % 2 * 2 + 1], p[i].ks);
+            const u32x2 lo = scaled4<C>(kc[i][kk / 2][kk % 2 * 2], p[i].ks);
+            const u32x2 hi = scaled4<C>(kc[i][kk / 2][kk % 2 * 2 + 1], p[i].ks);
             sc[0][i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
                 as_bf(u32x4{lo[0], lo[1], hi[0], hi[1]}), as_bf(r.q[0][kk]), sc[0][i], 0, 0, 0);
           }
@@ -259,7 +266,7 @@ __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8
         for (int j = 0; j < 8; ++j)
 #pragma unroll
           for (int c = 0; c < VW; ++c) {
-            const u32x2 x = C::four(vc[j][c], vs[j >> 2]);
+            const u32x2 x = scaled4<C>(vc[j][c], vs[j >> 2]);
             v[R::VW * j + 2 * c] = x[0], v[R::VW * j + 2 * c + 1] = x[1];
           }
         r.product(v, ph, pl);
@@ -442,6 +449,14 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
         kv[buf][0][row * CH + (chunk ^ k_swizzle(row & 15))] = u32x4{k0[0], k0[1], k1[0], k1[1]};
         kv[buf][1][row * CH + (chunk ^ v_swizzle(row))] = u32x4{v0[0], v0[1], v1[0], v1[1]};
       }
+      if (C::kPasses && __builtin_expect(top_of(raw_ks, vs) >= kMostBits, 0))
+#pragma unroll 1
+        for (int c = 0; c < 2 * CH / 8; ++c) {  // as they lie in LDS, eight threads to a row
+          const bool keys = c < CH / 8;
+          const int chunk = part * (CH / 8) + c % (CH / 8);
+          u32x4& x = kv[buf][keys ? 0 : 1][row * CH + (chunk ^ (keys ? k_swizzle(row & 15) : v_swizzle(row)))];
+          x = at_most(x);
+        }
       if ((wave & 1) == 0 && lane == 0) marks[buf][tile] = (wild ? 1 : 0) | (raw_out ? 4 : 0);
     };
     __syncthreads();  // the last segment's reads are done

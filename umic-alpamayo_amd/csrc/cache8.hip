@@ -495,6 +495,12 @@ __global__ __launch_bounds__(kThreads) void read_kernel(ReadArgs a) {
     C::values4(w[i][1], y);
 #pragma unroll
     for (int j = 0; j < 4; ++j) x[j] *= s[i], y[j] *= s[i];
+    if (C::kPasses && s[i] >= kMostScale)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {  // not fminf: NaN stays
+        x[j] = x[j] > kMost ? kMost : x[j] < -kMost ? -kMost : x[j];
+        y[j] = y[j] > kMost ? kMost : y[j] < -kMost ? -kMost : y[j];
+      }
     st_stream(reinterpret_cast<u32x4*>(to + (int64_t)i * kRows * D),
               u32x4{pack2(x[0], x[1]), pack2(x[2], x[3]), pack2(y[0], y[1]), pack2(y[2], y[3])});
   }

@@ -1,6 +1,7 @@
 // Codes of 8 bits with a scale for each block of 16 tokens and key head, a power of two.
 // A code has at most 8 significant bits, so that its value, code times scale, is a bf16
-// number: what is read back is what the attention sees, to the bit.
+// number: what is read back is what the attention sees, to the bit.  Only e4m3's can pass the
+// largest one (255 2^120 is rounded to 256 2^120): their value is that one.
 #pragma once
 
 #include "common.hpp"
@@ -17,9 +18,23 @@ int check_cache8(const umic_cache8_t* cache, int64_t& cap, int64_t table_w);
 template <int FORMAT>
 struct Codes;
 
+constexpr float kMost = 0x1.fep127f;      // bf16's largest number
+constexpr float kMostScale = 0x1p120f;    // from it on a code's value can pass it
+constexpr int kMostBits = (127 + 120) << 23;
 // 2^97.  From it on a scale, times a weight of the softmax, can pass what fp32 holds, and so
 // can products of codes with elements of q (wide_q).
 constexpr int kWideBits = (127 + 97) << 23;
+
+// Two bf16 numbers, infinite ones as the largest.
+__device__ __forceinline__ uint32_t at_most(uint32_t w) {
+  if ((w & 0x7fffu) == 0x7f80u) w -= 1u;
+  if ((w & 0x7fff0000u) == 0x7f800000u) w -= 0x10000u;
+  return w;
+}
+__device__ __forceinline__ u32x2 at_most(u32x2 v) { return u32x2{at_most(v[0]), at_most(v[1])}; }
+__device__ __forceinline__ u32x4 at_most(u32x4 v) {
+  return u32x4{at_most(v[0]), at_most(v[1]), at_most(v[2]), at_most(v[3])};
+}
 
 // Whether one of these bf16 numbers is 2^97 or more, infinite or NaN: the exponents' upper
 // three bits, both halves of a word at once.
@@ -35,6 +50,7 @@ __device__ __forceinline__ uint32_t wide_q(u32x4 v) {
 template <>
 struct Codes<UMIC_CODES_E4M3> {
   static constexpr int kTop = 7;
+  static constexpr bool kPasses = true;  // values can pass bf16's largest number
   // two bf16 numbers of the low (HI: high) half of w
   template <bool HI>
   static __device__ __forceinline__ uint32_t pair(uint32_t w, float scale = 1.0f) {
@@ -67,6 +83,7 @@ struct Codes<UMIC_CODES_E4M3> {
 template <>
 struct Codes<UMIC_CODES_INT8> {
   static constexpr int kTop = 6;
+  static constexpr bool kPasses = false;
   static __device__ __forceinline__ void values4(uint32_t w, float* x) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x[i] = (float)(int8_t)(w >> (8 * i));

@@ -3,8 +3,9 @@ decode step, twice the tokens of a pool.
 
 ``Pages8`` holds codes, ``torch.int8`` or ``torch.float8_e4m3fn``, and a scale for each
 block of ``BLOCK`` = 16 consecutive rows of a page, of one key head.  Scales are powers of
-two, so that a code times its scale is a bf16 number: what ``read`` gives is what
-``attention`` sees.  Requests, tables, slots and lengths are ``paged.plan_pages``'s.
+two, so that a code times its scale is a bf16 number (at the top of its range the largest
+one): what ``read`` gives is what ``attention`` sees.  Requests, tables, slots and lengths
+are ``paged.plan_pages``'s.
 
 Writing.  ``rotate_append`` is ``axial.rotate_append`` with the rows quantised, and
 ``append`` writes k as it comes.  A block's scale follows the largest magnitude a among
