@@ -575,9 +575,11 @@ typedef struct {
  * a code is x * 2^-e rounded to the nearest, ties to even (INT8: 127.5 to 127).  Where a
  * block's scale grows, its rows before n are rounded to the new one; its other rows
  * count as dropped, and are left as they are.  A NaN or an infinity among the values
- * makes its block's scale NaN, until the block is begun anew (n == 0).
+ * makes its block's scale NaN, until the block is begun anew (n == 0): rows before it in
+ * the block are lost, also where that token is dropped.
  * turn NULL: k's rows are written as they are (Hq 0, q_w and k_w NULL).  Else q and k are
- * turned, and normed, as by umic_axial_rope_bf16, to q_out [T, Hq, head_dim] (contiguous)
+ * turned, and normed, as by umic_axial_rope_bf16, but by angles that are rounded within a
+ * quarter turn (finer, and not its bits), to q_out [T, Hq, head_dim] (contiguous)
  * and the cache, k by way of bf16.  Strides of q, k and v: multiples of 8, pointers
  * 16-byte aligned.  A slot outside [0, pages * page_size) is not written.
  * No counterpart in the reference, whose cache holds 16-bit rows (cache.py:50-80).

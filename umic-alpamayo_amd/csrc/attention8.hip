@@ -160,8 +160,8 @@ constexpr int few8_of(int64_t D) { return D <= 128 ? 2 : 1; }
 // Up to 16 rows: attention.hip's kernel, a wave to 32 of a tile's 128 keys, the loads of a
 // step in flight while the one before is computed.
 // What bounds it: HBM where the keys are many (64 requests of 8000 keys 170 us, 6.2 TB/s);
-// a request of 3100 keys 11.6 us, of which 4 pass until its first keys are there and 3 to
-// join; of a step's 350 vector instructions int8 codes take 192 (one to a number, half one
+// a request of 3100 keys 10.5 us (bf16 rows 10.2 beside it; 10 to 14 from one process to
+// another), of which 4 pass until its first keys are there and 3 to join; of a step's 350 vector instructions int8 codes take 192 (one to a number, half one
 // to pair it) and e4m3's 80.
 template <int D, int FORMAT>
 __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8Args x) {

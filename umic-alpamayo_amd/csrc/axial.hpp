@@ -94,19 +94,19 @@ struct Raw<4> {
   __device__ __forceinline__ void pack(const float* f) { v = pack4(f); }
 };
 
+// Where the (cos, sin) of a token's pair lies among its D floats, if lanes of 8 pairs each
+// are to read theirs 16 bytes at a time side by side: [two pairs of a lane][lane].  (Pair by
+// pair, 64 bytes a lane, the reads met in their banks: 16381 tokens of 32 + 8 heads with
+// 8-bit rows 70 us for 63.)
+__device__ __forceinline__ int turn_at(int pair, int lanes) {
+  return ((pair >> 1 & 3) * lanes + (pair >> 3)) * 4 + (pair & 1) * 2;
+}
+
 // A lane holds VEC elements of each half of a head row; `group` lanes (a power
 // of two with the norm, whose sum runs over them; lanes past the row idle) hold
 // a row.  NT: stores past the caches, where the halves of a row are whole lines
 // (16381 tokens of 32 + 8 heads of 128: 72 us for 80; rows of 80, which are not,
 // 46 for 40).
-// Where the (cos, sin) of a token's pair lies among its D floats, if lanes of 8 pairs each
-// are to read theirs 16 bytes at a time side by side: [two pairs of a lane][lane].  (Pair by
-// pair, 64 bytes a lane, the reads met in their banks: 16381 tokens of 32 + 8 heads with
-// 8-bit rows 70 us for 68.)
-__device__ __forceinline__ int turn_at(int pair, int lanes) {
-  return ((pair >> 1 & 3) * lanes + (pair >> 3)) * 4 + (pair & 1) * 2;
-}
-
 // block: of a.tokens tokens; cs: [token][pair] (cos, sin) in LDS.  FINE: turn_of's, and
 // turn_at's order (VEC 8).
 template <int VEC, bool NORM, bool NT, bool FINE = false>
