@@ -108,3 +108,50 @@ def test_captured_append_of_another_order():
             ref8.store("int8", model[i], model[i + 2], x.double().numpy(), order.tolist())
         for got, want in zip(ref8.numbers(cache), model):
             assert (got == want).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("T", [1, 24, 25, 63, 64, 65, 1025, 2047, 2048, 2051, 4097])
+def test_any_number_of_tokens(kind, T):
+    """In order with and without a lead, in turn, in no order, with gaps."""
+    g = torch.Generator().manual_seed(T)
+    page, Hk, D = 32, 1, 64
+    room = 2 * T + 70
+    order = torch.randperm(room, generator=g)[:T].tolist()
+    for slots in (list(range(T)), list(range(7, T + 7)), in_turn(2, T, page)[:T], order,
+                  [-1 if i % 11 == 3 else s for i, s in enumerate(range(5, T + 5))]):
+        cache = new_cache(kind, -(-room // page) + 2, Hk, page, D)
+        model = list(ref8.numbers(cache))
+        k, v = (spread(g, T, Hk, D) for _ in range(2))
+        append(kind, cache, model, k, v, slots)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("name", ["prompts", "two halves", "shuffled"])
+def test_many_tokens(kind, name):
+    """More chunks than the chip holds workgroups: ragged prompts, whose blocks are whole but for
+    their ends; a prompt's odd rows, then its even ones; no order."""
+    T, page, Hk, D = 70001, 16, 1, 64
+    g = torch.Generator().manual_seed(3)
+    slots, at = [], 0
+    for i in range(9):
+        n = T // 9 if i < 8 else T - len(slots)
+        slots += range(at + 3 * i, at + 3 * i + n)
+        at += n + 64 - n % 16
+    if name == "two halves":
+        slots = list(range(1, T, 2)) + list(range(0, T, 2))
+    if name == "shuffled":
+        slots = torch.randperm(T + 100, generator=g)[:T].tolist()
+    slots[T // 2] = -1
+    cache = new_cache(kind, max(slots) // page + 1, Hk, page, D)
+    model = list(ref8.numbers(cache))
+    k, v = (spread(g, T, Hk, D) for _ in range(2))
+    append(kind, cache, model, k, v, slots)
+    q = bf16_randn(T, 2, D, gen=g).to(DEV)
+    plan = axial.AxisPlan(torch.zeros(D // 2), [0] * (D // 2), device=DEV)  # nothing turns
+    twin = new_cache(kind, cache.k.shape[0], Hk, page, D)
+    out = cache8.rotate_append(q, k.to(DEV), v.to(DEV), torch.zeros(1, T, dtype=torch.int64, device=DEV),
+                               plan, torch.tensor(slots, device=DEV), twin)
+    assert torch.equal(out, q)
+    for a, b in zip(cache, twin):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))

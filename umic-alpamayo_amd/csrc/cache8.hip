@@ -12,10 +12,11 @@
 // A block is its first token's workgroup's to write, with all tokens that the call brings to
 // it.  A wave finds them by its lanes where they stand within kSpan neighbours, and 16 there
 // are all.  Of a block with fewer the workgroup looks through all slots of the call, 8 bytes
-// a token, while positions and sines are on their way: tokens before the first one make it
-// another's, and with others behind it the block is done by itself, after the rest.  (Prompts
-// of one request have two such blocks; 4096 tokens of 64 requests 28.8 us, 28.0 without the
-// look, 64 single tokens 6.5 and 6.1.)  Behind those workgroups stand others that rotate q.
+// a token: tokens before the first one make it another's, and with others behind it the block
+// is done by itself, after the rest.  A prompt has two such blocks, at its ends, and single
+// tokens have no others.  (64 of them 6.3 us, 6.1 without the look; 16384 tokens of one
+// request 63 and 63, without a rotation, which hides some of it, 29 and 25.)  Behind those
+// workgroups stand others that rotate q.
 //
 // What bounds it: HBM at prompt sizes, 16381 tokens of 32 + 8 heads of 128 62 us, 5.9 TB/s
 // (a large copy 6.1); 3100 with the norm 19.3, of which 12 are their bytes', the rest the
@@ -99,7 +100,15 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
   }
   const int lane = threadIdx.x & (kWave - 1);
   const int waves = kWaves * a.split, parts = 2 * (int)a.Hk;
-  const int64_t t0 = (int64_t)(blockIdx.x / a.split) * a.chunk;
+  // Chunks in another order than workgroups: the first, then from the last one on, as a prompt's
+  // ends look through all slots, and what begins last ends the launch; and each 64 of them turned
+  // by as many places as it comes to, as ends of requests of one length are a power of two chunks
+  // apart, and in order all on a few CUs.
+  // (16384 tokens of 64 requests of 256: 63 us for 77.)
+  const unsigned chunks = a.blocks / a.split, nth_one = blockIdx.x / a.split;
+  unsigned chunk = nth_one ? chunks - nth_one : 0;
+  if ((chunk | 63) < chunks) chunk = (chunk & ~63u) | ((chunk + (chunk >> 6) * 37) & 63);
+  const int64_t t0 = (int64_t)chunk * a.chunk;
   const int mine = __builtin_amdgcn_readfirstlane(blockIdx.x % a.split * kWaves + threadIdx.x / kWave);
 
   // lane i: token t0 - (kSpan - 1) + i, its block and row; a slot outside the pool has none
@@ -111,16 +120,20 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
   };
   const int64_t slot = slot_of(a, lane);
   // The look through all slots: few are asked for here, beside the lanes' own.  (After them
-  // 64 single tokens took 7.2 us.)
+  // 64 single tokens took 7.0 us.)
   const bool wide = a.x.T > kSpan;  // no two tokens of fewer are further apart
-  constexpr int kSlots = 8;         // a thread's at a time
-  int64_t slots[kSlots];
-  auto load_slots = [&](const StoreArgs& a, int64_t t) {
+  constexpr int kPairs = 4;         // of slots, a thread's at a time
+  typedef int64_t pair_t __attribute__((ext_vector_type(2), aligned(8)));
+  constexpr int kLook = kPairs * 2 * kThreads;
+  auto token_of = [](int64_t i, int u) { return i + u * 2 * kThreads + threadIdx.x * 2; };
+  auto load_slots = [&](const StoreArgs& a, int64_t i, pair_t (&p)[kPairs]) {
 #pragma unroll
-    for (int u = 0; u < kSlots; ++u, t += kThreads) slots[u] = t < a.x.T ? a.x.slots[t] : -1;
+    for (int u = 0; u < kPairs; ++u)  // past the end the last pair again
+      p[u] = *reinterpret_cast<const pair_t*>(a.x.slots + min(token_of(i, u), a.x.T - 2));
   };
-  const bool few = a.x.T <= kSlots * kThreads;
-  if (wide && few) load_slots(a, threadIdx.x);
+  const bool few = a.x.T <= kLook;
+  pair_t ahead[kPairs];
+  if (wide && few) load_slots(a, 0, ahead);
   int axis = -1;
   uint64_t turn = 0;
   if constexpr (TURN) {
@@ -164,19 +177,25 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
   if (!now) return;
   if (!wide) open = 0;
   if (open) {
-    for (int64_t i = 0; i < a.x.T; i += kSlots * kThreads) {
-      if (!few) load_slots(a, i + threadIdx.x);
-      int blk[kSlots];
+    if (!few) load_slots(a, 0, ahead);
+    for (int64_t i = 0; i < a.x.T; i += kLook) {
+      uint32_t blk[2 * kPairs];  // without the bits above: one may seem to be a block's that is
+                                 // not, and gather() looks again
 #pragma unroll
-      for (int u = 0; u < kSlots; ++u) {  // the neighbours have been looked at
-        const uint64_t off = i + u * kThreads + threadIdx.x - base;
-        blk[u] = off < (uint64_t)(a.chunk + 2 * (kSpan - 1)) ? -1 : block_of(a, slots[u]);
-      }
+      for (int u = 0; u < kPairs; ++u)
+        for (int v = 0; v < 2; ++v) blk[2 * u + v] = (uint32_t)((uint64_t)ahead[u][v] / kBlockTokens);
+      if (i + kLook < a.x.T) load_slots(a, i + kLook, ahead);
+      if (i < base + kWave && i + kLook > base)  // the neighbours have been looked at
+#pragma unroll
+        for (int u = 0; u < 2 * kPairs; ++u) {
+          const int64_t t = min(token_of(i, u >> 1), a.x.T - 2) + (u & 1);
+          if ((uint64_t)(t - base) < (uint64_t)(a.chunk + 2 * (kSpan - 1))) blk[u] = ~0u;
+        }
 #pragma unroll 1
       for (uint32_t m = open; m; m &= m - 1) {
-        const int its = __builtin_amdgcn_readlane(block, kSpan - 1 + __builtin_ctz(m));
+        const uint32_t its = __builtin_amdgcn_readlane(block, kSpan - 1 + __builtin_ctz(m));
 #pragma unroll
-        for (int u = 0; u < kSlots; ++u) more |= blk[u] == its;
+        for (int u = 0; u < 2 * kPairs; ++u) more |= blk[u] == its;
       }
     }
     const bool any = __any(more);
@@ -189,15 +208,17 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
     if (threadIdx.x < kChunk) far_n[threadIdx.x] = 0;
     __syncthreads();
 #pragma unroll 1
-    for (int64_t i = 0; i < z.x.T; i += kSlots * kThreads) {
-      load_slots(z, i + threadIdx.x);
+    for (int64_t i = 0; i < z.x.T; i += kLook) {
+      load_slots(z, i, ahead);
 #pragma unroll 1
       for (uint32_t m = open; m; m &= m - 1) {
         const int c = __builtin_ctz(m), its = __builtin_amdgcn_readlane(block, kSpan - 1 + c);
 #pragma unroll
-        for (int u = 0; u < kSlots; ++u) {
-          const int64_t t = i + u * kThreads + threadIdx.x, off = t - base - (kSpan - 1 + c);
-          if (block_of(z, slots[u]) != its || (off >= 0 && off < kSpan)) continue;
+        for (int u = 0; u < 2 * kPairs; ++u) {
+          const int64_t t = token_of(i, u >> 1) + (u & 1), off = t - base - (kSpan - 1 + c);
+          // of the last pair for an odd one out, its second slot
+          const int64_t slot = ahead[u >> 1][t == z.x.T - 1 && !(u & 1) ? 1 : u & 1];
+          if (t >= z.x.T || block_of(z, slot) != its || (off >= 0 && off < kSpan)) continue;
           const int n = atomicAdd(&far_n[c], off < 0 ? kEarlier : 1) & (kEarlier - 1);
           if (off > 0 && n < kBlockTokens) far[c][n] = (int)(t - base);
         }
