@@ -3,10 +3,12 @@
 from __future__ import annotations
 
 
+import pytest
 import torch
 
 from test_cache8_host import FAKE, UNS, lib, pages8, struct  # noqa: F401
 from umic.kernels import cache8
+from umic.paged_cache import PagedArena
 
 
 def test_tokens_of_a_call(lib):  # noqa: F811
@@ -40,3 +42,9 @@ def test_rows_that_share_memory():
     assert cache8.empty(0, 2, 16, 64, torch.int8, "cpu").layout("x", -1).apart
     one = cache8.empty(1, 1, 16, 64, torch.int8, "cpu")
     assert one.layout("x", -1).apart and not one._replace(v=one.k).layout("x", -1).apart
+
+
+def test_codes_of_an_arena_of_rows():
+    ar = PagedArena(2, 2, 6, 2, 32, 64, 64, device="cpu")
+    with pytest.raises(ValueError, match="bf16 rows"):
+        ar.codes(0)

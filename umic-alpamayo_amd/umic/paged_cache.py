@@ -93,6 +93,8 @@ class PagedArena:
 
     def codes(self, layer: int) -> cache8.Pages8:
         """A layer's pages of 8-bit codes."""
+        if self.scales is None:
+            raise ValueError("PagedArena: its pages are bf16 rows, not codes")
         return self._codes[layer]
 
     def read(self, layer: int) -> tuple[torch.Tensor, torch.Tensor]:
