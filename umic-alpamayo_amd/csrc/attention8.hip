@@ -111,7 +111,8 @@ __device__ __forceinline__ u32x2 scaled4(uint32_t w, float scale) {
 __device__ __forceinline__ int top_of(float a, float b) {
   return max((int)__float_as_uint(a), (int)__float_as_uint(b));
 }
-__device__ __forceinline__ int top_of(const Tile& p) { return top_of(p.ks, p.vs); }
+// Of a tile that is there: a block that no token has come to can have any scale.
+__device__ __forceinline__ int top_of(const Tile& p) { return p.n ? top_of(p.ks, p.vs) : 0; }
 
 // attention.hpp's Deal with the remainder spread evenly, workgroup w beginning at w all /
 // nwg: where the workgroups of a segment come out even, none has parts of two (a request
@@ -161,8 +162,9 @@ constexpr int few8_of(int64_t D) { return D <= 128 ? 2 : 1; }
 // step in flight while the one before is computed.
 // What bounds it: HBM where the keys are many (64 requests of 8000 keys 170 us, 6.2 TB/s);
 // a request of 3100 keys 10.5 us (bf16 rows 10.2 beside it; 10 to 14 from one process to
-// another), of which 4 pass until its first keys are there and 3 to join; of a step's 350 vector instructions int8 codes take 192 (one to a number, half one
-// to pair it) and e4m3's 80.
+// another), of which 4 pass until its first keys are there and 3 to join; of a step's 350
+// vector instructions int8 codes take 192 (one to a number, half one to pair it) and e4m3's
+// 80.
 template <int D, int FORMAT>
 __global__ __launch_bounds__(kThreads, few8_of(D)) void attend8_few_kernel(Attn8Args x) {
   typedef Rows<D, 1, false> R;
@@ -454,7 +456,8 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 2 : 1) void attend8_many_kerne
         for (int c = 0; c < 2 * CH / 8; ++c) {  // as they lie in LDS, eight threads to a row
           const bool keys = c < CH / 8;
           const int chunk = part * (CH / 8) + c % (CH / 8);
-          u32x4& x = kv[buf][keys ? 0 : 1][row * CH + (chunk ^ (keys ? k_swizzle(row & 15) : v_swizzle(row)))];
+          u32x4& x = kv[buf][keys ? 0 : 1]
+                       [row * CH + (chunk ^ (keys ? k_swizzle(row & 15) : v_swizzle(row)))];
           x = at_most(x);
         }
       if ((wave & 1) == 0 && lane == 0) marks[buf][tile] = (wild ? 1 : 0) | (raw_out ? 4 : 0);
