@@ -53,7 +53,9 @@ struct StoreArgs {
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // x of another lane; all lanes are there.
-__device__ __forceinline__ int of_lane(int x, int lane) { return __builtin_amdgcn_ds_bpermute(lane * 4, x); }
+__device__ __forceinline__ int of_lane(int x, int lane) {
+  return __builtin_amdgcn_ds_bpermute(lane * 4, x);
+}
 
 __device__ __forceinline__ uint32_t max_halves(uint32_t a, uint32_t b) {
   typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
@@ -102,14 +104,13 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
   const int waves = kWaves * a.split, parts = 2 * (int)a.Hk;
   // Chunks in another order than workgroups: the first, then from the last one on, as a prompt's
   // ends look through all slots, and what begins last ends the launch; and each 64 of them turned
-  // by as many places as it comes to, as ends of requests of one length are a power of two chunks
-  // apart, and in order all on a few CUs.
-  // (16384 tokens of 64 requests of 256: 63 us for 77.)
+  // by another number of places, as ends of requests of one length are a power of two chunks
+  // apart, and in order all on a few CUs (16384 tokens of 64 requests of 256: 63 us for 77).
   const unsigned chunks = a.blocks / a.split, nth_one = blockIdx.x / a.split;
   unsigned chunk = nth_one ? chunks - nth_one : 0;
   if ((chunk | 63) < chunks) chunk = (chunk & ~63u) | ((chunk + (chunk >> 6) * 37) & 63);
   const int64_t t0 = (int64_t)chunk * a.chunk;
-  const int mine = __builtin_amdgcn_readfirstlane(blockIdx.x % a.split * kWaves + threadIdx.x / kWave);
+  const int mine = uniform(blockIdx.x % a.split * kWaves + threadIdx.x / kWave);
 
   // lane i: token t0 - (kSpan - 1) + i, its block and row; a slot outside the pool has none
   const int64_t base = t0 - (kSpan - 1);
@@ -303,9 +304,9 @@ __global__ __launch_bounds__(kThreads, D <= 128 ? 4 : 2) void store_kernel(Store
       const int its_turn = __builtin_popcountll(all & (((uint64_t)1 << place) - 1));
       int row0 = lane < n ? its_row : kBlockTokens;  // the lowest
       row0 = uniform(over16(row0, [](int x, int y) { return min(x, y); }));
-      const int64_t first = (int64_t)blk * kBlockTokens;
-      const int64_t page = first >> a.shift;
-      const int64_t r0 = first & (((int64_t)1 << a.shift) - 1);
+      const int64_t in_pool = (int64_t)blk * kBlockTokens;
+      const int64_t page = in_pool >> a.shift;
+      const int64_t r0 = in_pool & (((int64_t)1 << a.shift) - 1);
       int at_row[kPasses];  // its row, and times 16 where its sines are; negative: no token
       int of[kPasses];      // where it stands
 #pragma unroll
@@ -615,8 +616,8 @@ extern "C" int umic_cache8_append_bf16(
   } else if (Hq || q_w || k_w) {
     return UMIC_ERR_INVALID_ARG;
   }
-  if (T > 0x7fffffff || Hq > (1 << 16) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7) || !aligned16(q) ||
-      !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_w) || !aligned16(k_w))
+  if (T > 0x7fffffff || Hq > (1 << 16) || ((q_st | q_sh | k_st | k_sh | v_st | v_sh) & 7) ||
+      !aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(q_out) || !aligned16(q_w) || !aligned16(k_w))
     return UMIC_ERR_UNSUPPORTED;
   const umic_cache8_t& c = *cache;
   const int64_t D = c.head_dim;
@@ -655,7 +656,8 @@ extern "C" int umic_cache8_read_bf16(const umic_cache8_t* cache, void* k_out, vo
   if (B == 0 || rows == 0) return UMIC_OK;
   if (!k_out || !v_out || !table) return UMIC_ERR_INVALID_ARG;
   if (!kv_lens && (kv_len < 0 || kv_len > cap)) return UMIC_ERR_INVALID_ARG;
-  if (B > (1 << 20) || 2 * B * cache->heads > 0x7fffffff || rows > ((int64_t)1 << 31) || !aligned16(k_out) || !aligned16(v_out))
+  if (B > (1 << 20) || 2 * B * cache->heads > 0x7fffffff || rows > ((int64_t)1 << 31) ||
+      !aligned16(k_out) || !aligned16(v_out))
     return UMIC_ERR_UNSUPPORTED;
   const umic_cache8_t& c = *cache;
   const int64_t D = c.head_dim;
